@@ -1,0 +1,40 @@
+// paged_device.h — device helpers shared by the kernels over the paged cache.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "paged_index.h"
+
+namespace rlh {
+
+// f16 and bf16 as the kernels see them: eight in 16 bytes, values as f32.
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+struct HalfF16 {
+  typedef _Float16 T;
+  typedef f16x8_t V8;
+};
+struct HalfBF16 {
+  typedef __bf16 T;
+  typedef bf16x8_t V8;
+};
+
+// One batch as the kernels get it.
+struct Batch {
+  uint32_t n_seq, n_rows, max_q, max_kv, table_stride;
+  const uint32_t* q_start;
+  const uint32_t* kv_len;
+  const uint32_t* table;
+};
+
+__device__ __forceinline__ SeqView load_seq(const Batch& b, uint32_t s, bool* bad) {
+  return seq_view(b.q_start[s], b.q_start[s + 1], b.kv_len[s], b.n_rows, b.max_q, b.max_kv, bad);
+}
+
+__device__ __forceinline__ void raise(uint32_t* status, uint32_t bit) {
+  if (status) atomicOr(status, bit);
+}
+
+}  // namespace rlh

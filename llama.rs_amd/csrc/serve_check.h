@@ -1,0 +1,85 @@
+// serve_check.h — host-side checks shared by the batched serving operators.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/rlh_serve.h"
+#include "sampler.h"
+
+namespace rlh {
+
+inline int serve_error(int code, const std::string& msg) { return set_error(code, msg.c_str()); }
+
+inline uint32_t float_type_size(uint32_t ty) {
+  return ty == RLH_TYPE_F32 ? 4u : ty == RLH_TYPE_F16 || ty == RLH_TYPE_BF16 ? 2u : 0u;
+}
+
+inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+// Whether [a, a + na) and [b, b + nb) share a byte.
+inline bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + nb && y < x + na;
+}
+
+// Bytes from the first to the last value of n rows of `width` values.
+inline uint64_t row_bytes_span(uint64_t n, uint64_t stride, uint64_t width, uint32_t size) {
+  return n ? ((n - 1) * stride + width) * size : 0;
+}
+
+// Rows of `width` values of `size` bytes: pointer and stride as the kernels'
+// 16-byte accesses need them.
+inline int check_rows(const char* name, const void* p, uint64_t stride, uint64_t width, uint32_t size) {
+  if (!p) return serve_error(RLH_EINVAL, std::string(name) + " is null");
+  if (!aligned(p, 16)) return serve_error(RLH_EINVAL, std::string(name) + " is not aligned to 16 bytes");
+  if (stride < width) return serve_error(RLH_EINVAL, std::string(name) + ": stride below the row's width");
+  if (stride > (1ull << 32)) return serve_error(RLH_EINVAL, std::string(name) + ": stride above 2^32");
+  if (stride * size % 16) return serve_error(RLH_EINVAL, std::string(name) + ": stride is not a multiple of 16 bytes");
+  return RLH_OK;
+}
+
+// The pool and the batch (no device needed).
+int check_batch(const rlh_kv_pages* kv, const rlh_seqs* seqs, uint32_t n_head);
+
+// The current device, then pointers against it.
+class DeviceCheck {
+ public:
+  int begin() {
+    if (hipGetDevice(&dev_) == hipSuccess) return RLH_OK;
+    (void)hipGetLastError();
+    return serve_error(RLH_EDEVICE, "no HIP device available (librlh needs an MI355X / gfx950 GPU)");
+  }
+  int device() const { return dev_; }
+  // nullptr passes: a missing argument is found before
+  int operator()(const char* name, const void* p) const {
+    if (!p) return RLH_OK;
+    hipPointerAttribute_t a{};
+    if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+      (void)hipGetLastError();
+      return serve_error(RLH_EINVAL, std::string(name) + " is not device-accessible memory");
+    }
+    if (a.devicePointer == nullptr) return serve_error(RLH_EINVAL, std::string(name) + " is not device-accessible memory");
+    if (a.type == hipMemoryTypeDevice && a.device != dev_)
+      return serve_error(RLH_EINVAL, std::string(name) + " is memory of another device than the current one");
+    return RLH_OK;
+  }
+
+ private:
+  int dev_ = -1;
+};
+
+#define RLH_TRY(expr)            \
+  do {                           \
+    const int rc_ = (expr);      \
+    if (rc_ != RLH_OK) return rc_; \
+  } while (0)
+
+inline int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return RLH_OK;
+  return serve_error(RLH_EDEVICE, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+}  // namespace rlh

@@ -263,6 +263,55 @@ def sampling_params(temperature=0.7, top_k=40, top_p=0.95, repetition_penalty=1.
     return SamplingParams(temperature, top_k, top_p, repetition_penalty, repeat_last_n, seed)
 
 
+class KvPages(ctypes.Structure):
+    """rlh_kv_pages (include/rlh_serve.h): one layer's pool of key/value pages.
+    Pointers here and below are device addresses (e.g. a tensor's data_ptr())."""
+    _fields_ = [("type", ctypes.c_uint32), ("n_head_kv", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("n_pages", ctypes.c_uint64), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p)]
+
+
+class Seqs(ctypes.Structure):
+    """rlh_seqs: a ragged batch of sequences over the pages."""
+    _fields_ = [("n_seq", ctypes.c_uint32), ("n_rows", ctypes.c_uint32), ("max_q", ctypes.c_uint32),
+                ("max_kv", ctypes.c_uint32), ("table_stride", ctypes.c_uint32), ("q_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p)]
+
+
+class Rope(ctypes.Structure):
+    """rlh_rope: rotary frequencies and their scaling."""
+    _fields_ = [("rot_dim", ctypes.c_uint32), ("scaling", ctypes.c_uint32), ("theta", ctypes.c_double),
+                ("factor", ctypes.c_double), ("orig_ctx", ctypes.c_double), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double)]
+
+
+class AppendArgs(ctypes.Structure):
+    """rlh_append_args."""
+    _fields_ = [("in_type", ctypes.c_uint32), ("n_head", ctypes.c_uint32), ("q", ctypes.c_void_p),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_uint64),
+                ("k_stride", ctypes.c_uint64), ("v_stride", ctypes.c_uint64), ("q_norm", ctypes.c_void_p),
+                ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float), ("magnitude", ctypes.c_float),
+                ("freqs", ctypes.c_void_p), ("rot_dim", ctypes.c_uint32), ("interleaved", ctypes.c_uint32),
+                ("q_out", ctypes.c_void_p), ("q_out_stride", ctypes.c_uint64)]
+
+
+class AttnArgs(ctypes.Structure):
+    """rlh_attn_args."""
+    _fields_ = [("n_head", ctypes.c_uint32), ("window", ctypes.c_uint32), ("q", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p),
+                ("prefix_len", ctypes.c_void_p), ("shared_table", ctypes.c_void_p), ("shared_len", ctypes.c_uint32)]
+
+
+class RowSampling(ctypes.Structure):
+    """rlh_row_sampling: one row's options (in device memory, 16 bytes each)."""
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_uint32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
+
+
+SERVE_BAD_PAGE, SERVE_BAD_SEQ = 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS = 0, 1, 2
+
 _lib = None
 
 
@@ -368,6 +417,13 @@ def load():
         "rlh_synth_normal": (None, [U64, U64, U64, U64, F, F, P]),
         "rlh_synth_tensor": (I32, [U64, U64, U32, U64, U64, F, F, P, I32]),
         "rlh_synth_tokens": (None, [U64, U64, U32, P]),
+        "rlh_rope_freqs": (I32, [ctypes.POINTER(Rope), P, ctypes.POINTER(F)]),
+        "rlh_paged_append": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AppendArgs), P, P]),
+        "rlh_paged_attn_workspace": (U64, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs)]),
+        "rlh_paged_attn": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs), P, U64, P,
+                                 P]),
+        "rlh_sample_rows_workspace": (U64, [U64, U64]),
+        "rlh_sample_rows": (I32, [U32, P, U64, U64, U64, P, P, P, P, U64, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -452,6 +508,51 @@ def check(rc):
 
 def _p(a):
     return None if a is None else a.ctypes.data
+
+
+# ---- batched serving operators (include/rlh_serve.h) ------------------------------
+# Device addresses in, kernels enqueued on `stream` (a hipStream_t, None: the
+# null stream); nothing is allocated or waited for.
+
+def rope_freqs(rot_dim, theta, scaling=ROPE_PLAIN, factor=1.0, orig_ctx=0.0, beta_fast=32.0, beta_slow=1.0):
+    """(float64 frequencies in radians per position, magnitude)."""
+    r = Rope(rot_dim, scaling, theta, factor, orig_ctx, beta_fast, beta_slow)
+    f, m = np.empty(max(rot_dim // 2, 1), dtype=np.float64), ctypes.c_float()
+    check(load().rlh_rope_freqs(ctypes.byref(r), f.ctypes.data, ctypes.byref(m)))
+    return f, m.value
+
+
+def paged_append(kv, seqs, args, status=None, stream=None):
+    """Norms, position rotation and the append of k and v to their pages."""
+    rc = load().rlh_paged_append(kv, seqs, args, status, stream)
+    if rc:
+        check(rc)
+
+
+def paged_attn_workspace(kv, seqs, args):
+    """Workspace bytes of paged_attn for these arguments (0: none, or refused)."""
+    return load().rlh_paged_attn_workspace(kv, seqs, args)
+
+
+def paged_attn(kv, seqs, args, workspace=None, workspace_bytes=0, status=None, stream=None):
+    """Attention of a ragged batch over the pages."""
+    rc = load().rlh_paged_attn(kv, seqs, args, workspace, workspace_bytes, status, stream)
+    if rc:
+        check(rc)
+
+
+def sample_rows_workspace(n_rows, n):
+    """Workspace bytes of sample_rows."""
+    return load().rlh_sample_rows_workspace(n_rows, n)
+
+
+def sample_rows(logits_type, logits, n_rows, n, stride, options, u, tokens, workspace=None, workspace_bytes=0,
+                stream=None):
+    """One token per row of logits; options: n_rows RowSampling on the device."""
+    rc = load().rlh_sample_rows(logits_type, logits, n_rows, n, stride, options, u, tokens, workspace, workspace_bytes,
+                                stream)
+    if rc:
+        check(rc)
 
 
 class Model:
