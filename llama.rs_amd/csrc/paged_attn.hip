@@ -1,7 +1,11 @@
 // paged_attn.hip — attention of a ragged batch over the paged cache.
 #include <math.h>
 
+#include <algorithm>
+#include <atomic>
+
 #include "paged_device.h"
+#include "rlh_device.h"
 #include "serve_check.h"
 
 namespace rlh {
@@ -20,77 +24,903 @@ struct AttnParams {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kSmallRows = 16;    // rows of a KV head that the small kernel takes (the width of its MFMA)
+constexpr int kSmallTile = 128;   // positions that its four waves take per step
+constexpr int kTileRows = 128;    // rows of a tile of the tiled kernel
+constexpr int kTileKv = 64;       // positions of its steps
+// The maximum that probabilities are relative to is only moved when the
+// running maximum has grown by more than 8 (in units of log 2): until then
+// they stay below 2^8, which f16 holds as exactly as values below one.
+constexpr float kSlack = 8.0f;
 
-// Whole workgroup: the sequence that row `row` belongs to (n_seq: none).
-__device__ __forceinline__ uint32_t block_seq_of(const Batch& b, uint32_t row) {
-  uint32_t s = 0;
-  for (uint32_t i = 0; i < b.n_seq; i += blockDim.x) {
-    const uint32_t k = i + threadIdx.x;
-    s += (uint32_t)__syncthreads_count(k < b.n_seq && b.q_start[k + 1] <= row);
-  }
-  return s;
+#define RLH_CONST __attribute__((address_space(4)))
+#define RLH_LDS_PTR(T) __attribute__((address_space(3))) T
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+// A value every lane of the wave has.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint32_t load_uniform(const uint32_t* p, uint32_t i) {
+  return *((const RLH_CONST uint32_t*)p + uniform(i));
 }
 
-// One wave per (row, query head): 64 positions at a time.
-template <typename T, int D>
-__global__ void __launch_bounds__(64) k_attn_rows(AttnParams a) {
-  __shared__ float qs[D];
-  const uint32_t row = blockIdx.x, h = blockIdx.y, g = h / a.group;
-  const uint32_t s = block_seq_of(a.b, row);
-  if (s >= a.b.n_seq) return;
-  bool bad;
-  const SeqView sv = load_seq(a.b, s, &bad);
-  if (!sv.ok || row < sv.q0) {
-    if (threadIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
-    return;
+__device__ __forceinline__ float max_across_32(float x) {
+  const u32x2_t r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_across_16(float x) {
+  const u32x2_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_across_32(float x) {
+  const u32x2_t r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float sum_across_16(float x) {
+  const u32x2_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec4 = T __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4_t mfma16(vec8<_Float16> a, vec8<_Float16> b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mfma16(vec8<__bf16> a, vec8<__bf16> b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16_t mfma32(vec8<_Float16> a, vec8<_Float16> b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16_t mfma32(vec8<__bf16> a, vec8<__bf16> b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Columns of V as an MFMA operand: a group of 16 lanes names four rows of 16
+// values (lane t: row t / 4, values 4 (t % 4) .. + 3) and gets the transpose,
+// lane t the four rows' value t. Two of them make an operand's eight.
+template <typename T>
+__device__ __forceinline__ vec8<T> read_columns(const uint8_t RLH_LDS* a, const uint8_t RLH_LDS* b) {
+  const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RLH_LDS_PTR(s16x4_t)*)a);
+  const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((RLH_LDS_PTR(s16x4_t)*)b);
+  return __builtin_bit_cast(vec8<T>, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// Whether any of eight halves is infinite or NaN.
+template <typename T>
+__device__ __forceinline__ bool any_special(u32x4_t x) {
+  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) r |= (x[i] & e) == e || (x[i] >> 16 & e) == e;
+  return r;
+}
+
+// Element i (the same in every lane) of the vector that lane `src` holds.
+template <typename T>
+__device__ __forceinline__ float element(vec8<T> v, uint32_t i, int src) {
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+  const uint32_t x = i < 4 ? (i < 2 ? w[0] : w[1]) : (i < 6 ? w[2] : w[3]);
+  const uint32_t y = __shfl(x, src);
+  return (float)__builtin_bit_cast(T, (uint16_t)(i & 1 ? y >> 16 : y));
+}
+
+// Copies 16 bytes per lane to LDS from `dst` on (the same in every lane), in
+// lane order, without registers; counted by vmcnt. Written out so that the
+// compiler does not make every later read by columns wait for it: the step's
+// own wait and barrier order them. (m0 is reserved, which the compiler warns
+// of; named all the same, it orders this against the compiler's own uses.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Scores in units of log 2, from dots: s * scale, capped, biased.
+struct Scoring {
+  float mul;              // scale * log2(e), or with a cap 2 scale / cap * log2(e)
+  float cap2;             // softcap * log2(e)
+  bool capped, biased;
+};
+
+template <bool MOD>
+__device__ __forceinline__ float score(const Scoring& c, float dot, float slope2, int32_t away) {
+  float x = dot * c.mul;
+  if constexpr (MOD) {
+    // tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
+    if (c.capped) x = c.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f));
+    if (c.biased) x = fmaf(slope2, (float)away, x);
   }
-  const int lane = threadIdx.x;
-  const int32_t pos = (int32_t)(sv.kv_len - sv.q_len + (row - sv.q0));
-  const RowSpan span = row_span(pos, sv.kv_len, a.window, a.prefix_len ? a.prefix_len[s] : 0);
-  for (int d = lane; d < D; d += 64) qs[d] = (float)((const T*)a.q)[(size_t)row * a.q_stride + (size_t)h * D + d];
+  return x;
+}
+
+// What the partial results of one row look like: m, l and the D sums, by
+// source: prefix parts, then the parts of the sequence's own positions.
+struct Workspace {
+  float* prefix_o;   // [prefix_parts][n_rows * n_head][D]
+  float* prefix_ml;  // [prefix_parts][n_rows * n_head][2]
+  float* tile_o;     // [tile_parts][n_rows * n_head][D]
+  float* tile_ml;
+  float* item_o;     // [items * n_kv][16][D]
+  float* item_ml;    // [items * n_kv][16][2]
+  uint32_t* plan;    // [n_seq][2]: first item, items
+};
+
+struct Sizes {
+  uint32_t items;         // at most, of the small kernel (per KV head)
+  uint32_t item_goal;     // items that its work is divided into (and one more per sequence)
+  uint32_t tiles;         // at most, of the tiled kernel (per KV head)
+  uint32_t tile_parts;    // parts of the positions of a tile
+  uint32_t prefix_tiles;  // tiles over all rows
+  uint32_t prefix_parts;
+  bool small, tiled, merge;
+};
+
+struct Launch {
+  AttnParams a;
+  Scoring sc;
+  Workspace ws;
+  Sizes n;
+};
+
+struct SeqSpan {
+  SeqView v;
+  uint32_t rows;      // of a KV head: new rows times heads per KV head
+  int32_t p0;         // position of the first new row
+  int32_t begin, end; // positions that any of its rows sees (own ones: from shared_len)
+  uint32_t prefix;
+};
+
+__device__ __forceinline__ SeqSpan seq_span(const AttnParams& a, uint32_t s, bool* bad) {
+  SeqSpan r;
+  r.v = load_seq(a.b, s, bad);
+  r.rows = r.v.ok ? r.v.q_len * a.group : 0;
+  r.p0 = (int32_t)(r.v.kv_len - r.v.q_len);
+  r.prefix = a.prefix_len ? a.prefix_len[s] : 0;
+  r.begin = r.end = 0;
+  if (r.v.ok) {
+    const int32_t b = span_begin(row_span(r.p0, r.v.kv_len, a.window, r.prefix));
+    r.begin = (b > (int32_t)a.shared_len ? b : (int32_t)a.shared_len) & ~15;
+    r.end = span_end(row_span((int32_t)r.v.kv_len - 1, r.v.kv_len, a.window, r.prefix));
+  }
+  return r;
+}
+
+__device__ __forceinline__ uint32_t block_sum(uint32_t x, uint32_t* slots) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
   __syncthreads();
-  float m = -INFINITY, l = 0.0f, o[D / 64] = {};
-  for (int32_t j0 = span_begin(span); j0 < span_end(span); j0 += 64) {
-    const int32_t j = j0 + lane;
-    bool see = j < (int32_t)sv.kv_len && row_sees(span, j);
-    uint32_t page = 0;
-    if (see) {
-      page = j < (int32_t)a.shared_len ? a.shared_table[j >> a.page_shift]
-                                       : a.b.table[(size_t)s * a.b.table_stride + (j >> a.page_shift)];
-      if (page >= a.n_pages) {
-        raise(a.status, RLH_SERVE_BAD_PAGE);
-        see = false;
+  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return slots[0] + slots[1] + slots[2] + slots[3];
+}
+// Inclusive sum over the block's threads; *all receives the whole.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* slots, uint32_t* all) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const uint32_t o = __shfl_up(x, m);
+    if (lane >= (uint32_t)m) x += o;
+  }
+  __syncthreads();
+  if (lane == 63) slots[wave] = x;
+  __syncthreads();
+  uint32_t off = 0;
+  for (uint32_t i = 0; i < wave; i++) off += slots[i];
+  *all = slots[0] + slots[1] + slots[2] + slots[3];
+  return off + x;
+}
+
+// ---- few rows: single tokens and drafts -----------------------------------------
+// A block takes one KV head of one sequence (up to 16 rows) and a part of
+// its positions; each wave streams 32 positions at a time on its own: K
+// straight into MFMA operands (16x16x32: positions down, rows across), V
+// through the wave's LDS rows to be read by columns. Bound by HBM; the
+// positions are divided so that every part has the same length and the card
+// is filled once. Scores come out with a row per lane column, so the running
+// maximum and the sum are one register per lane, and the probabilities are
+// already the next product's operand if V's rows are taken in the order that
+// the lanes hold them: 4 (lane / 16) + i, and 16 more.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
+  constexpr int kStride = D * 2 + 32;    // bytes of a V row in LDS: 8 rows start in 8 different bank groups
+  constexpr int kSteps = D / 32;         // MFMAs of a score
+  constexpr int kLoads = D / 16;         // 1 KB loads of 32 V rows
+  constexpr int kLanes = D / 8;          // lanes of a row in them
+  constexpr int kOut = D / 16;
+  constexpr int kMergeStride = D + 4;
+  __shared__ __align__(16) uint8_t lds[kWaves * 32 * kStride > kWaves * 16 * kMergeStride * 4
+                                           ? kWaves * 32 * kStride : kWaves * 16 * kMergeStride * 4];
+  __shared__ float ml[kWaves][16][2];
+  __shared__ uint32_t slots[4];
+  __shared__ uint32_t mine[4];
+  const AttnParams& a = L.a;
+  const uint32_t t = threadIdx.x;
+  const uint32_t wave = uniform(t >> 6), lane = t & 63;
+  const uint32_t h = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
+  // the division of all sequences' positions, found by every block alike
+  uint32_t total = 0;
+  for (uint32_t s = t; s < a.b.n_seq; s += kThreads) {
+    bool bad;
+    const SeqSpan q = seq_span(a, s, &bad);
+    if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
+    if (q.rows && q.rows <= kSmallRows && q.end > q.begin) total += (uint32_t)(q.end - q.begin + kSmallTile - 1) / kSmallTile;
+  }
+  total = block_sum(total, slots);
+  const uint32_t per_item = (total + L.n.item_goal - 1) / L.n.item_goal;
+  uint32_t base = 0;
+  if (t == 0) mine[0] = 0xffffffffu;
+  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kThreads) {
+    const uint32_t s = s0 + t;
+    uint32_t n = 0, tiles = 0;
+    if (s < a.b.n_seq) {
+      bool bad;
+      const SeqSpan q = seq_span(a, s, &bad);
+      if (q.rows && q.rows <= kSmallRows) {
+        if (q.end > q.begin) tiles = (uint32_t)(q.end - q.begin + kSmallTile - 1) / kSmallTile;
+        n = tiles ? (tiles + per_item - 1) / per_item : 1;
       }
     }
-    const uint32_t slot = j & ((1u << a.page_shift) - 1);
-    const size_t at = see ? ((((size_t)page * a.n_kv + g) << a.page_shift) + slot) * D : 0;
-    float x = -INFINITY;
-    if (see) {
-      x = 0.0f;
-      for (int d = 0; d < D; d++) x = fmaf(qs[d], (float)((const T*)a.pool_k)[at + d], x);
-      x *= a.scale;
-      if (a.softcap > 0.0f) x = a.softcap * tanhf(x / a.softcap);
-      if (a.slopes) x = fmaf(a.slopes[h], (float)(j - pos), x);
+    uint32_t all;
+    const uint32_t upto = base + block_scan(n, slots, &all);
+    if (n && upto - n <= item && item < upto) {
+      mine[0] = s;
+      mine[1] = upto - n;
+      mine[2] = n;
+      mine[3] = tiles;
     }
-    float mx = x;
-    for (int w = 1; w < 64; w <<= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
-    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.0f : mn;
-    const float p = exp2f((x - base) * kLog2e), f = exp2f((m - base) * kLog2e);
-    float sum = p;
-    for (int w = 1; w < 64; w <<= 1) sum += __shfl_xor(sum, w);
-    l = l * f + sum;
-    m = mn;
-    for (int i = 0; i < D / 64; i++) o[i] *= f;
-    for (int k = 0; k < 64; k++) {
-      const float pk = __shfl(p, k);
-      if (!__shfl((int)see, k)) continue;
-      const size_t ak = (size_t)__shfl((unsigned long long)at, k);
-      for (int i = 0; i < D / 64; i++) o[i] = fmaf(pk, (float)((const T*)a.pool_v)[ak + i * 64 + lane], o[i]);
+    base += all;
+    __syncthreads();
+    if (base > item) break;
+  }
+  const uint32_t s = uniform(mine[0]);
+  if (s == 0xffffffffu) return;
+  const uint32_t first = uniform(mine[1]), n_items = uniform(mine[2]), tiles = uniform(mine[3]);
+  bool bad;
+  const SeqSpan sq = seq_span(a, s, &bad);
+  const uint32_t part = item - first, share = (tiles + n_items - 1) / n_items;
+  const int32_t from = sq.begin + (int32_t)(part * share * kSmallTile);
+  const int32_t to = min(sq.end, from + (int32_t)(share * kSmallTile));
+  if (t == 0 && part == 0 && h == 0) {
+    L.ws.plan[2 * s] = first;
+    L.ws.plan[2 * s + 1] = n_items;
+  }
+  // the lane's row
+  const uint32_t col = lane & 15, quad = lane >> 4;
+  const bool active = col < sq.rows;
+  const uint32_t qi = active ? col / a.group : 0, g = active ? col % a.group : 0;
+  const uint32_t row = sq.v.q0 + qi, head = h * a.group + g;
+  const int32_t pos = sq.p0 + (int32_t)qi;
+  const RowSpan span = row_span(pos, sq.v.kv_len, a.window, sq.prefix);
+  const RowSpan span0 = row_span(sq.p0, sq.v.kv_len, a.window, sq.prefix);
+  const RowSpan span1 = row_span((int32_t)sq.v.kv_len - 1, sq.v.kv_len, a.window, sq.prefix);
+  const float slope2 = MOD && L.sc.biased ? a.slopes[head] * kLog2e : 0.0f;
+  vec8<T> q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; i++) {
+    u32x4_t z = {0, 0, 0, 0};
+    if (active)
+      z = *(const u32x4_t*)((const T*)a.q + (size_t)row * a.q_stride + (size_t)head * D + i * 32 + quad * 8);
+    q[i] = __builtin_bit_cast(vec8<T>, z);
+  }
+  f32x4_t o[kOut];
+#pragma unroll
+  for (int i = 0; i < kOut; i++) o[i] = f32x4_t{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  uint8_t RLH_LDS* vrows = (uint8_t RLH_LDS*)lds + wave * 32 * kStride;
+  u32x4_t kr[2][kSteps], vr[kLoads];
+  const uint32_t* table = a.b.table + (size_t)s * a.b.table_stride;
+  const uint32_t page_mask = (1u << a.page_shift) - 1;
+  // whether the 16 positions at p hold any that a row sees
+  auto needed = [&](int32_t p) { return p < to && (p < span1.prefix || p + 16 > span0.lo); };
+  auto entry = [&](int32_t p) { return needed(p) ? load_uniform(table, (uint32_t)p >> a.page_shift) : 0u; };
+  uint32_t valid = 0;  // of the two groups in the registers
+  auto issue = [&](int32_t p, uint32_t e0, uint32_t e1) {
+    valid = 0;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int32_t pu = p + 16 * u;
+      uint32_t page = u ? e1 : e0;
+      bool ok = needed(pu);
+      if (ok && page >= a.n_pages) {
+        raise(lane == 0 ? a.status : nullptr, RLH_SERVE_BAD_PAGE);
+        ok = false;
+      }
+      if (!ok) page = 0;
+      valid |= ok ? 1u << u : 0u;
+      const size_t at = ((((size_t)page * a.n_kv + h) << a.page_shift) + (ok ? (uint32_t)pu & page_mask : 0)) * D;
+      const T* kp = (const T*)a.pool_k + at;
+      const T* vp = (const T*)a.pool_v + at;
+#pragma unroll
+      for (int i = 0; i < kSteps; i++)
+        kr[u][i] = *(const RLH_GLOBAL u32x4_t*)(kp + (col * D + i * 32 + quad * 8));
+#pragma unroll
+      for (int i = 0; i < kLoads / 2; i++)
+        vr[u * (kLoads / 2) + i] = *(const RLH_GLOBAL u32x4_t*)(vp + (i * 512 + lane * 8));
+    }
+  };
+  int32_t p = from + (int32_t)wave * 32;
+  if (p < to) {
+    issue(p, entry(p), entry(p + 16));
+    uint32_t e0 = entry(p + kSmallTile), e1 = entry(p + kSmallTile + 16);
+    for (; p < to; p += kSmallTile) {
+      const uint32_t ok = valid;
+      const bool full = ok == 3 && ((p >= span1.lo && p + 32 <= span0.hi) || p + 32 <= span0.prefix);
+      f32x4_t sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        sc[u] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) sc[u] = mfma16(__builtin_bit_cast(vec8<T>, kr[u][i]), q[i], sc[u]);
+      }
+      uint64_t special = 0;  // V rows with values that a zero would not silence
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+          const uint64_t b = __ballot(any_special<T>(vr[i]));
+#pragma unroll
+          for (int r = 0; r < 64 / kLanes; r++)
+            if (b >> (r * kLanes) & ((1ull << kLanes) - 1)) special |= 1ull << (i * (64 / kLanes) + r);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; i++)
+        *(RLH_LDS_PTR(u32x4_t)*)(vrows + (i * (64 / kLanes) + lane / kLanes) * kStride + (lane % kLanes) * 16) = vr[i];
+      if (p + kSmallTile < to) {
+        issue(p + kSmallTile, e0, e1);
+        e0 = entry(p + 2 * kSmallTile);
+        e1 = entry(p + 2 * kSmallTile + 16);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      float x[8];
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int32_t j = p + (i / 4) * 16 + (int32_t)quad * 4 + i % 4;
+        x[i] = score<MOD>(L.sc, sc[i / 4][i % 4], slope2, j - pos);
+        if (!full && !((ok >> (i / 4) & 1) && j < (int32_t)sq.v.kv_len && row_sees(span, j))) x[i] = -INFINITY;
+        top = fmaxf(top, x[i]);
+      }
+      top = max_across_16(max_across_32(top));
+      if (__ballot(top > m + kSlack)) {
+        const float mn = fmaxf(m, top);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < kOut; i++) o[i] *= f;
+        m = mn;
+      }
+      const float mb = m == -INFINITY ? 0.0f : m;
+      vec8<T> pr;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] - mb);
+        l += x[i];
+        pr[i] = (T)x[i];
+      }
+      while (special) {
+        // such a row is added to the rows that see it, one by one, and
+        // silenced for the product
+        const int32_t r = (int32_t)__builtin_ctzll(special);
+        special &= special - 1;
+        const int32_t j = p + r;
+        const bool see = (ok >> (r / 16) & 1) && j < (int32_t)sq.v.kv_len && row_sees(span, j);
+        const float pv = element<T>(pr, (uint32_t)(r / 16 * 4 + r % 4), (int)(col + 16 * (uint32_t)(r % 16 / 4)));
+#pragma unroll
+        for (int i = 0; i < kOut; i++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float v = (float)*(RLH_LDS_PTR(T)*)(vrows + r * kStride + (i * 16 + quad * 4 + e) * 2);
+            if (see) o[i][e] = fmaf(pv, v, o[i][e]);
+          }
+        if (lane < (uint32_t)kLanes) *(RLH_LDS_PTR(u32x4_t)*)(vrows + r * kStride + lane * 16) = u32x4_t{0, 0, 0, 0};
+      }
+      const uint8_t RLH_LDS* vc = vrows + (quad * 4 + col / 4) * kStride + col % 4 * 8;
+#pragma unroll
+      for (int i = 0; i < kOut; i++) o[i] = mfma16(read_columns<T>(vc + i * 32, vc + 16 * kStride + i * 32), pr, o[i]);
+    }
+  }
+  l = sum_across_16(sum_across_32(l));
+  // the four waves' results
+  __syncthreads();
+  float* ol = (float*)lds;
+#pragma unroll
+  for (int i = 0; i < kOut; i++) *(f32x4_t*)(ol + (wave * 16 + col) * kMergeStride + i * 16 + quad * 4) = o[i];
+  if (quad == 0) {
+    ml[wave][col][0] = m;
+    ml[wave][col][1] = l;
+  }
+  __syncthreads();
+  const uint32_t r = t / 16, c0 = (t % 16) * (D / 16);
+  if (r >= sq.rows) return;
+  float mm = -INFINITY, ls = 0.0f, acc[D / 16] = {};
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) mm = fmaxf(mm, ml[w][r][0]);
+  const float mb = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const float f = __builtin_amdgcn_exp2f(ml[w][r][0] - mb);
+    ls += ml[w][r][1] * f;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) acc[i] = fmaf(ol[(w * 16 + r) * kMergeStride + c0 + i], f, acc[i]);
+  }
+  if (n_items == 1 && a.shared_len == 0) {
+    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+    T* dst = (T*)a.out + (size_t)(sq.v.q0 + r / a.group) * a.out_stride + (size_t)(h * a.group + r % a.group) * D + c0;
+    typedef T VO __attribute__((ext_vector_type(D / 16)));
+    VO v;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) v[i] = (T)(acc[i] * inv);
+    *(VO*)dst = v;
+  } else {
+    const size_t at = ((size_t)item * a.n_kv + h) * kSmallRows + r;
+    float* dst = L.ws.item_o + at * D + c0;
+#pragma unroll
+    for (int i = 0; i < D / 16; i += 4) *(f32x4_t*)(dst + i) = f32x4_t{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+    if (c0 == 0) {
+      L.ws.item_ml[2 * at] = mm;
+      L.ws.item_ml[2 * at + 1] = ls;
+    }
+  }
+}
+
+// ---- many rows: prompts, and the shared prefix of the whole batch ------------------
+// A block takes 128 rows of one KV head (rows are tokens times heads per KV
+// head, so heads that share K and V share a tile) and walks 64 positions at
+// a time; K and V are copied into LDS by DMA, one step ahead, in 16-byte
+// pieces that are exchanged within a row so that the products' reads meet no
+// bank twice. Each wave has 32 rows: scores are K times Q^T (32x32x16:
+// positions down, rows across), so that a row is a lane column as above.
+template <int D>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
+  return D == 128 ? ((r & 3) << 2 | (r >> 2 & 3)) : ((r >> 1 & 1) << 2 | (r >> 2 & 3));
+}
+
+struct TileShared {
+  uint64_t special[2];  // positions of a step whose V row holds infinities or NaN
+  uint32_t slots[4];
+  int32_t range[4];
+  int32_t ranges[kWaves][8];
+};
+template <int D>
+constexpr uint32_t kTileLds = 4 * kTileKv * D * 2 + sizeof(TileShared);
+
+template <typename T, int D, bool MOD, bool PREFIX>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
+  constexpr int kRowB = D * 2;
+  constexpr int kBuf = kTileKv * kRowB;   // bytes of a K or V step
+  constexpr int kSteps = D / 16;
+  constexpr int kOut = D / 32;
+  constexpr int kLanes = D / 8;           // lanes of a row in a copy
+  constexpr int kCopies = 16 / (64 / kLanes);  // 1 KB copies of 16 rows
+  // K, V of two steps first: a copy's LDS address has 16 bits
+  extern __shared__ __align__(1024) uint8_t lds[];
+  TileShared& sh = *(TileShared*)(lds + 4 * kBuf);
+  uint32_t* slots = sh.slots;
+  int32_t* range = sh.range;
+  uint64_t* special = sh.special;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(RLH_LDS uint8_t*)lds;
+  const AttnParams& a = L.a;
+  const uint32_t t = threadIdx.x;
+  const uint32_t wave = uniform(t >> 6), lane = t & 63;
+  const uint32_t parts = PREFIX ? L.n.prefix_parts : L.n.tile_parts;
+  const uint32_t h = blockIdx.x % a.n_kv;
+  const uint32_t part = blockIdx.x / a.n_kv % parts;
+  const uint32_t tile = blockIdx.x / a.n_kv / parts;
+  // the tile's sequence (own positions), or all rows (the prefix)
+  uint32_t s = 0, row0 = 0, rows = 0, base = 0;
+  if constexpr (PREFIX) {
+    row0 = tile * kTileRows;
+    rows = a.b.n_rows * a.group;
+  } else {
+    if (t == 0) range[0] = -1;
+    for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kThreads) {
+      uint32_t n = 0, r = 0;
+      if (s0 + t < a.b.n_seq) {
+        bool bad;
+        const SeqView v = load_seq(a.b, s0 + t, &bad);
+        if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
+        r = v.ok ? v.q_len * a.group : 0;
+        if (r > kSmallRows) n = (r + kTileRows - 1) / kTileRows;
+      }
+      uint32_t all;
+      const uint32_t upto = base + block_scan(n, slots, &all);
+      if (n && upto - n <= tile && tile < upto) {
+        range[0] = (int32_t)(s0 + t);
+        range[1] = (int32_t)(upto - 1 - tile);  // the last rows, with the most positions, first
+        range[2] = (int32_t)r;
+      }
+      base += all;
+      __syncthreads();
+      if (base > tile && blockIdx.x != 0) break;
+    }
+    if (range[0] < 0) return;
+    s = uniform((uint32_t)range[0]);
+    row0 = uniform((uint32_t)range[1]) * kTileRows;
+    rows = uniform((uint32_t)range[2]);
+    __syncthreads();
+  }
+  // the lane's row
+  const uint32_t col = lane & 31, half = lane >> 5;
+  const uint32_t rr = row0 + wave * 32 + col;
+  bool active = rr < rows;
+  uint32_t row = rr / a.group, g = rr % a.group, sq = s;
+  if constexpr (PREFIX) {
+    uint32_t lo = 0, hi = a.b.n_seq;  // as many sequences end at or before the row as come before its own
+    while (lo < hi) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (active && a.b.q_start[mid + 1] <= row)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    sq = lo;
+    active = active && sq < a.b.n_seq;
+  }
+  SeqView sv{};
+  if (active) {
+    bool bad;
+    sv = load_seq(a.b, sq, &bad);
+    if constexpr (!PREFIX) row += sv.q0;
+    active = sv.ok && row >= sv.q0 && row < sv.q0 + sv.q_len;
+  }
+  const int32_t pos = (int32_t)(sv.kv_len - sv.q_len) + (int32_t)(row - sv.q0);
+  const uint32_t head = h * a.group + g;
+  const int32_t limit = PREFIX ? min((int32_t)a.shared_len, (int32_t)sv.kv_len) : (int32_t)sv.kv_len;
+  RowSpan span{0, 0, 0};
+  if (active) {
+    span = row_span(pos, sv.kv_len, a.window, a.prefix_len ? a.prefix_len[sq] : 0);
+    span.hi = min(span.hi, limit);
+    span.prefix = min(span.prefix, limit);
+  }
+  // positions that the wave's rows all see lie in [w_lo, w_hi) or below
+  // w_prefix; those that any sees in [b_lo, b_hi)
+  int32_t w_lo = active ? span.lo : 0, w_hi = active ? span.hi : 0x7fffffff, w_prefix = active ? span.prefix : 0x7fffffff;
+  int32_t b_lo = active ? max(span_begin(span), PREFIX ? 0 : (int32_t)a.shared_len) : 0x7fffffff;
+  int32_t b_hi = active ? span_end(span) : 0;
+  int32_t any_prefix = active ? span.prefix : 0, min_lo = active ? span.lo : 0x7fffffff;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    w_lo = max(w_lo, __shfl_xor(w_lo, d));
+    w_hi = min(w_hi, __shfl_xor(w_hi, d));
+    w_prefix = min(w_prefix, __shfl_xor(w_prefix, d));
+    b_lo = min(b_lo, __shfl_xor(b_lo, d));
+    b_hi = max(b_hi, __shfl_xor(b_hi, d));
+    any_prefix = max(any_prefix, __shfl_xor(any_prefix, d));
+    min_lo = min(min_lo, __shfl_xor(min_lo, d));
+  }
+  w_lo = (int32_t)uniform(w_lo);
+  w_hi = (int32_t)uniform(w_hi);
+  w_prefix = (int32_t)uniform(w_prefix);
+  const int32_t v_lo = (int32_t)uniform(b_lo), v_hi = (int32_t)uniform(b_hi);  // the wave's
+  if (lane == 0) {
+    int32_t* r = sh.ranges[wave];
+    r[0] = v_lo;
+    r[1] = v_hi;
+    r[2] = any_prefix;
+    r[3] = min_lo;
+    r[4] = w_lo;
+    r[5] = w_hi;
+    r[6] = w_prefix;
+  }
+  __syncthreads();
+  int32_t t_lo = 0x7fffffff, t_hi = 0, t_prefix = 0, t_min_lo = 0x7fffffff;  // the block's
+  int32_t c_lo = 0, c_hi = 0x7fffffff, c_prefix = 0x7fffffff;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const int32_t* r = sh.ranges[w];
+    t_lo = min(t_lo, r[0]);
+    t_hi = max(t_hi, r[1]);
+    t_prefix = max(t_prefix, r[2]);
+    t_min_lo = min(t_min_lo, r[3]);
+    c_lo = max(c_lo, r[4]);
+    c_hi = min(c_hi, r[5]);
+    c_prefix = min(c_prefix, r[6]);
+  }
+  c_lo = (int32_t)uniform(c_lo);
+  c_hi = (int32_t)uniform(c_hi);
+  c_prefix = (int32_t)uniform(c_prefix);
+  t_lo = (int32_t)uniform(t_lo & ~15);
+  t_hi = (int32_t)uniform(t_hi);
+  t_prefix = (int32_t)uniform(t_prefix);
+  t_min_lo = (int32_t)uniform(t_min_lo);
+  const uint32_t n_steps = t_hi > t_lo ? (uint32_t)(t_hi - t_lo + kTileKv - 1) / kTileKv : 0;
+  const uint32_t st0 = (uint32_t)((uint64_t)n_steps * part / parts), st1 = (uint32_t)((uint64_t)n_steps * (part + 1) / parts);
+
+  const float slope2 = MOD && L.sc.biased && active ? a.slopes[head] * kLog2e : 0.0f;
+  vec8<T> q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; i++) {
+    u32x4_t z = {0, 0, 0, 0};
+    if (active) z = *(const u32x4_t*)((const T*)a.q + (size_t)row * a.q_stride + (size_t)head * D + i * 16 + half * 8);
+    q[i] = __builtin_bit_cast(vec8<T>, z);
+  }
+  f32x16_t o[kOut];
+#pragma unroll
+  for (int i = 0; i < kOut; i++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  const uint32_t* table = PREFIX ? a.shared_table : a.b.table + (size_t)s * a.b.table_stride;
+  const uint32_t page_mask = (1u << a.page_shift) - 1;
+  auto needed = [&](int32_t p) { return p < t_hi && (p < t_prefix || p + 16 > t_min_lo); };
+  // the step's four groups of 16 positions whose page exists; the wave's own
+  // group is copied
+  auto copy = [&](int32_t p, uint32_t buf) -> uint32_t {
+    uint32_t ok = 0, page = 0, slot = 0;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int32_t pu = p + 16 * u;
+      if (!needed(pu)) continue;
+      const uint32_t e = load_uniform(table, (uint32_t)pu >> a.page_shift);
+      if (e >= a.n_pages) {
+        raise(t == 0 ? a.status : nullptr, RLH_SERVE_BAD_PAGE);
+        continue;
+      }
+      ok |= 1u << u;
+      if (u == (int)wave) {
+        page = e;
+        slot = (uint32_t)pu & page_mask;
+      }
+    }
+    const size_t at = ((((size_t)page * a.n_kv + h) << a.page_shift) + slot) * D;
+#pragma unroll
+    for (int i = 0; i < kCopies; i++) {
+      const uint32_t r = i * (64 / kLanes) + lane / kLanes;  // of the group's 16
+      const uint32_t c = (lane % kLanes) ^ swizzle<D>(r);
+      const uint32_t dst = lds0 + buf * 2 * kBuf + wave * 16 * kRowB + i * 1024;
+      copy_to_lds((const T*)a.pool_k + at + r * D + c * 8, dst);
+      copy_to_lds((const T*)a.pool_v + at + r * D + c * 8, dst + kBuf);
+    }
+    return ok;
+  };
+  uint32_t ok_next = 0;
+  if (st0 < st1) ok_next = copy(t_lo + (int32_t)st0 * kTileKv, 0);
+  for (uint32_t st = st0; st < st1; st++) {
+    const uint32_t buf = (st - st0) & 1;
+    const int32_t p = t_lo + (int32_t)st * kTileKv;
+    const uint32_t ok = ok_next;
+    if (t == 0) special[buf] = 0;  // last read two barriers ago
+    wait_vmcnt<0>();               // this wave's copies of the step have landed
+    lds_barrier();                 // ... everyone's; every wave is done with the other buffer
+    if (st + 1 < st1) ok_next = copy(p + kTileKv, buf ^ 1);
+    const uint8_t RLH_LDS* kb = (const uint8_t RLH_LDS*)lds + buf * 2 * kBuf;
+    uint8_t RLH_LDS* vb = (uint8_t RLH_LDS*)lds + buf * 2 * kBuf + kBuf;
+    const bool full = ok == 15 && ((p >= w_lo && p + kTileKv <= w_hi) || p + kTileKv <= w_prefix);
+    const bool none = p >= v_hi || p + kTileKv <= v_lo;
+    // values that a zero would not silence, in steps that not every row of
+    // the block sees whole
+    uint64_t odd = 0;
+    if (!(ok == 15 && ((p >= c_lo && p + kTileKv <= c_hi) || p + kTileKv <= c_prefix))) {
+#pragma unroll
+      for (int i = 0; i < kBuf / (kThreads * 16); i++) {
+        const uint32_t at = (i * kThreads + t) * 16;
+        if (any_special<T>(*(const RLH_LDS_PTR(u32x4_t)*)(vb + at)))
+          atomicOr((unsigned long long*)&special[buf], 1ull << (at / kRowB));
+      }
+      lds_barrier();
+      odd = special[buf];
+    }
+    f32x16_t sc[2];
+    float x[2][16];
+    vec8<T> pr[4];
+    if (!none) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) sc[u][e] = 0.0f;
+        const uint32_t r = u * 32 + col;
+        const uint8_t RLH_LDS* kp = kb + r * kRowB;
+        const uint32_t z = swizzle<D>(r);
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+          sc[u] = mfma32(__builtin_bit_cast(vec8<T>, *(const RLH_LDS_PTR(u32x4_t)*)(kp + ((2 * i + half) ^ z) * 16)), q[i], sc[u]);
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int32_t j = p + u * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4;
+          x[u][e] = score<MOD>(L.sc, sc[u][e], slope2, j - pos);
+          if (!full && !((ok >> (2 * u + e / 8) & 1) && row_sees(span, j) && (PREFIX || j >= (int32_t)a.shared_len))) x[u][e] = -INFINITY;
+          top = fmaxf(top, x[u][e]);
+        }
+      top = max_across_32(top);
+      if (__ballot(top > m + kSlack)) {
+        const float mn = fmaxf(m, top);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < kOut; i++) o[i] *= f;
+        m = mn;
+      }
+      const float mb = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          x[u][e] = __builtin_amdgcn_exp2f(x[u][e] - mb);
+          l += x[u][e];
+          pr[2 * u + e / 8][e % 8] = (T)x[u][e];
+        }
+    }
+    if (odd) {
+      if (!none) {
+        for (uint64_t left = odd; left; left &= left - 1) {
+          const int32_t r = (int32_t)__builtin_ctzll(left), j = p + r;
+          const bool see = active && (ok >> (r / 16) & 1) && row_sees(span, j) && (PREFIX || j >= (int32_t)a.shared_len);
+          float pv = 0.0f;
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++) {
+            const float c = element<T>(pr[ks], (uint32_t)(r % 16 / 8 * 4 + r % 4), (int)(col + 32 * (uint32_t)(r % 8 / 4)));
+            if (ks == r / 16) pv = c;
+          }
+#pragma unroll
+          for (int i = 0; i < kOut; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              const uint32_t d = i * 32 + (e / 4) * 8 + half * 4 + e % 4;
+              const float v = (float)*(const RLH_LDS_PTR(T)*)(vb + r * kRowB + ((d / 8) ^ swizzle<D>(r)) * 16 + d % 8 * 2);
+              if (see) o[i][e] = fmaf(pv, v, o[i][e]);
+            }
+        }
+      }
+      lds_barrier();
+      for (uint64_t left = odd; left; left &= left - 1) {
+        const uint32_t r = (uint32_t)__builtin_ctzll(left);
+        if (t < (uint32_t)kLanes) *(RLH_LDS_PTR(u32x4_t)*)(vb + r * kRowB + t * 16) = u32x4_t{0, 0, 0, 0};
+      }
+      lds_barrier();
+    }
+    if (!none) {
+      // V's rows 16 ks + 4 half + 0..3 and + 8, by columns 32 i + 16 (lane / 16 % 2) + 0..15
+      const uint32_t vr0 = half * 4 + lane % 16 / 4, vd = (lane >> 4 & 1) * 16 + lane % 4 * 4;
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) {
+        const uint32_t ra = ks * 16 + vr0, rb = ra + 8;
+#pragma unroll
+        for (int i = 0; i < kOut; i++) {
+          const uint32_t c = (i * 32 + vd) / 8, b = vd % 8 * 2;
+          o[i] = mfma32(read_columns<T>(vb + ra * kRowB + (c ^ swizzle<D>(ra)) * 16 + b,
+                                        vb + rb * kRowB + (c ^ swizzle<D>(rb)) * 16 + b),
+                        pr[ks], o[i]);
+        }
+      }
+    }
+  }
+  l = sum_across_32(l);
+  if (!active) return;
+  if (!PREFIX && parts == 1 && a.shared_len == 0) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* dst = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * D;
+#pragma unroll
+    for (int i = 0; i < kOut; i++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        vec4<T> v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = (T)(o[i][e + k] * inv);
+        *(vec4<T>*)(dst + i * 32 + (e / 4) * 8 + half * 4) = v;
+      }
+  } else {
+    const size_t at = ((size_t)part * a.b.n_rows + row) * a.n_head + head;
+    float* dst = (PREFIX ? L.ws.prefix_o : L.ws.tile_o) + at * D;
+    float* mlp = (PREFIX ? L.ws.prefix_ml : L.ws.tile_ml) + at * 2;
+#pragma unroll
+    for (int i = 0; i < kOut; i++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *(f32x4_t*)(dst + i * 32 + (e / 4) * 8 + half * 4) = f32x4_t{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+    if (half == 0) {
+      mlp[0] = m;
+      mlp[1] = l;
+    }
+  }
+}
+
+// ---- joining the parts of a row ------------------------------------------------------
+// A block takes 16 rows of one KV head of a sequence, 16 lanes to a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
+  constexpr int N = D / 16;
+  __shared__ uint32_t slots[4];
+  __shared__ uint32_t mine[2];
+  const AttnParams& a = L.a;
+  const uint32_t t = threadIdx.x;
+  const uint32_t h = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
+  uint32_t base = 0;
+  if (t == 0) mine[0] = 0xffffffffu;
+  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kThreads) {
+    uint32_t n = 0;
+    if (s0 + t < a.b.n_seq) {
+      bool bad;
+      const SeqView v = load_seq(a.b, s0 + t, &bad);
+      if (v.ok) n = (v.q_len * a.group + 15) / 16;
+    }
+    uint32_t all;
+    const uint32_t upto = base + block_scan(n, slots, &all);
+    if (n && upto - n <= tile && tile < upto) {
+      mine[0] = s0 + t;
+      mine[1] = tile - (upto - n);
+    }
+    base += all;
+    __syncthreads();
+    if (base > tile) break;
+  }
+  const uint32_t s = mine[0];
+  if (s == 0xffffffffu) return;
+  bool bad;
+  const SeqView sv = load_seq(a.b, s, &bad);
+  const uint32_t rows = sv.q_len * a.group;
+  const uint32_t r = mine[1] * 16 + t / 16, c0 = t % 16 * N;
+  if (r >= rows) return;
+  const uint32_t row = sv.q0 + r / a.group, head = h * a.group + r % a.group;
+  const bool small = rows <= kSmallRows;
+  const uint32_t n_prefix = a.shared_len ? L.n.prefix_parts : 0;
+  const uint32_t first = small ? L.ws.plan[2 * s] : 0;
+  const uint32_t n_own = small ? L.ws.plan[2 * s + 1] : L.n.tile_parts;
+  if (n_prefix == 0 && n_own == 1) return;  // written already
+  const size_t rh = (size_t)row * a.n_head + head, all = (size_t)a.b.n_rows * a.n_head;
+  auto place = [&](uint32_t i, const float** o, const float** ml) {
+    if (i < n_prefix) {
+      *o = L.ws.prefix_o + (i * all + rh) * D;
+      *ml = L.ws.prefix_ml + (i * all + rh) * 2;
+    } else if (small) {
+      const size_t at = ((size_t)(first + i - n_prefix) * a.n_kv + h) * kSmallRows + r;
+      *o = L.ws.item_o + at * D;
+      *ml = L.ws.item_ml + at * 2;
+    } else {
+      *o = L.ws.tile_o + ((i - n_prefix) * all + rh) * D;
+      *ml = L.ws.tile_ml + ((i - n_prefix) * all + rh) * 2;
+    }
+  };
+  const uint32_t n = n_prefix + n_own;
+  float m = -INFINITY, l = 0.0f, acc[N] = {};
+  for (uint32_t i = 0; i < n; i++) {
+    const float *o, *ml;
+    place(i, &o, &ml);
+    m = fmaxf(m, ml[0]);
+  }
+  const float mb = m == -INFINITY ? 0.0f : m;
+  for (uint32_t i = 0; i < n; i++) {
+    const float *o, *ml;
+    place(i, &o, &ml);
+    const float f = __builtin_amdgcn_exp2f(ml[0] - mb);
+    l = fmaf(ml[1], f, l);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      const f32x4_t v = *(const f32x4_t*)(o + c0 + k);
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[k + e] = fmaf(v[e], f, acc[k + e]);
     }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int i = 0; i < D / 64; i++)
-    ((T*)a.out)[(size_t)row * a.out_stride + (size_t)h * D + i * 64 + lane] = (T)(o[i] * inv);
+  typedef T VO __attribute__((ext_vector_type(N)));
+  VO v;
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = (T)(acc[i] * inv);
+  *(VO*)((T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + c0) = v;
+}
+
+constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into
+
+// Parts that the positions of `blocks` tiles are divided into: enough blocks
+// to fill the card twice, at least 256 positions each.
+uint32_t tile_parts(uint64_t blocks, uint64_t positions) {
+  if (blocks == 0 || blocks >= 512) return 1;
+  return (uint32_t)std::max<uint64_t>(1, std::min((512 + blocks - 1) / blocks, positions / 256));
 }
 
 int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
@@ -113,7 +943,99 @@ int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args
   return RLH_OK;
 }
 
-uint64_t attn_workspace(const rlh_kv_pages&, const rlh_seqs&, const rlh_attn_args&) { return 0; }
+// How the work of a call is divided, from sizes that the host knows.
+Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
+  Sizes n{};
+  const uint64_t group = args.n_head / kv.n_head_kv, rows = (uint64_t)q.n_rows * group;
+  const uint64_t own = q.max_kv > args.shared_len ? q.max_kv - args.shared_len : 0;
+  n.small = group <= kSmallRows;
+  n.tiled = q.max_q * group > kSmallRows;
+  if (n.small) {
+    n.item_goal = std::max(1u, kSmallBlocks / kv.n_head_kv);
+    n.items = q.n_seq + n.item_goal;
+  }
+  if (n.tiled) {
+    n.tiles = (uint32_t)(rows / kTileRows + std::min<uint64_t>(q.n_seq, rows / (kSmallRows + 1)));
+    n.tile_parts = tile_parts((uint64_t)n.tiles * kv.n_head_kv, own);
+  }
+  if (args.shared_len) {
+    n.prefix_tiles = (uint32_t)((rows + kTileRows - 1) / kTileRows);
+    n.prefix_parts = tile_parts((uint64_t)n.prefix_tiles * kv.n_head_kv, args.shared_len);
+  }
+  n.merge = args.shared_len || (n.small && own > kSmallTile) || n.tile_parts > 1;
+  return n;
+}
+
+// Places the workspace's parts from `base` on (null: counts only); bytes.
+uint64_t place_workspace(Workspace* w, uint8_t* base, const rlh_kv_pages& kv, const rlh_seqs& q,
+                         const rlh_attn_args& args, const Sizes& n) {
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    uint8_t* p = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  const uint64_t D = kv.head_dim, rows = (uint64_t)q.n_rows * args.n_head;
+  const uint64_t pr = args.shared_len ? n.prefix_parts * rows : 0;
+  const uint64_t tr = n.tiled && (n.tile_parts > 1 || args.shared_len) ? n.tile_parts * rows : 0;
+  const uint64_t ir = n.small && n.merge ? (uint64_t)n.items * kv.n_head_kv * kSmallRows : 0;
+  w->prefix_o = (float*)take(pr * D * 4);
+  w->prefix_ml = (float*)take(pr * 8);
+  w->tile_o = (float*)take(tr * D * 4);
+  w->tile_ml = (float*)take(tr * 8);
+  w->item_o = (float*)take(ir * D * 4);
+  w->item_ml = (float*)take(ir * 8);
+  w->plan = (uint32_t*)take(n.small ? (uint64_t)q.n_seq * 8 : 0);
+  return at;
+}
+
+uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
+  Workspace w;
+  return place_workspace(&w, nullptr, kv, q, args, attn_sizes(kv, q, args));
+}
+
+// The tiled kernels take more LDS than a launch may by default; said once per
+// device (idempotent, so two threads may).
+template <typename T, int D, bool MOD>
+int allow_tile_lds(int device) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return RLH_OK;
+  if (hipFuncSetAttribute((const void*)k_attn_tiles<T, D, MOD, true>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)kTileLds<D>) != hipSuccess ||
+      hipFuncSetAttribute((const void*)k_attn_tiles<T, D, MOD, false>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)kTileLds<D>) != hipSuccess) {
+    (void)hipGetLastError();
+    return serve_error(RLH_EDEVICE, "hipFuncSetAttribute (LDS of the tiled attention kernels)");
+  }
+  done.fetch_or(bit, std::memory_order_release);
+  return RLH_OK;
+}
+
+template <typename T, int D, bool MOD>
+int launch_attn(const Launch& L, int device, hipStream_t s) {
+  const uint32_t G = L.a.n_kv;
+  if (L.a.shared_len || L.n.tiled) RLH_TRY((allow_tile_lds<T, D, MOD>(device)));
+  if (L.a.shared_len)
+    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, true>), dim3(L.n.prefix_tiles * L.n.prefix_parts * G), dim3(kThreads),
+                       kTileLds<D>, s, L);
+  if (L.n.tiled)
+    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, false>), dim3(L.n.tiles * L.n.tile_parts * G), dim3(kThreads),
+                       kTileLds<D>, s, L);
+  if (L.n.small) hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), 0, s, L);
+  if (L.n.merge) {
+    const uint64_t rows = (uint64_t)L.a.b.n_rows * L.a.group;
+    const uint32_t tiles = (uint32_t)(rows / 16 + std::min<uint64_t>(L.a.b.n_seq, rows));
+    hipLaunchKernelGGL((k_attn_merge<T, D>), dim3(tiles * G), dim3(kThreads), 0, s, L);
+  }
+  return launched("rlh_paged_attn");
+}
+
+template <typename T>
+int launch_attn(const Launch& L, uint32_t dim, bool mod, int device, hipStream_t s) {
+  if (dim == 64) return mod ? launch_attn<T, 64, true>(L, device, s) : launch_attn<T, 64, false>(L, device, s);
+  return mod ? launch_attn<T, 128, true>(L, device, s) : launch_attn<T, 128, false>(L, device, s);
+}
 
 }  // namespace
 }  // namespace rlh
@@ -173,21 +1095,17 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   p.n_pages = (uint32_t)kv->n_pages;
   p.window = args->window;
   p.shared_len = args->shared_len;
-  const dim3 grid(seqs->n_rows, args->n_head);
-  hipStream_t s = (hipStream_t)stream;
-  const bool f16 = kv->type == RLH_TYPE_F16;
-  if (kv->head_dim == 64) {
-    if (f16)
-      hipLaunchKernelGGL((k_attn_rows<_Float16, 64>), grid, dim3(64), 0, s, p);
-    else
-      hipLaunchKernelGGL((k_attn_rows<__bf16, 64>), grid, dim3(64), 0, s, p);
-  } else {
-    if (f16)
-      hipLaunchKernelGGL((k_attn_rows<_Float16, 128>), grid, dim3(64), 0, s, p);
-    else
-      hipLaunchKernelGGL((k_attn_rows<__bf16, 128>), grid, dim3(64), 0, s, p);
-  }
-  return launched("rlh_paged_attn");
+  Launch L{};
+  L.a = p;
+  L.n = attn_sizes(*kv, *seqs, *args);
+  place_workspace(&L.ws, (uint8_t*)workspace, *kv, *seqs, *args, L.n);
+  L.sc.capped = args->softcap > 0.0f;
+  L.sc.biased = args->slopes != nullptr;
+  L.sc.mul = L.sc.capped ? 2.0f * args->scale / args->softcap * kLog2e : args->scale * kLog2e;
+  L.sc.cap2 = args->softcap * kLog2e;
+  const bool mod = L.sc.capped || L.sc.biased;
+  if (kv->type == RLH_TYPE_F16) return launch_attn<_Float16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
+  return launch_attn<__bf16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
 }
 
 }  // extern "C"
