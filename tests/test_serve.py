@@ -208,6 +208,7 @@ def test_sample_refuses():
                 dict(tokens=None), dict(tokens=A + 1)):
         assert call(**bad) == rlh.RLH_EINVAL, bad
     assert call(rows=1 << 23) == rlh.RLH_EUNSUP
+    assert call(rows=1 << 20, n=1 << 20, stride=1 << 20) == rlh.RLH_EUNSUP
     if rlh.sample_rows_workspace(2, 100):
         assert call(ws=None) == rlh.RLH_EINVAL
         assert call(size=rlh.sample_rows_workspace(2, 100) - 1) == rlh.RLH_EINVAL
