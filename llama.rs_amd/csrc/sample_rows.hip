@@ -11,27 +11,28 @@ namespace {
 // Two launches. The first reads the logits once: chunks of 4096 values, of
 // each its largest key, its mass relative to that, the largest key of every
 // 64 values, and, where a row's options may keep many tokens, a histogram of
-// counts and masses over eighths of a power of two. The second has a block
+// counts and masses over sixteenths of a power of two. The second has a block
 // per row and, as a rule, reads only the groups of 64 that can hold a token
 // next to the border of what is kept:
 //   top-k (small k): the k-th largest of the groups' maxima is at most the
 //     k-th largest value, so only groups that reach it are read
-//   else: the histogram names the bin that holds the border; its values are
-//     sorted, all above are kept
-// and then draws: over the list itself, or over the chunks' kept masses and
-// inside the one chunk that the draw falls into. A border bin (or list) of
-// more than kCand values takes a search over the whole row instead.
+//   else: the histogram names the bin that holds the border; only its values
+//     are looked at, all above are kept
+// A range of keys that holds the border is narrowed by histograms of 2048
+// bins until 64 values are left, which one wave sorts. The draw runs over the
+// list itself, or over the chunks' kept masses and inside the one chunk that
+// it falls into.
 constexpr int kMassBits = 42;  // masses in histograms: multiples of 2^-42 of a chunk's largest weight
 constexpr uint64_t kMaxRow = 1ull << 21;
 constexpr uint64_t kMaxRows = 1ull << 21;
 constexpr uint32_t kChunk = 4096;
 constexpr uint32_t kGroup = 64;
-constexpr uint32_t kBins = 384;        // 48 powers of two; the last one takes the rest
+constexpr uint32_t kBins = 640;        // 40 powers of two; the last one takes the rest
 constexpr int kScanThreads = 256;
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr uint32_t kCand = 2048;       // values sorted in LDS
-constexpr uint32_t kRadix = 2048;
+constexpr uint32_t kCand = 2048;       // values held in LDS
+constexpr uint32_t kFine = 2048;       // bins of a narrowing step
 constexpr uint32_t kListK = 1024;      // largest top-k that takes the groups' maxima
 
 // Ascending as the values are; NaN (either sign) and -infinity give 0.
@@ -45,13 +46,16 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // 2^y for y <= 0 (0 below 2^-1000, NaN and -infinity): Taylor's polynomial of
-// degree 11 of 2^f, |f| <= 1/2, off by less than 2^-47.
+// degree 9 of 2^f, |f| <= 1/2, off by less than 2^-37 (as the last place of
+// 10^11 of the mass, where two tokens' borders lie 10^-6 apart at best).
+// Rounding, scaling and conversion instructions of doubles run at a quarter
+// of the rate of sums and products, so y is rounded by adding 1.5 * 2^52,
+// whose low bits then are the exponent.
 __device__ __forceinline__ double exp2_neg(double y) {
-  const double n = rint(y);
-  const double f = (y - n) * 0.6931471805599453;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
+  const double big = 6755399441055744.0;
+  const double z = y + big;
+  const double f = (y - (z - big)) * 0.6931471805599453;
+  double p = 1.0 / 362880.0;
   p = fma(p, f, 1.0 / 40320.0);
   p = fma(p, f, 1.0 / 5040.0);
   p = fma(p, f, 1.0 / 720.0);
@@ -61,7 +65,8 @@ __device__ __forceinline__ double exp2_neg(double y) {
   p = fma(p, f, 0.5);
   p = fma(p, f, 1.0);
   p = fma(p, f, 1.0);
-  return y > -1000.0 ? ldexp(p, (int)n) : 0.0;
+  const uint64_t n = __builtin_bit_cast(uint64_t, z) << 52;  // (negative: the sum wraps as it should)
+  return y > -1000.0 ? __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + n) : 0.0;
 }
 
 // exp((x - top) / temperature) with `c` = log2(e) / temperature; 1 at the top
@@ -73,8 +78,8 @@ __device__ __forceinline__ double weight_of(uint32_t key, uint32_t top_key, doub
 __device__ __forceinline__ uint64_t mass_of(double w) { return (uint64_t)(w * (double)(1ull << kMassBits) + 0.5); }
 
 // Bin of a value below a row's or a chunk's largest (`base`: its edge
-// number): eighths of a power of two, from the top.
-__device__ __forceinline__ double edge_of(uint32_t key, double c) { return floor((double)value_of(key) * c * 8.0); }
+// number): sixteenths of a power of two, from the top.
+__device__ __forceinline__ double edge_of(uint32_t key, double c) { return floor((double)value_of(key) * c * 16.0); }
 __device__ __forceinline__ uint32_t bin_of(uint32_t key, uint32_t top_key, double base, double c) {
   if (key == top_key) return 0u;
   const double d = base - edge_of(key, c);
@@ -123,6 +128,9 @@ struct Space {
   }
 };
 
+constexpr uint32_t kCached = 2560;     // groups whose maxima are held in LDS
+constexpr uint32_t kMaxChunks = (uint32_t)(kMaxRow / kChunk) + 1;
+
 // A row's values are counted from the 16-byte line that its first one lies
 // in: value v of the lines is value v - shift of the row.
 template <typename T>
@@ -138,18 +146,24 @@ struct Row {
   __device__ __forceinline__ uint32_t key(uint32_t v) const {
     return v >= shift && v < shift + n ? key_of((float)x[v - shift]) : 0u;
   }
-  // the 16 / sizeof(T) keys from v on (v a multiple of that)
-  template <int V>
-  __device__ __forceinline__ void keys(uint32_t v, uint32_t (&k)[V]) const {
-    typedef T TV __attribute__((ext_vector_type(V)));
+  // the keys of the line at v (a multiple of V): its load, and what of it
+  // lies in the row
+  static constexpr int V = 16 / sizeof(T);
+  typedef T Line __attribute__((ext_vector_type(V)));
+  __device__ __forceinline__ Line line(uint32_t v) const {
+    Line a{};
     if (v >= shift && v + V <= shift + n) {
-      const TV a = *(const TV*)(x + ((size_t)v - shift));
-#pragma unroll
-      for (int i = 0; i < V; i++) k[i] = key_of((float)a[i]);
+      a = *(const Line*)(x + ((size_t)v - shift));
     } else {
 #pragma unroll
-      for (int i = 0; i < V; i++) k[i] = key(v + i);
+      for (int i = 0; i < V; i++)
+        if (v + i >= shift && v + i < shift + n) a[i] = x[v + i - shift];
     }
+    return a;
+  }
+  __device__ __forceinline__ void keys(uint32_t v, const Line& a, uint32_t (&k)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; i++) k[i] = v + i >= shift && v + i < shift + n ? key_of((float)a[i]) : 0u;
   }
 };
 
@@ -174,8 +188,11 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
     }
   }
   uint32_t k[N][V], top = 0;
+  typename Row<T>::Line line[N];
 #pragma unroll
-  for (int i = 0; i < N; i++) row.keys(chunk * kChunk + (i * kScanThreads + t) * V, k[i]);
+  for (int i = 0; i < N; i++) line[i] = row.line(chunk * kChunk + (i * kScanThreads + t) * V);
+#pragma unroll
+  for (int i = 0; i < N; i++) row.keys(chunk * kChunk + (i * kScanThreads + t) * V, line[i], k[i]);
 #pragma unroll
   for (int i = 0; i < N; i++) {
     uint32_t m = 0;
@@ -198,14 +215,19 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   const double tv = (double)value_of(top), base = edge_of(top, plan.c);
   double sum = 0.0;
   if (top != 0u) {
+    // an infinite top's own weight is 1, what lies below has none
+    const double tf = tv < INFINITY ? tv : 0x1p1000;
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const double w = weight_of(k[i][e], top, tv, plan.c);
+        const uint32_t ke = k[i][e];
+        // (key 0 is the value of a NaN)
+        double w = exp2_neg(((double)value_of(ke) - tf) * plan.c);
+        if (!(tv < INFINITY)) w = ke == top ? 1.0 : 0.0;
         sum += w;
-        if (plan.bins && k[i][e] != 0u) {
-          const uint32_t b = bin_of(k[i][e], top, base, plan.c);
+        if (plan.bins && ke != 0u) {
+          const uint32_t b = bin_of(ke, top, base, plan.c);
           atomicAdd(&count[b], 1u);
           atomicAdd((unsigned long long*)&bin[b], (unsigned long long)mass_of(w));
         }
@@ -223,138 +245,293 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
     }
 }
 
-// ---- block-wide sums and searches ---------------------------------------------------
-template <typename T>
-__device__ __forceinline__ T shfl_up_t(T v, int d) {
-  return __shfl_up(v, d);
+// ---- block-wide sums ------------------------------------------------------------------
+// The second kernel's code runs once per launch, from a cold instruction
+// cache: what is used often is called, not inlined (a row without filters
+// took 35 us with 47 KB of inlined code).
+
+// x moved between lanes by a DPP control; 0 where none comes.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp0(T x) {
+  constexpr int W = sizeof(T) / 4;
+  struct Words {
+    int w[W];
+  };
+  Words a = __builtin_bit_cast(Words, x);
+#pragma unroll
+  for (int i = 0; i < W; i++) a.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(T, a);
 }
-__device__ __forceinline__ uint64_t shfl_up_t(uint64_t v, int d) { return __shfl_up((unsigned long long)v, d); }
+template <typename T>
+__device__ __forceinline__ T lane_value(T x, int lane) {
+  constexpr int W = sizeof(T) / 4;
+  struct Words {
+    int w[W];
+  };
+  Words a = __builtin_bit_cast(Words, x);
+#pragma unroll
+  for (int i = 0; i < W; i++) a.w[i] = __builtin_amdgcn_readlane(a.w[i], lane);
+  return __builtin_bit_cast(T, a);
+}
+// Inclusive sum over the wave in lane order.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T x) {
+  x += dpp0<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += dpp0<0x112, 0xf>(x);
+  x += dpp0<0x114, 0xf>(x);
+  x += dpp0<0x118, 0xf>(x);
+  x += dpp0<0x142, 0xa>(x);  // row_bcast 15, 31
+  x += dpp0<0x143, 0xc>(x);
+  return x;
+}
 
 struct PickShared {
-  uint64_t sorted[kCand];     // (key, ~index), later sorted
-  uint32_t key[kCand];        // in index order
+  uint32_t key[kCand];        // gathered values, in index order
   uint32_t index[kCand];
   union {
-    uint32_t list[kCand];     // groups that are read
-    uint32_t hist[kRadix];
-    uint64_t mhist[kRadix];
+    struct {
+      uint32_t list[kCand];   // groups that are read
+      uint64_t bits[kCand];   // which of their values; later the values that are left
+    };
+    struct {
+      uint32_t count[kFine];
+      uint64_t mass[kFine];
+    } fine;
+    double kept[kMaxChunks];
   };
-  double slots[kWaves];
-  uint64_t slots64[kWaves];
-  uint32_t slots32[kWaves];
-  double bcast;
-  uint64_t bcast64;
+  uint32_t group[kCached];
+  double factor[kMaxChunks];  // of a chunk's weights; its largest key, its mass
+  double mass[kMaxChunks];
+  uint32_t top[kMaxChunks];
+  uint64_t slots[kWaves];
+  uint64_t before;
   uint32_t where[4];
 };
 
-// Inclusive sum of one value per thread in thread order; *all: the whole.
+// The largest key of group g.
+struct Groups {
+  const uint32_t* cached;
+  const uint32_t* all;
+  __device__ __forceinline__ uint32_t operator()(uint32_t g) const { return g < kCached ? cached[g] : all[g]; }
+};
+
+// Inclusive sum of one value per thread in thread order, and the whole.
 template <typename T>
-__device__ __forceinline__ T block_scan(T x, T* slots, T* all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T o = shfl_up_t(x, d);
-    if (lane >= d) x += o;
-  }
+struct Scan {
+  T upto, all;
+};
+template <typename T>
+__device__ __noinline__ Scan<T> block_scan(T x, PickShared* sh) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  x = wave_scan(x);
+  T* slots = (T*)sh->slots;
   __syncthreads();
   if (lane == 63) slots[wave] = x;
   __syncthreads();
-  T off = 0, sum = 0;
+  T v[kWaves], off = 0, sum = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) v[i] = slots[i];
 #pragma unroll
   for (int i = 0; i < kWaves; i++) {
-    if (i < wave) off += slots[i];
-    sum += slots[i];
+    off += i < wave ? v[i] : 0;
+    sum += v[i];
   }
-  *all = sum;
-  return off + x;
+  return Scan<T>{off + x, sum};
 }
 
-// The k-th largest of f(0..n-1) (k >= 1; 0 when fewer are above 0) by radix
-// descent, 11, 11 and 10 bits.
+__device__ __noinline__ double weight_called(uint32_t key, uint32_t top_key, double top, double c) {
+  return weight_of(key, top_key, top, c);
+}
+
+// The least key of [lo, hi] for which ok() holds (it does for hi, and for
+// all above one for which it does): the wave's lanes try 64 keys at a time.
 template <typename F>
-__device__ uint32_t kth_largest(PickShared& sh, uint32_t n, uint32_t k, F f) {
-  const uint32_t t = threadIdx.x;
-  uint32_t key = 0, above = 0;
-  for (int r = 0; r < 3; r++) {
-    const int shift = r == 0 ? 21 : r == 1 ? 10 : 0;
-    const uint32_t mask = r == 0 ? 0u : r == 1 ? 0xffe00000u : 0xfffffc00u;
-    __syncthreads();
-    for (uint32_t i = t; i < kRadix; i += kThreads) sh.hist[i] = 0;
-    if (t == 0) sh.where[0] = 0xffffffffu;
-    __syncthreads();
-    for (uint32_t i = t; i < n; i += kThreads) {
-      const uint32_t v = f(i);
-      if (v != 0u && ((v ^ key) & mask) == 0) atomicAdd(&sh.hist[(v >> shift) & (r == 2 ? 1023u : 2047u)], 1u);
+__device__ __forceinline__ uint32_t least_key(uint32_t lo, uint32_t hi, F ok) {
+  const uint32_t lane = threadIdx.x & 63;
+#pragma unroll 1
+  while (lo < hi) {
+    const uint32_t step = (hi - lo) / 64 + 1, off = lane * step;
+    const uint32_t k = off < hi - lo ? lo + off : hi;
+    const uint64_t yes = __ballot(ok(k));
+    if (!yes) {
+      lo = lane_value(k, 63) + 1;
+      continue;
     }
-    __syncthreads();
-    // two bins per thread, from the top
-    const uint32_t hi = kRadix - 1 - 2 * t, a = sh.hist[hi], b = sh.hist[hi - 1];
-    uint32_t all;
-    const uint32_t upto = above + block_scan<uint32_t>(a + b, sh.slots32, &all);
-    const uint32_t before = upto - a - b;
-    if (before < k && upto >= k) {
-      const bool first = before + a >= k;
-      sh.where[0] = first ? hi : hi - 1;
-      sh.where[1] = first ? before : before + a;
-    }
-    __syncthreads();
-    if (sh.where[0] == 0xffffffffu) return 0;
-    key |= sh.where[0] << shift;
-    above = sh.where[1];
+    const int f = __builtin_ctzll(yes);
+    hi = lane_value(k, f);
+    if (f > 0) lo = lane_value(k, f - 1) + 1;
   }
-  return key;
+  return lo;
+}
+
+// The border of what is kept: keys above `key`, and of equal ones indices up
+// to `index`.
+struct Border {
+  uint32_t key, index;
+};
+__device__ __forceinline__ bool kept(const Border& b, uint32_t key, uint32_t index) {
+  return key > b.key || (key == b.key && index <= b.index);
+}
+
+// What ends the kept tokens, and what is known of the keys above a range.
+struct Goal {
+  uint32_t k;        // values (2^32 - 1: no bound)
+  double p;          // mass (infinity: no bound)
+  uint32_t min_key;  // least key of min_p's weight
+  uint32_t top_key;
+  double top, c;
+};
+struct Range {
+  uint32_t lo, hi;   // holds the border
+  uint32_t above_k;  // values above hi, and their mass
+  double above_p;
+};
+
+// Narrows the range to one of its 2048 parts by the counts and masses of
+// get(0 .. n - 1); false if none of the three bounds ends within it.
+template <typename F>
+__device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goal, uint32_t n, F get) {
+  const uint32_t t = threadIdx.x, width = r.hi - r.lo;
+  const int shift = width < kFine ? 0 : 21 - __builtin_clz(width);
+  constexpr uint32_t kPer = kFine / kThreads;
+  __syncthreads();
+  for (uint32_t i = t; i < kFine; i += kThreads) {
+    sh.fine.count[i] = 0;
+    sh.fine.mass[i] = 0;
+  }
+  if (t == 0) sh.where[0] = 0xffffffffu;
+  __syncthreads();
+#pragma unroll 2
+  for (uint32_t i = t; i < n; i += kThreads) {
+    const uint32_t k = get(i);
+    if (k < r.lo || k > r.hi) continue;
+    const uint32_t b = (k - r.lo) >> shift;
+    atomicAdd(&sh.fine.count[b], 1u);
+    if (goal.p < INFINITY)
+      atomicAdd((unsigned long long*)&sh.fine.mass[b],
+                (unsigned long long)mass_of(weight_called(k, goal.top_key, goal.top, goal.c)));
+  }
+  __syncthreads();
+  // each thread's parts, from the top
+  uint32_t ck = 0;
+  uint64_t cp = 0;
+  for (uint32_t j = 0; j < kPer; j++) {
+    ck += sh.fine.count[kFine - 1 - t * kPer - j];
+    cp += sh.fine.mass[kFine - 1 - t * kPer - j];
+  }
+  uint32_t upto_k = block_scan<uint32_t>(ck, &sh).upto - ck;
+  uint64_t upto_p = goal.p < INFINITY ? block_scan<uint64_t>(cp, &sh).upto - cp : 0;
+  uint32_t mine = 0xffffffffu;
+  for (uint32_t j = 0; j < kPer; j++) {
+    const uint32_t b = kFine - 1 - t * kPer - j;
+    if (b > width >> shift) continue;
+    const uint64_t part = sh.fine.mass[b];
+    const uint32_t cnt = sh.fine.count[b];
+    if ((goal.k != 0xffffffffu && r.above_k + upto_k + cnt >= goal.k) ||
+        r.above_p + (double)(upto_p + part) * (1.0 / (double)(1ull << kMassBits)) >= goal.p ||
+        r.lo + (b << shift) < goal.min_key) {
+      mine = kFine - 1 - b;
+      break;
+    }
+    upto_k += cnt;
+    upto_p += part;
+  }
+  const uint64_t ends = __ballot(mine != 0xffffffffu);
+  if (ends && (int)(t & 63) == __builtin_ctzll(ends)) atomicMin(&sh.where[0], mine);
+  __syncthreads();
+  const uint32_t found = sh.where[0];
+  if (found == 0xffffffffu) return false;
+  const uint32_t b = kFine - 1 - found;
+  if (found == mine) {
+    sh.where[1] = upto_k;
+    sh.before = upto_p;
+  }
+  __syncthreads();
+  r.above_k += sh.where[1];
+  r.above_p += (double)sh.before * (1.0 / (double)(1ull << kMassBits));
+  r.lo += b << shift;
+  r.hi = r.lo + min(r.hi - r.lo, (1u << shift) - 1);
+  __syncthreads();
+  return true;
+}
+
+// How many of n equal values (key lo of a range that is one key) are kept.
+__device__ __forceinline__ uint32_t kept_equal(const Range& r, const Goal& goal, uint32_t n) {
+  uint32_t m = n;
+  if (goal.k != 0xffffffffu) m = min(m, goal.k > r.above_k ? goal.k - r.above_k : 0u);
+  if (goal.p < INFINITY) {
+    const double w = weight_called(r.lo, goal.top_key, goal.top, goal.c);
+    const double d = w > 0.0 ? ceil((goal.p - r.above_p) / w) : 0.0;
+    if (d < (double)m) m = d > 0.0 ? (uint32_t)d : 0u;
+  }
+  if (r.lo < goal.min_key) m = 0;
+  if (r.lo == goal.top_key) m = max(m, 1u);
+  return m;
 }
 
 // Every value with key in [lo, hi] into sh.key / sh.index, in index order;
 // false when there are more than kCand. Reads the groups that reach lo.
 template <typename T>
-__device__ bool gather(PickShared& sh, const Row<T>& row, const RowSpace& rs, uint32_t groups, uint32_t lo, uint32_t hi,
-                       uint32_t* count) {
+__device__ __forceinline__ bool gather(PickShared& sh, const Row<T>& row, const Groups& group, uint32_t groups,
+                                       uint32_t lo, uint32_t hi, uint32_t* count) {
   constexpr int V = 16 / sizeof(T);
   constexpr int kLanes = kGroup / V, kPer = 64 / kLanes;  // lanes of a group, groups of a wave
   const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
   uint32_t found = 0;
-  // in rounds of as many groups as the list holds
+  // rounds of neighbouring groups, eight per thread if the list holds those
+  // that reach lo, else four
+  uint32_t per = 2 * kCand / kThreads;
+#pragma unroll 1
   for (uint32_t g0 = 0; g0 < groups;) {
-    uint32_t listed = 0;
-    while (g0 < groups && listed + kThreads <= kCand) {
-      const uint32_t g = g0 + t;
-      const uint32_t yes = g < groups && rs.group[g] >= lo ? 1u : 0u;
-      uint32_t all;
-      const uint32_t at = listed + block_scan<uint32_t>(yes, sh.slots32, &all) - yes;
-      if (yes) sh.list[at] = g;
-      listed += all;
-      g0 += kThreads;
+    const uint32_t first = g0 + t * per;
+    uint32_t yes = 0;
+    for (uint32_t j = 0; j < per; j++) yes |= (first + j < groups && group(first + j) >= lo ? 1u : 0u) << j;
+    const Scan<uint32_t> places = block_scan<uint32_t>((uint32_t)__popc(yes), &sh);
+    uint32_t at = places.upto - (uint32_t)__popc(yes);
+    const uint32_t listed = places.all;
+    if (listed > kCand) {  // (not with four: those are kCand at most)
+      per = kCand / kThreads;
+      continue;
     }
+    for (; yes; yes &= yes - 1, at++) sh.list[at] = first + (uint32_t)__builtin_ctz(yes);
+    g0 += per * kThreads;
     __syncthreads();
-    // which values of each group: a bit per value
-    for (uint32_t i0 = wave * kPer; i0 < listed; i0 += kWaves * kPer) {
-      const uint32_t i = i0 + lane / kLanes;
-      uint64_t bits = 0;
-      if (i < listed) {
-        uint32_t k[V];
-        const uint32_t g = sh.list[i];
-        row.keys(g * kGroup + lane % kLanes * V, k);
+    // which values of each group: a bit per value; four groups' loads at a time
+    constexpr uint32_t kBatch = 4;
+#pragma unroll 1
+    for (uint32_t i0 = wave * kPer; i0 < listed; i0 += kBatch * kWaves * kPer) {
+      typename Row<T>::Line line[kBatch];
+      uint32_t v[kBatch];
 #pragma unroll
-        for (int e = 0; e < V; e++) bits |= (uint64_t)(k[e] >= lo && k[e] <= hi) << e;
-        bits <<= lane % kLanes * V;
+      for (uint32_t q = 0; q < kBatch; q++) {
+        const uint32_t i = i0 + q * kWaves * kPer + lane / kLanes;
+        v[q] = i < listed ? sh.list[i] * kGroup + lane % kLanes * V : 0u;
+        line[q] = row.line(v[q]);
       }
 #pragma unroll
-      for (int d = 1; d < kLanes; d <<= 1) bits |= __shfl_xor((unsigned long long)bits, d);
-      if (i < listed && lane % kLanes == 0) sh.sorted[i] = bits;
+      for (uint32_t q = 0; q < kBatch; q++) {
+        const uint32_t i = i0 + q * kWaves * kPer + lane / kLanes;
+        uint32_t k[V], b = 0;
+        row.keys(v[q], line[q], k);
+#pragma unroll
+        for (int e = 0; e < V; e++) b |= (k[e] >= lo && k[e] <= hi ? 1u : 0u) << e;
+        uint64_t bits = (uint64_t)b << (lane % kLanes * V);
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) bits |= __shfl_xor((unsigned long long)bits, d);
+        if (i < listed && lane % kLanes == 0) sh.bits[i] = bits;
+      }
     }
     __syncthreads();
-    // places of their values
-    for (uint32_t i0 = 0; i0 < listed; i0 += kThreads) {
-      const uint32_t i = i0 + t;
-      const uint64_t bits = i < listed ? sh.sorted[i] : 0;
-      uint32_t all;
-      uint32_t at = found + block_scan<uint32_t>((uint32_t)__popcll(bits), sh.slots32, &all) - (uint32_t)__popcll(bits);
-      const uint32_t g = i < listed ? sh.list[i] : 0;
-      for (uint64_t left = bits; left; left &= left - 1, at++)
-        if (at < kCand) sh.index[at] = g * kGroup + (uint32_t)__builtin_ctzll(left);
-      found += all;
-    }
+    // the places of their values: four neighbours per thread
+    uint32_t n = 0;
+    const uint32_t l0 = t * (kCand / kThreads);
+    for (uint32_t j = 0; j < kCand / kThreads; j++) n += l0 + j < listed ? (uint32_t)__popcll(sh.bits[l0 + j]) : 0u;
+    const Scan<uint32_t> values = block_scan<uint32_t>(n, &sh);
+    uint32_t to = found + values.upto - n;
+    for (uint32_t j = 0; j < kCand / kThreads && l0 + j < listed; j++)
+      for (uint64_t left = sh.bits[l0 + j]; left; left &= left - 1, to++)
+        if (to < kCand) sh.index[to] = sh.list[l0 + j] * kGroup + (uint32_t)__builtin_ctzll(left);
+    found += values.all;
     __syncthreads();
     if (found > kCand) return false;
   }
@@ -364,176 +541,103 @@ __device__ bool gather(PickShared& sh, const Row<T>& row, const RowSpace& rs, ui
   return true;
 }
 
-// sh.sorted = the gathered values, key descending and index ascending.
-__device__ void sort_gathered(PickShared& sh, uint32_t m) {
-  const uint32_t t = threadIdx.x;
-  uint32_t P = 2;
-  while (P < m) P <<= 1;
-  for (uint32_t i = t; i < P; i += kThreads)
-    sh.sorted[i] = i < m ? (uint64_t)sh.key[i] << 32 | (uint32_t)~sh.index[i] : 0ull;
-  __syncthreads();
-  if (P <= 64) {  // one wave, in registers
-    if (t < 64) {
-      uint64_t k = t < P ? sh.sorted[t] : 0ull;
-      for (uint32_t size = 2; size <= P; size <<= 1)
-        for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-          const uint64_t o = __shfl_xor((unsigned long long)k, (int)stride);
-          const bool larger = ((t & size) == 0) == ((t & stride) == 0);
-          k = (k > o) == larger ? k : o;
-        }
-      if (t < P) sh.sorted[t] = k;
-    }
-    __syncthreads();
-    return;
-  }
-  for (uint32_t size = 2; size <= P; size <<= 1)
-    for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-      for (uint32_t q = t; q < P / 2; q += kThreads) {
-        const uint32_t i = 2 * stride * (q / stride) + q % stride, j = i + stride;
-        const bool desc = (i & size) == 0;
-        const uint64_t a = sh.sorted[i], b = sh.sorted[j];
-        if ((a < b) == desc) {
-          sh.sorted[i] = b;
-          sh.sorted[j] = a;
-        }
-      }
-      __syncthreads();
-    }
-}
-
-// The border: kept are keys above `key` and, of equal ones, indices up to `index`.
-struct Border {
-  uint32_t key, index;
-};
-__device__ __forceinline__ bool kept(const Border& b, uint32_t key, uint32_t index) {
-  return key > b.key || (key == b.key && index <= b.index);
-}
-
-// The border within the sorted values: `k` more by count, mass up to goal_p
-// on top of `above`, weights of at least min_p; none of the three reached:
-// the last one. `force`: the first of them is the row's first, always kept.
-__device__ Border cut_sorted(PickShared& sh, uint32_t m, const RowPlan& plan, uint32_t k, double above, double goal_p,
-                             uint32_t top_key, bool force) {
-  const uint32_t t = threadIdx.x;
-  const double top = (double)value_of(top_key);
-  if (t == 0) sh.where[0] = m;  // values kept
-  __syncthreads();
-  double run = above;
-  for (uint32_t i0 = 0; i0 < m; i0 += kThreads) {
-    const uint32_t i = i0 + t;
-    const double w = i < m ? weight_of((uint32_t)(sh.sorted[i] >> 32), top_key, top, plan.c) : 0.0;
-    double all;
-    const double upto = run + block_scan<double>(w, sh.slots, &all);
-    // dropped: past k, reached before it, or too light
-    if (i < m && (i >= k || (plan.by_p && upto - w >= goal_p) || w < plan.min_p) && !(force && i == 0))
-      atomicMin(&sh.where[0], i);
-    run += all;
-    __syncthreads();
-  }
-  const uint32_t n = sh.where[0];
-  __syncthreads();
-  if (n == 0) return Border{0xffffffffu, 0u};
-  const uint64_t last = sh.sorted[n - 1];
-  return Border{(uint32_t)(last >> 32), ~(uint32_t)last};
-}
-
-// The border by a search over the whole row: radix descent on counts and on
-// masses (whole numbers, so their order does not matter) side by side.
+// The index of the nth (from 1) value that equals key.
 template <typename T>
-__device__ Border search_row(PickShared& sh, const Row<T>& row, const RowPlan& plan, uint32_t goal_k, double share_p,
-                             uint32_t top_key) {
-  const uint32_t t = threadIdx.x;
-  const double top = (double)value_of(top_key);
-  const uint32_t lines = row.lines();
-  Border border{1u, 0xffffffffu};
-  auto nth_equal = [&](uint32_t key, uint32_t nth) {  // index of the nth (from 1) value that equals key
-    uint32_t seen = 0;
-    for (uint32_t v0 = 0; v0 < lines; v0 += kThreads) {
-      const uint32_t v = v0 + t, yes = v < lines && row.key(v) == key ? 1u : 0u;
-      uint32_t all;
-      const uint32_t upto = seen + block_scan<uint32_t>(yes, sh.slots32, &all);
-      if (yes && upto == nth) sh.where[2] = v;
-      seen += all;
-      if (seen >= nth) break;
+__device__ __noinline__ uint32_t nth_equal(PickShared* sh, const Row<T> row, uint32_t key, uint32_t nth) {
+  uint32_t seen = 0;
+  for (uint32_t v0 = 0; v0 < row.lines() && seen < nth; v0 += kThreads) {
+    const uint32_t v = v0 + threadIdx.x, yes = v < row.lines() && row.key(v) == key ? 1u : 0u;
+    const Scan<uint32_t> c = block_scan<uint32_t>(yes, sh);
+    if (yes && seen + c.upto == nth) sh->where[2] = v;
+    seen += c.all;
+  }
+  __syncthreads();
+  const uint32_t v = sh->where[2];
+  __syncthreads();
+  return v;
+}
+
+// The border within a range: gathers it (after narrowing over the whole row
+// while it holds too many), narrows the gathered list, sorts what is left.
+// *gathered: values in sh.key / sh.index if they are the whole of the first
+// range, else 2^32 - 1.
+template <typename T>
+__device__ __noinline__ Border find_border(PickShared* shp, const Row<T> row, const Groups group, uint32_t groups,
+                                           Range r, const Goal& goal, uint32_t* gathered) {
+  PickShared& sh = *shp;
+  const uint32_t t = threadIdx.x, lane = t & 63;
+  uint32_t m = 0;
+  bool whole = true;
+#pragma unroll 1
+  while (!gather(sh, row, group, groups, r.lo, r.hi, &m)) {
+    whole = false;
+    if (r.lo == r.hi) {
+      // more equal values than the list holds
+      uint32_t part = 0;
+      for (uint32_t v = t; v < row.lines(); v += kThreads) part += row.key(v) == r.lo ? 1u : 0u;
+      const uint32_t n = kept_equal(r, goal, block_scan<uint32_t>(part, shp).all);
+      *gathered = 0xffffffffu;
+      return n ? Border{r.lo, nth_equal(shp, row, r.lo, n)} : Border{r.lo + 1, 0xffffffffu};
     }
-    __syncthreads();
-    return sh.where[2];
-  };
-  auto tighten = [&](uint32_t key, uint32_t index) {
-    if (key > border.key || (key == border.key && index < border.index)) border = Border{key, index};
-  };
-  if (plan.by_k) {
-    const uint32_t key = kth_largest(sh, lines, goal_k, [&](uint32_t v) { return row.key(v); });
-    if (key != 0u) {
-      uint32_t part = 0, above = 0;
-      for (uint32_t v = t; v < lines; v += kThreads) part += row.key(v) > key ? 1u : 0u;
-      block_scan<uint32_t>(part, sh.slots32, &above);
-      __syncthreads();
-      tighten(key, nth_equal(key, goal_k - above));
+    if (!narrow(sh, r, goal, row.lines(), [&](uint32_t v) { return row.key(v); })) {
+      *gathered = 0xffffffffu;
+      return Border{r.lo, 0xffffffffu};
     }
   }
-  if (plan.by_p) {
-    uint64_t part = 0, sum = 0;
-    for (uint32_t v = t; v < lines; v += kThreads) part += mass_of(weight_of(row.key(v), top_key, top, plan.c));
-    block_scan<uint64_t>(part, sh.slots64, &sum);
-    const double goal = share_p * (double)sum;
-    uint32_t key = 0;
-    uint64_t above = 0;
-    for (int r = 0; r < 3; r++) {
-      const int shift = r == 0 ? 21 : r == 1 ? 10 : 0;
-      const uint32_t mask = r == 0 ? 0u : r == 1 ? 0xffe00000u : 0xfffffc00u;
-      __syncthreads();
-      for (uint32_t i = t; i < kRadix; i += kThreads) sh.mhist[i] = 0;
-      if (t == 0) sh.where[0] = 0;
-      __syncthreads();
-      for (uint32_t v = t; v < lines; v += kThreads) {
-        const uint32_t k = row.key(v);
-        if (k != 0u && ((k ^ key) & mask) == 0)
-          atomicAdd((unsigned long long*)&sh.mhist[(k >> shift) & (r == 2 ? 1023u : 2047u)],
-                    (unsigned long long)mass_of(weight_of(k, top_key, top, plan.c)));
+  *gathered = whole ? m : 0xffffffffu;
+  if (m > 64) {
+    while (r.lo != r.hi) {
+      if (!narrow(sh, r, goal, m, [&](uint32_t i) { return sh.key[i]; })) return Border{r.lo, 0xffffffffu};
+      uint32_t in = 0;
+      for (uint32_t i = t; i < m; i += kThreads) in += sh.key[i] >= r.lo && sh.key[i] <= r.hi ? 1u : 0u;
+      if (block_scan<uint32_t>(in, shp).all <= 64) break;
+    }
+  }
+  // what is left, in index order: four neighbours per thread
+  uint32_t in = 0;
+  const uint32_t i0 = t * (kCand / kThreads);
+  for (uint32_t j = 0; j < kCand / kThreads; j++)
+    in |= (i0 + j < m && sh.key[i0 + j] >= r.lo && sh.key[i0 + j] <= r.hi ? 1u : 0u) << j;
+  const Scan<uint32_t> places = block_scan<uint32_t>((uint32_t)__popc(in), shp);
+  const uint32_t left = places.all;
+  uint32_t at = places.upto - (uint32_t)__popc(in);
+  for (; in; in &= in - 1, at++) {
+    const uint32_t i = i0 + (uint32_t)__builtin_ctz(in);
+    sh.bits[at] = (uint64_t)sh.key[i] << 32 | (uint32_t)~sh.index[i];
+  }
+  __syncthreads();
+  if (left > 64) {  // equal values
+    const uint32_t n = kept_equal(r, goal, left);
+    return n ? Border{r.lo, ~(uint32_t)sh.bits[n - 1]} : Border{r.lo + 1, 0xffffffffu};
+  }
+  if (t < 64) {
+    uint64_t k = lane < left ? sh.bits[lane] : 0ull;
+#pragma unroll 1
+    for (uint32_t size = 2; size <= 64; size <<= 1)
+#pragma unroll 1
+      for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
+        const uint64_t o = __shfl_xor((unsigned long long)k, (int)stride);
+        const bool larger = ((lane & size) == 0) == ((lane & stride) == 0);
+        k = (k > o) == larger ? k : o;
       }
-      __syncthreads();
-      const uint32_t hi = kRadix - 1 - 2 * t;
-      const uint64_t a = sh.mhist[hi], b = sh.mhist[hi - 1];
-      uint64_t all;
-      const uint64_t upto = above + block_scan<uint64_t>(a + b, sh.slots64, &all);
-      const uint64_t before = upto - a - b;
-      auto reached = [&](uint64_t v) { return v > 0 && (double)v >= goal; };
-      if (!reached(before) && reached(upto)) {
-        const bool first = reached(before + a);
-        sh.where[0] = first ? hi : hi - 1;
-        sh.bcast64 = first ? before : before + a;
-      }
-      __syncthreads();
-      key |= sh.where[0] << shift;
-      above = sh.bcast64;
+    const uint32_t key = (uint32_t)(k >> 32);
+    const double w = lane < left ? weight_called(key, goal.top_key, goal.top, goal.c) : 0.0;
+    const double before = r.above_p + (wave_scan(w) - w);
+    const bool keep = lane < left && ((goal.k == 0xffffffffu || r.above_k + lane < goal.k) && before < goal.p &&
+                                      key >= goal.min_key);
+    uint64_t dropped = __ballot(!keep);
+    if (left && r.above_k == 0 && lane_value((uint32_t)(k >> 32), 0) == goal.top_key) dropped &= ~1ull;  // the row's first
+    const uint32_t n = dropped ? (uint32_t)__builtin_ctzll(dropped) : 64u;
+    const uint64_t last = lane_value(k, n ? (int)n - 1 : 0);
+    if (t == 0) {
+      sh.where[0] = n ? (uint32_t)(last >> 32) : r.hi + 1;
+      sh.where[1] = n ? ~(uint32_t)last : 0xffffffffu;
     }
-    const uint64_t w = mass_of(weight_of(key, top_key, top, plan.c));
-    uint32_t nth = 1;
-    if (w > 0) {
-      const double d = (goal - (double)above) / (double)w;
-      nth = d > 1.0 ? (uint32_t)fmin(d, (double)kMaxRow) : 1u;
-      while (nth > 1 && (double)(above + (uint64_t)(nth - 1) * w) >= goal) nth--;
-      while ((double)(above + (uint64_t)nth * w) < goal && nth < row.n) nth++;
-    }
-    tighten(key, nth_equal(key, nth));
   }
-  if (plan.min_p > 0.0) {
-    // the lightest key that still has min_p (the first is kept whatever it has)
-    uint32_t lo = 1, hi = top_key;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (weight_of(mid, top_key, top, plan.c) >= plan.min_p)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
-    if (weight_of(top_key, top_key, top, plan.c) < plan.min_p)
-      tighten(top_key, nth_equal(top_key, 1));
-    else
-      tighten(lo, 0xffffffffu);
-  }
-  return border;
+  __syncthreads();
+  const Border b{sh.where[0], sh.where[1]};
+  __syncthreads();
+  return b;
 }
 
 template <typename T>
@@ -543,30 +647,43 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
   __shared__ PickShared sh;
   const uint32_t t = threadIdx.x, r = blockIdx.x, lane = t & 63, wave = t >> 6;
   const rlh_row_sampling o = options[r];
-  const RowPlan plan = row_plan(o, n);
+  const float u = us[r];
   const RowSpace rs = space.row(r);
   const Row<T> row(logits, stride, n, r);
   const uint32_t chunks = (row.lines() + kChunk - 1) / kChunk, groups = (row.lines() + kGroup - 1) / kGroup;
+  // what the first launch left, all loads at once: a chain of loads that wait
+  // for each other costs most of the time here
   uint32_t top_key = 0;
-  for (uint32_t i = t; i < chunks; i += kThreads) top_key = max(top_key, rs.top[i]);
+  uint32_t g[kCached / kThreads];
+#pragma unroll
+  for (uint32_t j = 0; j < kCached / kThreads; j++) g[j] = j * kThreads + t < groups ? rs.group[j * kThreads + t] : 0u;
+  for (uint32_t i = t; i < chunks; i += kThreads) {
+    const uint32_t k = rs.top[i];
+    sh.top[i] = k;
+    sh.mass[i] = rs.mass[i];  // (not written, and not used, where the plan asks for no masses)
+    top_key = max(top_key, k);
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < kCached / kThreads; j++) sh.group[j * kThreads + t] = g[j];
+  const Groups group{sh.group, rs.group};
+  const RowPlan plan = row_plan(o, n);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, d));
-  if (lane == 0) sh.slots32[wave] = top_key;
+  uint32_t* tops = (uint32_t*)sh.slots;
+  if (lane == 0) tops[wave] = top_key;
+  if (t == 0) sh.where[0] = 0xffffffffu;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; i++) top_key = max(top_key, sh.slots32[i]);
-  __syncthreads();
+  for (int i = 0; i < kWaves; i++) top_key = max(top_key, tops[i]);
   if (top_key == 0u) {
     if (t == 0) tokens[r] = 0;
     return;
   }
   if (plan.greedy) {
     // the first group that holds it, the first of its values
-    if (t == 0) sh.where[0] = 0xffffffffu;
-    __syncthreads();
-    for (uint32_t g = t; g < groups; g += kThreads)
-      if (rs.group[g] == top_key) {
-        atomicMin(&sh.where[0], g);
+    for (uint32_t i = t; i < groups; i += kThreads)
+      if (group(i) == top_key) {
+        atomicMin(&sh.where[0], i);
         break;
       }
     __syncthreads();
@@ -577,199 +694,228 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
     }
     return;
   }
-  const double top = (double)value_of(top_key);
+  const double top = (double)value_of(top_key), c = plan.c;
   // masses of chunks are relative to their own largest weight
-  auto chunk_factor = [&](uint32_t ch) { return weight_of(rs.top[ch], top_key, top, plan.c); };
-  double sum = 0.0;
+  Goal goal{plan.by_k ? o.top_k : 0xffffffffu, INFINITY, 0u, top_key, top, c};
   if (plan.mass) {
     double part = 0.0;
-    for (uint32_t i = t; i < chunks; i += kThreads) part += chunk_factor(i) * rs.mass[i];
-    block_scan<double>(part, sh.slots, &sum);
-    __syncthreads();
+    for (uint32_t i = t; i < chunks; i += kThreads) {
+      const double f = weight_called(sh.top[i], top_key, top, c);
+      sh.factor[i] = f;
+      part += f * sh.mass[i];
+    }
+    const double sum = block_scan<double>(part, &sh).all;
+    if (plan.by_p) goal.p = (double)o.top_p * sum;
   }
-  const double goal_p = (double)o.top_p * sum;
-  const float u = us[r];
+  if (plan.min_p > 0.0) {
+    const uint32_t lo = least_key(1, top_key, [&](uint32_t k) { return weight_called(k, top_key, top, c) >= plan.min_p; });
+    goal.min_key = plan.min_p > 1.0 ? top_key + 1 : lo;
+  }
   const double uu = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
+  const double base = edge_of(top_key, c);
 
   Border border{0u, 0xffffffffu};  // everything
-  uint32_t border_bin = kBins, gathered = 0;  // the bin that holds it, and its values in sh.key / sh.index
+  uint32_t border_bin = kBins, m = 0xffffffffu;
   if (plan.list) {
-    const uint32_t lo = max(kth_largest(sh, groups, o.top_k, [&](uint32_t g) { return rs.group[g]; }), 1u);
-    uint32_t m;
-    if (gather(sh, row, rs, groups, lo, 0xffffffffu, &m)) {
-      sort_gathered(sh, m);
-      border = cut_sorted(sh, m, plan, o.top_k, 0.0, goal_p, top_key, true);
-      // the draw over the list, which is in index order
-      double total = 0.0;
-      double w[kCand / kThreads];
+    // a key that at least k groups reach, to a 2048th of the maxima's span
+    uint32_t least = 0xffffffffu;
+    for (uint32_t i = t; i < groups; i += kThreads) least = min(least, group(i) ? group(i) : 0xffffffffu);
 #pragma unroll
-      for (uint32_t j = 0; j < kCand / kThreads; j++) {
-        const uint32_t i = t * (kCand / kThreads) + j;
-        w[j] = i < m && kept(border, sh.key[i], sh.index[i]) ? weight_of(sh.key[i], top_key, top, plan.c) : 0.0;
-        total += w[j];
-      }
-      double all;
-      double run = block_scan<double>(total, sh.slots, &all) - total;
-      const double goal = uu * all;
-      if (t == 0) sh.where[3] = 0xffffffffu;
-      __syncthreads();
+    for (int d = 1; d < 64; d <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d));
+    __syncthreads();
+    if (lane == 0) tops[wave] = least;
+    __syncthreads();
 #pragma unroll
-      for (uint32_t j = 0; j < kCand / kThreads; j++) {
-        run += w[j];
-        if (w[j] > 0.0 && run > goal) atomicMin(&sh.where[3], t * (kCand / kThreads) + j);
-      }
-      __syncthreads();
-      if (sh.where[3] == 0xffffffffu) {  // u at its upper end: the last one with mass
-        if (t == 0) sh.where[2] = 0;
-        __syncthreads();
-#pragma unroll
-        for (uint32_t j = 0; j < kCand / kThreads; j++)
-          if (w[j] > 0.0) atomicMax(&sh.where[2], t * (kCand / kThreads) + j);
-        __syncthreads();
-        if (t == 0) tokens[r] = sh.index[sh.where[2]] - row.shift;
-        return;
-      }
-      if (t == 0) tokens[r] = sh.index[sh.where[3]] - row.shift;
-      return;
-    }
-    border = search_row(sh, row, plan, o.top_k, (double)o.top_p, top_key);
+    for (int i = 0; i < kWaves; i++) least = min(least, tops[i]);
+    Range range{least, top_key, 0u, 0.0};
+    const Goal by_count{o.top_k, INFINITY, 0u, top_key, top, c};
+    const bool enough = narrow(sh, range, by_count, groups, [&](uint32_t i) { return group(i); });
+    range = Range{enough ? range.lo : 1u, 0xffffffffu, 0u, 0.0};
+    border = find_border(&sh, row, group, groups, range, goal, &m);
   } else if (plan.bins) {
     // the row's histogram, one bin per thread, chunk after chunk
-    const double base = edge_of(top_key, plan.c);
-    uint32_t cnt = 0;
-    double mass = 0.0;
-    if (t < kBins) {
-      for (uint32_t ch = 0; ch < chunks; ch++) {
-        const uint32_t ck = rs.top[ch];
-        if (ck == 0u) continue;
-        const uint32_t off = bin_of(ck, top_key, base, plan.c);
-        if (t < off) continue;
-        if (t < kBins - 1) {
-          cnt += rs.count[(uint64_t)ch * kBins + t - off];
-          mass += chunk_factor(ch) * (double)rs.bin[(uint64_t)ch * kBins + t - off];
-        }
-      }
-    }
-    mass *= 1.0 / (double)(1ull << kMassBits);
-    uint32_t all32;
-    double alld;
-    const uint32_t upto_k = block_scan<uint32_t>(cnt, sh.slots32, &all32);
-    const double upto_p = block_scan<double>(mass, sh.slots, &alld);
+    for (uint32_t i = t; i < chunks; i += kThreads) sh.list[i] = sh.top[i] ? bin_of(sh.top[i], top_key, base, c) : kBins;
     if (t == 0) sh.where[0] = kBins - 1;
     __syncthreads();
-    // the first bin at which one of the three ends
-    uint32_t min_bin = kBins;
-    if (plan.min_p > 0.0) {
-      // (NaN: an infinite top, whose bin holds all that have mass)
-      const double d = base - floor((top * plan.c + log2(fmin(plan.min_p, 1.0))) * 8.0);
-      min_bin = d >= (double)(kBins - 1) ? kBins : d > 0.0 ? (uint32_t)d : 0u;
-    }
-    if (t < kBins - 1 &&
-        ((plan.by_k && upto_k >= o.top_k) || (plan.by_p && upto_p >= goal_p) || t >= min_bin))
-      atomicMin(&sh.where[0], t);
-    __syncthreads();
-    const uint32_t bin = sh.where[0];
-    __syncthreads();
-    if (t == bin) {
-      sh.where[1] = upto_k - cnt;
-      sh.bcast = upto_p - mass;
-    }
-    __syncthreads();
-    const uint32_t above_k = sh.where[1];
-    const double above_p = sh.bcast;
-    if (bin < kBins - 1) {
-      // the bin's keys: bins fall as keys rise
-      auto first_key = [&](uint32_t b) {  // the least key of bin b or above
-        uint32_t lo = 1, hi = top_key;
-        while (lo < hi) {
-          const uint32_t mid = lo + (hi - lo) / 2;
-          if (bin_of(mid, top_key, base, plan.c) <= b)
-            hi = mid;
-          else
-            lo = mid + 1;
-        }
-        return lo;
-      };
-      if (t < 2) sh.where[2 + t] = t == 0 ? first_key(bin) : bin == 0 ? top_key + 1 : first_key(bin - 1);
-      __syncthreads();
-      const uint32_t lo = sh.where[2], hi = sh.where[3] - 1;
-      uint32_t m;
-      if (gather(sh, row, rs, groups, lo, hi, &m)) {
-        sort_gathered(sh, m);
-        border = cut_sorted(sh, m, plan, plan.by_k ? o.top_k - above_k : 0xffffffffu, above_p, goal_p, top_key, bin == 0);
-        if (border.key == 0xffffffffu) border = Border{hi + 1, 0xffffffffu};  // the bins above, and nothing of this one
-        border_bin = bin;
-        gathered = m;
-      } else {
-        border = search_row(sh, row, plan, o.top_k, (double)o.top_p, top_key);
-      }
-    }
-  }
-  // the draw over the chunks' kept masses, then within one chunk
-  const double base = edge_of(top_key, plan.c);
-  auto chunk_kept = [&](uint32_t ch) {  // a whole wave; every lane gets the sum
-    double s = 0.0;
-    if (border_bin < kBins) {  // the bins above the border's, and what is kept of that one
-      const uint32_t off = bin_of(rs.top[ch], top_key, base, plan.c);
-      for (uint32_t i = lane; off + i < border_bin; i += 64) s += (double)rs.bin[(uint64_t)ch * kBins + i];
-      s *= chunk_factor(ch) * (1.0 / (double)(1ull << kMassBits));
-      for (uint32_t i = lane; i < gathered; i += 64)
-        if (sh.index[i] / kChunk == ch && kept(border, sh.key[i], sh.index[i])) s += weight_of(sh.key[i], top_key, top, plan.c);
-    } else {
-      for (uint32_t i = lane; i < kChunk; i += 64) {
-        const uint32_t v = ch * kChunk + i, k = row.key(v);
-        if (k != 0u && kept(border, k, v)) s += weight_of(k, top_key, top, plan.c);
-      }
-    }
+    constexpr uint32_t kEach = (kBins + kThreads - 1) / kThreads;  // neighbouring bins
+    uint32_t cnt[kEach] = {};
+    double mass[kEach] = {};
+#pragma unroll 4
+    for (uint32_t ch = 0; ch < chunks; ch++) {
+      const uint32_t off = sh.list[ch];
+      const double f = sh.factor[ch] * (1.0 / (double)(1ull << kMassBits));
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    return s;
-  };
-  __syncthreads();
-  double* kept_mass = (double*)sh.sorted;  // [chunks], at most 513
-  for (uint32_t ch = wave; ch < chunks; ch += kWaves) {
-    const bool some = rs.top[ch] != 0u && rs.top[ch] >= border.key;
-    const double s = !some ? 0.0 : border.key == 0u ? chunk_factor(ch) * rs.mass[ch] : chunk_kept(ch);
-    if (lane == 0) kept_mass[ch] = s;
+      for (uint32_t j = 0; j < kEach; j++) {
+        // (bin 0 is read and not used where the chunk has none)
+        const uint32_t b = t * kEach + j;
+        const bool in = b >= off && b < kBins - 1;
+        const uint64_t at = (uint64_t)ch * kBins + (in ? b - off : 0u);
+        const uint32_t n1 = rs.count[at];
+        const double m1 = (double)rs.bin[at];
+        cnt[j] += in ? n1 : 0u;
+        mass[j] += in ? f * m1 : 0.0;
+      }
+    }
+    uint32_t sum_k = 0;
+    double sum_p = 0.0;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; j++) {
+      sum_k += cnt[j];
+      sum_p += mass[j];
+    }
+    uint32_t upto_k = block_scan<uint32_t>(sum_k, &sh).upto - sum_k;
+    double upto_p = block_scan<double>(sum_p, &sh).upto - sum_p;
+    // the first bin at which one of the three ends
+    const uint32_t min_bin = goal.min_key == 0u ? kBins : bin_of(min(goal.min_key, top_key), top_key, base, c);
+    const uint32_t before_k = upto_k;
+    const double before_p = upto_p;
+    uint32_t mine = kBins;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; j++) {
+      const uint32_t b = t * kEach + j;
+      upto_k += cnt[j];
+      upto_p += mass[j];
+      if (mine == kBins && b < kBins - 1 && ((plan.by_k && upto_k >= o.top_k) || (plan.by_p && upto_p >= goal.p) || b >= min_bin)) mine = b;
+    }
+    const uint64_t ends = __ballot(mine < kBins);
+    if (ends && (int)lane == __builtin_ctzll(ends)) atomicMin(&sh.where[0], mine);
+    __syncthreads();
+    border_bin = sh.where[0];
+    __syncthreads();
+    if (border_bin < kBins - 1) {
+      if (border_bin / kEach == t) {
+        uint32_t k = before_k;
+        double p = before_p;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++)
+          if (t * kEach + j < border_bin) {
+            k += cnt[j];
+            p += mass[j];
+          }
+        sh.where[1] = k;
+        sh.before = __builtin_bit_cast(uint64_t, p);
+      }
+      // the bin's keys: bins fall as keys rise
+      auto from_bin = [&](uint32_t b) { return least_key(1, top_key, [&](uint32_t k) { return bin_of(k, top_key, base, c) <= b; }); };
+      const uint32_t lo = from_bin(border_bin), hi = border_bin == 0 ? top_key : from_bin(border_bin - 1) - 1;
+      __syncthreads();
+      const Range range{lo, hi, sh.where[1], __builtin_bit_cast(double, sh.before)};
+      border = find_border(&sh, row, group, groups, range, goal, &m);
+    } else {
+      border_bin = kBins;
+    }
   }
   __syncthreads();
-  double total = 0.0;
-  const double mine = t < chunks ? kept_mass[t] : 0.0;
-  const double upto = block_scan<double>(mine, sh.slots, &total);
-  const double goal = uu * total;
+  uint32_t per = 0, ch = 0;  // neighbours per thread of the list; or the draw's chunk
+  double before = 0.0, draw = 0.0;
+  const bool from_list = plan.list && m != 0xffffffffu;
+  if (from_list) {
+    per = (m + kThreads - 1) / kThreads;
+  } else {
+    // the draw over the chunks' kept masses
+    if (border.key == 0u) {
+      for (uint32_t q = t; q < chunks; q += kThreads) sh.kept[q] = sh.top[q] ? sh.factor[q] * sh.mass[q] : 0.0;
+    } else {
+#pragma unroll 1
+      for (uint32_t q = wave; q < chunks; q += kWaves) {
+        const uint32_t ck = sh.top[q];
+        double s = 0.0;
+        if (ck != 0u && ck >= border.key) {
+          if (border_bin < kBins && m != 0xffffffffu) {
+            // the bins above the border's, and what is kept of that one
+            const uint32_t off = bin_of(ck, top_key, base, c);
+#pragma unroll
+            for (uint32_t j = 0; j < kBins / 64; j++) {
+              const uint32_t i = j * 64 + lane;
+              const double x = (double)rs.bin[(uint64_t)q * kBins + i];
+              s += off + i < border_bin ? x : 0.0;
+            }
+            s *= sh.factor[q] * (1.0 / (double)(1ull << kMassBits));
+            for (uint32_t i = lane; i < m; i += 64)
+              if (sh.index[i] / kChunk == q && kept(border, sh.key[i], sh.index[i])) s += weight_called(sh.key[i], top_key, top, c);
+          } else {
+#pragma unroll 4
+            for (uint32_t i = lane; i < kChunk; i += 64) {
+              const uint32_t v = q * kChunk + i, k = row.key(v);
+              if (k != 0u && kept(border, k, v)) s += weight_of(k, top_key, top, c);
+            }
+          }
+        }
+        s = wave_scan(s);
+        if (lane == 63) sh.kept[q] = s;
+      }
+    }
+    if (t == 0) {
+      sh.where[0] = 0xffffffffu;
+      sh.where[1] = 0;
+    }
+    __syncthreads();
+    // two chunks per thread (there are at most 513)
+    const double a = 2 * t < chunks ? sh.kept[2 * t] : 0.0, b = 2 * t + 1 < chunks ? sh.kept[2 * t + 1] : 0.0;
+    const Scan<double> sums = block_scan<double>(a + b, &sh);
+    const double at = sums.upto - (a + b);
+    draw = uu * sums.all;
+    if (a > 0.0) {
+      if (at + a > draw) atomicMin(&sh.where[0], 2 * t);
+      atomicMax(&sh.where[1], 2 * t);
+    }
+    if (b > 0.0) {
+      if (at + a + b > draw) atomicMin(&sh.where[0], 2 * t + 1);
+      atomicMax(&sh.where[1], 2 * t + 1);
+    }
+    __syncthreads();
+    ch = sh.where[0] != 0xffffffffu ? sh.where[0] : sh.where[1];
+    if (ch / 2 == t) sh.before = __builtin_bit_cast(uint64_t, ch % 2 ? at + a : at);
+    __syncthreads();
+    before = __builtin_bit_cast(double, sh.before);
+  }
   if (t == 0) {
-    sh.where[0] = 0xffffffffu;
-    sh.where[1] = 0;
     sh.where[2] = 0xffffffffu;
     sh.where[3] = 0;
   }
-  __syncthreads();
-  if (mine > 0.0) {
-    if (upto > goal) atomicMin(&sh.where[0], t);
-    atomicMax(&sh.where[1], t);
+  // the draw over neighbouring values per thread, so that sums in thread order
+  // are in index order
+  constexpr uint32_t kPer = kChunk / kThreads, V = Row<T>::V;
+  double w[kPer], s = 0.0;
+  uint32_t at[kPer], k[kPer];
+  if (from_list) {
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; j++) {
+      const uint32_t i = t * per + j;
+      const bool in = j < per && i < m;
+      at[j] = in ? sh.index[i] : 0u;
+      k[j] = in ? sh.key[i] : 0u;
+    }
+  } else {
+    typename Row<T>::Line line[kPer / V];
+#pragma unroll
+    for (uint32_t j = 0; j < kPer / V; j++) line[j] = row.line(ch * kChunk + t * kPer + j * V);
+#pragma unroll
+    for (uint32_t j = 0; j < kPer / V; j++) row.keys(ch * kChunk + t * kPer + j * V, line[j], *(uint32_t(*)[V])(k + j * V));
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; j++) at[j] = ch * kChunk + t * kPer + j;
   }
-  __syncthreads();
-  const uint32_t ch = sh.where[0] != 0xffffffffu ? sh.where[0] : sh.where[1];
-  if (t == ch) sh.bcast = upto - mine;
-  // consecutive values per thread, so that sums in thread order are in index order
-  constexpr uint32_t kPer = kChunk / kThreads;
-  double w[kPer], s = 0.0, all;
 #pragma unroll
   for (uint32_t j = 0; j < kPer; j++) {
-    const uint32_t v = ch * kChunk + t * kPer + j, k = row.key(v);
-    w[j] = k != 0u && kept(border, k, v) ? weight_of(k, top_key, top, plan.c) : 0.0;
+    w[j] = k[j] != 0u && kept(border, k[j], at[j]) ? weight_called(k[j], top_key, top, c) : 0.0;
     s += w[j];
   }
-  double run = block_scan<double>(s, sh.slots, &all) - s + sh.bcast;
+  const Scan<double> sums = block_scan<double>(s, &sh);
+  double run = sums.upto - s + before;
+  if (from_list) draw = uu * sums.all;
+  uint32_t hit = 0xffffffffu, last = 0xffffffffu;
 #pragma unroll
   for (uint32_t j = 0; j < kPer; j++) {
     run += w[j];
-    const uint32_t v = ch * kChunk + t * kPer + j;
-    if (w[j] > 0.0 && run > goal) atomicMin(&sh.where[2], v);
-    if (w[j] >= 0x1p-43) atomicMax(&sh.where[3], v);
+    if (hit == 0xffffffffu && w[j] > 0.0 && run > draw) hit = at[j];
+    if (w[j] >= 0x1p-43) last = at[j];
   }
+  // one lane of a wave speaks for it: the sums rise and the indices with them
+  const uint64_t hits = __ballot(hit != 0xffffffffu), lasts = __ballot(last != 0xffffffffu);
+  if (hits && (int)lane == __builtin_ctzll(hits)) atomicMin(&sh.where[2], hit);
+  if (lasts && (int)lane == 63 - __builtin_clzll(lasts)) atomicMax(&sh.where[3], last);
   __syncthreads();
-  // (none past the goal: u at its upper end, or sums that differ in their last bits)
+  // (none past the draw: u at its upper end, or sums that differ in their last bits)
   if (t == 0) tokens[r] = (sh.where[2] != 0xffffffffu ? sh.where[2] : sh.where[3]) - row.shift;
 }
 
