@@ -60,8 +60,8 @@ typedef struct rlh_kv_pages {
  * and rows behind the last sequence are left as they were. max_q and max_kv
  * bound the new rows and kv_len of every sequence (max_kv <= table_stride *
  * page_size < 2^30): work is divided by them, so near bounds are faster.
- * n_seq < 2^16, n_rows <= 2^23, n_rows * n_head <= 2^27 and n_seq * n_head_kv
- * <= 2^22 (RLH_EUNSUP beyond). */
+ * n_seq < 2^16, n_rows <= 2^23, n_rows * n_head <= 2^25 and n_seq * n_head_kv
+ * <= 2^21 (RLH_EUNSUP beyond). */
 typedef struct rlh_seqs {
   uint32_t n_seq, n_rows, max_q, max_kv, table_stride;
   const uint32_t* q_start;

@@ -27,8 +27,8 @@ int check_batch(const rlh_kv_pages* kv, const rlh_seqs* seqs, uint32_t n_head) {
   if (seqs->n_seq > 65535) return serve_error(RLH_EUNSUP, "more than 65535 sequences");
   if (seqs->n_rows > 0x800000u) return serve_error(RLH_EUNSUP, "more than 2^23 rows");
   // launches hold fewer than 2^24 blocks
-  if ((uint64_t)seqs->n_rows * n_head > (1ull << 27)) return serve_error(RLH_EUNSUP, "n_rows * n_head above 2^27");
-  if ((uint64_t)seqs->n_seq * kv->n_head_kv > (1ull << 22)) return serve_error(RLH_EUNSUP, "n_seq * n_head_kv above 2^22");
+  if ((uint64_t)seqs->n_rows * n_head > (1ull << 25)) return serve_error(RLH_EUNSUP, "n_rows * n_head above 2^25");
+  if ((uint64_t)seqs->n_seq * kv->n_head_kv > (1ull << 21)) return serve_error(RLH_EUNSUP, "n_seq * n_head_kv above 2^21");
   if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;  // nothing to do
   if (!seqs->q_start || !seqs->kv_len || !seqs->table) return serve_error(RLH_EINVAL, "a batch array is null");
   if (!aligned(seqs->q_start, 4) || !aligned(seqs->kv_len, 4) || !aligned(seqs->table, 4))

@@ -162,7 +162,10 @@ struct Sizes {
   uint32_t tile_parts;    // parts of the positions of a tile
   uint32_t prefix_tiles;  // tiles over all rows
   uint32_t prefix_parts;
+  uint32_t small_rows;    // sequences of up to so many rows of a KV head go to the small kernel
   bool small, tiled, merge;
+  bool merge_small;       // only its sequences have parts to join
+  uint32_t merge_rows;    // then: blocks per sequence and KV head
 };
 
 struct Launch {
@@ -195,29 +198,49 @@ __device__ __forceinline__ SeqSpan seq_span(const AttnParams& a, uint32_t s, boo
   return r;
 }
 
-__device__ __forceinline__ uint32_t block_sum(uint32_t x, uint32_t* slots) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return slots[0] + slots[1] + slots[2] + slots[3];
+// x moved between lanes by a DPP control; 0 where none comes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-// Inclusive sum over the block's threads; *all receives the whole.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* slots, uint32_t* all) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t o = __shfl_up(x, m);
-    if (lane >= (uint32_t)m) x += o;
+// Inclusive sum over the wave in lane order.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += dpp0<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += dpp0<0x112, 0xf>(x);
+  x += dpp0<0x114, 0xf>(x);
+  x += dpp0<0x118, 0xf>(x);
+  x += dpp0<0x142, 0xa>(x);  // row_bcast 15, 31
+  x += dpp0<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t x, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+// Finds item `item` of a list in which sequence s has parts(s) items, one
+// after the other: every wave for itself, 64 sequences at a time (no
+// barriers). False if the list ends before it.
+struct Found {
+  uint32_t s, first, n;  // the sequence, its first item, its items
+};
+template <typename F>
+__device__ __forceinline__ bool find_item(uint32_t n_seq, uint32_t item, F parts, Found* f) {
+  uint32_t base = 0;
+  for (uint32_t s0 = 0; s0 < n_seq; s0 += 64) {
+    const uint32_t s = s0 + (threadIdx.x & 63);
+    const uint32_t n = s < n_seq ? parts(s) : 0;
+    const uint32_t upto = base + wave_scan(n);
+    const uint64_t hit = __ballot(upto > item);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      f->s = s0 + (uint32_t)l;
+      f->n = lane_value(n, l);
+      f->first = lane_value(upto, l) - f->n;
+      return true;
+    }
+    base = lane_value(upto, 63);
   }
-  __syncthreads();
-  if (lane == 63) slots[wave] = x;
-  __syncthreads();
-  uint32_t off = 0;
-  for (uint32_t i = 0; i < wave; i++) off += slots[i];
-  *all = slots[0] + slots[1] + slots[2] + slots[3];
-  return off + x;
+  return false;
 }
 
 // ---- few rows: single tokens and drafts -----------------------------------------
@@ -241,52 +264,46 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
   __shared__ __align__(16) uint8_t lds[kWaves * 32 * kStride > kWaves * 16 * kMergeStride * 4
                                            ? kWaves * 32 * kStride : kWaves * 16 * kMergeStride * 4];
   __shared__ float ml[kWaves][16][2];
-  __shared__ uint32_t slots[4];
-  __shared__ uint32_t mine[4];
   const AttnParams& a = L.a;
   const uint32_t t = threadIdx.x;
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
   const uint32_t h = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
-  // the division of all sequences' positions, found by every block alike
-  uint32_t total = 0;
-  for (uint32_t s = t; s < a.b.n_seq; s += kThreads) {
-    bool bad;
-    const SeqSpan q = seq_span(a, s, &bad);
-    if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
-    if (q.rows && q.rows <= kSmallRows && q.end > q.begin) total += (uint32_t)(q.end - q.begin + kSmallTile - 1) / kSmallTile;
-  }
-  total = block_sum(total, slots);
-  const uint32_t per_item = (total + L.n.item_goal - 1) / L.n.item_goal;
-  uint32_t base = 0;
-  if (t == 0) mine[0] = 0xffffffffu;
-  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kThreads) {
-    const uint32_t s = s0 + t;
-    uint32_t n = 0, tiles = 0;
+  // the division of all sequences' positions, found by every wave alike
+  auto tiles_of = [&](uint32_t s, bool* bad, bool* mine) -> uint32_t {
+    const SeqSpan q = seq_span(a, s, bad);
+    *mine = q.rows != 0 && q.rows <= kSmallRows;
+    return *mine && q.end > q.begin ? (uint32_t)(q.end - q.begin + kSmallTile - 1) / kSmallTile : 0;
+  };
+  uint32_t total = 0, tiles0 = 0;  // (tiles0: of the first 64 sequences, which are not looked at twice)
+  bool mine0 = false;
+  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64) {
+    const uint32_t s = s0 + lane;
+    uint32_t n = 0;
     if (s < a.b.n_seq) {
-      bool bad;
-      const SeqSpan q = seq_span(a, s, &bad);
-      if (q.rows && q.rows <= kSmallRows) {
-        if (q.end > q.begin) tiles = (uint32_t)(q.end - q.begin + kSmallTile - 1) / kSmallTile;
-        n = tiles ? (tiles + per_item - 1) / per_item : 1;
+      bool bad, mine;
+      n = tiles_of(s, &bad, &mine);
+      if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
+      if (s0 == 0) {
+        tiles0 = n;
+        mine0 = mine;
       }
     }
-    uint32_t all;
-    const uint32_t upto = base + block_scan(n, slots, &all);
-    if (n && upto - n <= item && item < upto) {
-      mine[0] = s;
-      mine[1] = upto - n;
-      mine[2] = n;
-      mine[3] = tiles;
-    }
-    base += all;
-    __syncthreads();
-    if (base > item) break;
+    total += n;
   }
-  const uint32_t s = uniform(mine[0]);
-  if (s == 0xffffffffu) return;
-  const uint32_t first = uniform(mine[1]), n_items = uniform(mine[2]), tiles = uniform(mine[3]);
+  total = lane_value(wave_scan(total), 63);
+  const uint32_t per_item = (total + L.n.item_goal - 1) / L.n.item_goal;
+  Found f;
+  if (!find_item(a.b.n_seq, item, [&](uint32_t s) {
+        uint32_t n = tiles0;
+        bool bad, mine = mine0;
+        if (s >= 64) n = tiles_of(s, &bad, &mine);
+        return n ? (n + per_item - 1) / per_item : mine ? 1u : 0u;
+      }, &f))
+    return;
+  const uint32_t s = f.s, first = f.first, n_items = f.n;
   bool bad;
   const SeqSpan sq = seq_span(a, s, &bad);
+  const uint32_t tiles = sq.end > sq.begin ? (uint32_t)(sq.end - sq.begin + kSmallTile - 1) / kSmallTile : 0;
   const uint32_t part = item - first, share = (tiles + n_items - 1) / n_items;
   const int32_t from = sq.begin + (int32_t)(part * share * kSmallTile);
   const int32_t to = min(sq.end, from + (int32_t)(share * kSmallTile));
@@ -488,8 +505,6 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
 
 struct TileShared {
   uint64_t special[2];  // positions of a step whose V row holds infinities or NaN
-  uint32_t slots[4];
-  int32_t range[4];
   int32_t ranges[kWaves][8];
 };
 template <int D>
@@ -506,8 +521,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
   // K, V of two steps first: a copy's LDS address has 16 bits
   extern __shared__ __align__(1024) uint8_t lds[];
   TileShared& sh = *(TileShared*)(lds + 4 * kBuf);
-  uint32_t* slots = sh.slots;
-  int32_t* range = sh.range;
   uint64_t* special = sh.special;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(RLH_LDS uint8_t*)lds;
   const AttnParams& a = L.a;
@@ -518,37 +531,29 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
   const uint32_t part = blockIdx.x / a.n_kv % parts;
   const uint32_t tile = blockIdx.x / a.n_kv / parts;
   // the tile's sequence (own positions), or all rows (the prefix)
-  uint32_t s = 0, row0 = 0, rows = 0, base = 0;
+  uint32_t s = 0, row0 = 0, rows = 0;
   if constexpr (PREFIX) {
     row0 = tile * kTileRows;
     rows = a.b.n_rows * a.group;
   } else {
-    if (t == 0) range[0] = -1;
-    for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kThreads) {
-      uint32_t n = 0, r = 0;
-      if (s0 + t < a.b.n_seq) {
+    if (blockIdx.x == 0)
+      for (uint32_t i = t; i < a.b.n_seq; i += kThreads) {
         bool bad;
-        const SeqView v = load_seq(a.b, s0 + t, &bad);
-        if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
-        r = v.ok ? v.q_len * a.group : 0;
-        if (r > kSmallRows) n = (r + kTileRows - 1) / kTileRows;
+        load_seq(a.b, i, &bad);
+        if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
       }
-      uint32_t all;
-      const uint32_t upto = base + block_scan(n, slots, &all);
-      if (n && upto - n <= tile && tile < upto) {
-        range[0] = (int32_t)(s0 + t);
-        range[1] = (int32_t)(upto - 1 - tile);  // the last rows, with the most positions, first
-        range[2] = (int32_t)r;
-      }
-      base += all;
-      __syncthreads();
-      if (base > tile && blockIdx.x != 0) break;
-    }
-    if (range[0] < 0) return;
-    s = uniform((uint32_t)range[0]);
-    row0 = uniform((uint32_t)range[1]) * kTileRows;
-    rows = uniform((uint32_t)range[2]);
-    __syncthreads();
+    Found f;
+    if (!find_item(a.b.n_seq, tile, [&](uint32_t i) {
+          bool bad;
+          const SeqView v = load_seq(a.b, i, &bad);
+          const uint32_t r = v.ok ? v.q_len * a.group : 0;
+          return r > L.n.small_rows ? (r + kTileRows - 1) / kTileRows : 0u;
+        }, &f))
+      return;
+    s = f.s;
+    row0 = (f.n - 1 - (tile - f.first)) * kTileRows;  // the last rows, with the most positions, first
+    bool bad;
+    rows = load_seq(a.b, s, &bad).q_len * a.group;
   }
   // the lane's row
   const uint32_t col = lane & 31, half = lane >> 5;
@@ -831,81 +836,104 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
 }
 
 // ---- joining the parts of a row ------------------------------------------------------
-// A block takes 16 rows of one KV head of a sequence, 16 lanes to a row.
+// A wave takes a row of a query head, its four groups of 16 lanes every
+// fourth part: all maxima at once, then the parts' values, four parts' loads
+// of a group at a time. Bound by latency (a part of a row is 512 bytes at a
+// place of its own).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
-  constexpr int N = D / 16;
-  __shared__ uint32_t slots[4];
-  __shared__ uint32_t mine[2];
+  constexpr int N = D / 16;   // values per lane
+  constexpr uint32_t kAhead = 4;
   const AttnParams& a = L.a;
-  const uint32_t t = threadIdx.x;
-  const uint32_t h = blockIdx.x % a.n_kv, tile = blockIdx.x / a.n_kv;
-  uint32_t base = 0;
-  if (t == 0) mine[0] = 0xffffffffu;
-  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kThreads) {
-    uint32_t n = 0;
-    if (s0 + t < a.b.n_seq) {
-      bool bad;
-      const SeqView v = load_seq(a.b, s0 + t, &bad);
-      if (v.ok) n = (v.q_len * a.group + 15) / 16;
-    }
-    uint32_t all;
-    const uint32_t upto = base + block_scan(n, slots, &all);
-    if (n && upto - n <= tile && tile < upto) {
-      mine[0] = s0 + t;
-      mine[1] = tile - (upto - n);
-    }
-    base += all;
-    __syncthreads();
-    if (base > tile) break;
-  }
-  const uint32_t s = mine[0];
-  if (s == 0xffffffffu) return;
+  const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  uint32_t s = 0, row, head, r;
+  SeqView sv;
   bool bad;
-  const SeqView sv = load_seq(a.b, s, &bad);
-  const uint32_t rows = sv.q_len * a.group;
-  const uint32_t r = mine[1] * 16 + t / 16, c0 = t % 16 * N;
-  if (r >= rows) return;
-  const uint32_t row = sv.q0 + r / a.group, head = h * a.group + r % a.group;
-  const bool small = rows <= kSmallRows;
+  if (L.n.merge_small) {  // blocks: (sequence, four rows, KV head)
+    const uint32_t h = blockIdx.x % a.n_kv, i = blockIdx.x / a.n_kv;
+    s = i / L.n.merge_rows;
+    sv = load_seq(a.b, s, &bad);
+    r = i % L.n.merge_rows * kWaves + wave;
+    row = sv.q0 + r / a.group;
+    head = h * a.group + r % a.group;
+  } else {  // waves: (row, head)
+    const uint32_t w = blockIdx.x * kWaves + wave;
+    row = w / a.n_head;
+    head = w % a.n_head;
+    if (row >= a.b.n_rows) return;
+    for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64)
+      s += (uint32_t)__popcll(__ballot(s0 + lane < a.b.n_seq && a.b.q_start[s0 + lane + 1] <= row));
+    if (s >= a.b.n_seq) return;
+    sv = load_seq(a.b, s, &bad);
+    if (row < sv.q0) return;
+    r = (row - sv.q0) * a.group + head % a.group;
+  }
+  if (!sv.ok || r >= sv.q_len * a.group) return;
+  const bool small = sv.q_len * a.group <= L.n.small_rows;
+  if (L.n.merge_small && !small) return;
   const uint32_t n_prefix = a.shared_len ? L.n.prefix_parts : 0;
-  const uint32_t first = small ? L.ws.plan[2 * s] : 0;
-  const uint32_t n_own = small ? L.ws.plan[2 * s + 1] : L.n.tile_parts;
+  const uint32_t first = small ? load_uniform(L.ws.plan, 2 * s) : 0;
+  const uint32_t n_own = small ? load_uniform(L.ws.plan, 2 * s + 1) : L.n.tile_parts;
   if (n_prefix == 0 && n_own == 1) return;  // written already
+  const uint32_t h = head / a.group;
   const size_t rh = (size_t)row * a.n_head + head, all = (size_t)a.b.n_rows * a.n_head;
-  auto place = [&](uint32_t i, const float** o, const float** ml) {
-    if (i < n_prefix) {
-      *o = L.ws.prefix_o + (i * all + rh) * D;
-      *ml = L.ws.prefix_ml + (i * all + rh) * 2;
-    } else if (small) {
-      const size_t at = ((size_t)(first + i - n_prefix) * a.n_kv + h) * kSmallRows + r;
-      *o = L.ws.item_o + at * D;
-      *ml = L.ws.item_ml + at * 2;
-    } else {
-      *o = L.ws.tile_o + ((i - n_prefix) * all + rh) * D;
-      *ml = L.ws.tile_ml + ((i - n_prefix) * all + rh) * 2;
-    }
-  };
   const uint32_t n = n_prefix + n_own;
-  float m = -INFINITY, l = 0.0f, acc[N] = {};
-  for (uint32_t i = 0; i < n; i++) {
+  auto place = [&](uint32_t i, const float** o, const float** ml) {
+    size_t at;
+    if (i < n_prefix) {
+      at = i * all + rh;
+      *o = L.ws.prefix_o;
+      *ml = L.ws.prefix_ml;
+    } else if (small) {
+      at = ((size_t)(first + i - n_prefix) * a.n_kv + h) * kSmallRows + r;
+      *o = L.ws.item_o;
+      *ml = L.ws.item_ml;
+    } else {
+      at = (i - n_prefix) * all + rh;
+      *o = L.ws.tile_o;
+      *ml = L.ws.tile_ml;
+    }
+    *o += at * D;
+    *ml += at * 2;
+  };
+  float m = -INFINITY;
+  for (uint32_t i = lane; i < n; i += 64) {
     const float *o, *ml;
     place(i, &o, &ml);
     m = fmaxf(m, ml[0]);
   }
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  m = max_across_16(max_across_32(m));
   const float mb = m == -INFINITY ? 0.0f : m;
-  for (uint32_t i = 0; i < n; i++) {
-    const float *o, *ml;
-    place(i, &o, &ml);
-    const float f = __builtin_amdgcn_exp2f(ml[0] - mb);
-    l = fmaf(ml[1], f, l);
+  const uint32_t quad = lane / 16, c0 = lane % 16 * N;
+  float l = 0.0f, acc[N] = {};
+  for (uint32_t i0 = quad; i0 < n; i0 += 4 * kAhead) {
+    f32x4_t v[kAhead][N / 4];
+    float mi[kAhead], li[kAhead];
 #pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      const f32x4_t v = *(const f32x4_t*)(o + c0 + k);
+    for (uint32_t q = 0; q < kAhead; q++) {
+      const uint32_t i = i0 + 4 * q;
+      const float *o, *ml;
+      place(i < n ? i : i0, &o, &ml);
+      mi[q] = i < n ? ml[0] : -INFINITY;
+      li[q] = ml[1];
 #pragma unroll
-      for (int e = 0; e < 4; e++) acc[k + e] = fmaf(v[e], f, acc[k + e]);
+      for (int k = 0; k < N / 4; k++) v[q][k] = *(const f32x4_t*)(o + c0 + 4 * k);
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < kAhead; q++) {
+      if (i0 + 4 * q >= n) continue;
+      const float f = __builtin_amdgcn_exp2f(mi[q] - mb);
+      l = fmaf(li[q], f, l);
+#pragma unroll
+      for (int k = 0; k < N; k++) acc[k] = fmaf(v[q][k / 4][k % 4], f, acc[k]);
     }
   }
+  l = sum_across_16(sum_across_32(l));
+#pragma unroll
+  for (int k = 0; k < N; k++) acc[k] = sum_across_16(sum_across_32(acc[k]));
+  if (quad != 0) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   typedef T VO __attribute__((ext_vector_type(N)));
   VO v;
@@ -916,11 +944,11 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
 
 constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into
 
-// Parts that the positions of `blocks` tiles are divided into: enough blocks
-// to fill the card twice, at least 256 positions each.
+// Parts that the positions of `blocks` tiles are divided into: as many as let
+// all blocks run at once (two to a CU), of at least 256 positions.
 uint32_t tile_parts(uint64_t blocks, uint64_t positions) {
-  if (blocks == 0 || blocks >= 512) return 1;
-  return (uint32_t)std::max<uint64_t>(1, std::min((512 + blocks - 1) / blocks, positions / 256));
+  if (blocks == 0) return 1;
+  return (uint32_t)std::max<uint64_t>(1, std::min(512 / blocks, positions / 256));
 }
 
 int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
@@ -948,14 +976,16 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
   Sizes n{};
   const uint64_t group = args.n_head / kv.n_head_kv, rows = (uint64_t)q.n_rows * group;
   const uint64_t own = q.max_kv > args.shared_len ? q.max_kv - args.shared_len : 0;
-  n.small = group <= kSmallRows;
   n.tiled = q.max_q * group > kSmallRows;
+  // a single sequence goes to one of the two kernels as a whole
+  n.small = group <= kSmallRows && !(n.tiled && q.n_seq == 1);
+  n.small_rows = n.small ? kSmallRows : 0;
   if (n.small) {
     n.item_goal = std::max(1u, kSmallBlocks / kv.n_head_kv);
     n.items = q.n_seq + n.item_goal;
   }
   if (n.tiled) {
-    n.tiles = (uint32_t)(rows / kTileRows + std::min<uint64_t>(q.n_seq, rows / (kSmallRows + 1)));
+    n.tiles = (uint32_t)(rows / kTileRows + std::min<uint64_t>(q.n_seq, rows / (n.small_rows + 1)));
     n.tile_parts = tile_parts((uint64_t)n.tiles * kv.n_head_kv, own);
   }
   if (args.shared_len) {
@@ -963,6 +993,8 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
     n.prefix_parts = tile_parts((uint64_t)n.prefix_tiles * kv.n_head_kv, args.shared_len);
   }
   n.merge = args.shared_len || (n.small && own > kSmallTile) || n.tile_parts > 1;
+  n.merge_small = !args.shared_len && n.tile_parts <= 1;
+  n.merge_rows = (uint32_t)(std::min<uint64_t>(kSmallRows, q.max_q * group) + kWaves - 1) / kWaves;
   return n;
 }
 
@@ -1024,9 +1056,9 @@ int launch_attn(const Launch& L, int device, hipStream_t s) {
                        kTileLds<D>, s, L);
   if (L.n.small) hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), 0, s, L);
   if (L.n.merge) {
-    const uint64_t rows = (uint64_t)L.a.b.n_rows * L.a.group;
-    const uint32_t tiles = (uint32_t)(rows / 16 + std::min<uint64_t>(L.a.b.n_seq, rows));
-    hipLaunchKernelGGL((k_attn_merge<T, D>), dim3(tiles * G), dim3(kThreads), 0, s, L);
+    const uint64_t blocks = L.n.merge_small ? (uint64_t)L.a.b.n_seq * L.n.merge_rows * G
+                                            : ((uint64_t)L.a.b.n_rows * L.a.n_head + kWaves - 1) / kWaves;
+    hipLaunchKernelGGL((k_attn_merge<T, D>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, L);
   }
   return launched("rlh_paged_attn");
 }
