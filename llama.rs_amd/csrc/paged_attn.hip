@@ -28,7 +28,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kSmallRows = 16;    // rows of a KV head that the small kernel takes (the width of its MFMA)
 constexpr int kSmallTile = 128;   // positions that its four waves take per step
-constexpr int kTileRows = 128;    // rows of a tile of the tiled kernel
+constexpr int kTileWaves = 8;
+constexpr int kTileRows = 32 * kTileWaves;  // rows of a tile of the tiled kernel
 constexpr int kTileKv = 64;       // positions of its steps
 // The maximum that probabilities are relative to is only moved when the
 // running maximum has grown by more than 8 (in units of log 2): until then
@@ -125,22 +126,21 @@ __device__ __forceinline__ void copy_to_lds(const void* src, uint32_t dst) {
 }
 #pragma clang diagnostic pop
 
-// Scores in units of log 2, from dots: s * scale, capped, biased.
+// Scores in units of log 2. Without cap and bias they are dot * mul, and the
+// product is only formed in the exponential's argument (mul > 0: the largest
+// dot has the largest score).
 struct Scoring {
-  float mul;              // scale * log2(e), or with a cap 2 scale / cap * log2(e)
+  float mul;              // |scale| * log2(e), or with a cap 2 scale / cap * log2(e)
   float cap2;             // softcap * log2(e)
+  uint32_t flip;          // sign bits of two halves: q is negated where scale < 0
   bool capped, biased;
 };
 
-template <bool MOD>
 __device__ __forceinline__ float score(const Scoring& c, float dot, float slope2, int32_t away) {
   float x = dot * c.mul;
-  if constexpr (MOD) {
-    // tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
-    if (c.capped) x = c.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f));
-    if (c.biased) x = fmaf(slope2, (float)away, x);
-  }
-  return x;
+  // tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
+  if (c.capped) x = c.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f));
+  return c.biased ? fmaf(slope2, (float)away, x) : x;
 }
 
 // What the partial results of one row look like: m, l and the D sums, by
@@ -327,8 +327,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
     u32x4_t z = {0, 0, 0, 0};
     if (active)
       z = *(const u32x4_t*)((const T*)a.q + (size_t)row * a.q_stride + (size_t)head * D + i * 32 + quad * 8);
-    q[i] = __builtin_bit_cast(vec8<T>, z);
+    q[i] = __builtin_bit_cast(vec8<T>, z ^ L.sc.flip);
   }
+  const float mul = MOD ? 1.0f : L.sc.mul;
   f32x4_t o[kOut];
 #pragma unroll
   for (int i = 0; i < kOut; i++) o[i] = f32x4_t{0, 0, 0, 0};
@@ -400,15 +401,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
       }
       __builtin_amdgcn_sched_barrier(0);
       float x[8];
-      float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const int32_t j = p + (i / 4) * 16 + (int32_t)quad * 4 + i % 4;
-        x[i] = score<MOD>(L.sc, sc[i / 4][i % 4], slope2, j - pos);
-        if (!full && !((ok >> (i / 4) & 1) && j < (int32_t)sq.v.kv_len && row_sees(span, j))) x[i] = -INFINITY;
-        top = fmaxf(top, x[i]);
+        x[i] = MOD ? score(L.sc, sc[i / 4][i % 4], slope2, j - pos) : sc[i / 4][i % 4];
       }
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int32_t j = p + (i / 4) * 16 + (int32_t)quad * 4 + i % 4;
+          x[i] = (row_sees(span, j) & (bool)(ok >> (i / 4) & 1)) ? x[i] : -INFINITY;
+        }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
       top = max_across_16(max_across_32(top));
+      if constexpr (!MOD) top *= mul;
       if (__ballot(top > m + kSlack)) {
         const float mn = fmaxf(m, top);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
       vec8<T> pr;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - mb);
+        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], mul, -mb));
         l += x[i];
         pr[i] = (T)x[i];
       }
@@ -431,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
         const int32_t r = (int32_t)__builtin_ctzll(special);
         special &= special - 1;
         const int32_t j = p + r;
-        const bool see = (ok >> (r / 16) & 1) && j < (int32_t)sq.v.kv_len && row_sees(span, j);
+        const bool see = (ok >> (r / 16) & 1) && row_sees(span, j);
         const float pv = element<T>(pr, (uint32_t)(r / 16 * 4 + r % 4), (int)(col + 16 * (uint32_t)(r % 16 / 4)));
 #pragma unroll
         for (int i = 0; i < kOut; i++)
@@ -492,12 +501,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
 }
 
 // ---- many rows: prompts, and the shared prefix of the whole batch ------------------
-// A block takes 128 rows of one KV head (rows are tokens times heads per KV
+// A block takes 256 rows of one KV head (rows are tokens times heads per KV
 // head, so heads that share K and V share a tile) and walks 64 positions at
 // a time; K and V are copied into LDS by DMA, one step ahead, in 16-byte
 // pieces that are exchanged within a row so that the products' reads meet no
-// bank twice. Each wave has 32 rows: scores are K times Q^T (32x32x16:
-// positions down, rows across), so that a row is a lane column as above.
+// bank twice. Each of eight waves has 32 rows: scores are K times Q^T
+// (32x32x16: positions down, rows across), so that a row is a lane column as
+// above. What bounds it: a step's 32 MFMAs take 1024 cycles of a SIMD and its
+// exponentials, maxima and sums as many, and the two overlap only between
+// two waves that are at different places; copies are issued at 48 cycles a
+// KB, so four waves per tile would spend 1550 cycles a step on them.
 template <int D>
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   return D == 128 ? ((r & 3) << 2 | (r >> 2 & 3)) : ((r >> 1 & 1) << 2 | (r >> 2 & 3));
@@ -505,19 +518,21 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
 
 struct TileShared {
   uint64_t special[2];  // positions of a step whose V row holds infinities or NaN
-  int32_t ranges[kWaves][8];
+  int32_t ranges[kTileWaves][8];
 };
 template <int D>
 constexpr uint32_t kTileLds = 4 * kTileKv * D * 2 + sizeof(TileShared);
 
 template <typename T, int D, bool MOD, bool PREFIX>
-__global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
+__global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   constexpr int kRowB = D * 2;
   constexpr int kBuf = kTileKv * kRowB;   // bytes of a K or V step
   constexpr int kSteps = D / 16;
   constexpr int kOut = D / 32;
   constexpr int kLanes = D / 8;           // lanes of a row in a copy
-  constexpr int kCopies = 16 / (64 / kLanes);  // 1 KB copies of 16 rows
+  constexpr int kThreads = 64 * kTileWaves;
+  constexpr int kMine = kTileKv / kTileWaves;           // positions of a step that a wave copies
+  constexpr int kCopies = kMine / (64 / kLanes);        // in 1 KB pieces
   // K, V of two steps first: a copy's LDS address has 16 bits
   extern __shared__ __align__(1024) uint8_t lds[];
   TileShared& sh = *(TileShared*)(lds + 4 * kBuf);
@@ -622,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
   int32_t t_lo = 0x7fffffff, t_hi = 0, t_prefix = 0, t_min_lo = 0x7fffffff;  // the block's
   int32_t c_lo = 0, c_hi = 0x7fffffff, c_prefix = 0x7fffffff;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) {
+  for (int w = 0; w < kTileWaves; w++) {
     const int32_t* r = sh.ranges[w];
     t_lo = min(t_lo, r[0]);
     t_hi = max(t_hi, r[1]);
@@ -648,8 +663,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
   for (int i = 0; i < kSteps; i++) {
     u32x4_t z = {0, 0, 0, 0};
     if (active) z = *(const u32x4_t*)((const T*)a.q + (size_t)row * a.q_stride + (size_t)head * D + i * 16 + half * 8);
-    q[i] = __builtin_bit_cast(vec8<T>, z);
+    q[i] = __builtin_bit_cast(vec8<T>, z ^ L.sc.flip);
   }
+  const float mul = MOD ? 1.0f : L.sc.mul;
   f32x16_t o[kOut];
 #pragma unroll
   for (int i = 0; i < kOut; i++)
@@ -659,47 +675,63 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
 
   const uint32_t* table = PREFIX ? a.shared_table : a.b.table + (size_t)s * a.b.table_stride;
   const uint32_t page_mask = (1u << a.page_shift) - 1;
-  auto needed = [&](int32_t p) { return p < t_hi && (p < t_prefix || p + 16 > t_min_lo); };
-  // the step's four groups of 16 positions whose page exists; the wave's own
-  // group is copied
-  auto copy = [&](int32_t p, uint32_t buf) -> uint32_t {
-    uint32_t ok = 0, page = 0, slot = 0;
+  // Page ids of 16 steps, a group of 16 positions per lane (the id, or none),
+  // loaded some steps before their first use
+  constexpr uint32_t kNone = 0xffffffffu;
+  auto look_up = [&](uint32_t step) -> uint32_t {
+    const int32_t g = t_lo + (int32_t)step * kTileKv + 16 * (int32_t)lane;
+    // whether the group holds positions that a row sees
+    if (!((g < t_hi) & ((g < t_prefix) | (g + 16 > t_min_lo)))) return kNone;
+    const uint32_t e = table[(uint32_t)g >> a.page_shift];
+    if (e < a.n_pages) return e;
+    if (wave == 0) raise(a.status, RLH_SERVE_BAD_PAGE);
+    return kNone;
+  };
+  uint32_t from[kCopies];  // of the wave's positions, what each lane copies
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int32_t pu = p + 16 * u;
-      if (!needed(pu)) continue;
-      const uint32_t e = load_uniform(table, (uint32_t)pu >> a.page_shift);
-      if (e >= a.n_pages) {
-        raise(t == 0 ? a.status : nullptr, RLH_SERVE_BAD_PAGE);
-        continue;
-      }
-      ok |= 1u << u;
-      if (u == (int)wave) {
-        page = e;
-        slot = (uint32_t)pu & page_mask;
-      }
-    }
-    const size_t at = ((((size_t)page * a.n_kv + h) << a.page_shift) + slot) * D;
+  for (int i = 0; i < kCopies; i++) {
+    const uint32_t r = wave * kMine + i * (64 / kLanes) + lane / kLanes;  // of the step
+    from[i] = r % 16 * D + ((lane % kLanes) ^ swizzle<D>(r)) * 8;
+  }
+  // copies the wave's positions of the step at p, whose groups are lanes
+  // 4 k .. 4 k + 3 of `pages`
+  auto copy = [&](int32_t p, uint32_t pages, uint32_t k, uint32_t buf) {
+    const uint32_t u = wave * kMine / 16;
+    const uint32_t page = lane_value(pages, (int)(4 * k + u));
+    const bool exists = page != kNone;
+    const uint32_t slot = exists ? (uint32_t)(p + 16 * (int32_t)u) & page_mask : 0u;
+    const size_t at = ((((size_t)(exists ? page : 0u) * a.n_kv + h) << a.page_shift) + slot) * D;
+    const uint32_t dst = lds0 + buf * 2 * kBuf + wave * kMine * kRowB;
 #pragma unroll
     for (int i = 0; i < kCopies; i++) {
-      const uint32_t r = i * (64 / kLanes) + lane / kLanes;  // of the group's 16
-      const uint32_t c = (lane % kLanes) ^ swizzle<D>(r);
-      const uint32_t dst = lds0 + buf * 2 * kBuf + wave * 16 * kRowB + i * 1024;
-      copy_to_lds((const T*)a.pool_k + at + r * D + c * 8, dst);
-      copy_to_lds((const T*)a.pool_v + at + r * D + c * 8, dst + kBuf);
+      copy_to_lds((const T*)a.pool_k + at + from[i], dst + i * 1024);
+      copy_to_lds((const T*)a.pool_v + at + from[i], dst + i * 1024 + kBuf);
     }
-    return ok;
   };
-  uint32_t ok_next = 0;
-  if (st0 < st1) ok_next = copy(t_lo + (int32_t)st0 * kTileKv, 0);
+  // Two waves share a SIMD; left alone they go through products and
+  // exponentials in step and take turns at both.
+  if (wave >= kTileWaves / 2) __builtin_amdgcn_s_setprio(2);
+  uint32_t pages = kNone, next_pages = kNone;
+  uint64_t exist = 0;  // the groups of `pages` whose page exists
+  if (st0 < st1) {
+    pages = look_up(st0);
+    exist = __ballot(pages != kNone);
+    copy(t_lo + (int32_t)st0 * kTileKv, pages, 0, 0);
+  }
   for (uint32_t st = st0; st < st1; st++) {
     const uint32_t buf = (st - st0) & 1;
     const int32_t p = t_lo + (int32_t)st * kTileKv;
-    const uint32_t ok = ok_next;
+    const uint32_t k = (st - st0) & 15;
+    const uint32_t ok = (uint32_t)(exist >> (4 * k)) & 15;
     if (t == 0) special[buf] = 0;  // last read two barriers ago
     wait_vmcnt<0>();               // this wave's copies of the step have landed
     lds_barrier();                 // ... everyone's; every wave is done with the other buffer
-    if (st + 1 < st1) ok_next = copy(p + kTileKv, buf ^ 1);
+    if (k == 8) next_pages = look_up(st + 8);
+    if (k == 15) {
+      pages = next_pages;
+      exist = __ballot(pages != kNone);
+    }
+    if (st + 1 < st1) copy(p + kTileKv, pages, (k + 1) & 15, buf ^ 1);
     const uint8_t RLH_LDS* kb = (const uint8_t RLH_LDS*)lds + buf * 2 * kBuf;
     uint8_t RLH_LDS* vb = (uint8_t RLH_LDS*)lds + buf * 2 * kBuf + kBuf;
     const bool full = ok == 15 && ((p >= w_lo && p + kTileKv <= w_hi) || p + kTileKv <= w_prefix);
@@ -718,7 +750,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
       odd = special[buf];
     }
     f32x16_t sc[2];
-    float x[2][16];
     vec8<T> pr[4];
     if (!none) {
 #pragma unroll
@@ -732,17 +763,27 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
         for (int i = 0; i < kSteps; i++)
           sc[u] = mfma32(__builtin_bit_cast(vec8<T>, *(const RLH_LDS_PTR(u32x4_t)*)(kp + ((2 * i + half) ^ z) * 16)), q[i], sc[u]);
       }
-      float top = -INFINITY;
+      if constexpr (MOD) {
 #pragma unroll
-      for (int u = 0; u < 2; u++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int32_t j = p + u * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4;
-          x[u][e] = score<MOD>(L.sc, sc[u][e], slope2, j - pos);
-          if (!full && !((ok >> (2 * u + e / 8) & 1) && row_sees(span, j) && (PREFIX || j >= (int32_t)a.shared_len))) x[u][e] = -INFINITY;
-          top = fmaxf(top, x[u][e]);
-        }
+          for (int e = 0; e < 16; e++)
+            sc[u][e] = score(L.sc, sc[u][e], slope2, p + u * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4 - pos);
+      }
+      if (!full) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int32_t j = p + u * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4;
+            sc[u][e] = (row_sees(span, j) & (bool)(ok >> (2 * u + e / 8) & 1)) ? sc[u][e] : -INFINITY;
+          }
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; i++) top = fmaxf(top, sc[i / 16][i % 16]);
       top = max_across_32(top);
+      if constexpr (!MOD) top *= mul;
       if (__ballot(top > m + kSlack)) {
         const float mn = fmaxf(m, top);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -756,16 +797,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_tiles(Launch L) {
       for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-          x[u][e] = __builtin_amdgcn_exp2f(x[u][e] - mb);
-          l += x[u][e];
-          pr[2 * u + e / 8][e % 8] = (T)x[u][e];
+          const float x = __builtin_amdgcn_exp2f(fmaf(sc[u][e], mul, -mb));
+          l += x;
+          pr[2 * u + e / 8][e % 8] = (T)x;
         }
     }
     if (odd) {
       if (!none) {
         for (uint64_t left = odd; left; left &= left - 1) {
           const int32_t r = (int32_t)__builtin_ctzll(left), j = p + r;
-          const bool see = active && (ok >> (r / 16) & 1) && row_sees(span, j) && (PREFIX || j >= (int32_t)a.shared_len);
+          const bool see = active && (ok >> (r / 16) & 1) && row_sees(span, j);
           float pv = 0.0f;
 #pragma unroll
           for (int ks = 0; ks < 4; ks++) {
@@ -945,10 +986,10 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
 constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into
 
 // Parts that the positions of `blocks` tiles are divided into: as many as let
-// all blocks run at once (two to a CU), of at least 256 positions.
+// all blocks run at once (one to a CU), of at least 256 positions.
 uint32_t tile_parts(uint64_t blocks, uint64_t positions) {
   if (blocks == 0) return 1;
-  return (uint32_t)std::max<uint64_t>(1, std::min(512 / blocks, positions / 256));
+  return (uint32_t)std::max<uint64_t>(1, std::min(256 / blocks, positions / 256));
 }
 
 int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
@@ -1049,10 +1090,10 @@ int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
   if (L.a.shared_len || L.n.tiled) RLH_TRY((allow_tile_lds<T, D, MOD>(device)));
   if (L.a.shared_len)
-    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, true>), dim3(L.n.prefix_tiles * L.n.prefix_parts * G), dim3(kThreads),
+    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, true>), dim3(L.n.prefix_tiles * L.n.prefix_parts * G), dim3(64 * kTileWaves),
                        kTileLds<D>, s, L);
   if (L.n.tiled)
-    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, false>), dim3(L.n.tiles * L.n.tile_parts * G), dim3(kThreads),
+    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, false>), dim3(L.n.tiles * L.n.tile_parts * G), dim3(64 * kTileWaves),
                        kTileLds<D>, s, L);
   if (L.n.small) hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), 0, s, L);
   if (L.n.merge) {
@@ -1133,9 +1174,11 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   place_workspace(&L.ws, (uint8_t*)workspace, *kv, *seqs, *args, L.n);
   L.sc.capped = args->softcap > 0.0f;
   L.sc.biased = args->slopes != nullptr;
-  L.sc.mul = L.sc.capped ? 2.0f * args->scale / args->softcap * kLog2e : args->scale * kLog2e;
+  const float scale = fabsf(args->scale);
+  L.sc.mul = L.sc.capped ? 2.0f * scale / args->softcap * kLog2e : scale * kLog2e;
   L.sc.cap2 = args->softcap * kLog2e;
-  const bool mod = L.sc.capped || L.sc.biased;
+  L.sc.flip = args->scale < 0.0f ? 0x80008000u : 0u;
+  const bool mod = L.sc.capped || L.sc.biased || !(scale > 0.0f);
   if (kv->type == RLH_TYPE_F16) return launch_attn<_Float16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
   return launch_attn<__bf16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
 }
