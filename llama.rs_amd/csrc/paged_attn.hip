@@ -136,11 +136,11 @@ struct Scoring {
   bool capped, biased;
 };
 
-__device__ __forceinline__ float score(const Scoring& c, float dot, float slope2, int32_t away) {
+__device__ __forceinline__ float score(const Scoring& c, float dot, float slope2, float away) {
   float x = dot * c.mul;
   // tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
   if (c.capped) x = c.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f));
-  return c.biased ? fmaf(slope2, (float)away, x) : x;
+  return c.biased ? fmaf(slope2, away, x) : x;
 }
 
 // What the partial results of one row look like: m, l and the D sums, by
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const int32_t j = p + (i / 4) * 16 + (int32_t)quad * 4 + i % 4;
-        x[i] = MOD ? score(L.sc, sc[i / 4][i % 4], slope2, j - pos) : sc[i / 4][i % 4];
+        x[i] = MOD ? score(L.sc, sc[i / 4][i % 4], slope2, (float)(j - pos)) : sc[i / 4][i % 4];
       }
       if (!full) {
 #pragma unroll
@@ -711,6 +711,28 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   // Two waves share a SIMD; left alone they go through products and
   // exponentials in step and take turns at both.
   if (wave >= kTileWaves / 2) __builtin_amdgcn_s_setprio(2);
+  // operands: K's row 32 u + col, values 16 i + 8 half + 0..7; V's rows 16 ks +
+  // 4 half + 0..3 and + 8, by columns 32 i + 16 (lane / 16 % 2) + 0..15
+  const uint32_t va = half * 4 + lane % 16 / 4, vb8 = va + 8;
+  uint32_t v_at[2][kOut], k_at[kSteps];
+#pragma unroll
+  for (int i = 0; i < kOut; i++) {
+    const uint32_t d = i * 32 + (lane >> 4 & 1) * 16 + lane % 4 * 4;
+    v_at[0][i] = va * kRowB + ((d / 8) ^ swizzle<D>(va)) * 16 + d % 8 * 2;
+    v_at[1][i] = vb8 * kRowB + ((d / 8) ^ swizzle<D>(vb8)) * 16 + d % 8 * 2;
+  }
+#pragma unroll
+  for (int i = 0; i < kSteps; i++) k_at[i] = col * kRowB + ((2 * i + half) ^ swizzle<D>(col)) * 16;
+  auto load_v = [&](const uint8_t RLH_LDS* vb, int ks, vec8<T> (&f)[kOut]) {
+#pragma unroll
+    for (int i = 0; i < kOut; i++)
+      f[i] = read_columns<T>(vb + v_at[0][i] + ks * 16 * kRowB, vb + v_at[1][i] + ks * 16 * kRowB);
+  };
+  auto load_k = [&](const uint8_t RLH_LDS* kb, int u, vec8<T> (&f)[kSteps]) {
+#pragma unroll
+    for (int i = 0; i < kSteps; i++)
+      f[i] = __builtin_bit_cast(vec8<T>, *(const RLH_LDS_PTR(u32x4_t)*)(kb + k_at[i] + u * 32 * kRowB));
+  };
   uint32_t pages = kNone, next_pages = kNone;
   uint64_t exist = 0;  // the groups of `pages` whose page exists
   if (st0 < st1) {
@@ -752,32 +774,36 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
     f32x16_t sc[2];
     vec8<T> pr[4];
     if (!none) {
+      // reads well ahead of the products (one read takes some 250 cycles)
+      vec8<T> k0[kSteps], k1[kSteps];
+      load_k(kb, 0, k0);
+      load_k(kb, 1, k1);
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
+      for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int e = 0; e < 16; e++) sc[u][e] = 0.0f;
-        const uint32_t r = u * 32 + col;
-        const uint8_t RLH_LDS* kp = kb + r * kRowB;
-        const uint32_t z = swizzle<D>(r);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < kSteps; i++)
-          sc[u] = mfma32(__builtin_bit_cast(vec8<T>, *(const RLH_LDS_PTR(u32x4_t)*)(kp + ((2 * i + half) ^ z) * 16)), q[i], sc[u]);
-      }
+      for (int i = 0; i < kSteps; i++) sc[0] = mfma32(k0[i], q[i], sc[0]);
+#pragma unroll
+      for (int i = 0; i < kSteps; i++) sc[1] = mfma32(k1[i], q[i], sc[1]);
+      // the lane's first position; the others are constants away (opaque, so
+      // that 32 of them are not kept in registers from step to step)
+      int32_t j0 = p + (int32_t)half * 4;
+      asm volatile("" : "+v"(j0));
       if constexpr (MOD) {
+        const float away = (float)(j0 - pos);
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++)
-            sc[u][e] = score(L.sc, sc[u][e], slope2, p + u * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4 - pos);
+        for (int i = 0; i < 32; i++) sc[i / 16][i % 16] = score(L.sc, sc[i / 16][i % 16], slope2, away + (float)(i / 4 * 8 + i % 4));
       }
       if (!full) {
+        const int32_t lo = span.lo - j0, hi = span.hi - j0, pre = span.prefix - j0;
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const int32_t j = p + u * 32 + (e / 4) * 8 + (int32_t)half * 4 + e % 4;
-            sc[u][e] = (row_sees(span, j) & (bool)(ok >> (2 * u + e / 8) & 1)) ? sc[u][e] : -INFINITY;
-          }
+        for (int i = 0; i < 32; i++) {
+          const int32_t d = i / 4 * 8 + i % 4;
+          const bool see = ((d >= lo) & (d < hi)) | (d < pre);
+          sc[i / 16][i % 16] = (see & (bool)(ok >> (i / 8) & 1)) ? sc[i / 16][i % 16] : -INFINITY;
+        }
       }
       float top = sc[0][0];
 #pragma unroll
@@ -831,18 +857,16 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
       lds_barrier();
     }
     if (!none) {
-      // V's rows 16 ks + 4 half + 0..3 and + 8, by columns 32 i + 16 (lane / 16 % 2) + 0..15
-      const uint32_t vr0 = half * 4 + lane % 16 / 4, vd = (lane >> 4 & 1) * 16 + lane % 4 * 4;
+      vec8<T> f[2][kOut];
+      load_v(vb, 0, f[0]);
+      load_v(vb, 1, f[1]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int ks = 0; ks < 4; ks++) {
-        const uint32_t ra = ks * 16 + vr0, rb = ra + 8;
 #pragma unroll
-        for (int i = 0; i < kOut; i++) {
-          const uint32_t c = (i * 32 + vd) / 8, b = vd % 8 * 2;
-          o[i] = mfma32(read_columns<T>(vb + ra * kRowB + (c ^ swizzle<D>(ra)) * 16 + b,
-                                        vb + rb * kRowB + (c ^ swizzle<D>(rb)) * 16 + b),
-                        pr[ks], o[i]);
-        }
+        for (int i = 0; i < kOut; i++) o[i] = mfma32(f[ks % 2][i], pr[ks], o[i]);
+        if (ks < 2) load_v(vb, ks + 2, f[ks % 2]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
