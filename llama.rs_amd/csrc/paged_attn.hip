@@ -27,7 +27,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kSmallRows = 16;    // rows of a KV head that the small kernel takes (the width of its MFMA)
-constexpr int kSmallTile = 128;   // positions that its four waves take per step
 constexpr int kTileWaves = 8;
 constexpr int kTileRows = 32 * kTileWaves;  // rows of a tile of the tiled kernel
 constexpr int kTileKv = 64;       // positions of its steps
@@ -253,21 +252,23 @@ __device__ __forceinline__ bool find_item(uint32_t n_seq, uint32_t item, F parts
 // maximum and the sum are one register per lane, and the probabilities are
 // already the next product's operand if V's rows are taken in the order that
 // the lanes hold them: 4 (lane / 16) + i, and 16 more.
-template <typename T, int D, bool MOD>
-__global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
+template <int D, int W>
+constexpr uint32_t kSmallLds = (W * 32 * (D * 2 + 32) > W * 16 * (D + 4) * 4 ? W * 32 * (D * 2 + 32) : W * 16 * (D + 4) * 4) + W * 128;
+
+template <typename T, int D, bool MOD, int W>
+__device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uint8_t* lds) {
   constexpr int kStride = D * 2 + 32;    // bytes of a V row in LDS: 8 rows start in 8 different bank groups
   constexpr int kSteps = D / 32;         // MFMAs of a score
   constexpr int kLoads = D / 16;         // 1 KB loads of 32 V rows
   constexpr int kLanes = D / 8;          // lanes of a row in them
   constexpr int kOut = D / 16;
   constexpr int kMergeStride = D + 4;
-  __shared__ __align__(16) uint8_t lds[kWaves * 32 * kStride > kWaves * 16 * kMergeStride * 4
-                                           ? kWaves * 32 * kStride : kWaves * 16 * kMergeStride * 4];
-  __shared__ float ml[kWaves][16][2];
+  constexpr int kSmallTile = 32 * W;     // positions that the waves take per step
+  float(*ml)[16][2] = (float(*)[16][2])(lds + kSmallLds<D, W> - W * 128);
   const AttnParams& a = L.a;
   const uint32_t t = threadIdx.x;
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
-  const uint32_t h = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
+  const uint32_t h = block % a.n_kv, item = block / a.n_kv;
   // the division of all sequences' positions, found by every wave alike
   auto tiles_of = [&](uint32_t s, bool* bad, bool* mine) -> uint32_t {
     const SeqSpan q = seq_span(a, s, bad);
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
     if (s < a.b.n_seq) {
       bool bad, mine;
       n = tiles_of(s, &bad, &mine);
-      if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
+      if (bad && block == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
       if (s0 == 0) {
         tiles0 = n;
         mine0 = mine;
@@ -467,37 +468,44 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
     ml[wave][col][1] = l;
   }
   __syncthreads();
-  const uint32_t r = t / 16, c0 = (t % 16) * (D / 16);
+  constexpr int kRowLanes = 4 * W, N = D / kRowLanes;  // threads and values of a row
+  const uint32_t r = t / kRowLanes, c0 = (t % kRowLanes) * N;
   if (r >= sq.rows) return;
-  float mm = -INFINITY, ls = 0.0f, acc[D / 16] = {};
+  float mm = -INFINITY, ls = 0.0f, acc[N] = {};
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) mm = fmaxf(mm, ml[w][r][0]);
+  for (int w = 0; w < W; w++) mm = fmaxf(mm, ml[w][r][0]);
   const float mb = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) {
+  for (int w = 0; w < W; w++) {
     const float f = __builtin_amdgcn_exp2f(ml[w][r][0] - mb);
     ls += ml[w][r][1] * f;
 #pragma unroll
-    for (int i = 0; i < D / 16; i++) acc[i] = fmaf(ol[(w * 16 + r) * kMergeStride + c0 + i], f, acc[i]);
+    for (int i = 0; i < N; i++) acc[i] = fmaf(ol[(w * 16 + r) * kMergeStride + c0 + i], f, acc[i]);
   }
   if (n_items == 1 && a.shared_len == 0) {
     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
     T* dst = (T*)a.out + (size_t)(sq.v.q0 + r / a.group) * a.out_stride + (size_t)(h * a.group + r % a.group) * D + c0;
-    typedef T VO __attribute__((ext_vector_type(D / 16)));
+    typedef T VO __attribute__((ext_vector_type(N)));
     VO v;
 #pragma unroll
-    for (int i = 0; i < D / 16; i++) v[i] = (T)(acc[i] * inv);
+    for (int i = 0; i < N; i++) v[i] = (T)(acc[i] * inv);
     *(VO*)dst = v;
   } else {
     const size_t at = ((size_t)item * a.n_kv + h) * kSmallRows + r;
     float* dst = L.ws.item_o + at * D + c0;
 #pragma unroll
-    for (int i = 0; i < D / 16; i += 4) *(f32x4_t*)(dst + i) = f32x4_t{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
+    for (int i = 0; i < N; i++) dst[i] = acc[i];
     if (c0 == 0) {
       L.ws.item_ml[2 * at] = mm;
       L.ws.item_ml[2 * at + 1] = ls;
     }
   }
+}
+
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  small_block<T, D, MOD, kWaves>(L, blockIdx.x, lds);
 }
 
 // ---- many rows: prompts, and the shared prefix of the whole batch ------------------
@@ -523,8 +531,8 @@ struct TileShared {
 template <int D>
 constexpr uint32_t kTileLds = 4 * kTileKv * D * 2 + sizeof(TileShared);
 
-template <typename T, int D, bool MOD, bool PREFIX>
-__global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
+template <typename T, int D, bool MOD>
+__device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool prefix, uint8_t* lds) {
   constexpr int kRowB = D * 2;
   constexpr int kBuf = kTileKv * kRowB;   // bytes of a K or V step
   constexpr int kSteps = D / 16;
@@ -533,25 +541,24 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   constexpr int kThreads = 64 * kTileWaves;
   constexpr int kMine = kTileKv / kTileWaves;           // positions of a step that a wave copies
   constexpr int kCopies = kMine / (64 / kLanes);        // in 1 KB pieces
-  // K, V of two steps first: a copy's LDS address has 16 bits
-  extern __shared__ __align__(1024) uint8_t lds[];
+  // K, V of two steps first
   TileShared& sh = *(TileShared*)(lds + 4 * kBuf);
   uint64_t* special = sh.special;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(RLH_LDS uint8_t*)lds;
   const AttnParams& a = L.a;
   const uint32_t t = threadIdx.x;
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
-  const uint32_t parts = PREFIX ? L.n.prefix_parts : L.n.tile_parts;
-  const uint32_t h = blockIdx.x % a.n_kv;
-  const uint32_t part = blockIdx.x / a.n_kv % parts;
-  const uint32_t tile = blockIdx.x / a.n_kv / parts;
+  const uint32_t parts = prefix ? L.n.prefix_parts : L.n.tile_parts;
+  const uint32_t h = block % a.n_kv;
+  const uint32_t part = block / a.n_kv % parts;
+  const uint32_t tile = block / a.n_kv / parts;
   // the tile's sequence (own positions), or all rows (the prefix)
   uint32_t s = 0, row0 = 0, rows = 0;
-  if constexpr (PREFIX) {
+  if (prefix) {
     row0 = tile * kTileRows;
     rows = a.b.n_rows * a.group;
   } else {
-    if (blockIdx.x == 0)
+    if (block == 0)
       for (uint32_t i = t; i < a.b.n_seq; i += kThreads) {
         bool bad;
         load_seq(a.b, i, &bad);
@@ -575,7 +582,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   const uint32_t rr = row0 + wave * 32 + col;
   bool active = rr < rows;
   uint32_t row = rr / a.group, g = rr % a.group, sq = s;
-  if constexpr (PREFIX) {
+  if (prefix) {
     uint32_t lo = 0, hi = a.b.n_seq;  // as many sequences end at or before the row as come before its own
     while (lo < hi) {
       const uint32_t mid = (lo + hi) / 2;
@@ -591,12 +598,12 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   if (active) {
     bool bad;
     sv = load_seq(a.b, sq, &bad);
-    if constexpr (!PREFIX) row += sv.q0;
+    if (!prefix) row += sv.q0;
     active = sv.ok && row >= sv.q0 && row < sv.q0 + sv.q_len;
   }
   const int32_t pos = (int32_t)(sv.kv_len - sv.q_len) + (int32_t)(row - sv.q0);
   const uint32_t head = h * a.group + g;
-  const int32_t limit = PREFIX ? min((int32_t)a.shared_len, (int32_t)sv.kv_len) : (int32_t)sv.kv_len;
+  const int32_t limit = prefix ? min((int32_t)a.shared_len, (int32_t)sv.kv_len) : (int32_t)sv.kv_len;
   RowSpan span{0, 0, 0};
   if (active) {
     span = row_span(pos, sv.kv_len, a.window, a.prefix_len ? a.prefix_len[sq] : 0);
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   // positions that the wave's rows all see lie in [w_lo, w_hi) or below
   // w_prefix; those that any sees in [b_lo, b_hi)
   int32_t w_lo = active ? span.lo : 0, w_hi = active ? span.hi : 0x7fffffff, w_prefix = active ? span.prefix : 0x7fffffff;
-  int32_t b_lo = active ? max(span_begin(span), PREFIX ? 0 : (int32_t)a.shared_len) : 0x7fffffff;
+  int32_t b_lo = active ? max(span_begin(span), prefix ? 0 : (int32_t)a.shared_len) : 0x7fffffff;
   int32_t b_hi = active ? span_end(span) : 0;
   int32_t any_prefix = active ? span.prefix : 0, min_lo = active ? span.lo : 0x7fffffff;
 #pragma unroll
@@ -673,7 +680,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
     for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  const uint32_t* table = PREFIX ? a.shared_table : a.b.table + (size_t)s * a.b.table_stride;
+  const uint32_t* table = prefix ? a.shared_table : a.b.table + (size_t)s * a.b.table_stride;
   const uint32_t page_mask = (1u << a.page_shift) - 1;
   // Page ids of 16 steps, a group of 16 positions per lane (the id, or none),
   // loaded some steps before their first use
@@ -872,7 +879,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
   }
   l = sum_across_32(l);
   if (!active) return;
-  if (!PREFIX && parts == 1 && a.shared_len == 0) {
+  if (!prefix && parts == 1 && a.shared_len == 0) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* dst = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * D;
 #pragma unroll
@@ -886,8 +893,8 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
       }
   } else {
     const size_t at = ((size_t)part * a.b.n_rows + row) * a.n_head + head;
-    float* dst = (PREFIX ? L.ws.prefix_o : L.ws.tile_o) + at * D;
-    float* mlp = (PREFIX ? L.ws.prefix_ml : L.ws.tile_ml) + at * 2;
+    float* dst = (prefix ? L.ws.prefix_o : L.ws.tile_o) + at * D;
+    float* mlp = (prefix ? L.ws.prefix_ml : L.ws.tile_ml) + at * 2;
 #pragma unroll
     for (int i = 0; i < kOut; i++)
 #pragma unroll
@@ -898,6 +905,20 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_tiles(Launch L) {
       mlp[1] = l;
     }
   }
+}
+
+// Prefix tiles, tiles and items of few rows in one launch: each kind leaves
+// parts of the card idle that the others fill.
+template <typename T, int D, bool MOD>
+__global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  const uint32_t n_prefix = L.n.prefix_tiles * L.n.prefix_parts * L.a.n_kv;
+  const uint32_t n_tiles = n_prefix + L.n.tiles * L.n.tile_parts * L.a.n_kv;
+  const uint32_t b = blockIdx.x;
+  if (b < n_tiles)
+    tile_block<T, D, MOD>(L, b < n_prefix ? b : b - n_prefix, b < n_prefix, lds);
+  else
+    small_block<T, D, MOD, kTileWaves>(L, b - n_tiles, lds);
 }
 
 // ---- joining the parts of a row ------------------------------------------------------
@@ -1057,7 +1078,8 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
     n.prefix_tiles = (uint32_t)((rows + kTileRows - 1) / kTileRows);
     n.prefix_parts = tile_parts((uint64_t)n.prefix_tiles * kv.n_head_kv, args.shared_len);
   }
-  n.merge = args.shared_len || (n.small && own > kSmallTile) || n.tile_parts > 1;
+  const uint32_t step = 32 * (args.shared_len || n.tiled ? kTileWaves : kWaves);  // of the few rows' blocks
+  n.merge = args.shared_len || (n.small && own > step) || n.tile_parts > 1;
   n.merge_small = !args.shared_len && n.tile_parts <= 1;
   n.merge_rows = (uint32_t)(std::min<uint64_t>(kSmallRows, q.max_q * group) + kWaves - 1) / kWaves;
   return n;
@@ -1091,17 +1113,17 @@ uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_att
   return place_workspace(&w, nullptr, kv, q, args, attn_sizes(kv, q, args));
 }
 
-// The tiled kernels take more LDS than a launch may by default; said once per
+// The mixed kernels take more LDS than a launch may by default; said once per
 // device (idempotent, so two threads may).
+template <int D>
+constexpr uint32_t kMixedLds = kTileLds<D> > kSmallLds<D, kTileWaves> ? kTileLds<D> : kSmallLds<D, kTileWaves>;
 template <typename T, int D, bool MOD>
-int allow_tile_lds(int device) {
+int allow_mixed_lds(int device) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_acquire) & bit) return RLH_OK;
-  if (hipFuncSetAttribute((const void*)k_attn_tiles<T, D, MOD, true>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (int)kTileLds<D>) != hipSuccess ||
-      hipFuncSetAttribute((const void*)k_attn_tiles<T, D, MOD, false>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (int)kTileLds<D>) != hipSuccess) {
+  if (hipFuncSetAttribute((const void*)k_attn_mixed<T, D, MOD>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)kMixedLds<D>) != hipSuccess) {
     (void)hipGetLastError();
     return serve_error(RLH_EDEVICE, "hipFuncSetAttribute (LDS of the tiled attention kernels)");
   }
@@ -1112,14 +1134,13 @@ int allow_tile_lds(int device) {
 template <typename T, int D, bool MOD>
 int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
-  if (L.a.shared_len || L.n.tiled) RLH_TRY((allow_tile_lds<T, D, MOD>(device)));
-  if (L.a.shared_len)
-    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, true>), dim3(L.n.prefix_tiles * L.n.prefix_parts * G), dim3(64 * kTileWaves),
-                       kTileLds<D>, s, L);
-  if (L.n.tiled)
-    hipLaunchKernelGGL((k_attn_tiles<T, D, MOD, false>), dim3(L.n.tiles * L.n.tile_parts * G), dim3(64 * kTileWaves),
-                       kTileLds<D>, s, L);
-  if (L.n.small) hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), 0, s, L);
+  if (L.a.shared_len || L.n.tiled) {
+    RLH_TRY((allow_mixed_lds<T, D, MOD>(device)));
+    const uint32_t blocks = (L.n.prefix_tiles * L.n.prefix_parts + L.n.tiles * L.n.tile_parts + L.n.items) * G;
+    hipLaunchKernelGGL((k_attn_mixed<T, D, MOD>), dim3(blocks), dim3(64 * kTileWaves), kMixedLds<D>, s, L);
+  } else {
+    hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), (kSmallLds<D, kWaves>), s, L);
+  }
   if (L.n.merge) {
     const uint64_t blocks = L.n.merge_small ? (uint64_t)L.a.b.n_seq * L.n.merge_rows * G
                                             : ((uint64_t)L.a.b.n_rows * L.a.n_head + kWaves - 1) / kWaves;
