@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include "paged_device.h"
+#include "rlh_device.h"
 #include "serve_check.h"
 
 namespace rlh {
@@ -22,6 +23,10 @@ namespace {
 // bins until 64 values are left, which one wave sorts. The draw runs over the
 // list itself, or over the chunks' kept masses and inside the one chunk that
 // it falls into.
+// A pointer that a called function must know to be of global memory: loads
+// through a generic one are counted with LDS reads, so that each of those
+// waits for every load before it.
+
 constexpr int kMassBits = 42;  // masses in histograms: multiples of 2^-42 of a chunk's largest weight
 constexpr uint64_t kMaxRow = 1ull << 21;
 constexpr uint64_t kMaxRows = 1ull << 21;
@@ -32,6 +37,7 @@ constexpr int kScanThreads = 256;
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr uint32_t kCand = 2048;       // values held in LDS
+constexpr uint32_t kListed = 2560;     // groups read at a time
 constexpr uint32_t kFine = 2048;       // bins of a narrowing step
 constexpr uint32_t kListK = 1024;      // largest top-k that takes the groups' maxima
 
@@ -41,20 +47,21 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   if (!(x > -INFINITY)) return 0u;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+constexpr uint32_t kLeastKey = 0x00800000u, kMostKey = 0xff800000u;  // of the lowest finite value, of infinity
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// 2^y for y <= 0 (0 below 2^-1000, NaN and -infinity): Taylor's polynomial of
-// degree 9 of 2^f, |f| <= 1/2, off by less than 2^-37 (as the last place of
-// 10^11 of the mass, where two tokens' borders lie 10^-6 apart at best).
-// Rounding, scaling and conversion instructions of doubles run at a quarter
-// of the rate of sums and products, so y is rounded by adding 1.5 * 2^52,
-// whose low bits then are the exponent.
-__device__ __forceinline__ double exp2_neg(double y) {
-  const double big = 6755399441055744.0;
-  const double z = y + big;
-  const double f = (y - (z - big)) * 0.6931471805599453;
+constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds, and the sum's low bits are the integer
+
+// 2^y for -1000 <= y <= 0: Taylor's polynomial of degree 9 of 2^f, |f| <= 1/2,
+// off by less than 2^-37 (as the last place of 10^11 of the mass, where two
+// tokens' borders lie 10^-6 apart at best). Rounding, scaling and conversion
+// instructions of doubles run at a quarter of the rate of sums and products,
+// so y is rounded by adding kRound.
+__device__ __forceinline__ double exp2_within(double y) {
+  const double z = y + kRound;
+  const double f = (y - (z - kRound)) * 0.6931471805599453;
   double p = 1.0 / 362880.0;
   p = fma(p, f, 1.0 / 40320.0);
   p = fma(p, f, 1.0 / 5040.0);
@@ -66,8 +73,10 @@ __device__ __forceinline__ double exp2_neg(double y) {
   p = fma(p, f, 1.0);
   p = fma(p, f, 1.0);
   const uint64_t n = __builtin_bit_cast(uint64_t, z) << 52;  // (negative: the sum wraps as it should)
-  return y > -1000.0 ? __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + n) : 0.0;
+  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + n);
 }
+// 0 below 2^-1000, NaN and -infinity.
+__device__ __forceinline__ double exp2_neg(double y) { return y > -1000.0 ? exp2_within(y) : 0.0; }
 
 // exp((x - top) / temperature) with `c` = log2(e) / temperature; 1 at the top
 // itself (so infinite tops share the mass), 0 for what has none.
@@ -75,15 +84,46 @@ __device__ __forceinline__ double weight_of(uint32_t key, uint32_t top_key, doub
   if (key == top_key) return 1.0;
   return key == 0u ? 0.0 : exp2_neg(((double)value_of(key) - top) * c);
 }
+__device__ __noinline__ double weight_called(uint32_t key, uint32_t top_key, double top, double c) {
+  return weight_of(key, top_key, top, c);
+}
 __device__ __forceinline__ uint64_t mass_of(double w) { return (uint64_t)(w * (double)(1ull << kMassBits) + 0.5); }
 
-// Bin of a value below a row's or a chunk's largest (`base`: its edge
-// number): sixteenths of a power of two, from the top.
-__device__ __forceinline__ double edge_of(uint32_t key, double c) { return floor((double)value_of(key) * c * 16.0); }
+// Bins of a histogram: the value's logarithm of its weight, rounded to
+// sixteenths of a power of two and counted from the largest's (`base`) down.
+__device__ __forceinline__ double edge_of(double x16) { return (x16 + kRound) - kRound; }
+__device__ __forceinline__ double edge_of(uint32_t key, double c) { return edge_of((double)value_of(key) * (c * 16.0)); }
 __device__ __forceinline__ uint32_t bin_of(uint32_t key, uint32_t top_key, double base, double c) {
   if (key == top_key) return 0u;
   const double d = base - edge_of(key, c);
   return key != 0u && d < (double)(kBins - 1) ? (uint32_t)d : kBins - 1;
+}
+// Their words: a bin's count from bit 51 on, below it its mass as multiples of
+// 2^-38 of the weight at the bin's middle. A value's weight is 2^(-1/32) to
+// 2^(1/32) of that (at most 2^(1/16) where numbers above 2^51 are rounded), so
+// 4096 of them fit 51 bits, and each is rounded by 2^-39 of itself, however
+// small the bin's weights are.
+constexpr int kBinShift = 51;
+constexpr uint64_t kBinMask = (1ull << kBinShift) - 1;
+constexpr double kBinUnit = 0x1p-38;
+// 2^(f / 16) for |f| <= 1/2 in those units: Taylor's polynomial of degree 5,
+// off by less than 2^-42.
+__device__ __forceinline__ uint64_t bin_word(double f) {
+  constexpr double g = 0.6931471805599453 / 16.0;
+  double p = g * g * g * g * g / 120.0;
+  p = fma(p, f, g * g * g * g / 24.0);
+  p = fma(p, f, g * g * g / 6.0);
+  p = fma(p, f, g * g / 2.0);
+  p = fma(p, f, g);
+  p = fma(p, f, 1.0);
+  // (the low bits of a sum with 2^52 are the rounded integer)
+  return (__builtin_bit_cast(uint64_t, fma(p, 1.0 / kBinUnit, 0x1p52)) & kBinMask) | 1ull << kBinShift;
+}
+
+// A unit of bin b's mass, as a share of the top's weight.
+__device__ __forceinline__ double bin_weight(uint32_t b, double base, double top, double c) {
+  if (!(top < INFINITY)) return b == 0 ? kBinUnit : 0.0;
+  return exp2_neg(((base - (double)b) - top * (c * 16.0)) * (1.0 / 16.0)) * kBinUnit;
 }
 
 // What a row's options ask for.
@@ -109,7 +149,6 @@ struct RowSpace {
   uint32_t* group;   // [groups]
   uint32_t* top;     // [chunks]
   double* mass;      // [chunks]
-  uint32_t* count;   // [chunks][kBins]
   uint64_t* bin;     // [chunks][kBins]
 };
 struct Space {
@@ -121,8 +160,7 @@ struct Space {
     RowSpace s;
     s.bin = (uint64_t*)p;
     s.mass = (double*)(p + (uint64_t)chunks * kBins * 8);
-    s.count = (uint32_t*)(p + (uint64_t)chunks * (kBins * 8 + 8));
-    s.top = s.count + (uint64_t)chunks * kBins;
+    s.top = (uint32_t*)(p + (uint64_t)chunks * (kBins * 8 + 8));
     s.group = s.top + chunks;
     return s;
   }
@@ -135,10 +173,10 @@ constexpr uint32_t kMaxChunks = (uint32_t)(kMaxRow / kChunk) + 1;
 // in: value v of the lines is value v - shift of the row.
 template <typename T>
 struct Row {
-  const T* x;
+  const RLH_GLOBAL T* x;
   uint32_t n, shift;
   __device__ __forceinline__ Row(const T* logits, uint64_t stride, uint32_t n_, uint32_t r) {
-    x = logits + (size_t)r * stride;
+    x = (const RLH_GLOBAL T*)(logits + (size_t)r * stride);
     n = n_;
     shift = (uint32_t)((uintptr_t)x & 15) / sizeof(T);
   }
@@ -146,26 +184,34 @@ struct Row {
   __device__ __forceinline__ uint32_t key(uint32_t v) const {
     return v >= shift && v < shift + n ? key_of((float)x[v - shift]) : 0u;
   }
-  // the keys of the line at v (a multiple of V): its load, and what of it
-  // lies in the row
+  // the line at v (a multiple of V); NaN where it lies outside of the row
   static constexpr int V = 16 / sizeof(T);
   typedef T Line __attribute__((ext_vector_type(V)));
   __device__ __forceinline__ Line line(uint32_t v) const {
-    Line a{};
+    Line a;
     if (v >= shift && v + V <= shift + n) {
-      a = *(const Line*)(x + ((size_t)v - shift));
+      a = *(const RLH_GLOBAL Line*)(x + ((size_t)v - shift));
     } else {
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (v + i >= shift && v + i < shift + n) a[i] = x[v + i - shift];
+      for (int i = 0; i < V; i++) a[i] = v + i >= shift && v + i < shift + n ? x[v + i - shift] : (T)__builtin_nanf("");
     }
     return a;
   }
-  __device__ __forceinline__ void keys(uint32_t v, const Line& a, uint32_t (&k)[V]) const {
-#pragma unroll
-    for (int i = 0; i < V; i++) k[i] = v + i >= shift && v + i < shift + n ? key_of((float)a[i]) : 0u;
-  }
 };
+
+// The larger of x and of what lane ^ 1, ^ 2, and then the mirrored lane of 8 or
+// 16 hold: after all of them the largest of the lanes.
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float x) {
+  return fmaxf(x, __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(__float_as_uint(x), __float_as_uint(x), CTRL, 0xf, 0xf, false)));
+}
+template <int LANES>
+__device__ __forceinline__ float max_of_lanes(float x) {
+  x = max_dpp<0xb1>(x);   // quad_perm 1, 0, 3, 2
+  x = max_dpp<0x4e>(x);   // quad_perm 2, 3, 0, 1
+  x = max_dpp<0x141>(x);  // row_half_mirror
+  return LANES == 16 ? max_dpp<0x140>(x) : x;  // row_mirror
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, uint32_t n, uint64_t stride,
@@ -173,7 +219,6 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   constexpr int V = 16 / sizeof(T);
   constexpr int N = kChunk / kScanThreads / V;  // lines per thread
   constexpr int kGroupLanes = kGroup / V;
-  __shared__ uint32_t count[kBins];
   __shared__ uint64_t bin[kBins];
   __shared__ uint32_t tops[kScanThreads / 64];
   __shared__ double sums[kScanThreads / 64];
@@ -182,27 +227,21 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   const RowSpace rs = space.row(r);
   const Row<T> row(logits, stride, n, r);
   if (plan.bins) {
-    for (uint32_t i = t; i < kBins; i += kScanThreads) {
-      count[i] = 0;
-      bin[i] = 0;
-    }
+    for (uint32_t i = t; i < kBins; i += kScanThreads) bin[i] = 0;
   }
-  uint32_t k[N][V], top = 0;
   typename Row<T>::Line line[N];
 #pragma unroll
   for (int i = 0; i < N; i++) line[i] = row.line(chunk * kChunk + (i * kScanThreads + t) * V);
-#pragma unroll
-  for (int i = 0; i < N; i++) row.keys(chunk * kChunk + (i * kScanThreads + t) * V, line[i], k[i]);
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < N; i++) {
-    uint32_t m = 0;
+    float m = -INFINITY;  // (NaN is not larger)
 #pragma unroll
-    for (int e = 0; e < V; e++) m = max(m, k[i][e]);
-#pragma unroll
-    for (int d = 1; d < kGroupLanes; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+    for (int e = 0; e < V; e++) m = fmaxf(m, (float)line[i][e]);
+    const uint32_t km = key_of(max_of_lanes<kGroupLanes>(m));
     const uint32_t g = (chunk * kChunk + (i * kScanThreads + t) * V) / kGroup;
-    if (t % kGroupLanes == 0 && g < space.groups) rs.group[g] = m;
-    top = max(top, m);
+    if (t % kGroupLanes == 0 && g < space.groups) rs.group[g] = km;
+    top = max(top, km);
   }
 #pragma unroll
   for (int d = kGroupLanes; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
@@ -214,23 +253,39 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   if (!plan.mass) return;
   const double tv = (double)value_of(top), base = edge_of(top, plan.c);
   double sum = 0.0;
-  if (top != 0u) {
-    // an infinite top's own weight is 1, what lies below has none
-    const double tf = tv < INFINITY ? tv : 0x1p1000;
+  if (top != 0u && plan.bins) {
+    const double c16 = plan.c * 16.0;
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const uint32_t ke = k[i][e];
-        // (key 0 is the value of a NaN)
-        double w = exp2_neg(((double)value_of(ke) - tf) * plan.c);
-        if (!(tv < INFINITY)) w = ke == top ? 1.0 : 0.0;
+        const float x = (float)line[i][e];
+        const double x16 = (double)x * c16, edge = edge_of(x16), d = base - edge;
+        if (d < (double)(kBins - 1))  // (not for NaN, and not for an infinite top)
+          atomicAdd((unsigned long long*)&bin[(uint32_t)__builtin_bit_cast(uint64_t, d + kRound)],
+                    (unsigned long long)bin_word(x16 - edge));
+        else if (x == (float)tv)
+          atomicAdd((unsigned long long*)&bin[0], (unsigned long long)bin_word(0.0));
+        else if (x > -INFINITY)  // 2^-39 of the top's weight or less
+          sum += weight_called(key_of(x), top, tv, plan.c);
+      }
+    __syncthreads();
+    for (uint32_t i = t; i < kBins; i += kScanThreads) {
+      const uint64_t x = bin[i];
+      rs.bin[(uint64_t)chunk * kBins + i] = x;
+      sum += bin_weight(i, base, tv, plan.c) * (double)(x & kBinMask);
+    }
+  } else if (top != 0u) {
+    // an infinite top's own weight is 1, what lies below has none
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float x = (float)line[i][e];
+        // (what has no weight is given 2^-1000 of the top's, which no sum holds)
+        double w = exp2_within(fmax(((double)x - tv) * plan.c, -1000.0));
+        if (!(tv < INFINITY)) w = x == (float)tv ? 1.0 : 0.0;
         sum += w;
-        if (plan.bins && ke != 0u) {
-          const uint32_t b = bin_of(ke, top, base, plan.c);
-          atomicAdd(&count[b], 1u);
-          atomicAdd((unsigned long long*)&bin[b], (unsigned long long)mass_of(w));
-        }
       }
   }
 #pragma unroll
@@ -238,11 +293,6 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   if ((t & 63) == 0) sums[t >> 6] = sum;
   __syncthreads();
   if (t == 0) rs.mass[chunk] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  if (plan.bins)
-    for (uint32_t i = t; i < kBins; i += kScanThreads) {
-      rs.count[(uint64_t)chunk * kBins + i] = count[i];
-      rs.bin[(uint64_t)chunk * kBins + i] = bin[i];
-    }
 }
 
 // ---- block-wide sums ------------------------------------------------------------------
@@ -290,14 +340,21 @@ struct PickShared {
   uint32_t index[kCand];
   union {
     struct {
-      uint32_t list[kCand];   // groups that are read
-      uint64_t bits[kCand];   // which of their values; later the values that are left
+      uint64_t bits[kListed];  // which of the listed groups' values; later the values that are left
+      uint16_t list[kListed];  // groups that are read, from the round's first
     };
     struct {
       uint32_t count[kFine];
       uint64_t mass[kFine];
     } fine;
-    double kept[kMaxChunks];
+    struct {
+      double kept[kMaxChunks];
+      double weight[kBins];           // of a unit of a bin's mass
+      uint32_t first[kMaxChunks + 1];  // of a chunk's values in key / index
+      uint32_t off[kMaxChunks];       // of a chunk's bins from the row's
+      uint64_t units[kThreads / 2];
+      uint32_t count[kThreads / 2];
+    };
   };
   uint32_t group[kCached];
   double factor[kMaxChunks];  // of a chunk's weights; its largest key, its mass
@@ -310,8 +367,8 @@ struct PickShared {
 
 // The largest key of group g.
 struct Groups {
-  const uint32_t* cached;
-  const uint32_t* all;
+  const RLH_LDS uint32_t* cached;
+  const RLH_GLOBAL uint32_t* all;
   __device__ __forceinline__ uint32_t operator()(uint32_t g) const { return g < kCached ? cached[g] : all[g]; }
 };
 
@@ -337,10 +394,6 @@ __device__ __noinline__ Scan<T> block_scan(T x, PickShared* sh) {
     sum += v[i];
   }
   return Scan<T>{off + x, sum};
-}
-
-__device__ __noinline__ double weight_called(uint32_t key, uint32_t top_key, double top, double c) {
-  return weight_of(key, top_key, top, c);
 }
 
 // The least key of [lo, hi] for which ok() holds (it does for hi, and for
@@ -373,6 +426,27 @@ __device__ __forceinline__ bool kept(const Border& b, uint32_t key, uint32_t ind
   return key > b.key || (key == b.key && index <= b.index);
 }
 
+// f(place, value) for the row's places [from, to) (from: a multiple of 8), by
+// `threads` threads of which this is number `mine`; four loads at a time.
+template <typename T, typename F>
+__device__ __forceinline__ void visit_lines(const Row<T>& row, uint32_t from, uint32_t to, uint32_t mine, uint32_t threads,
+                                            F f) {
+  constexpr uint32_t V = Row<T>::V;
+#pragma unroll 1
+  for (uint32_t v0 = from + mine * V; v0 < to; v0 += 4 * threads * V) {
+    typename Row<T>::Line line[4];
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) line[q] = row.line(v0 + q * threads * V);
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) {
+      const uint32_t v = v0 + q * threads * V;
+#pragma unroll
+      for (uint32_t e = 0; e < V; e++)
+        if (v < to) f(v + e, (float)line[q][e]);
+    }
+  }
+}
+
 // What ends the kept tokens, and what is known of the keys above a range.
 struct Goal {
   uint32_t k;        // values (2^32 - 1: no bound)
@@ -387,10 +461,11 @@ struct Range {
   double above_p;
 };
 
-// Narrows the range to one of its 2048 parts by the counts and masses of
-// get(0 .. n - 1); false if none of the three bounds ends within it.
+// Narrows the range to one of its 2048 parts by the counts and masses of the
+// keys that visit(f) calls f with; false if none of the three bounds ends
+// within it.
 template <typename F>
-__device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goal, uint32_t n, F get) {
+__device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goal, F visit) {
   const uint32_t t = threadIdx.x, width = r.hi - r.lo;
   const int shift = width < kFine ? 0 : 21 - __builtin_clz(width);
   constexpr uint32_t kPer = kFine / kThreads;
@@ -401,16 +476,14 @@ __device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goa
   }
   if (t == 0) sh.where[0] = 0xffffffffu;
   __syncthreads();
-#pragma unroll 2
-  for (uint32_t i = t; i < n; i += kThreads) {
-    const uint32_t k = get(i);
-    if (k < r.lo || k > r.hi) continue;
+  visit([&](uint32_t k) {
+    if (k < r.lo || k > r.hi) return;
     const uint32_t b = (k - r.lo) >> shift;
     atomicAdd(&sh.fine.count[b], 1u);
     if (goal.p < INFINITY)
       atomicAdd((unsigned long long*)&sh.fine.mass[b],
                 (unsigned long long)mass_of(weight_called(k, goal.top_key, goal.top, goal.c)));
-  }
+  });
   __syncthreads();
   // each thread's parts, from the top
   uint32_t ck = 0;
@@ -474,13 +547,17 @@ __device__ __forceinline__ uint32_t kept_equal(const Range& r, const Goal& goal,
 template <typename T>
 __device__ __forceinline__ bool gather(PickShared& sh, const Row<T>& row, const Groups& group, uint32_t groups,
                                        uint32_t lo, uint32_t hi, uint32_t* count) {
-  constexpr int V = 16 / sizeof(T);
-  constexpr int kLanes = kGroup / V, kPer = 64 / kLanes;  // lanes of a group, groups of a wave
+  constexpr uint32_t V = Row<T>::V;
+  constexpr uint32_t kLanes = kGroup / V;  // of a group; a wave takes V groups
+  constexpr uint64_t kEach = ~0ull / ((1ull << kLanes) - 1);  // a lane's bits
+  // the range as values (the keys of -infinity and NaN are below lo)
+  const float least = value_of(max(lo, kLeastKey)), most = value_of(min(hi, kMostKey));
+  const uint32_t outside = row.lines() + V;  // of the row (a place that no line has)
   const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
   uint32_t found = 0;
   // rounds of neighbouring groups, eight per thread if the list holds those
-  // that reach lo, else four
-  uint32_t per = 2 * kCand / kThreads;
+  // that reach lo, else five
+  uint32_t per = 8;
 #pragma unroll 1
   for (uint32_t g0 = 0; g0 < groups;) {
     const uint32_t first = g0 + t * per;
@@ -489,48 +566,73 @@ __device__ __forceinline__ bool gather(PickShared& sh, const Row<T>& row, const 
     const Scan<uint32_t> places = block_scan<uint32_t>((uint32_t)__popc(yes), &sh);
     uint32_t at = places.upto - (uint32_t)__popc(yes);
     const uint32_t listed = places.all;
-    if (listed > kCand) {  // (not with four: those are kCand at most)
-      per = kCand / kThreads;
+    if (listed > kListed) {  // (not with five: those are kListed at most)
+      per = kListed / kThreads;
       continue;
     }
-    for (; yes; yes &= yes - 1, at++) sh.list[at] = first + (uint32_t)__builtin_ctz(yes);
-    g0 += per * kThreads;
+    for (; yes; yes &= yes - 1, at++) sh.list[at] = (uint16_t)(first - g0 + (uint32_t)__builtin_ctz(yes));
     __syncthreads();
-    // which values of each group: a bit per value; four groups' loads at a time
-    constexpr uint32_t kBatch = 4;
+    // which values of each group, 16 groups' loads at a time. A wave's V
+    // groups leave V words: word e has value e of each lane
+    constexpr uint32_t kBatch = 16;
 #pragma unroll 1
-    for (uint32_t i0 = wave * kPer; i0 < listed; i0 += kBatch * kWaves * kPer) {
+    for (uint32_t i0 = wave * V; i0 < listed; i0 += kBatch * kWaves * V) {
       typename Row<T>::Line line[kBatch];
-      uint32_t v[kBatch];
 #pragma unroll
       for (uint32_t q = 0; q < kBatch; q++) {
-        const uint32_t i = i0 + q * kWaves * kPer + lane / kLanes;
-        v[q] = i < listed ? sh.list[i] * kGroup + lane % kLanes * V : 0u;
-        line[q] = row.line(v[q]);
+        if (i0 + q * kWaves * V >= listed) break;
+        const uint32_t i = i0 + q * kWaves * V + lane / kLanes;
+        line[q] = row.line(i < listed ? (g0 + sh.list[i]) * kGroup + lane % kLanes * V : outside);
       }
 #pragma unroll
       for (uint32_t q = 0; q < kBatch; q++) {
-        const uint32_t i = i0 + q * kWaves * kPer + lane / kLanes;
-        uint32_t k[V], b = 0;
-        row.keys(v[q], line[q], k);
+        if (i0 + q * kWaves * V >= listed) break;
+        uint64_t word = 0;
 #pragma unroll
-        for (int e = 0; e < V; e++) b |= (k[e] >= lo && k[e] <= hi ? 1u : 0u) << e;
-        uint64_t bits = (uint64_t)b << (lane % kLanes * V);
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1) bits |= __shfl_xor((unsigned long long)bits, d);
-        if (i < listed && lane % kLanes == 0) sh.bits[i] = bits;
+        for (uint32_t e = 0; e < V; e++) {
+          const float x = (float)line[q][e];
+          const uint64_t in = __ballot(x >= least && x <= most);
+          word = lane == e ? in : word;
+        }
+        const uint32_t i = i0 + q * kWaves * V + lane;
+        if (lane < V) sh.bits[i] = word;
       }
     }
     __syncthreads();
-    // the places of their values: four neighbours per thread
+    // the places of their values: five neighbours per thread
+    auto values_of = [&](uint32_t i) {  // bit e * kLanes + lane
+      uint64_t x = 0;
+#pragma unroll
+      for (uint32_t e = 0; e < V; e++)
+        x |= (sh.bits[i / V * V + e] >> (i % V * kLanes) & ((1ull << kLanes) - 1)) << (e * kLanes);
+      return x;
+    };
     uint32_t n = 0;
-    const uint32_t l0 = t * (kCand / kThreads);
-    for (uint32_t j = 0; j < kCand / kThreads; j++) n += l0 + j < listed ? (uint32_t)__popcll(sh.bits[l0 + j]) : 0u;
+    uint64_t own[kListed / kThreads];
+    const uint32_t l0 = t * (kListed / kThreads);
+#pragma unroll
+    for (uint32_t j = 0; j < kListed / kThreads; j++) {
+      own[j] = l0 + j < listed ? values_of(l0 + j) : 0ull;
+      n += (uint32_t)__popcll(own[j]);
+    }
     const Scan<uint32_t> values = block_scan<uint32_t>(n, &sh);
     uint32_t to = found + values.upto - n;
-    for (uint32_t j = 0; j < kCand / kThreads && l0 + j < listed; j++)
-      for (uint64_t left = sh.bits[l0 + j]; left; left &= left - 1, to++)
-        if (to < kCand) sh.index[to] = sh.list[l0 + j] * kGroup + (uint32_t)__builtin_ctzll(left);
+#pragma unroll
+    for (uint32_t j = 0; j < kListed / kThreads; j++) {
+      uint64_t left = own[j];
+#pragma unroll 1
+      while (left) {  // the lanes in order, of each its values
+        uint64_t any = left;
+#pragma unroll
+        for (uint32_t e = kLanes; e < 64; e <<= 1) any |= any >> e;
+        const uint32_t l = (uint32_t)__builtin_ctzll(any);
+        uint64_t of_lane = left >> l & kEach;
+        left &= ~(kEach << l);
+        for (; of_lane; of_lane &= of_lane - 1, to++)
+          if (to < kCand) sh.index[to] = (g0 + sh.list[l0 + j]) * kGroup + l * V + (uint32_t)__builtin_ctzll(of_lane) / kLanes;
+      }
+    }
+    g0 += per * kThreads;
     found += values.all;
     __syncthreads();
     if (found > kCand) return false;
@@ -563,7 +665,7 @@ __device__ __noinline__ uint32_t nth_equal(PickShared* sh, const Row<T> row, uin
 // range, else 2^32 - 1.
 template <typename T>
 __device__ __noinline__ Border find_border(PickShared* shp, const Row<T> row, const Groups group, uint32_t groups,
-                                           Range r, const Goal& goal, uint32_t* gathered) {
+                                           Range r, const Goal goal, uint32_t* gathered) {
   PickShared& sh = *shp;
   const uint32_t t = threadIdx.x, lane = t & 63;
   uint32_t m = 0;
@@ -579,7 +681,12 @@ __device__ __noinline__ Border find_border(PickShared* shp, const Row<T> row, co
       *gathered = 0xffffffffu;
       return n ? Border{r.lo, nth_equal(shp, row, r.lo, n)} : Border{r.lo + 1, 0xffffffffu};
     }
-    if (!narrow(sh, r, goal, row.lines(), [&](uint32_t v) { return row.key(v); })) {
+    const float least = value_of(max(r.lo, kLeastKey)), most = value_of(min(r.hi, kMostKey));
+    if (!narrow(sh, r, goal, [&](auto f) {
+          visit_lines(row, 0u, row.lines(), t, (uint32_t)kThreads, [&](uint32_t, float x) {
+            if (x >= least && x <= most) f(key_of(x));
+          });
+        })) {
       *gathered = 0xffffffffu;
       return Border{r.lo, 0xffffffffu};
     }
@@ -587,7 +694,9 @@ __device__ __noinline__ Border find_border(PickShared* shp, const Row<T> row, co
   *gathered = whole ? m : 0xffffffffu;
   if (m > 64) {
     while (r.lo != r.hi) {
-      if (!narrow(sh, r, goal, m, [&](uint32_t i) { return sh.key[i]; })) return Border{r.lo, 0xffffffffu};
+      if (!narrow(sh, r, goal, [&](auto f) {
+            for (uint32_t i = t; i < m; i += kThreads) f(sh.key[i]);
+          })) return Border{r.lo, 0xffffffffu};
       uint32_t in = 0;
       for (uint32_t i = t; i < m; i += kThreads) in += sh.key[i] >= r.lo && sh.key[i] <= r.hi ? 1u : 0u;
       if (block_scan<uint32_t>(in, shp).all <= 64) break;
@@ -611,15 +720,15 @@ __device__ __noinline__ Border find_border(PickShared* shp, const Row<T> row, co
     return n ? Border{r.lo, ~(uint32_t)sh.bits[n - 1]} : Border{r.lo + 1, 0xffffffffu};
   }
   if (t < 64) {
-    uint64_t k = lane < left ? sh.bits[lane] : 0ull;
-#pragma unroll 1
-    for (uint32_t size = 2; size <= 64; size <<= 1)
-#pragma unroll 1
-      for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-        const uint64_t o = __shfl_xor((unsigned long long)k, (int)stride);
-        const bool larger = ((lane & size) == 0) == ((lane & stride) == 0);
-        k = (k > o) == larger ? k : o;
-      }
+    // each by the number of larger ones (no two are equal)
+    const uint64_t own = lane < left ? sh.bits[lane] : 0ull;
+    uint32_t rank = 0;
+#pragma unroll 8
+    for (uint32_t i = 0; i < left; i++) rank += sh.bits[i] > own ? 1u : 0u;
+    if (lane < left) sh.bits[64 + rank] = own;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t k = lane < left ? sh.bits[64 + lane] : 0ull;
     const uint32_t key = (uint32_t)(k >> 32);
     const double w = lane < left ? weight_called(key, goal.top_key, goal.top, goal.c) : 0.0;
     const double before = r.above_p + (wave_scan(w) - w);
@@ -665,7 +774,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
   }
 #pragma unroll
   for (uint32_t j = 0; j < kCached / kThreads; j++) sh.group[j * kThreads + t] = g[j];
-  const Groups group{sh.group, rs.group};
+  const Groups group{(const RLH_LDS uint32_t*)sh.group, (const RLH_GLOBAL uint32_t*)rs.group};
   const RowPlan plan = row_plan(o, n);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top_key = max(top_key, (uint32_t)__shfl_xor((int)top_key, d));
@@ -729,76 +838,76 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
     for (int i = 0; i < kWaves; i++) least = min(least, tops[i]);
     Range range{least, top_key, 0u, 0.0};
     const Goal by_count{o.top_k, INFINITY, 0u, top_key, top, c};
-    const bool enough = narrow(sh, range, by_count, groups, [&](uint32_t i) { return group(i); });
+    const bool enough = narrow(sh, range, by_count, [&](auto f) {
+      for (uint32_t i = t; i < groups; i += kThreads) f(group(i));
+    });
     range = Range{enough ? range.lo : 1u, 0xffffffffu, 0u, 0.0};
     border = find_border(&sh, row, group, groups, range, goal, &m);
   } else if (plan.bins) {
-    // the row's histogram, one bin per thread, chunk after chunk
-    for (uint32_t i = t; i < chunks; i += kThreads) sh.list[i] = sh.top[i] ? bin_of(sh.top[i], top_key, base, c) : kBins;
-    if (t == 0) sh.where[0] = kBins - 1;
+    // the row's histogram, 16 powers of two at a time until one of the three
+    // bounds ends: a bin per thread, half of the chunks for each half of the
+    // block. (One block reads 31 GB/s whatever it asks for at once, so it asks
+    // for little: all 640 bins of 38 chunks took 10 us.) The row's bins lie
+    // off[chunk] before the chunk's.
+    for (uint32_t i = t; i < chunks; i += kThreads) sh.off[i] = sh.top[i] ? bin_of(sh.top[i], top_key, base, c) : kBins;
+    if (t == 0) sh.where[0] = 0xffffffffu;
     __syncthreads();
-    constexpr uint32_t kEach = (kBins + kThreads - 1) / kThreads;  // neighbouring bins
-    uint32_t cnt[kEach] = {};
-    double mass[kEach] = {};
-#pragma unroll 4
-    for (uint32_t ch = 0; ch < chunks; ch++) {
-      const uint32_t off = sh.list[ch];
-      const double f = sh.factor[ch] * (1.0 / (double)(1ull << kMassBits));
-#pragma unroll
-      for (uint32_t j = 0; j < kEach; j++) {
-        // (bin 0 is read and not used where the chunk has none)
-        const uint32_t b = t * kEach + j;
-        const bool in = b >= off && b < kBins - 1;
-        const uint64_t at = (uint64_t)ch * kBins + (in ? b - off : 0u);
-        const uint32_t n1 = rs.count[at];
-        const double m1 = (double)rs.bin[at];
-        cnt[j] += in ? n1 : 0u;
-        mass[j] += in ? f * m1 : 0.0;
-      }
-    }
-    uint32_t sum_k = 0;
-    double sum_p = 0.0;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; j++) {
-      sum_k += cnt[j];
-      sum_p += mass[j];
-    }
-    uint32_t upto_k = block_scan<uint32_t>(sum_k, &sh).upto - sum_k;
-    double upto_p = block_scan<double>(sum_p, &sh).upto - sum_p;
-    // the first bin at which one of the three ends
+    constexpr uint32_t kHalf = kThreads / 2;
     const uint32_t min_bin = goal.min_key == 0u ? kBins : bin_of(min(goal.min_key, top_key), top_key, base, c);
-    const uint32_t before_k = upto_k;
-    const double before_p = upto_p;
-    uint32_t mine = kBins;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; j++) {
-      const uint32_t b = t * kEach + j;
-      upto_k += cnt[j];
-      upto_p += mass[j];
-      if (mine == kBins && b < kBins - 1 && ((plan.by_k && upto_k >= o.top_k) || (plan.by_p && upto_p >= goal.p) || b >= min_bin)) mine = b;
-    }
-    const uint64_t ends = __ballot(mine < kBins);
-    if (ends && (int)lane == __builtin_ctzll(ends)) atomicMin(&sh.where[0], mine);
-    __syncthreads();
-    border_bin = sh.where[0];
-    __syncthreads();
-    if (border_bin < kBins - 1) {
-      if (border_bin / kEach == t) {
-        uint32_t k = before_k;
-        double p = before_p;
-#pragma unroll
-        for (uint32_t j = 0; j < kEach; j++)
-          if (t * kEach + j < border_bin) {
-            k += cnt[j];
-            p += mass[j];
-          }
-        sh.where[1] = k;
-        sh.before = __builtin_bit_cast(uint64_t, p);
+    uint32_t above_k = 0;
+    double above_p = 0.0;
+#pragma unroll 1
+    for (uint32_t b0 = 0; b0 < kBins - 1; b0 += kHalf) {
+      const uint32_t b = b0 + t % kHalf;
+      uint32_t cnt = 0;
+      uint64_t units = 0;  // (2^21 values of up to 2^38.1: below 2^60)
+#pragma unroll 8
+      for (uint32_t ch = t / kHalf; ch < chunks; ch += 2) {
+        // (bin 0 is read and not used where the chunk has none)
+        const uint32_t off = sh.off[ch];
+        const bool in = b >= off && b < kBins - 1;
+        const uint64_t x = rs.bin[(uint64_t)ch * kBins + (in ? b - off : 0u)];
+        cnt += in ? (uint32_t)(x >> kBinShift) : 0u;
+        units += in ? x & kBinMask : 0ull;
       }
+      if (t >= kHalf) {
+        sh.units[t - kHalf] = units;
+        sh.count[t - kHalf] = cnt;
+        cnt = 0;
+        units = 0;
+      }
+      __syncthreads();
+      if (t < kHalf) {
+        units += sh.units[t];
+        cnt += sh.count[t];
+      }
+      const double mass = t < kHalf ? (double)units * bin_weight(b, base, top, c) : 0.0;
+      const Scan<uint32_t> sum_k = block_scan<uint32_t>(cnt, &sh);
+      const Scan<double> sum_p = block_scan<double>(mass, &sh);
+      // the first bin at which one of the three ends
+      const bool ends = t < kHalf && b < kBins - 1 &&
+                        ((plan.by_k && above_k + sum_k.upto >= o.top_k) || (plan.by_p && above_p + sum_p.upto >= goal.p) || b >= min_bin);
+      const uint64_t any = __ballot(ends);
+      if (any && (int)lane == __builtin_ctzll(any)) atomicMin(&sh.where[0], b);
+      __syncthreads();
+      border_bin = sh.where[0];
+      if (t < kHalf && b == border_bin) {
+        sh.where[1] = above_k + sum_k.upto - cnt;
+        sh.before = __builtin_bit_cast(uint64_t, above_p + (sum_p.upto - mass));
+      }
+      if (border_bin != 0xffffffffu) break;
+      above_k += sum_k.all;
+      above_p += sum_p.all;
+    }
+    if (border_bin < kBins - 1) {
       // the bin's keys: bins fall as keys rise
       auto from_bin = [&](uint32_t b) { return least_key(1, top_key, [&](uint32_t k) { return bin_of(k, top_key, base, c) <= b; }); };
-      const uint32_t lo = from_bin(border_bin), hi = border_bin == 0 ? top_key : from_bin(border_bin - 1) - 1;
+      // the first half of the waves looks for the bin's end, the others for the next one's
+      const bool low = wave < kWaves / 2;
+      const uint32_t edge = low || border_bin > 0 ? from_bin(low ? border_bin : border_bin - 1) : top_key + 1;
+      if (lane == 0 && wave % (kWaves / 2) == 0) sh.where[low ? 2 : 3] = edge;
       __syncthreads();
+      const uint32_t lo = sh.where[2], hi = sh.where[3] - 1;
       const Range range{lo, hi, sh.where[1], __builtin_bit_cast(double, sh.before)};
       border = find_border(&sh, row, group, groups, range, goal, &m);
     } else {
@@ -816,29 +925,45 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
     if (border.key == 0u) {
       for (uint32_t q = t; q < chunks; q += kThreads) sh.kept[q] = sh.top[q] ? sh.factor[q] * sh.mass[q] : 0.0;
     } else {
+      const float least = value_of(max(border.key, kLeastKey));
+      const bool by_bins = border_bin < kBins && m != 0xffffffffu;
+      if (by_bins) {
+        // where each chunk's values begin in the list
+        for (uint32_t i = t; i <= m; i += kThreads) {
+          const uint32_t upto = i < m ? sh.index[i] / kChunk : chunks;
+          for (uint32_t q = i ? sh.index[i - 1] / kChunk + 1 : 0u; q <= upto; q++) sh.first[q] = i;
+        }
+        for (uint32_t i = t; i < kBins; i += kThreads) sh.weight[i] = bin_weight(i, base, top, c);
+        for (uint32_t i = t; i < chunks; i += kThreads) sh.off[i] = sh.top[i] ? bin_of(sh.top[i], top_key, base, c) : kBins;
+        __syncthreads();
+      }
 #pragma unroll 1
       for (uint32_t q = wave; q < chunks; q += kWaves) {
         const uint32_t ck = sh.top[q];
         double s = 0.0;
         if (ck != 0u && ck >= border.key) {
-          if (border_bin < kBins && m != 0xffffffffu) {
+          if (by_bins) {
             // the bins above the border's, and what is kept of that one
-            const uint32_t off = bin_of(ck, top_key, base, c);
+            const uint32_t off = sh.off[q];
+#pragma unroll 1
+            for (uint32_t i0 = 0; off + i0 < border_bin; i0 += kBins / 2) {
+              uint64_t x[kBins / 128];
 #pragma unroll
-            for (uint32_t j = 0; j < kBins / 64; j++) {
-              const uint32_t i = j * 64 + lane;
-              const double x = (double)rs.bin[(uint64_t)q * kBins + i];
-              s += off + i < border_bin ? x : 0.0;
+              for (uint32_t j = 0; j < kBins / 128; j++) x[j] = rs.bin[(uint64_t)q * kBins + i0 + j * 64 + lane];
+#pragma unroll
+              for (uint32_t j = 0; j < kBins / 128; j++) {
+                const uint32_t b = off + i0 + j * 64 + lane;
+                if (b < border_bin) s += sh.weight[b] * (double)(x[j] & kBinMask);
+              }
             }
-            s *= sh.factor[q] * (1.0 / (double)(1ull << kMassBits));
-            for (uint32_t i = lane; i < m; i += 64)
-              if (sh.index[i] / kChunk == q && kept(border, sh.key[i], sh.index[i])) s += weight_called(sh.key[i], top_key, top, c);
+            for (uint32_t i = sh.first[q] + lane; i < sh.first[q + 1]; i += 64)
+              if (kept(border, sh.key[i], sh.index[i])) s += weight_called(sh.key[i], top_key, top, c);
           } else {
-#pragma unroll 4
-            for (uint32_t i = lane; i < kChunk; i += 64) {
-              const uint32_t v = q * kChunk + i, k = row.key(v);
-              if (k != 0u && kept(border, k, v)) s += weight_of(k, top_key, top, c);
-            }
+            visit_lines(row, q * kChunk, (q + 1) * kChunk, lane, 64u, [&](uint32_t v, float x) {
+              if (!(x >= least)) return;
+              const uint32_t k = key_of(x);
+              if (kept(border, k, v)) s += weight_called(k, top_key, top, c);
+            });
           }
         }
         s = wave_scan(s);
@@ -891,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
 #pragma unroll
     for (uint32_t j = 0; j < kPer / V; j++) line[j] = row.line(ch * kChunk + t * kPer + j * V);
 #pragma unroll
-    for (uint32_t j = 0; j < kPer / V; j++) row.keys(ch * kChunk + t * kPer + j * V, line[j], *(uint32_t(*)[V])(k + j * V));
+    for (uint32_t j = 0; j < kPer; j++) k[j] = key_of((float)line[j / V][j % V]);
 #pragma unroll
     for (uint32_t j = 0; j < kPer; j++) at[j] = ch * kChunk + t * kPer + j;
   }
@@ -925,7 +1050,7 @@ Space sample_space(void* base, uint64_t n) {
   // a row may begin up to 7 values into its first line
   s.chunks = (uint32_t)((n + 7 + kChunk - 1) / kChunk);
   s.groups = (uint32_t)((n + 7 + kGroup - 1) / kGroup);
-  s.row_bytes = ((uint64_t)s.chunks * (kBins * 12 + 12) + (uint64_t)s.groups * 4 + 255) / 256 * 256;
+  s.row_bytes = ((uint64_t)s.chunks * (kBins * 8 + 12) + (uint64_t)s.groups * 4 + 255) / 256 * 256;
   return s;
 }
 
