@@ -135,10 +135,12 @@ struct Scoring {
   bool capped, biased;
 };
 
+// tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
+__device__ __forceinline__ float capped(const Scoring& c, float dot) {
+  return fmaf(-2.0f * c.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * c.mul) + 1.0f), c.cap2);
+}
 __device__ __forceinline__ float score(const Scoring& c, float dot, float slope2, float away) {
-  float x = dot * c.mul;
-  // tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
-  if (c.capped) x = c.cap2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f));
+  const float x = c.capped ? capped(c, dot) : dot * c.mul;
   return c.biased ? fmaf(slope2, away, x) : x;
 }
 
@@ -321,7 +323,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   const RowSpan span = row_span(pos, sq.v.kv_len, a.window, sq.prefix);
   const RowSpan span0 = row_span(sq.p0, sq.v.kv_len, a.window, sq.prefix);
   const RowSpan span1 = row_span((int32_t)sq.v.kv_len - 1, sq.v.kv_len, a.window, sq.prefix);
-  const float slope2 = MOD && L.sc.biased ? a.slopes[head] * kLog2e : 0.0f;
+  const float slope2 = MOD && a.slopes ? a.slopes[head] * kLog2e : 0.0f;
   vec8<T> q[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; i++) {
@@ -664,7 +666,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   const uint32_t n_steps = t_hi > t_lo ? (uint32_t)(t_hi - t_lo + kTileKv - 1) / kTileKv : 0;
   const uint32_t st0 = (uint32_t)((uint64_t)n_steps * part / parts), st1 = (uint32_t)((uint64_t)n_steps * (part + 1) / parts);
 
-  const float slope2 = MOD && L.sc.biased && active ? a.slopes[head] * kLog2e : 0.0f;
+  const float slope2 = MOD && a.slopes && active ? a.slopes[head] * kLog2e : 0.0f;
   vec8<T> q[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; i++) {
@@ -798,10 +800,22 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
       // that 32 of them are not kept in registers from step to step)
       int32_t j0 = p + (int32_t)half * 4;
       asm volatile("" : "+v"(j0));
+      float far = 0.0f;  // what all of the row's scores lack
       if constexpr (MOD) {
-        const float away = (float)(j0 - pos);
+        if (L.sc.capped) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) sc[i / 16][i % 16] = score(L.sc, sc[i / 16][i % 16], slope2, away + (float)(i / 4 * 8 + i % 4));
+          for (int i = 0; i < 32; i++) sc[i / 16][i % 16] = capped(L.sc, sc[i / 16][i % 16]);
+        }
+        if (L.sc.biased) {
+          // slope * distance = far + near + slope * (0 .. 59): far that of the
+          // step's first position, near the rest up to the lane's first
+          far = slope2 * (float)(p - pos);
+          const float near = fmaf(slope2, (float)(j0 - pos), -far);
+          const float mul1 = L.sc.capped ? 1.0f : L.sc.mul;
+#pragma unroll
+          for (int i = 0; i < 32; i++)
+            sc[i / 16][i % 16] = fmaf(sc[i / 16][i % 16], mul1, fmaf(slope2, (float)(i / 4 * 8 + i % 4), near));
+        }
       }
       if (!full) {
         const int32_t lo = span.lo - j0, hi = span.hi - j0, pre = span.prefix - j0;
@@ -816,7 +830,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
 #pragma unroll
       for (int i = 1; i < 32; i++) top = fmaxf(top, sc[i / 16][i % 16]);
       top = max_across_32(top);
-      if constexpr (!MOD) top *= mul;
+      top = MOD ? top + far : top * mul;
       if (__ballot(top > m + kSlack)) {
         const float mn = fmaxf(m, top);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -825,7 +839,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
         for (int i = 0; i < kOut; i++) o[i] *= f;
         m = mn;
       }
-      const float mb = m == -INFINITY ? 0.0f : m;
+      const float mb = (m == -INFINITY ? 0.0f : m) - far;
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -1218,12 +1232,13 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   L.n = attn_sizes(*kv, *seqs, *args);
   place_workspace(&L.ws, (uint8_t*)workspace, *kv, *seqs, *args, L.n);
   L.sc.capped = args->softcap > 0.0f;
-  L.sc.biased = args->slopes != nullptr;
   const float scale = fabsf(args->scale);
   L.sc.mul = L.sc.capped ? 2.0f * scale / args->softcap * kLog2e : scale * kLog2e;
   L.sc.cap2 = args->softcap * kLog2e;
   L.sc.flip = args->scale < 0.0f ? 0x80008000u : 0u;
-  const bool mod = L.sc.capped || L.sc.biased || !(scale > 0.0f);
+  // (a scale of zero, which the exponential could not take in, goes with a bias of zero)
+  L.sc.biased = args->slopes || (!L.sc.capped && scale == 0.0f);
+  const bool mod = L.sc.capped || L.sc.biased;
   if (kv->type == RLH_TYPE_F16) return launch_attn<_Float16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
   return launch_attn<__bf16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
 }
