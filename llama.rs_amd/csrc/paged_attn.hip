@@ -162,12 +162,18 @@ struct Sizes {
   uint32_t tiles;         // at most, of the tiled kernel (per KV head)
   uint32_t tile_parts;    // parts of the positions of a tile
   uint32_t prefix_tiles;  // tiles over all rows
-  uint32_t prefix_parts;
+  uint32_t prefix_parts;  // of all but the last of them
+  uint32_t last_parts;    // of the last, which may have fewer rows
   uint32_t small_rows;    // sequences of up to so many rows of a KV head go to the small kernel
   bool small, tiled, merge;
   bool merge_small;       // only its sequences have parts to join
   uint32_t merge_rows;    // then: blocks per sequence and KV head
 };
+
+// Blocks of a KV head for the shared prefix.
+__host__ __device__ inline uint32_t prefix_blocks(const Sizes& n) {
+  return n.prefix_tiles ? (n.prefix_tiles - 1) * n.prefix_parts + n.last_parts : 0;
+}
 
 struct Launch {
   AttnParams a;
@@ -550,10 +556,13 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   const AttnParams& a = L.a;
   const uint32_t t = threadIdx.x;
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
-  const uint32_t parts = prefix ? L.n.prefix_parts : L.n.tile_parts;
-  const uint32_t h = block % a.n_kv;
-  const uint32_t part = block / a.n_kv % parts;
-  const uint32_t tile = block / a.n_kv / parts;
+  const uint32_t h = block % a.n_kv, of_head = block / a.n_kv;
+  uint32_t parts = prefix ? L.n.prefix_parts : L.n.tile_parts, tile = of_head / parts, part = of_head % parts;
+  if (prefix && tile >= L.n.prefix_tiles - 1) {
+    tile = L.n.prefix_tiles - 1;
+    part = of_head - tile * parts;
+    parts = L.n.last_parts;
+  }
   // the tile's sequence (own positions), or all rows (the prefix)
   uint32_t s = 0, row0 = 0, rows = 0;
   if (prefix) {
@@ -926,7 +935,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
-  const uint32_t n_prefix = L.n.prefix_tiles * L.n.prefix_parts * L.a.n_kv;
+  const uint32_t n_prefix = prefix_blocks(L.n) * L.a.n_kv;
   const uint32_t n_tiles = n_prefix + L.n.tiles * L.n.tile_parts * L.a.n_kv;
   const uint32_t b = blockIdx.x;
   if (b < n_tiles)
@@ -971,7 +980,10 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
   if (!sv.ok || r >= sv.q_len * a.group) return;
   const bool small = sv.q_len * a.group <= L.n.small_rows;
   if (L.n.merge_small && !small) return;
-  const uint32_t n_prefix = a.shared_len ? L.n.prefix_parts : 0;
+  const uint32_t in_head = row * a.group + head % a.group;  // among all rows of its KV head
+  const uint32_t n_prefix = !a.shared_len                                       ? 0
+                            : in_head / kTileRows + 1 < L.n.prefix_tiles ? L.n.prefix_parts
+                                                                        : L.n.last_parts;
   const uint32_t first = small ? load_uniform(L.ws.plan, 2 * s) : 0;
   const uint32_t n_own = small ? load_uniform(L.ws.plan, 2 * s + 1) : L.n.tile_parts;
   if (n_prefix == 0 && n_own == 1) return;  // written already
@@ -1090,7 +1102,17 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
   }
   if (args.shared_len) {
     n.prefix_tiles = (uint32_t)((rows + kTileRows - 1) / kTileRows);
-    n.prefix_parts = tile_parts((uint64_t)n.prefix_tiles * kv.n_head_kv, args.shared_len);
+    n.prefix_parts = n.last_parts = tile_parts((uint64_t)n.prefix_tiles * kv.n_head_kv, args.shared_len);
+    // A last tile of up to 128 rows has one wave per SIMD, whose steps take
+    // about 0.55 of the time, and is divided into fewer parts (576 rows of a
+    // KV head against 16384 positions: 12, 12 and 8 parts instead of 10 each,
+    // 70 us instead of 75).
+    const uint64_t most = 256 / kv.n_head_kv, last = rows - (uint64_t)(n.prefix_tiles - 1) * kTileRows;
+    const uint64_t p = std::min<uint64_t>(most * 20 / (20 * n.prefix_tiles - 9), args.shared_len / 256);
+    if (n.prefix_tiles > 1 && last <= kTileRows / 2 && p > n.prefix_parts) {
+      n.prefix_parts = (uint32_t)p;
+      n.last_parts = (uint32_t)std::min(p, most - (n.prefix_tiles - 1) * p);
+    }
   }
   const uint32_t step = 32 * (args.shared_len || n.tiled ? kTileWaves : kWaves);  // of the few rows' blocks
   n.merge = args.shared_len || (n.small && own > step) || n.tile_parts > 1;
@@ -1150,7 +1172,7 @@ int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
   if (L.a.shared_len || L.n.tiled) {
     RLH_TRY((allow_mixed_lds<T, D, MOD>(device)));
-    const uint32_t blocks = (L.n.prefix_tiles * L.n.prefix_parts + L.n.tiles * L.n.tile_parts + L.n.items) * G;
+    const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts + L.n.items) * G;
     hipLaunchKernelGGL((k_attn_mixed<T, D, MOD>), dim3(blocks), dim3(64 * kTileWaves), kMixedLds<D>, s, L);
   } else {
     hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), (kSmallLds<D, kWaves>), s, L);

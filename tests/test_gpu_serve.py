@@ -692,3 +692,101 @@ def test_refused_on_the_device():
         assert b"workspace" in lib.rlh_last_error()
     torch.cuda.synchronize()
     assert torch.all(out == 7.0)
+
+
+# ---- divisions of the work, scales, long rows --------------------------------------
+
+ATTN_MORE = {
+    # 320 rows of a KV head: a whole tile and one of 64 rows, divided into fewer parts
+    "shared uneven": dict(seqs=[(4, 4608 + 4 + i) for i in range(20)], heads=32, kv=8, dim=64, page=64, ty=rlh.BF16,
+                          shared=4608),
+    "shared uneven all masks": dict(seqs=[(4, 4608 + 4 + 7 * i) for i in range(20)], heads=32, kv=8, dim=64, page=64,
+                                    ty=rlh.F16, shared=4608, cap=10.0, bias=True, window=2000, prefix=[300 * i for i in range(20)]),
+    # a bias that grows with positions behind a row's own
+    "prefix bias": dict(seqs=[(300, 300), (70, 500), (1, 700)], heads=8, kv=4, dim=128, page=16, ty=rlh.BF16, bias=True,
+                        prefix=[250, 499, 700]),
+    "cap and bias": dict(seqs=[(100, 1100), (1, 1500)], heads=12, kv=4, dim=128, page=32, ty=rlh.F16, bias=True, cap=4.0,
+                         q_scale=4.0),
+    "mixed with drafts": dict(seqs=[(300, 310), (2, 900), (1, 33), (4, 4), (0, 5), (90, 2000)], heads=16, kv=4, dim=64, page=16,
+                              ty=rlh.F16, pad_seqs=2, pad_rows=4),
+}
+
+
+@pytest.mark.parametrize("name", list(ATTN_MORE))
+def test_attention_more(name):
+    case = dict(ATTN_MORE[name])
+    heads = case["heads"]
+    print("attention", name, case, flush=True)
+    b, q, out, opts = attn_case(seed=len(name), **case)
+    st = status_word()
+    run_attn(b, q, out, heads, status=st, **opts)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    check_attn(b, q, out, heads, opts)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.2, 0.3])
+@pytest.mark.parametrize("name", ["decode ragged", "mixed", "cap", "bias", "shared drafts"])
+def test_attention_scales(name, scale):
+    case = dict(ATTN[name])
+    heads = case["heads"]
+    b, q, out, opts = attn_case(seed=13, **case)
+    run_attn(b, q, out, heads, scale=scale, **opts)
+    torch.cuda.synchronize()
+    want, bound = ref.attention(b, q[:, :heads * b.dim].view(-1, heads, b.dim), heads, scale, opts["cap"], opts["slopes"],
+                                opts["window"], opts["prefix"])
+    got = out[:, :heads * b.dim].double().view(-1, heads, b.dim)
+    assert torch.all((got - want).abs()[:b.n_live] <= bound[:b.n_live] + 1e-30)
+
+
+@pytest.mark.parametrize("ty", [rlh.F32, rlh.F16, rlh.BF16])
+@pytest.mark.parametrize("n,shift", [(300001, 0), (300001, 1), (163841, 3), (131072, 0)])
+def test_sample_long_rows(n, shift, ty):
+    """More groups of 64 than are held or listed at a time; rows that begin
+    inside a 16-byte line."""
+    rows = [(1.0, 0, 0.9, 0.0), (20.0, 0, 0.9, 0.0), (1.0, 1000, 0.99, 0.0), (1.5, 20000, 1.0, 0.0), (1.0, 0, 1.0, 1e-4),
+            (1.0, 0, 1.0, 0.0), (0.7, 40, 0.95, 0.0), (0.0, 0, 1.0, 0.0)]
+    g = torch.Generator().manual_seed(n + ty + shift)
+    x = 2.0 * torch.randn((len(rows), n + 9), generator=g)
+    x = x.to(TORCH[ty]).cuda()[:, shift:]
+    u = np.random.default_rng(n + ty).random(len(rows)).astype(np.float32)
+    got = run_sample(x, ty, rows, u, n=n)
+    host = x[:, :n].double().cpu().numpy()
+    for r, opt in enumerate(rows):
+        assert got[r] == ref.sample(host[r], *opt, u[r]), (r, opt, u[r])
+
+
+def test_sample_long_ties():
+    """Many more equal values than are held, over all groups, and a border in
+    the middle of them."""
+    n = 200003
+    xs, rows, us = [], [], []
+    for opt in [(1.0, 1000, 1.0, 0.0), (1.0, 0, 0.37, 0.0), (1.0, 150000, 0.5, 0.0), (1.0, 0, 1.0, 1.0), (0.5, 700, 0.8, 0.5),
+                (1.0, 0, 1.0, 0.0)]:
+        for kind in range(3):
+            v = np.zeros(n, np.float32)
+            if kind == 1:
+                v[::2] = -1.0
+            if kind == 2:
+                v[:] = -np.inf
+                v[5::3] = 4.0
+                v[100::1000] = 4.5
+            xs.append(v)
+            rows.append(opt)
+            us.append(0.123 + 0.04 * len(us))
+    u = np.array(us, np.float32)
+    got = run_sample(torch.tensor(np.stack(xs)).cuda(), rlh.F32, rows, u)
+    for r, opt in enumerate(rows):
+        assert got[r] == ref.sample(xs[r], *opt, u[r]), (r, opt)
+
+
+def test_sample_longest_row():
+    n = 1 << 21
+    g = torch.Generator().manual_seed(1)
+    x = (3.0 * torch.randn((4, n), generator=g)).half().cuda()
+    rows = [(1.0, 0, 0.9, 0.0), (1.0, 50, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (0.8, 5000, 0.99, 1e-5)]
+    u = np.array([0.3, 0.6, 0.9, 0.99], np.float32)
+    got = run_sample(x, rlh.F16, rows, u)
+    host = x.double().cpu().numpy()
+    for r, opt in enumerate(rows):
+        assert got[r] == ref.sample(host[r], *opt, u[r]), (r, opt)
