@@ -166,6 +166,7 @@ struct Sizes {
   uint32_t last_parts;    // of the last, which may have fewer rows
   uint32_t small_rows;    // sequences of up to so many rows of a KV head go to the small kernel
   bool small, tiled, merge;
+  bool whole;             // the small kernel's sequences are not divided
   bool merge_small;       // only its sequences have parts to join
   uint32_t merge_rows;    // then: blocks per sequence and KV head
 };
@@ -300,7 +301,8 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
     total += n;
   }
   total = lane_value(wave_scan(total), 63);
-  const uint32_t per_item = (total + L.n.item_goal - 1) / L.n.item_goal;
+  // (without a launch that joins parts, there are none)
+  const uint32_t per_item = L.n.merge ? (total + L.n.item_goal - 1) / L.n.item_goal : total;
   Found f;
   if (!find_item(a.b.n_seq, item, [&](uint32_t s) {
         uint32_t n = tiles0;
@@ -510,10 +512,10 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   }
 }
 
-template <typename T, int D, bool MOD>
-__global__ void __launch_bounds__(kThreads, 2) k_attn_small(Launch L) {
+template <typename T, int D, bool MOD, int W>
+__global__ void __launch_bounds__(64 * W, 2) k_attn_small(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
-  small_block<T, D, MOD, kWaves>(L, blockIdx.x, lds);
+  small_block<T, D, MOD, W>(L, blockIdx.x, lds);
 }
 
 // ---- many rows: prompts, and the shared prefix of the whole batch ------------------
@@ -1054,6 +1056,13 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
   *(VO*)((T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + c0) = v;
 }
 
+// Up to so many positions, and while all blocks run at once, a sequence of few
+// rows is not divided: its block then has eight waves (a step of 256 positions
+// takes 2 us) and there is no second launch (8 sequences of 250: 8.6 us
+// instead of 7.0 + 4.0, of 500: 10.6 instead of 6.9 + 4.0, of 777: 12.6
+// instead of 7.7 + 4.2; 61 of 500, in 488 blocks: 26.4 instead of 24.4 + 4.8,
+// 128 of 250: 37.3 instead of 27.6 + 3.8).
+constexpr uint32_t kWhole = 512;
 constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into
 
 // Parts that the positions of `blocks` tiles are divided into: as many as let
@@ -1093,8 +1102,9 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
   n.small = group <= kSmallRows && !(n.tiled && q.n_seq == 1);
   n.small_rows = n.small ? kSmallRows : 0;
   if (n.small) {
-    n.item_goal = std::max(1u, kSmallBlocks / kv.n_head_kv);
-    n.items = q.n_seq + n.item_goal;
+    n.whole = !n.tiled && !args.shared_len && q.max_kv <= kWhole && q.n_seq * kv.n_head_kv <= 256;
+    n.item_goal = n.whole ? 1 : std::max(1u, kSmallBlocks / kv.n_head_kv);
+    n.items = q.n_seq + (n.whole ? 0 : n.item_goal);
   }
   if (n.tiled) {
     n.tiles = (uint32_t)(rows / kTileRows + std::min<uint64_t>(q.n_seq, rows / (n.small_rows + 1)));
@@ -1115,7 +1125,7 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
     }
   }
   const uint32_t step = 32 * (args.shared_len || n.tiled ? kTileWaves : kWaves);  // of the few rows' blocks
-  n.merge = args.shared_len || (n.small && own > step) || n.tile_parts > 1;
+  n.merge = args.shared_len || (n.small && !n.whole && own > step) || n.tile_parts > 1;
   n.merge_small = !args.shared_len && n.tile_parts <= 1;
   n.merge_rows = (uint32_t)(std::min<uint64_t>(kSmallRows, q.max_q * group) + kWaves - 1) / kWaves;
   return n;
@@ -1154,12 +1164,14 @@ uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_att
 template <int D>
 constexpr uint32_t kMixedLds = kTileLds<D> > kSmallLds<D, kTileWaves> ? kTileLds<D> : kSmallLds<D, kTileWaves>;
 template <typename T, int D, bool MOD>
-int allow_mixed_lds(int device) {
+int allow_lds(int device) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_acquire) & bit) return RLH_OK;
   if (hipFuncSetAttribute((const void*)k_attn_mixed<T, D, MOD>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (int)kMixedLds<D>) != hipSuccess) {
+                          (int)kMixedLds<D>) != hipSuccess ||
+      hipFuncSetAttribute((const void*)k_attn_small<T, D, MOD, kTileWaves>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)kSmallLds<D, kTileWaves>) != hipSuccess) {
     (void)hipGetLastError();
     return serve_error(RLH_EDEVICE, "hipFuncSetAttribute (LDS of the tiled attention kernels)");
   }
@@ -1171,11 +1183,15 @@ template <typename T, int D, bool MOD>
 int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
   if (L.a.shared_len || L.n.tiled) {
-    RLH_TRY((allow_mixed_lds<T, D, MOD>(device)));
+    RLH_TRY((allow_lds<T, D, MOD>(device)));
     const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts + L.n.items) * G;
     hipLaunchKernelGGL((k_attn_mixed<T, D, MOD>), dim3(blocks), dim3(64 * kTileWaves), kMixedLds<D>, s, L);
+  } else if (L.n.whole) {
+    RLH_TRY((allow_lds<T, D, MOD>(device)));
+    hipLaunchKernelGGL((k_attn_small<T, D, MOD, kTileWaves>), dim3(L.n.items * G), dim3(64 * kTileWaves),
+                       (kSmallLds<D, kTileWaves>), s, L);
   } else {
-    hipLaunchKernelGGL((k_attn_small<T, D, MOD>), dim3(L.n.items * G), dim3(kThreads), (kSmallLds<D, kWaves>), s, L);
+    hipLaunchKernelGGL((k_attn_small<T, D, MOD, kWaves>), dim3(L.n.items * G), dim3(kThreads), (kSmallLds<D, kWaves>), s, L);
   }
   if (L.n.merge) {
     const uint64_t blocks = L.n.merge_small ? (uint64_t)L.a.b.n_seq * L.n.merge_rows * G

@@ -707,6 +707,10 @@ ATTN_MORE = {
                         prefix=[250, 499, 700]),
     "cap and bias": dict(seqs=[(100, 1100), (1, 1500)], heads=12, kv=4, dim=128, page=32, ty=rlh.F16, bias=True, cap=4.0,
                          q_scale=4.0),
+    # short sequences: one block each, or (more blocks than run at once) divided
+    "decode short": dict(seqs=[(1, 1 + (i * 37) % 500) for i in range(40)], heads=8, kv=2, dim=128, page=16, ty=rlh.BF16),
+    "decode many short": dict(seqs=[(1, 1 + (i * 37) % 250) for i in range(140)], heads=8, kv=2, dim=128, page=16, ty=rlh.BF16),
+    "decode many shorter": dict(seqs=[(1, 1 + (i * 37) % 128) for i in range(140)], heads=8, kv=2, dim=64, page=32, ty=rlh.F16),
     "mixed with drafts": dict(seqs=[(300, 310), (2, 900), (1, 33), (4, 4), (0, 5), (90, 2000)], heads=16, kv=4, dim=64, page=16,
                               ty=rlh.F16, pad_seqs=2, pad_rows=4),
 }
