@@ -275,7 +275,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   constexpr int kSmallTile = 32 * W;     // positions that the waves take per step
   float(*ml)[16][2] = (float(*)[16][2])(lds + kSmallLds<D, W> - W * 128);
   const AttnParams& a = L.a;
-  const uint32_t t = threadIdx.x;
+  const uint32_t t = threadIdx.x % (64 * W);
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
   const uint32_t h = block % a.n_kv, item = block / a.n_kv;
   // the division of all sequences' positions, found by every wave alike
@@ -309,8 +309,11 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
         bool bad, mine = mine0;
         if (s >= 64) n = tiles_of(s, &bad, &mine);
         return n ? (n + per_item - 1) / per_item : mine ? 1u : 0u;
-      }, &f))
+      }, &f)) {
+    __syncthreads();  // as often as a neighbour in the same block
+    __syncthreads();
     return;
+  }
   const uint32_t s = f.s, first = f.first, n_items = f.n;
   bool bad;
   const SeqSpan sq = seq_span(a, s, &bad);
@@ -940,10 +943,12 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
   const uint32_t n_prefix = prefix_blocks(L.n) * L.a.n_kv;
   const uint32_t n_tiles = n_prefix + L.n.tiles * L.n.tile_parts * L.a.n_kv;
   const uint32_t b = blockIdx.x;
-  if (b < n_tiles)
+  if (b < n_tiles) {
     tile_block<T, D, MOD>(L, b < n_prefix ? b : b - n_prefix, b < n_prefix, lds);
-  else
-    small_block<T, D, MOD, kTileWaves>(L, b - n_tiles, lds);
+  } else {  // two items, of four waves each
+    const uint32_t half = uniform(threadIdx.x / kThreads);
+    small_block<T, D, MOD, kWaves>(L, 2 * (b - n_tiles) + half, lds + half * kSmallLds<D, kWaves>);
+  }
 }
 
 // ---- joining the parts of a row ------------------------------------------------------
@@ -1124,8 +1129,7 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
       n.last_parts = (uint32_t)std::min(p, most - (n.prefix_tiles - 1) * p);
     }
   }
-  const uint32_t step = 32 * (args.shared_len || n.tiled ? kTileWaves : kWaves);  // of the few rows' blocks
-  n.merge = args.shared_len || (n.small && !n.whole && own > step) || n.tile_parts > 1;
+  n.merge = args.shared_len || (n.small && !n.whole && own > 32 * kWaves) || n.tile_parts > 1;
   n.merge_small = !args.shared_len && n.tile_parts <= 1;
   n.merge_rows = (uint32_t)(std::min<uint64_t>(kSmallRows, q.max_q * group) + kWaves - 1) / kWaves;
   return n;
@@ -1162,7 +1166,7 @@ uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_att
 // The mixed kernels take more LDS than a launch may by default; said once per
 // device (idempotent, so two threads may).
 template <int D>
-constexpr uint32_t kMixedLds = kTileLds<D> > kSmallLds<D, kTileWaves> ? kTileLds<D> : kSmallLds<D, kTileWaves>;
+constexpr uint32_t kMixedLds = kTileLds<D> > 2 * kSmallLds<D, kWaves> ? kTileLds<D> : 2 * kSmallLds<D, kWaves>;
 template <typename T, int D, bool MOD>
 int allow_lds(int device) {
   static std::atomic<uint64_t> done{0};
@@ -1184,7 +1188,7 @@ int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
   if (L.a.shared_len || L.n.tiled) {
     RLH_TRY((allow_lds<T, D, MOD>(device)));
-    const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts + L.n.items) * G;
+    const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts) * G + (L.n.items * G + 1) / 2;
     hipLaunchKernelGGL((k_attn_mixed<T, D, MOD>), dim3(blocks), dim3(64 * kTileWaves), kMixedLds<D>, s, L);
   } else if (L.n.whole) {
     RLH_TRY((allow_lds<T, D, MOD>(device)));
