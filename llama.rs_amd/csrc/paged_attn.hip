@@ -19,7 +19,6 @@ struct AttnParams {
   const float* slopes;
   const uint32_t *prefix_len, *shared_table;
   uint32_t* status;
-  float scale, softcap;
   uint32_t n_head, n_kv, group, page_shift, n_pages, window, shared_len;
 };
 
@@ -255,12 +254,17 @@ __device__ __forceinline__ bool find_item(uint32_t n_seq, uint32_t item, F parts
 // A block takes one KV head of one sequence (up to 16 rows) and a part of
 // its positions; each wave streams 32 positions at a time on its own: K
 // straight into MFMA operands (16x16x32: positions down, rows across), V
-// through the wave's LDS rows to be read by columns. Bound by HBM; the
-// positions are divided so that every part has the same length and the card
-// is filled once. Scores come out with a row per lane column, so the running
-// maximum and the sum are one register per lane, and the probabilities are
-// already the next product's operand if V's rows are taken in the order that
-// the lanes hold them: 4 (lane / 16) + i, and 16 more.
+// through the wave's LDS rows to be read by columns. Scores come out with a
+// row per lane column, so the running maximum and the sum are one register per
+// lane, and the probabilities are already the next product's operand if V's
+// rows are taken in the order that the lanes hold them: 4 (lane / 16) + i, and
+// 16 more. Probabilities are rounded to the pool's type for that product (off
+// by half a step of each; the sum takes them unrounded), all else is f32.
+// Bound by HBM: 61 tokens of 32 heads on 940 MB of pages take 166 us (5.7
+// TB/s; a copy of 2 GiB moves 5.1), 3 of 64 heads on 459 MB 90 us. The
+// positions are divided so that the parts are of one length and fill the card
+// once; a single short sequence costs the chain of loads from its start to its
+// pages (6 us) and the second launch that joins the parts (4 us).
 template <int D, int W>
 constexpr uint32_t kSmallLds = (W * 32 * (D * 2 + 32) > W * 16 * (D + 4) * 4 ? W * 32 * (D * 2 + 32) : W * 16 * (D + 4) * 4) + W * 128;
 
@@ -531,7 +535,13 @@ __global__ void __launch_bounds__(64 * W, 2) k_attn_small(Launch L) {
 // above. What bounds it: a step's 32 MFMAs take 1024 cycles of a SIMD and its
 // exponentials, maxima and sums as many, and the two overlap only between
 // two waves that are at different places; copies are issued at 48 cycles a
-// KB, so four waves per tile would spend 1550 cycles a step on them.
+// KB, so four waves per tile would spend 1550 cycles a step on them. 4096
+// tokens of 64 heads: 275 GFLOP in 303 us, 907 TFLOP/s (a product of 16384^3
+// reaches 1357; tiles of 128 rows took 382 us, operand reads that do not run
+// ahead of the products 349). A cap adds an exponential and a reciprocal per
+// score; a bias is linear in the position, so that a row's share at the step's
+// first position is kept out of the scores and joins the running maximum only
+// (5 prompts of 6895 tokens with a bias: 147 us with it in each score, 107).
 template <int D>
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   return D == 128 ? ((r & 3) << 2 | (r >> 2 & 3)) : ((r >> 1 & 1) << 2 | (r >> 2 & 3));
@@ -935,8 +945,11 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   }
 }
 
-// Prefix tiles, tiles and items of few rows in one launch: each kind leaves
-// parts of the card idle that the others fill.
+// Prefix tiles, tiles and items of few rows in one launch, long blocks first:
+// each kind leaves parts of the card idle that the others fill (64 tokens of
+// 32 heads behind 4096 shared positions: 28 us, in launches of their own
+// 20 + 17; 72 of 64 heads behind 16384: 70 us, apart 65 + 14 + 5; a prompt
+// alone loses 1 % by it).
 template <typename T, int D, bool MOD>
 __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -955,7 +968,8 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
 // A wave takes a row of a query head, its four groups of 16 lanes every
 // fourth part: all maxima at once, then the parts' values, four parts' loads
 // of a group at a time. Bound by latency (a part of a row is 512 bytes at a
-// place of its own).
+// place of its own): 4 us for a single sequence, 8 for 2048 rows and heads of
+// 17 parts (36 MB).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
   constexpr int N = D / 16;   // values per lane
@@ -1068,10 +1082,12 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
 // instead of 7.7 + 4.2; 61 of 500, in 488 blocks: 26.4 instead of 24.4 + 4.8,
 // 128 of 250: 37.3 instead of 27.6 + 3.8).
 constexpr uint32_t kWhole = 512;
-constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into
+constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into (three to a CU)
 
 // Parts that the positions of `blocks` tiles are divided into: as many as let
-// all blocks run at once (one to a CU), of at least 256 positions.
+// all blocks run at once (one to a CU), of at least 256 positions (of 128,
+// what 64 tokens behind 4096 shared positions take grows from 33 + 8 us to
+// 41 + 11).
 uint32_t tile_parts(uint64_t blocks, uint64_t positions) {
   if (blocks == 0) return 1;
   return (uint32_t)std::max<uint64_t>(1, std::min(256 / blocks, positions / 256));
@@ -1260,8 +1276,6 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   p.prefix_len = args->prefix_len;
   p.shared_table = args->shared_table;
   p.status = status;
-  p.scale = args->scale;
-  p.softcap = args->softcap;
   p.n_head = args->n_head;
   p.n_kv = kv->n_head_kv;
   p.group = args->n_head / kv->n_head_kv;
