@@ -16,7 +16,7 @@
  *    says host; plain host memory, or memory of another device, is RLH_EINVAL.
  *    Data and workspaces are aligned to 16 bytes, strides count elements and
  *    span a multiple of 16 bytes, index arrays are aligned to 4 bytes, rotary
- *    frequencies to 8.
+ *    frequencies to 8. What a call writes overlaps nothing else of it.
  *  - The calls enqueue kernels on `stream` (a hipStream_t, NULL for the null
  *    stream), allocate nothing and do not synchronize, so they may be captured
  *    into a graph; lengths, positions, page ids and sampling options are read

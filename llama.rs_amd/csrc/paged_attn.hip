@@ -536,8 +536,8 @@ __global__ void __launch_bounds__(64 * W, 2) k_attn_small(Launch L) {
 // exponentials, maxima and sums as many, and the two overlap only between
 // two waves that are at different places; copies are issued at 48 cycles a
 // KB, so four waves per tile would spend 1550 cycles a step on them. 4096
-// tokens of 64 heads: 275 GFLOP in 303 us, 907 TFLOP/s (a product of 16384^3
-// reaches 1357; tiles of 128 rows took 382 us, operand reads that do not run
+// tokens of 64 heads: 275 GFLOP in 303 us, 907 TFLOP/s (340 us in a row of
+// passes; a product of 16384^3 reaches 1357 TFLOP/s; there, tiles of 128 rows took 382 us, operand reads that do not run
 // ahead of the products 349). A cap adds an exponential and a reciprocal per
 // score; a bias is linear in the position, so that a row's share at the step's
 // first position is kept out of the scores and joins the running maximum only
@@ -1093,6 +1093,12 @@ uint32_t tile_parts(uint64_t blocks, uint64_t positions) {
   return (uint32_t)std::max<uint64_t>(1, std::min(256 / blocks, positions / 256));
 }
 
+// A score in units of log 2 per unit of the dot product (of 2 / softcap with a cap).
+float score_factor(const rlh_attn_args& args) {
+  const float scale = fabsf(args.scale);
+  return args.softcap > 0.0f ? 2.0f * scale / args.softcap * kLog2e : scale * kLog2e;
+}
+
 int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
   if (!args) return serve_error(RLH_EINVAL, "null argument");
   RLH_TRY(check_batch(kv, seqs, args->n_head));
@@ -1110,6 +1116,9 @@ int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args
   if (overlap(args->q, row_bytes_span(seqs->n_rows, args->q_stride, w, 2), args->out,
               row_bytes_span(seqs->n_rows, args->out_stride, w, 2)))
     return serve_error(RLH_EINVAL, "out overlaps q");
+  if (overlaps_pool(*kv, args->out, row_bytes_span(seqs->n_rows, args->out_stride, w, 2)))
+    return serve_error(RLH_EINVAL, "out overlaps the pool");
+  if (!isfinite(score_factor(*args))) return serve_error(RLH_EINVAL, "scale, or scale / softcap, is out of range");
   return RLH_OK;
 }
 
@@ -1249,6 +1258,11 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   if (need > workspace_bytes)
     return serve_error(RLH_EINVAL, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
   if (need && !aligned(workspace, 16)) return serve_error(RLH_EINVAL, "workspace is not aligned to 16 bytes");
+  const uint64_t w = (uint64_t)args->n_head * kv->head_dim;
+  if (overlap(workspace, need, args->q, row_bytes_span(seqs->n_rows, args->q_stride, w, 2)) ||
+      overlap(workspace, need, args->out, row_bytes_span(seqs->n_rows, args->out_stride, w, 2)) ||
+      overlaps_pool(*kv, workspace, need))
+    return serve_error(RLH_EINVAL, "workspace overlaps q, out or the pool");
   DeviceCheck dev;
   RLH_TRY(dev.begin());
   RLH_TRY(dev("k pages", kv->k));
@@ -1288,12 +1302,11 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   L.n = attn_sizes(*kv, *seqs, *args);
   place_workspace(&L.ws, (uint8_t*)workspace, *kv, *seqs, *args, L.n);
   L.sc.capped = args->softcap > 0.0f;
-  const float scale = fabsf(args->scale);
-  L.sc.mul = L.sc.capped ? 2.0f * scale / args->softcap * kLog2e : scale * kLog2e;
+  L.sc.mul = score_factor(*args);
   L.sc.cap2 = args->softcap * kLog2e;
   L.sc.flip = args->scale < 0.0f ? 0x80008000u : 0u;
   // (a scale of zero, which the exponential could not take in, goes with a bias of zero)
-  L.sc.biased = args->slopes || (!L.sc.capped && scale == 0.0f);
+  L.sc.biased = args->slopes || (!L.sc.capped && L.sc.mul == 0.0f);
   const bool mod = L.sc.capped || L.sc.biased;
   if (kv->type == RLH_TYPE_F16) return launch_attn<_Float16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
   return launch_attn<__bf16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);

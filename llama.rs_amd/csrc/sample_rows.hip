@@ -1102,6 +1102,12 @@ int rlh_sample_rows(uint32_t type, const void* logits, uint64_t n_rows, uint64_t
   if (need > workspace_bytes)
     return serve_error(RLH_EINVAL, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
   if (need && !aligned(workspace, 16)) return serve_error(RLH_EINVAL, "workspace is not aligned to 16 bytes");
+  const uint64_t span = row_bytes_span(n_rows, stride, n, size);
+  if (overlap(workspace, need, logits, span) || overlap(workspace, need, options, n_rows * sizeof(*options)) ||
+      overlap(workspace, need, u, n_rows * 4) || overlap(workspace, need, tokens, n_rows * 4) ||
+      overlap(tokens, n_rows * 4, logits, span) || overlap(tokens, n_rows * 4, options, n_rows * sizeof(*options)) ||
+      overlap(tokens, n_rows * 4, u, n_rows * 4))
+    return serve_error(RLH_EINVAL, "workspace or tokens overlap another argument");
   DeviceCheck dev;
   RLH_TRY(dev.begin());
   RLH_TRY(dev("logits", logits));

@@ -40,6 +40,14 @@ inline int check_rows(const char* name, const void* p, uint64_t stride, uint64_t
   return RLH_OK;
 }
 
+// Bytes of the pool's k, and of its v; whether [p, p + n) meets one of them.
+inline uint64_t pool_bytes(const rlh_kv_pages& kv) {
+  return kv.n_pages * kv.n_head_kv * kv.page_size * kv.head_dim * 2;
+}
+inline bool overlaps_pool(const rlh_kv_pages& kv, const void* p, uint64_t n) {
+  return overlap(p, n, kv.k, pool_bytes(kv)) || overlap(p, n, kv.v, pool_bytes(kv));
+}
+
 // The pool and the batch (no device needed).
 int check_batch(const rlh_kv_pages* kv, const rlh_seqs* seqs, uint32_t n_head);
 

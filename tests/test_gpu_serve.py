@@ -794,3 +794,20 @@ def test_sample_longest_row():
     host = x.double().cpu().numpy()
     for r, opt in enumerate(rows):
         assert got[r] == ref.sample(host[r], *opt, u[r]), (r, opt)
+
+
+def test_append_with_starts_that_fall():
+    """A row that lies in no sequence, though the starts name one by their
+    count: left as it was, and the status says so."""
+    b = ref.Batch([(5, 40), (5, 40), (5, 40)], 2, 128, 16, rlh.F16, seed=3)
+    b.q_start.copy_(torch.tensor([0, 30, 5, 10], dtype=torch.int32)[:b.q_start.numel()])
+    x = append_inputs(b, 4, rlh.F32, 5)
+    q_out = torch.full((b.n_rows, 4 * 128), 7.0, dtype=torch.float16, device="cuda")
+    k = b.k.clone()
+    st = status_word()
+    run_append(b, x, rlh.F32, 4, q_out, None, None, None, 1.0, 0, False, st)
+    torch.cuda.synchronize()
+    assert int(st) == rlh.SERVE_BAD_SEQ
+    assert torch.all(q_out[10:] == 7.0) and torch.all(q_out[:5] == 7.0)
+    changed = torch.any(torch.any(b.k != k, dim=3), dim=1)
+    assert int(changed.sum()) <= 5

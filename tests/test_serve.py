@@ -315,3 +315,64 @@ def test_what_rows_see(shim):
                            sees.ctypes.data_as(ctypes.c_void_p), 64)
             seen = np.nonzero(sees[:kv])[0]
             assert out[0] <= seen.min() and seen.max() < out[1]
+
+
+# ---- arguments that overlap, factors out of range ---------------------------------------
+
+@pytest.mark.parametrize("field,value", [("q_out", A), ("q_out", 2 * A + 64), ("q", A), ("k", 2 * A), ("v", A + 65536 - 16)])
+def test_append_refuses_the_pool(field, value):
+    args = good()
+    args["app"][field] = value
+    kv, seqs, app, _ = structs(args)
+    assert rlh.load().rlh_paged_append(kv, seqs, app, None, None) == rlh.RLH_EINVAL
+    assert b"overlap" in rlh.load().rlh_last_error()
+
+
+def test_attention_refuses_overlaps():
+    lib = rlh.load()
+    args = good()
+    args["att"]["out"] = 2 * A + 65536 - 16
+    kv, seqs, _, att = structs(args)
+    assert lib.rlh_paged_attn(kv, seqs, att, 16 * A, 1 << 40, None, None) == rlh.RLH_EINVAL
+    assert b"overlaps the pool" in lib.rlh_last_error()
+    kv, seqs, _, att = structs(good())
+    need = rlh.paged_attn_workspace(kv, seqs, att)
+    assert need > 0
+    for ws in (6 * A, 7 * A + 16, A, 2 * A + 32, 6 * A - need + 16):
+        assert lib.rlh_paged_attn(kv, seqs, att, ws, 1 << 40, None, None) == rlh.RLH_EINVAL
+        assert b"workspace overlaps" in lib.rlh_last_error()
+
+
+@pytest.mark.parametrize("scale,cap", [(3e38, 0.0), (-3e38, 0.0), (1.0, 1e-40), (1e30, 1e-30)])
+def test_attention_refuses_factors_past_f32(scale, cap):
+    args = good()
+    args["att"].update(scale=scale, softcap=cap)
+    kv, seqs, _, att = structs(args)
+    assert rlh.load().rlh_paged_attn(kv, seqs, att, 16 * A, 1 << 40, None, None) == rlh.RLH_EINVAL
+    assert rlh.load().rlh_paged_attn_workspace(kv, seqs, att) == 0
+
+
+def test_sample_refuses_overlaps():
+    lib = rlh.load()
+    need = rlh.sample_rows_workspace(2, 100)
+    assert need > 0
+
+    def call(logits=A, options=2 * A, u=3 * A, tokens=4 * A, ws=16 * A):
+        return lib.rlh_sample_rows(rlh.F32, logits, 2, 100, 100, options, u, tokens, ws, 1 << 40, None)
+
+    for bad in (dict(ws=A), dict(ws=2 * A), dict(ws=3 * A), dict(ws=4 * A), dict(ws=A - need + 16), dict(tokens=A + 796),
+                dict(tokens=2 * A + 4), dict(tokens=3 * A + 4)):
+        assert call(**bad) == rlh.RLH_EINVAL, bad
+        assert b"overlap" in lib.rlh_last_error()
+
+
+@pytest.mark.parametrize("n_seq,n_rows", [(65535, 6), (2, (1 << 23)), (2, (1 << 19) + 1)])
+def test_sizes_past_a_launch(n_seq, n_rows):
+    """n_seq * n_head_kv and n_rows * n_head beyond what a launch holds."""
+    args = good()
+    args["kv"].update(n_head_kv=64, n_pages=1)
+    args["att"]["n_head"] = args["app"]["n_head"] = 64
+    args["seqs"].update(n_seq=n_seq, n_rows=n_rows)
+    kv, seqs, app, att = structs(args)
+    assert rlh.load().rlh_paged_attn(kv, seqs, att, 16 * A, 1 << 40, None, None) == rlh.RLH_EUNSUP
+    assert rlh.load().rlh_paged_append(kv, seqs, app, None, None) == rlh.RLH_EUNSUP
