@@ -25,12 +25,14 @@ namespace {
 // it falls into.
 // Masses are doubles and integers, so that no order of summing changes them
 // and a border is where 64 bits put it to 10^-11 of the mass. That bounds the
-// first launch: 192 rows of 151936 f32 values (117 MB) take 17 to 20 us where
-// only maxima are asked for (6.0 TB/s), 37 with masses and 44 with histograms.
+// first launch: 192 rows of 151936 f32 values (117 MB) take 17 to 19 us where
+// only maxima are asked for (6.0 TB/s), 33 with masses and 41 with histograms,
+// where every SIMD issues vector instructions in 95 % of the cycles (34 and 41
+// per value and lane, 18 and 16 of them of doubles).
 // The second is bound by chains of loads and block-wide sums from a cold start
 // (top-k 40: 17 us) and, where the border lies deep, by what one compute unit
 // reads (31 GB/s: a nucleus of 0.9 of a row as normal numbers have it, 54 us).
-// 192 rows of options of every kind: 90 us; one row of top-k 40: 21.
+// 192 rows of options of every kind: 87 us; one row of top-k 40: 21.
 
 constexpr int kMassBits = 42;  // masses within a range: multiples of 2^-42 of the row's largest weight
 constexpr uint64_t kMaxRow = 1ull << 21;
@@ -64,21 +66,47 @@ constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds, 
 // tokens' borders lie 10^-6 apart at best). Rounding, scaling and conversion
 // instructions of doubles run at a quarter of the rate of sums and products,
 // so y is rounded by adding kRound.
-__device__ __forceinline__ double exp2_within(double y) {
-  const double z = y + kRound;
-  const double f = (y - (z - kRound)) * 0.6931471805599453;
-  double p = 1.0 / 362880.0;
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
+struct Exp2 {
+  double round, c9, c8, c7, c6, c5, c4, c3, c2, c1;
+};
+__device__ __forceinline__ double exp2_within(double y, const Exp2& q) {
+  const double z = y + q.round;
+  const double f = y - (z - q.round);
+  double p = q.c9;
+  p = fma(p, f, q.c8);
+  p = fma(p, f, q.c7);
+  p = fma(p, f, q.c6);
+  p = fma(p, f, q.c5);
+  p = fma(p, f, q.c4);
+  p = fma(p, f, q.c3);
+  p = fma(p, f, q.c2);
+  p = fma(p, f, q.c1);
   p = fma(p, f, 1.0);
   const uint64_t n = __builtin_bit_cast(uint64_t, z) << 52;  // (negative: the sum wraps as it should)
   return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + n);
+}
+constexpr double power(double x, int n) { return n ? x * power(x, n - 1) : 1.0; }
+constexpr double kLn2 = 0.6931471805599453;
+constexpr Exp2 kExp2 = {kRound,
+                        power(kLn2, 9) / 362880.0,
+                        power(kLn2, 8) / 40320.0,
+                        power(kLn2, 7) / 5040.0,
+                        power(kLn2, 6) / 720.0,
+                        power(kLn2, 5) / 120.0,
+                        power(kLn2, 4) / 24.0,
+                        power(kLn2, 3) / 6.0,
+                        power(kLn2, 2) / 2.0,
+                        kLn2};
+__device__ __forceinline__ double exp2_within(double y) { return exp2_within(y, kExp2); }
+__device__ __forceinline__ double opaque(double x) {
+  asm("" : "+s"(x));
+  return x;
+}
+// The same factors in scalar registers, of which the compiler knows no value:
+// else it moves each into vector registers before every use.
+__device__ __forceinline__ Exp2 exp2_factors() {
+  return Exp2{opaque(kExp2.round), opaque(kExp2.c9), opaque(kExp2.c8), opaque(kExp2.c7), opaque(kExp2.c6),
+              opaque(kExp2.c5),    opaque(kExp2.c4), opaque(kExp2.c3), opaque(kExp2.c2), opaque(kExp2.c1)};
 }
 // 0 below 2^-1000, NaN and -infinity.
 __device__ __forceinline__ double exp2_neg(double y) { return y > -1000.0 ? exp2_within(y) : 0.0; }
@@ -113,16 +141,22 @@ constexpr uint64_t kBinMask = (1ull << kBinShift) - 1;
 constexpr double kBinUnit = 0x1p-38;
 // 2^(f / 16) for |f| <= 1/2 in those units: Taylor's polynomial of degree 5,
 // off by less than 2^-42.
-__device__ __forceinline__ uint64_t bin_word(double f) {
-  constexpr double g = 0.6931471805599453 / 16.0;
-  double p = g * g * g * g * g / 120.0;
-  p = fma(p, f, g * g * g * g / 24.0);
-  p = fma(p, f, g * g * g / 6.0);
-  p = fma(p, f, g * g / 2.0);
-  p = fma(p, f, g);
+struct BinExp2 {
+  double c5, c4, c3, c2, c1, unit, big;
+};
+__device__ __forceinline__ uint64_t bin_word(double f, const BinExp2& q) {
+  double p = q.c5;
+  p = fma(p, f, q.c4);
+  p = fma(p, f, q.c3);
+  p = fma(p, f, q.c2);
+  p = fma(p, f, q.c1);
   p = fma(p, f, 1.0);
   // (the low bits of a sum with 2^52 are the rounded integer)
-  return (__builtin_bit_cast(uint64_t, fma(p, 1.0 / kBinUnit, 0x1p52)) & kBinMask) | 1ull << kBinShift;
+  return (__builtin_bit_cast(uint64_t, fma(p, q.unit, q.big)) & kBinMask) | 1ull << kBinShift;
+}
+__device__ __forceinline__ BinExp2 bin_factors() {
+  constexpr double g = kLn2 / 16.0, c5 = power(g, 5) / 120.0, c4 = power(g, 4) / 24.0, c3 = power(g, 3) / 6.0, c2 = g * g / 2.0;
+  return BinExp2{opaque(c5), opaque(c4), opaque(c3), opaque(c2), opaque(g), opaque(1.0 / kBinUnit), opaque(0x1p52)};
 }
 
 // A unit of bin b's mass, as a share of the top's weight.
@@ -230,6 +264,8 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   __shared__ uint32_t tops[kScanThreads / 64];
   __shared__ double sums[kScanThreads / 64];
   const uint32_t t = threadIdx.x, chunk = blockIdx.x % space.chunks, r = blockIdx.x / space.chunks;
+  const Exp2 exp2 = exp2_factors();
+  const BinExp2 bin_exp2 = bin_factors();
   const RowPlan plan = row_plan(options[r], n);
   const RowSpace rs = space.row(r);
   const Row<T> row(logits, stride, n, r);
@@ -237,8 +273,15 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
     for (uint32_t i = t; i < kBins; i += kScanThreads) bin[i] = 0;
   }
   typename Row<T>::Line line[N];
+  if (chunk * kChunk >= row.shift && (chunk + 1) * kChunk <= row.shift + n) {
+    // (all within the row, as most are)
+    const RLH_GLOBAL T* x = row.x + ((size_t)chunk * kChunk - row.shift);
 #pragma unroll
-  for (int i = 0; i < N; i++) line[i] = row.line(chunk * kChunk + (i * kScanThreads + t) * V);
+    for (int i = 0; i < N; i++) line[i] = *(const RLH_GLOBAL typename Row<T>::Line*)(x + (i * kScanThreads + t) * V);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) line[i] = row.line(chunk * kChunk + (i * kScanThreads + t) * V);
+  }
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < N; i++) {
@@ -256,23 +299,24 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kScanThreads / 64; i++) top = max(top, tops[i]);
+  top = (uint32_t)__builtin_amdgcn_readfirstlane((int)top);  // (the block's: known to be uniform from here)
   if (t == 0) rs.top[chunk] = top;
   if (!plan.mass) return;
   const double tv = (double)value_of(top), base = edge_of(top, plan.c);
   double sum = 0.0;
   if (top != 0u && plan.bins) {
-    const double c16 = plan.c * 16.0;
+    const double c16 = plan.c * 16.0, round = exp2.round;
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
         const float x = (float)line[i][e];
-        const double x16 = (double)x * c16, edge = edge_of(x16), d = base - edge;
+        const double x16 = (double)x * c16, edge = (x16 + round) - round, d = base - edge;
         if (d < (double)(kBins - 1))  // (not for NaN, and not for an infinite top)
-          atomicAdd((unsigned long long*)&bin[(uint32_t)__builtin_bit_cast(uint64_t, d + kRound)],
-                    (unsigned long long)bin_word(x16 - edge));
+          atomicAdd((unsigned long long*)&bin[(uint32_t)__builtin_bit_cast(uint64_t, d + round)],
+                    (unsigned long long)bin_word(x16 - edge, bin_exp2));
         else if (x == (float)tv)
-          atomicAdd((unsigned long long*)&bin[0], (unsigned long long)bin_word(0.0));
+          atomicAdd((unsigned long long*)&bin[0], (unsigned long long)bin_word(0.0, bin_exp2));
         else if (x > -INFINITY)  // 2^-39 of the top's weight or less
           sum += weight_called(key_of(x), top, tv, plan.c);
       }
@@ -283,16 +327,18 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
       sum += bin_weight(i, base, tv, plan.c) * (double)(x & kBinMask);
     }
   } else if (top != 0u) {
-    // an infinite top's own weight is 1, what lies below has none
+    const bool finite = tv < INFINITY;
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
         const float x = (float)line[i][e];
-        // (what has no weight is given 2^-1000 of the top's, which no sum holds)
-        double w = exp2_within(fmax(((double)x - tv) * plan.c, -1000.0));
-        if (!(tv < INFINITY)) w = x == (float)tv ? 1.0 : 0.0;
-        sum += w;
+        // (what has no weight is given 2^-1000 of the top's, which no sum holds;
+        // an infinite top's own weight is 1, what lies below has none)
+        if (finite)
+          sum += exp2_within(fmax(((double)x - tv) * plan.c, -1000.0), exp2);
+        else
+          sum += x == (float)tv ? 1.0 : 0.0;
       }
   }
 #pragma unroll
