@@ -100,9 +100,11 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(AppendParams a) {
   const uint32_t row = blockIdx.x;
   // the row's sequence: as many end at or before it as come before it
   uint32_t s = 0;
-  for (uint32_t i = 0; i < a.b.n_seq; i += kThreads) {
-    const uint32_t k = i + threadIdx.x;
-    s += (uint32_t)__syncthreads_count(k < a.b.n_seq && a.b.q_start[k + 1] <= row);
+  if (a.b.n_seq <= kThreads) {
+    const uint32_t k = threadIdx.x;
+    s = (uint32_t)__syncthreads_count(k < a.b.n_seq && a.b.q_start[k + 1] <= row);
+  } else {
+    s = count_upto(a.b.q_start + 1, 1, a.b.n_seq, row);
   }
   if (s >= a.b.n_seq) return;  // behind the last sequence
   bool bad;

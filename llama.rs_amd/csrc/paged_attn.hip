@@ -153,6 +153,7 @@ struct Workspace {
   float* item_o;     // [items * n_kv][16][D]
   float* item_ml;    // [items * n_kv][16][2]
   uint32_t* plan;    // [n_seq][2]: first item, items
+  uint32_t* tiles;   // [n_seq][2]: first tile, tiles (where `planned`)
 };
 
 struct Sizes {
@@ -166,6 +167,7 @@ struct Sizes {
   uint32_t small_rows;    // sequences of up to so many rows of a KV head go to the small kernel
   bool small, tiled, merge;
   bool whole;             // the small kernel's sequences are not divided
+  bool planned;           // a launch before found where each sequence's items and tiles begin
   bool merge_small;       // only its sequences have parts to join
   uint32_t merge_rows;    // then: blocks per sequence and KV head
 };
@@ -250,6 +252,25 @@ __device__ __forceinline__ bool find_item(uint32_t n_seq, uint32_t item, F parts
   return false;
 }
 
+// The same in a list that k_attn_plan left.
+__device__ __forceinline__ bool find_planned(const uint32_t* plan, uint32_t n_seq, uint32_t item, Found* f) {
+  const uint32_t n = count_upto(plan, 2, n_seq, item);
+  if (n == 0) return false;
+  f->s = n - 1;
+  f->first = load_uniform(plan, 2 * f->s);
+  f->n = load_uniform(plan, 2 * f->s + 1);
+  return item < f->first + f->n;
+}
+
+// Steps of a block of W waves over the positions of sequence s, and whether it
+// is one of few rows.
+template <int W>
+__device__ __forceinline__ uint32_t small_steps(const AttnParams& a, uint32_t s, bool* bad, bool* mine) {
+  const SeqSpan q = seq_span(a, s, bad);
+  *mine = q.rows != 0 && q.rows <= kSmallRows;
+  return *mine && q.end > q.begin ? (uint32_t)(q.end - q.begin + 32 * W - 1) / (32 * W) : 0;
+}
+
 // ---- few rows: single tokens and drafts -----------------------------------------
 // A block takes one KV head of one sequence (up to 16 rows) and a part of
 // its positions; each wave streams 32 positions at a time on its own: K
@@ -283,37 +304,39 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
   const uint32_t h = block % a.n_kv, item = block / a.n_kv;
   // the division of all sequences' positions, found by every wave alike
-  auto tiles_of = [&](uint32_t s, bool* bad, bool* mine) -> uint32_t {
-    const SeqSpan q = seq_span(a, s, bad);
-    *mine = q.rows != 0 && q.rows <= kSmallRows;
-    return *mine && q.end > q.begin ? (uint32_t)(q.end - q.begin + kSmallTile - 1) / kSmallTile : 0;
-  };
-  uint32_t total = 0, tiles0 = 0;  // (tiles0: of the first 64 sequences, which are not looked at twice)
-  bool mine0 = false;
-  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-    const uint32_t s = s0 + lane;
-    uint32_t n = 0;
-    if (s < a.b.n_seq) {
-      bool bad, mine;
-      n = tiles_of(s, &bad, &mine);
-      if (bad && block == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
-      if (s0 == 0) {
-        tiles0 = n;
-        mine0 = mine;
-      }
-    }
-    total += n;
-  }
-  total = lane_value(wave_scan(total), 63);
-  // (without a launch that joins parts, there are none)
-  const uint32_t per_item = L.n.merge ? (total + L.n.item_goal - 1) / L.n.item_goal : total;
+  auto tiles_of = [&](uint32_t s, bool* bad, bool* mine) { return small_steps<W>(a, s, bad, mine); };
   Found f;
-  if (!find_item(a.b.n_seq, item, [&](uint32_t s) {
-        uint32_t n = tiles0;
-        bool bad, mine = mine0;
-        if (s >= 64) n = tiles_of(s, &bad, &mine);
-        return n ? (n + per_item - 1) / per_item : mine ? 1u : 0u;
-      }, &f)) {
+  bool found;
+  if (L.n.planned) {
+    found = find_planned(L.ws.plan, a.b.n_seq, item, &f);
+  } else {
+    uint32_t total = 0, tiles0 = 0;  // (tiles0: of the first 64 sequences, which are not looked at twice)
+    bool mine0 = false;
+    for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64) {
+      const uint32_t s = s0 + lane;
+      uint32_t n = 0;
+      if (s < a.b.n_seq) {
+        bool bad, mine;
+        n = tiles_of(s, &bad, &mine);
+        if (bad && block == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
+        if (s0 == 0) {
+          tiles0 = n;
+          mine0 = mine;
+        }
+      }
+      total += n;
+    }
+    total = lane_value(wave_scan(total), 63);
+    // (without a launch that joins parts, there are none)
+    const uint32_t per_item = L.n.merge ? (total + L.n.item_goal - 1) / L.n.item_goal : total;
+    found = find_item(a.b.n_seq, item, [&](uint32_t s) {
+      uint32_t n = tiles0;
+      bool bad, mine = mine0;
+      if (s >= 64) n = tiles_of(s, &bad, &mine);
+      return n ? (n + per_item - 1) / per_item : mine ? 1u : 0u;
+    }, &f);
+  }
+  if (!found) {
     __syncthreads();  // as often as a neighbour in the same block
     __syncthreads();
     return;
@@ -325,7 +348,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   const uint32_t part = item - first, share = (tiles + n_items - 1) / n_items;
   const int32_t from = sq.begin + (int32_t)(part * share * kSmallTile);
   const int32_t to = min(sq.end, from + (int32_t)(share * kSmallTile));
-  if (t == 0 && part == 0 && h == 0) {
+  if (!L.n.planned && t == 0 && part == 0 && h == 0) {
     L.ws.plan[2 * s] = first;
     L.ws.plan[2 * s + 1] = n_items;
   }
@@ -547,6 +570,14 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   return D == 128 ? ((r & 3) << 2 | (r >> 2 & 3)) : ((r >> 1 & 1) << 2 | (r >> 2 & 3));
 }
 
+// Tiles of sequence s.
+__device__ __forceinline__ uint32_t tiles_of_seq(const Launch& L, uint32_t s) {
+  bool bad;
+  const SeqView v = load_seq(L.a.b, s, &bad);
+  const uint32_t r = v.ok ? v.q_len * L.a.group : 0;
+  return r > L.n.small_rows ? (r + kTileRows - 1) / kTileRows : 0u;
+}
+
 struct TileShared {
   uint64_t special[2];  // positions of a step whose V row holds infinities or NaN
   int32_t ranges[kTileWaves][8];
@@ -584,19 +615,15 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
     row0 = tile * kTileRows;
     rows = a.b.n_rows * a.group;
   } else {
-    if (block == 0)
+    if (block == 0 && !L.n.planned)
       for (uint32_t i = t; i < a.b.n_seq; i += kThreads) {
         bool bad;
         load_seq(a.b, i, &bad);
         if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
       }
     Found f;
-    if (!find_item(a.b.n_seq, tile, [&](uint32_t i) {
-          bool bad;
-          const SeqView v = load_seq(a.b, i, &bad);
-          const uint32_t r = v.ok ? v.q_len * a.group : 0;
-          return r > L.n.small_rows ? (r + kTileRows - 1) / kTileRows : 0u;
-        }, &f))
+    if (L.n.planned ? !find_planned(L.ws.tiles, a.b.n_seq, tile, &f)
+                    : !find_item(a.b.n_seq, tile, [&](uint32_t i) { return tiles_of_seq(L, i); }, &f))
       return;
     s = f.s;
     row0 = (f.n - 1 - (tile - f.first)) * kTileRows;  // the last rows, with the most positions, first
@@ -991,8 +1018,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
     row = w / a.n_head;
     head = w % a.n_head;
     if (row >= a.b.n_rows) return;
-    for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64)
-      s += (uint32_t)__popcll(__ballot(s0 + lane < a.b.n_seq && a.b.q_start[s0 + lane + 1] <= row));
+    s = count_upto(a.b.q_start + 1, 1, a.b.n_seq, row);
     if (s >= a.b.n_seq) return;
     sv = load_seq(a.b, s, &bad);
     if (row < sv.q0) return;
@@ -1082,6 +1108,74 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
 // instead of 7.7 + 4.2; 61 of 500, in 488 blocks: 26.4 instead of 24.4 + 4.8,
 // 128 of 250: 37.3 instead of 27.6 + 3.8).
 constexpr uint32_t kWhole = 512;
+// ---- many sequences -------------------------------------------------------------------
+// Where each sequence's items and tiles begin, by one block. Up to kPlanned
+// sequences every wave of the other kernels finds that out by itself, which
+// costs less than a launch; beyond, their loops over all sequences would take
+// longer than the attention (2048 of 300 positions: 5 + 448 us instead of 1024).
+constexpr uint32_t kPlanned = 256;
+constexpr int kPlanThreads = 1024;
+
+__global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
+  __shared__ uint32_t sums[2][kPlanThreads / 64];
+  const AttnParams& a = L.a;
+  const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  // the inclusive sums over the block of two values per thread, and the whole
+  auto scan = [&](uint32_t (&x)[2], uint32_t (&all)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) x[i] = wave_scan(x[i]);
+    __syncthreads();
+    if (lane == 63)
+#pragma unroll
+      for (int i = 0; i < 2; i++) sums[i][wave] = x[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      all[i] = 0;
+      for (uint32_t w = 0; w < kPlanThreads / 64; w++) {
+        const uint32_t v = sums[i][w];
+        x[i] += w < wave ? v : 0u;
+        all[i] += v;
+      }
+    }
+  };
+  uint32_t per_item = 0;
+  if (L.n.small) {
+    uint32_t n[2] = {0, 0}, all[2];
+    for (uint32_t s = t; s < a.b.n_seq; s += kPlanThreads) {
+      bool bad, mine;
+      n[0] += small_steps<kWaves>(a, s, &bad, &mine);
+    }
+    scan(n, all);
+    per_item = L.n.merge ? (all[0] + L.n.item_goal - 1) / L.n.item_goal : all[0];
+  }
+  uint32_t before[2] = {0, 0};
+  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kPlanThreads) {
+    const uint32_t s = s0 + t;
+    uint32_t n[2] = {0, 0}, all[2];
+    if (s < a.b.n_seq) {
+      bool bad, mine;
+      const uint32_t steps = small_steps<kWaves>(a, s, &bad, &mine);
+      if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
+      if (L.n.small) n[0] = steps ? (steps + per_item - 1) / per_item : mine ? 1u : 0u;
+      if (L.n.tiled) n[1] = tiles_of_seq(L, s);
+    }
+    uint32_t upto[2] = {n[0], n[1]};
+    scan(upto, all);
+    if (s < a.b.n_seq)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        uint32_t* p = i ? L.ws.tiles : L.ws.plan;
+        if (i ? L.n.tiled : L.n.small) {
+          p[2 * s] = before[i] + upto[i] - n[i];
+          p[2 * s + 1] = n[i];
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < 2; i++) before[i] += all[i];
+  }
+}
+
 constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into (three to a CU)
 
 // Parts that the positions of `blocks` tiles are divided into: as many as let
@@ -1155,6 +1249,7 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
     }
   }
   n.merge = args.shared_len || (n.small && !n.whole && own > 32 * kWaves) || n.tile_parts > 1;
+  n.planned = q.n_seq > kPlanned && (n.small || n.tiled);
   n.merge_small = !args.shared_len && n.tile_parts <= 1;
   n.merge_rows = (uint32_t)(std::min<uint64_t>(kSmallRows, q.max_q * group) + kWaves - 1) / kWaves;
   return n;
@@ -1180,6 +1275,7 @@ uint64_t place_workspace(Workspace* w, uint8_t* base, const rlh_kv_pages& kv, co
   w->item_o = (float*)take(ir * D * 4);
   w->item_ml = (float*)take(ir * 8);
   w->plan = (uint32_t*)take(n.small ? (uint64_t)q.n_seq * 8 : 0);
+  w->tiles = (uint32_t*)take(n.planned && n.tiled ? (uint64_t)q.n_seq * 8 : 0);
   return at;
 }
 
@@ -1211,6 +1307,7 @@ int allow_lds(int device) {
 template <typename T, int D, bool MOD>
 int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
+  if (L.n.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, L);
   if (L.a.shared_len || L.n.tiled) {
     RLH_TRY((allow_lds<T, D, MOD>(device)));
     const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts) * G + (L.n.items * G + 1) / 2;

@@ -811,3 +811,53 @@ def test_append_with_starts_that_fall():
     assert torch.all(q_out[10:] == 7.0) and torch.all(q_out[:5] == 7.0)
     changed = torch.any(torch.any(b.k != k, dim=3), dim=1)
     assert int(changed.sum()) <= 5
+
+
+# ---- more sequences than a wave looks at by itself -----------------------------------
+
+ATTN_MANY = {
+    "tokens": dict(seqs=[(1, 1 + (i * 61) % 700) for i in range(1100)], heads=4, kv=2, dim=64, page=16, ty=rlh.F16),
+    "tokens short": dict(seqs=[(1, 1 + (i * 37) % 128) for i in range(259)], heads=2, kv=1, dim=64, page=16, ty=rlh.BF16),
+    "tokens and prompts": dict(seqs=[((0, 1, 20, 2)[i % 4], 30 + (i * 37) % 300) for i in range(300)] + [(300, 310)], heads=8,
+                               kv=2, dim=64, page=16, ty=rlh.BF16, pad_seqs=3, pad_rows=2),
+    "wide groups": dict(seqs=[(1, 1 + (i * 37) % 200) for i in range(280)], heads=20, kv=1, dim=64, page=32, ty=rlh.F16),
+    "shared": dict(seqs=[(1 + i % 7 // 6 * 8, 80 + (i * 37) % 200) for i in range(270)], heads=4, kv=1, dim=64, page=16,
+                   ty=rlh.F16, shared=64),
+}
+
+
+@pytest.mark.parametrize("name", list(ATTN_MANY))
+def test_attention_many_sequences(name):
+    case = dict(ATTN_MANY[name])
+    heads = case["heads"]
+    print("attention", name, flush=True)
+    b, q, out, opts = attn_case(seed=len(name), **case)
+    st = status_word()
+    run_attn(b, q, out, heads, status=st, **opts)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    check_attn(b, q, out, heads, opts)
+    # one that contradicts the bounds
+    b.kv_len[260 % len(case["seqs"])] = b.max_kv + 1
+    run_attn(b, q, torch.empty_like(out), heads, status=st, **opts)
+    torch.cuda.synchronize()
+    rows = case["seqs"][260 % len(case["seqs"])][0]
+    assert int(st) == (rlh.SERVE_BAD_SEQ if rows else 0)
+
+
+def test_append_many_sequences():
+    seqs = [((0, 1, 3, 1)[i % 4], 5 + (i * 37) % 90) for i in range(600)]
+    b = ref.Batch(seqs, 1, 64, 16, rlh.F16, seed=8, pad_seqs=2, pad_rows=3)
+    x = append_inputs(b, 2, rlh.F16, 5)
+    q_out = torch.full((b.n_rows, 2 * 64), 7.0, dtype=torch.float16, device="cuda")
+    st = status_word()
+    run_append(b, x, rlh.F16, 2, q_out, None, None, None, 1.0, 0, False, st)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    xs = x[:, :4 * 64].view(b.n_rows, 4, 64)
+    assert torch.equal(q_out[:b.n_live], xs[:b.n_live, :2].reshape(-1, 128)) and torch.all(q_out[b.n_live:] == 7.0)
+    for s, (rows, n) in enumerate(seqs):
+        for i in range(rows):
+            p, r = n - rows + i, int(b.starts[s]) + i
+            assert torch.equal(b.k[b.page_of(s, p), :, p % 16], xs[r, 2:3])
+            assert torch.equal(b.v[b.page_of(s, p), :, p % 16], xs[r, 3:4])
