@@ -7,19 +7,7 @@
 
 namespace rlh {
 
-// f16 and bf16 as the kernels see them: eight in 16 bytes, values as f32.
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
-struct HalfF16 {
-  typedef _Float16 T;
-  typedef f16x8_t V8;
-};
-struct HalfBF16 {
-  typedef __bf16 T;
-  typedef bf16x8_t V8;
-};
 
 // One batch as the kernels get it.
 struct Batch {
