@@ -167,7 +167,8 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
  * temperature <= 0 (or NaN): the first of the order. NaN logits have no mass;
  * at +infinity only those logits have; a row without a value above -infinity
  * gives 0. Masses below 2^-43 of the largest may count as none. u outside
- * [0, 1) (or NaN) is taken as the nearer end (0). n <= 2^21, n_rows <= 2^21
+ * [0, 1) (or NaN) is taken as the nearer end (0); at 1 and above the token is
+ * the last kept one of at least 2^-43 of the largest weight. n <= 2^21, n_rows <= 2^21
  * and n_rows * n <= 2^35. The token does not depend on the run: masses are
  * summed in a fixed order, or as whole numbers. */
 typedef struct rlh_row_sampling {

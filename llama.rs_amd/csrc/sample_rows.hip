@@ -35,6 +35,7 @@ namespace {
 // 192 rows of options of every kind: 87 us; one row of top-k 40: 21.
 
 constexpr int kMassBits = 42;  // masses within a range: multiples of 2^-42 of the row's largest weight
+constexpr double kLeastWeight = 0x1p-43;  // of the largest: a token of less is not taken for the last one
 constexpr uint64_t kMaxRow = 1ull << 21;
 constexpr uint64_t kMaxRows = 1ull << 21;
 constexpr uint32_t kChunk = 4096;
@@ -969,7 +970,8 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
   }
   __syncthreads();
   uint32_t per = 0, ch = 0;  // neighbours per thread of the list; or the draw's chunk
-  double before = 0.0, draw = 0.0;
+  double before = 0.0, draw = 0.0, least_weight = kLeastWeight;
+  const bool at_end = !(uu < 1.0);  // nothing exceeds the draw: the last that has weight
   const bool from_list = plan.list && m != 0xffffffffu;
   if (from_list) {
     per = (m + kThreads - 1) / kThreads;
@@ -1033,16 +1035,26 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
     const Scan<double> sums = block_scan<double>(a + b, &sh);
     const double at = sums.upto - (a + b);
     draw = uu * sums.all;
-    if (a > 0.0) {
-      if (at + a > draw) atomicMin(&sh.where[0], 2 * t);
-      atomicMax(&sh.where[1], 2 * t);
-    }
-    if (b > 0.0) {
-      if (at + a + b > draw) atomicMin(&sh.where[0], 2 * t + 1);
-      atomicMax(&sh.where[1], 2 * t + 1);
+    if (!at_end) {
+      if (a > 0.0 && at + a > draw) atomicMin(&sh.where[0], 2 * t);
+      if (b > 0.0 && at + a + b > draw) atomicMin(&sh.where[0], 2 * t + 1);
     }
     __syncthreads();
-    ch = sh.where[0] != 0xffffffffu ? sh.where[0] : sh.where[1];
+    ch = sh.where[0];
+    if (ch == 0xffffffffu) {
+      // the last chunk that has a kept weight of kLeastWeight: its largest is
+      // kept if any is (the row's largest always: there is one)
+      if (b > 0.0 && weight_called(sh.top[2 * t + 1], top_key, top, c) >= kLeastWeight)
+        atomicMax(&sh.where[1], 2 * t + 1);
+      else if (a > 0.0 && weight_called(sh.top[2 * t], top_key, top, c) >= kLeastWeight)
+        atomicMax(&sh.where[1], 2 * t);
+      __syncthreads();
+      ch = sh.where[1];
+    } else {
+      // (found by sums of another order than those below: the draw may lie past
+      // the chunk's end by their last bits, and the chunk may have little weight)
+      least_weight *= fmin(1.0, sh.kept[ch]);
+    }
     if (ch / 2 == t) sh.before = __builtin_bit_cast(uint64_t, ch % 2 ? at + a : at);
     __syncthreads();
     before = __builtin_bit_cast(double, sh.before);
@@ -1081,19 +1093,21 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
   const Scan<double> sums = block_scan<double>(s, &sh);
   double run = sums.upto - s + before;
   if (from_list) draw = uu * sums.all;
+  if (at_end) draw = INFINITY;
   uint32_t hit = 0xffffffffu, last = 0xffffffffu;
 #pragma unroll
   for (uint32_t j = 0; j < kPer; j++) {
     run += w[j];
     if (hit == 0xffffffffu && w[j] > 0.0 && run > draw) hit = at[j];
-    if (w[j] >= 0x1p-43) last = at[j];
+    if (w[j] >= least_weight) last = at[j];
   }
   // one lane of a wave speaks for it: the sums rise and the indices with them
   const uint64_t hits = __ballot(hit != 0xffffffffu), lasts = __ballot(last != 0xffffffffu);
   if (hits && (int)lane == __builtin_ctzll(hits)) atomicMin(&sh.where[2], hit);
   if (lasts && (int)lane == 63 - __builtin_clzll(lasts)) atomicMax(&sh.where[3], last);
   __syncthreads();
-  // (none past the draw: u at its upper end, or sums that differ in their last bits)
+  // (none past the draw: u at its upper end, or sums that differ in their last
+  // bits; a token of least_weight there is)
   if (t == 0) tokens[r] = (sh.where[2] != 0xffffffffu ? sh.where[2] : sh.where[3]) - row.shift;
 }
 
