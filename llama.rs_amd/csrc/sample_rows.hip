@@ -23,9 +23,13 @@ namespace {
 // bins until 64 values are left, which one wave sorts. The draw runs over the
 // list itself, or over the chunks' kept masses and inside the one chunk that
 // it falls into.
-// Masses are doubles and integers, so that no order of summing changes them
-// and a border is where 64 bits put it to 10^-11 of the mass. That bounds the
-// first launch: 192 rows of 151936 f32 values (117 MB) take 17 to 19 us where
+// Masses are doubles and integers, so that no order of summing changes them.
+// A weight is off by 2^-37 of itself, a value in a bin by 2^-39 more, and
+// narrowing rounds each to 2^-43 of the range's largest: a border is where 64
+// bits put it to 2^-36 of the mass. What lies below the histogram (2^-39.9 of
+// the largest) is searched as one more bin, down to 2^-43; if no bound ends
+// there either, the rest is dropped.
+// The doubles bound the first launch: 192 rows of 151936 f32 values (117 MB) take 17 to 19 us where
 // only maxima are asked for (6.0 TB/s), 33 with masses and 41 with histograms,
 // where every SIMD issues vector instructions in 95 % of the cycles (34 and 41
 // per value and lane, 18 and 16 of them of doubles).
@@ -34,7 +38,7 @@ namespace {
 // reads (31 GB/s: a nucleus of 0.9 of a row as normal numbers have it, 54 us).
 // 192 rows of options of every kind: 87 us; one row of top-k 40: 21.
 
-constexpr int kMassBits = 42;  // masses within a range: multiples of 2^-42 of the row's largest weight
+constexpr int kMassBits = 42;  // masses within a range: multiples of 2^-42 of the largest weight in it
 constexpr double kLeastWeight = 0x1p-43;  // of the largest: a token of less is not taken for the last one
 constexpr uint64_t kMaxRow = 1ull << 21;
 constexpr uint64_t kMaxRows = 1ull << 21;
@@ -63,8 +67,8 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds, and the sum's low bits are the integer
 
 // 2^y for -1000 <= y <= 0: Taylor's polynomial of degree 9 of 2^f, |f| <= 1/2,
-// off by less than 2^-37 (as the last place of 10^11 of the mass, where two
-// tokens' borders lie 10^-6 apart at best). Rounding, scaling and conversion
+// off by less than 2^-37 (7 10^-12, where two tokens' borders lie 10^-6 of the
+// mass apart at best). Rounding, scaling and conversion
 // instructions of doubles run at a quarter of the rate of sums and products,
 // so y is rounded by adding kRound.
 struct Exp2 {
@@ -121,8 +125,6 @@ __device__ __forceinline__ double weight_of(uint32_t key, uint32_t top_key, doub
 __device__ __noinline__ double weight_called(uint32_t key, uint32_t top_key, double top, double c) {
   return weight_of(key, top_key, top, c);
 }
-__device__ __forceinline__ uint64_t mass_of(double w) { return (uint64_t)(w * (double)(1ull << kMassBits) + 0.5); }
-
 // Bins of a histogram: the value's logarithm of its weight, rounded to
 // sixteenths of a power of two and counted from the largest's (`base`) down.
 __device__ __forceinline__ double edge_of(double x16) { return (x16 + kRound) - kRound; }
@@ -529,6 +531,12 @@ __device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goa
     sh.fine.mass[i] = 0;
   }
   if (t == 0) sh.where[0] = 0xffffffffu;
+  // (2^21 values of at most 2^42 units: below 2^64)
+  double unit = 0.0, units = 0.0;  // of a mass; in a weight of one
+  if (goal.p < INFINITY) {
+    unit = fmax(weight_called(min(r.hi, goal.top_key), goal.top_key, goal.top, goal.c), kLeastWeight) * (1.0 / (double)(1ull << kMassBits));
+    units = 1.0 / unit;
+  }
   __syncthreads();
   visit([&](uint32_t k) {
     if (k < r.lo || k > r.hi) return;
@@ -536,7 +544,7 @@ __device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goa
     atomicAdd(&sh.fine.count[b], 1u);
     if (goal.p < INFINITY)
       atomicAdd((unsigned long long*)&sh.fine.mass[b],
-                (unsigned long long)mass_of(weight_called(k, goal.top_key, goal.top, goal.c)));
+                (unsigned long long)(weight_called(k, goal.top_key, goal.top, goal.c) * units + 0.5));
   });
   __syncthreads();
   // each thread's parts, from the top
@@ -555,7 +563,7 @@ __device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goa
     const uint64_t part = sh.fine.mass[b];
     const uint32_t cnt = sh.fine.count[b];
     if ((goal.k != 0xffffffffu && r.above_k + upto_k + cnt >= goal.k) ||
-        r.above_p + (double)(upto_p + part) * (1.0 / (double)(1ull << kMassBits)) >= goal.p ||
+        r.above_p + (double)(upto_p + part) * unit >= goal.p ||
         r.lo + (b << shift) < goal.min_key) {
       mine = kFine - 1 - b;
       break;
@@ -575,7 +583,7 @@ __device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goa
   }
   __syncthreads();
   r.above_k += sh.where[1];
-  r.above_p += (double)sh.before * (1.0 / (double)(1ull << kMassBits));
+  r.above_p += (double)sh.before * unit;
   r.lo += b << shift;
   r.hi = r.lo + min(r.hi - r.lo, (1u << shift) - 1);
   __syncthreads();
@@ -953,20 +961,23 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(const T* logits, uint3
       above_k += sum_k.all;
       above_p += sum_p.all;
     }
-    if (border_bin < kBins - 1) {
-      // the bin's keys: bins fall as keys rise
-      auto from_bin = [&](uint32_t b) { return least_key(1, top_key, [&](uint32_t k) { return bin_of(k, top_key, base, c) <= b; }); };
-      // the first half of the waves looks for the bin's end, the others for the next one's
-      const bool low = wave < kWaves / 2;
-      const uint32_t edge = low || border_bin > 0 ? from_bin(low ? border_bin : border_bin - 1) : top_key + 1;
-      if (lane == 0 && wave % (kWaves / 2) == 0) sh.where[low ? 2 : 3] = edge;
-      __syncthreads();
-      const uint32_t lo = sh.where[2], hi = sh.where[3] - 1;
-      const Range range{lo, hi, sh.where[1], __builtin_bit_cast(double, sh.before)};
-      border = find_border(&sh, row, group, groups, range, goal, &m);
-    } else {
-      border_bin = kBins;
-    }
+    // the bin's keys: bins fall as keys rise. Where no bound ends within the
+    // bins, one may among what lies below them and has weight
+    const bool deep = border_bin == 0xffffffffu;
+    if (deep) border_bin = kBins - 1;
+    auto from_bin = [&](uint32_t b) { return least_key(1, top_key, [&](uint32_t k) { return bin_of(k, top_key, base, c) <= b; }); };
+    // the first half of the waves looks for the bin's end, the others for the next one's
+    const bool low = wave < kWaves / 2;
+    uint32_t edge = top_key + 1;
+    if (low && deep)
+      edge = least_key(1, top_key, [&](uint32_t k) { return weight_called(k, top_key, top, c) >= kLeastWeight; });
+    else if (low || border_bin > 0)
+      edge = from_bin(low ? border_bin : border_bin - 1);
+    if (lane == 0 && wave % (kWaves / 2) == 0) sh.where[low ? 2 : 3] = edge;
+    __syncthreads();
+    const uint32_t lo = sh.where[2], hi = sh.where[3] - 1;
+    const Range range{lo, hi, deep ? above_k : sh.where[1], deep ? above_p : __builtin_bit_cast(double, sh.before)};
+    border = find_border(&sh, row, group, groups, range, goal, &m);
   }
   __syncthreads();
   uint32_t per = 0, ch = 0;  // neighbours per thread of the list; or the draw's chunk

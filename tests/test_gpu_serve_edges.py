@@ -75,3 +75,72 @@ def test_sample_inside_a_chunk_of_little_weight():
         rows.append((1.0, 0, 1.0, 0.0))
         us.append(at * w / 4904.0)
     compare_samples(xs, rows, us)
+
+
+# ---- borders far below the largest weight ------------------------------------------
+
+DEEP = [(1.0, 2000, 1.0, 0.0), (1.0, 5000, 1.0, 0.0), (1.0, 0, 1.0, 4e-13), (1.0, 3000, 1.0, 5e-13), (0.5, 2000, 1.0, 0.0),
+        (1.0, 5999, 1.0, 0.0), (2.0, 2000, 1.0, 0.0)]
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("kind", ["spread", "equal", "steps"])
+def test_sample_borders_below_the_histograms(kind, shift):
+    """One likely token, and thousands at some 2^-41 of it among which top-k
+    or min-p ends."""
+    rng = np.random.default_rng(11)
+    n = 6000 if kind == "spread" else 20000
+    xs, rows, us = [], [], []
+    for opt in DEEP:
+        for u in (1.0, 1 - 2.0 ** -24, 0.3):
+            v = rng.normal(-28.4, 0.3, n).astype(np.float32)
+            if kind == "equal":
+                v[:] = -28.4
+            if kind == "steps":
+                v = np.round(v * 8) / 8
+            v *= opt[0]
+            v[rng.integers(0, n)] = 0.0
+            xs.append(v.astype(np.float32))
+            rows.append(opt)
+            us.append(u)
+    compare_samples(xs, rows, us, shift=shift)
+
+
+def test_sample_long_flat_row_behind_one_token():
+    """151936 logits, one 28 above the rest: what top-k leaves is less than a
+    step of u away from 1, the whole rest is more."""
+    n = 151936
+    xs, rows, us = [], [], []
+    for k in (1200, 2000, 30000):
+        v = np.zeros(n, np.float32)
+        v[0] = 28.0
+        xs.append(v)
+        rows.append((1.0, k, 1.0, 0.0))
+        us.append(1 - 2.0 ** -24)
+    compare_samples(xs, rows, us)
+
+
+def test_sample_draws_in_a_deep_tail():
+    """The draw falls among tokens of 2^-40.4 of the largest: inside the first
+    top_k, and where 64 bits put it as far as the masses go, 2^-37 of the
+    largest: 11 tokens."""
+    n = 1 << 18
+    v = np.full(n, -28.0, np.float32)
+    v[0] = 0.0
+    k = 120000
+    u = np.full(2, 1 - 2.0 ** -24, np.float32)
+    got = run_sample(torch.tensor(np.stack([v, v])).cuda(), rlh.F32, [(1.0, k, 1.0, 0.0)] * 2, u)
+    want = ref.sample(v, 1.0, k, 1.0, 0.0, u[0])
+    assert 0 < want < k and abs(int(got[1]) - want) <= 11
+
+
+def test_sample_nucleus_that_ends_deep():
+    """top-p that ends among equal tokens of 2^-40.4 of the largest: the last
+    kept one is where 64 bits put it to 2^-36 of the mass, 21 tokens."""
+    n = 1 << 18
+    v = np.full(n, -28.0, np.float32)
+    v[5] = 0.0
+    p = np.float32(1 - 2.0 ** -23)
+    got = run_sample(torch.tensor(np.stack([v, v])).cuda(), rlh.F32, [(1.0, 0, p, 0.0)] * 2, np.ones(2, np.float32))
+    want = ref.sample(v, 1.0, 0, p, 0.0, np.float32(1.0))
+    assert 1000 < want < n - 1000 and abs(int(got[1]) - want) <= 21
