@@ -333,7 +333,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
       uint32_t n = tiles0;
       bool bad, mine = mine0;
       if (s >= 64) n = tiles_of(s, &bad, &mine);
-      return n ? (n + per_item - 1) / per_item : mine ? 1u : 0u;
+      return n ? items_of(n, per_item) : mine ? 1u : 0u;
     }, &f);
   }
   if (!found) {
@@ -1141,13 +1141,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
   };
   uint32_t per_item = 0;
   if (L.n.small) {
-    uint32_t n[2] = {0, 0}, all[2];
+    uint32_t mine_all = 0;  // of up to 64 sequences
     for (uint32_t s = t; s < a.b.n_seq; s += kPlanThreads) {
       bool bad, mine;
-      n[0] += small_steps<kWaves>(a, s, &bad, &mine);
+      mine_all += small_steps<kWaves>(a, s, &bad, &mine);
     }
+    uint32_t n[2] = {mine_all & 0xffff, mine_all >> 16}, all[2];
     scan(n, all);
-    per_item = L.n.merge ? (all[0] + L.n.item_goal - 1) / L.n.item_goal : all[0];
+    const uint64_t total = all[0] + ((uint64_t)all[1] << 16);
+    per_item = steps_per_item(total, L.n.merge ? L.n.item_goal : 1);
   }
   uint32_t before[2] = {0, 0};
   for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kPlanThreads) {
@@ -1157,7 +1159,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
       bool bad, mine;
       const uint32_t steps = small_steps<kWaves>(a, s, &bad, &mine);
       if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
-      if (L.n.small) n[0] = steps ? (steps + per_item - 1) / per_item : mine ? 1u : 0u;
+      if (L.n.small) n[0] = steps ? items_of(steps, per_item) : mine ? 1u : 0u;
       if (L.n.tiled) n[1] = tiles_of_seq(L, s);
     }
     uint32_t upto[2] = {n[0], n[1]};

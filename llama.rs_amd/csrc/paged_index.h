@@ -53,4 +53,13 @@ RLH_HD bool row_sees(const RowSpan& r, int32_t j) { return ((j >= r.lo) & (j < r
 RLH_HD int32_t span_begin(const RowSpan& first) { return first.prefix > 0 ? 0 : first.lo; }
 RLH_HD int32_t span_end(const RowSpan& last) { return last.hi > last.prefix ? last.hi : last.prefix; }
 
+// Steps of an item when the `steps` of all sequences (fewer than 2^24 each, so
+// that 32 bits hold the sum of 256 of them, not of 65535) are divided into
+// `goal` items: the sequences' own, rounded up, are at most `goal` and one each.
+RLH_HD uint32_t steps_per_item(uint64_t steps, uint32_t goal) {
+  const uint64_t n = (steps + goal - 1) / goal;
+  return n < 1u << 24 ? (uint32_t)n : 1u << 24;
+}
+RLH_HD uint32_t items_of(uint32_t steps, uint32_t per_item) { return (steps + per_item - 1) / per_item; }
+
 }  // namespace rlh
