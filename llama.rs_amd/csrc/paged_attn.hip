@@ -133,13 +133,37 @@ struct Scoring {
   uint32_t flip;          // sign bits of two halves: q is negated where scale < 0
   bool capped, biased;
 };
+// What the kernels' variants do to a score: nothing, cap and bias, or the same
+// with a cap above kNarrowCap (a variant of its own: the wide form beside the
+// other in one kernel made prompts with a bias 3 % slower).
+enum { kPlain = 0, kMod = 1, kWideCap = 2 };
+
+// Up to this cap a score may be off by 2^-23 of the cap (a probability by
+// 2^-17 of itself); above, tanh's own size counts.
+constexpr float kNarrowCap = 64.0f;
+// Larger caps are taken as this one, which changes no score below 2^88 in f32.
+constexpr float kMostCap = 0x1p100f;
 
 // tanh(y) = 1 - 2 / (exp(2 y) + 1): off by 2^-23 of the cap, at any y
 __device__ __forceinline__ float capped(const Scoring& c, float dot) {
   return fmaf(-2.0f * c.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(dot * c.mul) + 1.0f), c.cap2);
 }
+// Below |y| = 1/4 by the series y (1 - y^2 / 3 + 2 y^4 / 15 - 17 y^6 / 315 + 62
+// y^8 / 2835), off by 2^-26 of itself; x = dot * mul is y times 2 log2(e). The
+// products with the cap then cancel: a cap of any size leaves small scores as they are.
+__device__ __forceinline__ float capped_wide(const Scoring& c, float dot) {
+  constexpr float a = 0.34657359f, a2 = a * a;  // ln(2) / 2
+  const float x = dot * c.mul, z = x * x;
+  float p = a2 * a2 * a2 * a2 * 62.0f / 2835.0f;
+  p = fmaf(p, z, -a2 * a2 * a2 * 17.0f / 315.0f);
+  p = fmaf(p, z, a2 * a2 * 2.0f / 15.0f);
+  p = fmaf(p, z, -a2 / 3.0f);
+  p = fmaf(p, z, 1.0f);
+  return fabsf(x) < 0.72134752f ? x * (c.cap2 * a) * p : capped(c, dot);
+}
+template <int MOD>
 __device__ __forceinline__ float score(const Scoring& c, float dot, float slope2, float away) {
-  const float x = c.capped ? capped(c, dot) : dot * c.mul;
+  const float x = MOD == kWideCap ? capped_wide(c, dot) : c.capped ? capped(c, dot) : dot * c.mul;
   return c.biased ? fmaf(slope2, away, x) : x;
 }
 
@@ -289,7 +313,7 @@ __device__ __forceinline__ uint32_t small_steps(const AttnParams& a, uint32_t s,
 template <int D, int W>
 constexpr uint32_t kSmallLds = (W * 32 * (D * 2 + 32) > W * 16 * (D + 4) * 4 ? W * 32 * (D * 2 + 32) : W * 16 * (D + 4) * 4) + W * 128;
 
-template <typename T, int D, bool MOD, int W>
+template <typename T, int D, int MOD, int W>
 __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uint8_t* lds) {
   constexpr int kStride = D * 2 + 32;    // bytes of a V row in LDS: 8 rows start in 8 different bank groups
   constexpr int kSteps = D / 32;         // MFMAs of a score
@@ -445,7 +469,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const int32_t j = p + (i / 4) * 16 + (int32_t)quad * 4 + i % 4;
-        x[i] = MOD ? score(L.sc, sc[i / 4][i % 4], slope2, (float)(j - pos)) : sc[i / 4][i % 4];
+        x[i] = MOD ? score<MOD>(L.sc, sc[i / 4][i % 4], slope2, (float)(j - pos)) : sc[i / 4][i % 4];
       }
       if (!full) {
 #pragma unroll
@@ -542,7 +566,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   }
 }
 
-template <typename T, int D, bool MOD, int W>
+template <typename T, int D, int MOD, int W>
 __global__ void __launch_bounds__(64 * W, 2) k_attn_small(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
   small_block<T, D, MOD, W>(L, blockIdx.x, lds);
@@ -585,7 +609,7 @@ struct TileShared {
 template <int D>
 constexpr uint32_t kTileLds = 4 * kTileKv * D * 2 + sizeof(TileShared);
 
-template <typename T, int D, bool MOD>
+template <typename T, int D, int MOD>
 __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool prefix, uint8_t* lds) {
   constexpr int kRowB = D * 2;
   constexpr int kBuf = kTileKv * kRowB;   // bytes of a K or V step
@@ -853,7 +877,10 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
       asm volatile("" : "+v"(j0));
       float far = 0.0f;  // what all of the row's scores lack
       if constexpr (MOD) {
-        if (L.sc.capped) {
+        if constexpr (MOD == kWideCap) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) sc[i / 16][i % 16] = capped_wide(L.sc, sc[i / 16][i % 16]);
+        } else if (L.sc.capped) {
 #pragma unroll
           for (int i = 0; i < 32; i++) sc[i / 16][i % 16] = capped(L.sc, sc[i / 16][i % 16]);
         }
@@ -977,7 +1004,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
 // 32 heads behind 4096 shared positions: 28 us, in launches of their own
 // 20 + 17; 72 of 64 heads behind 16384: 70 us, apart 65 + 14 + 5; a prompt
 // alone loses 1 % by it).
-template <typename T, int D, bool MOD>
+template <typename T, int D, int MOD>
 __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
   const uint32_t n_prefix = prefix_blocks(L.n) * L.a.n_kv;
@@ -1192,7 +1219,7 @@ uint32_t tile_parts(uint64_t blocks, uint64_t positions) {
 // A score in units of log 2 per unit of the dot product (of 2 / softcap with a cap).
 float score_factor(const rlh_attn_args& args) {
   const float scale = fabsf(args.scale);
-  return args.softcap > 0.0f ? 2.0f * scale / args.softcap * kLog2e : scale * kLog2e;
+  return args.softcap > 0.0f ? 2.0f * scale / fminf(args.softcap, kMostCap) * kLog2e : scale * kLog2e;
 }
 
 int check_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
@@ -1290,7 +1317,7 @@ uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_att
 // device (idempotent, so two threads may).
 template <int D>
 constexpr uint32_t kMixedLds = kTileLds<D> > 2 * kSmallLds<D, kWaves> ? kTileLds<D> : 2 * kSmallLds<D, kWaves>;
-template <typename T, int D, bool MOD>
+template <typename T, int D, int MOD>
 int allow_lds(int device) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
@@ -1306,7 +1333,7 @@ int allow_lds(int device) {
   return RLH_OK;
 }
 
-template <typename T, int D, bool MOD>
+template <typename T, int D, int MOD>
 int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
   if (L.n.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, L);
@@ -1329,10 +1356,16 @@ int launch_attn(const Launch& L, int device, hipStream_t s) {
   return launched("rlh_paged_attn");
 }
 
+template <typename T, int D>
+int launch_attn(const Launch& L, int mod, int device, hipStream_t s) {
+  return mod == kPlain ? launch_attn<T, D, kPlain>(L, device, s)
+         : mod == kMod ? launch_attn<T, D, kMod>(L, device, s)
+                       : launch_attn<T, D, kWideCap>(L, device, s);
+}
+
 template <typename T>
-int launch_attn(const Launch& L, uint32_t dim, bool mod, int device, hipStream_t s) {
-  if (dim == 64) return mod ? launch_attn<T, 64, true>(L, device, s) : launch_attn<T, 64, false>(L, device, s);
-  return mod ? launch_attn<T, 128, true>(L, device, s) : launch_attn<T, 128, false>(L, device, s);
+int launch_attn(const Launch& L, uint32_t dim, int mod, int device, hipStream_t s) {
+  return dim == 64 ? launch_attn<T, 64>(L, mod, device, s) : launch_attn<T, 128>(L, mod, device, s);
 }
 
 }  // namespace
@@ -1402,11 +1435,11 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   place_workspace(&L.ws, (uint8_t*)workspace, *kv, *seqs, *args, L.n);
   L.sc.capped = args->softcap > 0.0f;
   L.sc.mul = score_factor(*args);
-  L.sc.cap2 = args->softcap * kLog2e;
+  L.sc.cap2 = fminf(args->softcap, kMostCap) * kLog2e;
   L.sc.flip = args->scale < 0.0f ? 0x80008000u : 0u;
   // (a scale of zero, which the exponential could not take in, goes with a bias of zero)
   L.sc.biased = args->slopes || (!L.sc.capped && L.sc.mul == 0.0f);
-  const bool mod = L.sc.capped || L.sc.biased;
+  const int mod = args->softcap > kNarrowCap ? kWideCap : L.sc.capped || L.sc.biased ? kMod : kPlain;
   if (kv->type == RLH_TYPE_F16) return launch_attn<_Float16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
   return launch_attn<__bf16>(L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
 }

@@ -6,7 +6,7 @@ import torch
 
 import rlh
 import serve_ref as ref
-from test_gpu_serve import run_sample
+from test_gpu_serve import ATTN, attn_case, check_attn, run_attn, run_sample
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +144,77 @@ def test_sample_nucleus_that_ends_deep():
     got = run_sample(torch.tensor(np.stack([v, v])).cuda(), rlh.F32, [(1.0, 0, p, 0.0)] * 2, np.ones(2, np.float32))
     want = ref.sample(v, 1.0, 0, p, 0.0, np.float32(1.0))
     assert 1000 < want < n - 1000 and abs(int(got[1]) - want) <= 21
+
+
+# ---- attention: caps, flat rows ------------------------------------------------------
+
+class Shared:
+    """`n_seq` sequences of `rows` new rows whose pages are the same ones."""
+
+    def __init__(self, k, v, n_seq, rows, heads, ty, page=64):
+        n, kv, dim = k.shape
+        pages = -(-n // page)
+        pool = torch.zeros((2, pages * page, kv, dim), dtype=torch.float64)
+        pool[0, :n], pool[1, :n] = k, v
+        pool = pool.view(2, pages, page, kv, dim).transpose(2, 3).contiguous().to(TORCH[ty]).cuda()
+        self.k, self.v, self.heads, self.dim, self.rows, self.n, self.kv_heads = pool[0], pool[1], heads, dim, rows, n, kv
+        self.table = torch.arange(pages, dtype=torch.int32).repeat(n_seq, 1).cuda()
+        self.q_start = (rows * torch.arange(n_seq + 1, dtype=torch.int32)).cuda()
+        self.kv_len = torch.full((n_seq,), n, dtype=torch.int32).cuda()
+        self.kv = rlh.KvPages(ty, kv, dim, page, pages, self.k.data_ptr(), self.v.data_ptr())
+        self.seqs = rlh.Seqs(n_seq, n_seq * rows, rows, n, pages, self.q_start.data_ptr(), self.kv_len.data_ptr(),
+                             self.table.data_ptr())
+
+    def run(self, q, scale, cap=0.0):
+        out = torch.full_like(q, 7.0)
+        args = rlh.AttnArgs(self.heads, 0, q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0), scale, cap, None, None,
+                            None, 0)
+        need = rlh.paged_attn_workspace(self.kv, self.seqs, args)
+        ws = torch.full((need + 16,), 0xff, dtype=torch.uint8, device="cuda")
+        rlh.paged_attn(self.kv, self.seqs, args, ws.data_ptr(), ws.numel() // 16 * 16, None,
+                       torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return out
+
+
+U = 2.0 ** -24
+
+
+@pytest.mark.parametrize("cap", [65.0, 1e3, 1e5, 1e8, 1e30, 3.4e38])
+@pytest.mark.parametrize("size", [1.0, 40.0])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_caps_far_above_the_scores(rows, size, cap):
+    """tanh's relative error counts, not the cap's: a score is off by what
+    the dot product is, (dim + 8) 2^-24 sum |q k|, and 16 half steps of its own
+    size for the cap's terms and the exponent's argument. That scales a
+    probability once in the sum with v and once in the sum below it; the rest
+    is the probabilities' rounding (of the smallest: to multiples of 2^-24), f32
+    sums of n terms and the result's rounding."""
+    n, heads, kv, dim, ty = 300, 4, 2, 128, rlh.F16
+    g = torch.Generator().manual_seed(rows)
+    k, v = [torch.randn((n, kv, dim), generator=g).half().double() for _ in range(2)]
+    q = (size * torch.randn((rows, heads * dim), generator=g)).half()
+    scale = float(np.float32(dim ** -0.5))
+    out = Shared(k, v, 1, rows, heads, ty).run(q.cuda(), scale, cap).double().cpu().view(rows, heads, dim)
+    cap = float(np.float32(cap))
+    see = torch.arange(n)[None, :] <= torch.arange(n - rows, n)[:, None]
+    half = torch.finfo(torch.float16).eps / 2
+    for h in range(heads):
+        qh, kh, vh = q.double().view(rows, heads, dim)[:, h], k[:, h // 2], v[:, h // 2]
+        t = scale * (qh @ kh.T)
+        ds = ((dim + 8) * U * scale * (qh.abs() @ kh.abs().T) + 16 * U * t.abs()).amax(1, keepdim=True)
+        p = torch.softmax(torch.where(see, cap * torch.tanh(t / cap), -float("inf")), 1)
+        want, near = p @ vh, p @ vh.abs()
+        bound = want.abs() * half + near * (half + 2 * (ds + n * U)) + 2.0 ** -25 * (see.double() @ vh.abs())
+        assert torch.all((out[:, h] - want).abs() <= bound), (h, float(((out[:, h] - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("cap", [65.0, 1e4])
+@pytest.mark.parametrize("name", ["everything", "shared everything", "cap 64", "mixed", "decode ragged", "bias", "shared"])
+def test_attention_larger_caps(name, cap):
+    """Caps above 64 beside every mask, type and head size."""
+    case = dict(ATTN[name], cap=cap, q_scale=12.0)
+    b, q, out, opts = attn_case(seed=21, **case)
+    run_attn(b, q, out, case["heads"], **opts)
+    torch.cuda.synchronize()
+    check_attn(b, q, out, case["heads"], opts)
