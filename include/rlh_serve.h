@@ -127,7 +127,8 @@ int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_app
  * A row that sees nothing, or only scores of minus infinity, is zero. q and
  * out are [n_rows][n_head][head_dim] of the pool's type with row strides, and
  * must not overlap. Scores, maxima and sums are f32; the probabilities are
- * rounded to the pool's type for the product with V. A cap of up to 64 puts a
+ * rounded to the pool's type for the product with V (in f16, those below 2^-21
+ * of the largest so far to multiples of 2^-31 of it). A cap of up to 64 puts a
  * score off by 2^-23 of the cap, a larger one by 2^-21 of the score; above 2^100
  * it is taken as 2^100.
  *

@@ -31,8 +31,14 @@ constexpr int kTileRows = 32 * kTileWaves;  // rows of a tile of the tiled kerne
 constexpr int kTileKv = 64;       // positions of its steps
 // The maximum that probabilities are relative to is only moved when the
 // running maximum has grown by more than 8 (in units of log 2): until then
-// they stay below 2^8, which f16 holds as exactly as values below one.
+// they stay below 2^8 times the factor below, which f16 holds.
 constexpr float kSlack = 8.0f;
+// Probabilities of f16 are formed 2^7 larger, just below f16's largest, in the
+// products with V and in their sums alike: what lies below 2^-14 of the maximum
+// would lose bits as f16 and vanish below 2^-25, though the sum counts it (20000
+// positions 17.5 below one: all of their share of the result). bf16 has f32's exponents.
+template <typename T>
+constexpr float kLift = __is_same(T, _Float16) ? 7.0f : 0.0f;
 
 #define RLH_CONST __attribute__((address_space(4)))
 #define RLH_LDS_PTR(T) __attribute__((address_space(3))) T
@@ -491,7 +497,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
         for (int i = 0; i < kOut; i++) o[i] *= f;
         m = mn;
       }
-      const float mb = m == -INFINITY ? 0.0f : m;
+      const float mb = (m == -INFINITY ? 0.0f : m) - kLift<T>;
       vec8<T> pr;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -917,7 +923,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
         for (int i = 0; i < kOut; i++) o[i] *= f;
         m = mn;
       }
-      const float mb = (m == -INFINITY ? 0.0f : m) - far;
+      const float mb = (m == -INFINITY ? 0.0f : m) - far - kLift<T>;
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll

@@ -218,3 +218,28 @@ def test_attention_larger_caps(name, cap):
     run_attn(b, q, out, case["heads"], **opts)
     torch.cuda.synchronize()
     check_attn(b, q, out, case["heads"], opts)
+
+
+@pytest.mark.parametrize("top", ["first", "last"])
+@pytest.mark.parametrize("n_seq,rows,kv", [(100, 1, 8), (20, 64, 8)])
+def test_attention_flat_rows_in_f16(n_seq, rows, kv, top):
+    """One score 17.5 above thousands of equal ones: each has less than 2^-25
+    of its weight, all of them what counts (the first's value is zero).
+    The result is off by its own rounding, by f32's sums, and by what half a step of
+    f16's smallest, 2^-25, is of probabilities of up to 2^7 and more: 2^-32 a position."""
+    n, dim, group = 20000, 128, 4
+    k = torch.zeros((n, kv, dim), dtype=torch.float64)
+    v = torch.ones((n, kv, dim), dtype=torch.float64)
+    at = 0 if top == "first" else n - rows
+    k[at, :, 0] = 17.5
+    v[at] = 0.0
+    q = torch.zeros((n_seq * rows, kv * group, dim), dtype=torch.float16)
+    q[:, :, 0] = 8.0
+    b = Shared(k, v, n_seq, rows, kv * group, rlh.F16)
+    out = b.run(q.view(n_seq * rows, -1).cuda(), 0.125).double().view(n_seq, rows, kv * group * dim)
+    seen = torch.arange(n - rows, n, dtype=torch.float64, device="cuda")[None, :, None] + 1
+    w = float(np.exp(-17.5))
+    L = 1 + (seen - 1) * w
+    want = (seen - 1) * w / L
+    bound = want * (2.0 ** -11 + 2 * (40 + n) * U) + seen * 2.0 ** -32 / L + 2.0 ** -25
+    assert torch.all((out - want).abs() <= bound), (float(out.min()), float(out.max()), float(want.min()))
