@@ -137,9 +137,12 @@ int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_app
  * page_size]) and are read once for the whole batch; the sequences' own
  * table entries before shared_len / page_size are not read.
  *
- * The workspace size follows from the sizes alone (heads, n_seq, n_rows, max_q,
- * max_kv, shared_len) and may be 0, as it is for arguments that
- * rlh_paged_attn refuses. */
+ * The workspace size follows from the sizes alone (heads, head_dim, n_seq,
+ * n_rows, max_q, max_kv, shared_len) and may be 0, as it is for arguments that
+ * rlh_paged_attn refuses. It is enough for every call with these heads and n_seq,
+ * n_rows, max_q, max_kv and shared_len up to these (a smaller batch may take
+ * more than a larger one, as its work is divided into more parts): asked for
+ * a host's limits, it is made once. */
 typedef struct rlh_attn_args {
   uint32_t n_head, window;
   const void* q;

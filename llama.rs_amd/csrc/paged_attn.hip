@@ -1213,6 +1213,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
 
 constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into (three to a CU)
 
+uint32_t item_goal(uint32_t n_head_kv) { return std::max(1u, kSmallBlocks / n_head_kv); }
+
 // Parts that the positions of `blocks` tiles are divided into: as many as let
 // all blocks run at once (one to a CU), of at least 256 positions (of 128,
 // what 64 tokens behind 4096 shared positions take grows from 33 + 8 us to
@@ -1262,7 +1264,7 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
   n.small_rows = n.small ? kSmallRows : 0;
   if (n.small) {
     n.whole = !n.tiled && !args.shared_len && q.max_kv <= kWhole && q.n_seq * kv.n_head_kv <= 256;
-    n.item_goal = n.whole ? 1 : std::max(1u, kSmallBlocks / kv.n_head_kv);
+    n.item_goal = n.whole ? 1 : item_goal(kv.n_head_kv);
     n.items = q.n_seq + (n.whole ? 0 : n.item_goal);
   }
   if (n.tiled) {
@@ -1290,33 +1292,64 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
   return n;
 }
 
+// Values and records of a workspace's parts.
+struct Room {
+  uint64_t prefix, tile, item;  // partial results of a row and head (or of an item's row)
+  uint64_t plan, tiles;         // sequences
+};
+
+// What a call takes.
+Room attn_room(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args, const Sizes& n) {
+  const uint64_t rows = (uint64_t)q.n_rows * args.n_head;
+  Room r{};
+  r.prefix = args.shared_len ? n.prefix_parts * rows : 0;
+  r.tile = n.tiled && (n.tile_parts > 1 || args.shared_len) ? n.tile_parts * rows : 0;
+  r.item = n.small && n.merge ? (uint64_t)n.items * kv.n_head_kv * kSmallRows : 0;
+  r.plan = n.small ? q.n_seq : 0;
+  r.tiles = n.planned && n.tiled ? q.n_seq : 0;
+  return r;
+}
+
+// What no call with n_seq, n_rows, max_q, max_kv and shared_len up to these
+// takes more of. Parts let their tiles' blocks run at once: parts * tiles *
+// n_head_kv <= 256, where tiles of 256 rows hold all rows of a KV head, so
+// that parts * rows <= 2^16 if there is more than one part (for a last prefix
+// tile of up to 128 rows as well: 20 (tiles - 1/2) < 20 tiles - 9).
+Room attn_room_within(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
+  const uint64_t group = args.n_head / kv.n_head_kv, rows = (uint64_t)q.n_rows * args.n_head;
+  auto divided = [&](uint64_t positions) {  // 0: never
+    const uint64_t parts = tile_parts(kv.n_head_kv, positions);
+    return parts > 1 ? std::min<uint64_t>(256 * kTileRows, parts * rows) : 0;
+  };
+  const bool tiled = q.max_q * group > kSmallRows, small = group <= kSmallRows;
+  const bool whole = q.max_kv <= kWhole && q.n_seq * kv.n_head_kv <= 256 && (!tiled || q.n_seq == 1);
+  Room r{};
+  if (args.shared_len) r.prefix = std::max(rows, divided(args.shared_len));
+  if (tiled) r.tile = std::max(args.shared_len ? rows : 0, divided(q.max_kv));
+  if (small && (args.shared_len || (!whole && q.max_kv > 32 * kWaves)))
+    r.item = ((uint64_t)q.n_seq + item_goal(kv.n_head_kv)) * kv.n_head_kv * kSmallRows;
+  r.plan = small ? q.n_seq : 0;
+  r.tiles = q.n_seq > kPlanned && tiled ? q.n_seq : 0;
+  return r;
+}
+
 // Places the workspace's parts from `base` on (null: counts only); bytes.
-uint64_t place_workspace(Workspace* w, uint8_t* base, const rlh_kv_pages& kv, const rlh_seqs& q,
-                         const rlh_attn_args& args, const Sizes& n) {
+uint64_t place_workspace(Workspace* w, uint8_t* base, uint64_t dim, const Room& r) {
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     uint8_t* p = base ? base + at : nullptr;
     at += (bytes + 255) / 256 * 256;
     return p;
   };
-  const uint64_t D = kv.head_dim, rows = (uint64_t)q.n_rows * args.n_head;
-  const uint64_t pr = args.shared_len ? n.prefix_parts * rows : 0;
-  const uint64_t tr = n.tiled && (n.tile_parts > 1 || args.shared_len) ? n.tile_parts * rows : 0;
-  const uint64_t ir = n.small && n.merge ? (uint64_t)n.items * kv.n_head_kv * kSmallRows : 0;
-  w->prefix_o = (float*)take(pr * D * 4);
-  w->prefix_ml = (float*)take(pr * 8);
-  w->tile_o = (float*)take(tr * D * 4);
-  w->tile_ml = (float*)take(tr * 8);
-  w->item_o = (float*)take(ir * D * 4);
-  w->item_ml = (float*)take(ir * 8);
-  w->plan = (uint32_t*)take(n.small ? (uint64_t)q.n_seq * 8 : 0);
-  w->tiles = (uint32_t*)take(n.planned && n.tiled ? (uint64_t)q.n_seq * 8 : 0);
+  w->prefix_o = (float*)take(r.prefix * dim * 4);
+  w->prefix_ml = (float*)take(r.prefix * 8);
+  w->tile_o = (float*)take(r.tile * dim * 4);
+  w->tile_ml = (float*)take(r.tile * 8);
+  w->item_o = (float*)take(r.item * dim * 4);
+  w->item_ml = (float*)take(r.item * 8);
+  w->plan = (uint32_t*)take(r.plan * 8);
+  w->tiles = (uint32_t*)take(r.tiles * 8);
   return at;
-}
-
-uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
-  Workspace w;
-  return place_workspace(&w, nullptr, kv, q, args, attn_sizes(kv, q, args));
 }
 
 // The mixed kernels take more LDS than a launch may by default; said once per
@@ -1383,7 +1416,8 @@ extern "C" {
 
 uint64_t rlh_paged_attn_workspace(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
   if (check_attn(kv, seqs, args) != RLH_OK || seqs->n_seq == 0 || seqs->n_rows == 0) return 0;
-  return attn_workspace(*kv, *seqs, *args);
+  Workspace w;
+  return place_workspace(&w, nullptr, kv->head_dim, attn_room_within(*kv, *seqs, *args));
 }
 
 int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args, void* workspace,
@@ -1391,7 +1425,9 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   RLH_TRY(check_attn(kv, seqs, args));
   if (!aligned(status, 4)) return serve_error(RLH_EINVAL, "status is not aligned to 4 bytes");
   if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;
-  const uint64_t need = attn_workspace(*kv, *seqs, *args);
+  Launch L{};
+  L.n = attn_sizes(*kv, *seqs, *args);
+  const uint64_t need = place_workspace(&L.ws, (uint8_t*)workspace, kv->head_dim, attn_room(*kv, *seqs, *args, L.n));
   if (need && !workspace) return serve_error(RLH_EINVAL, "workspace is null");
   if (need > workspace_bytes)
     return serve_error(RLH_EINVAL, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
@@ -1435,10 +1471,7 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   p.n_pages = (uint32_t)kv->n_pages;
   p.window = args->window;
   p.shared_len = args->shared_len;
-  Launch L{};
   L.a = p;
-  L.n = attn_sizes(*kv, *seqs, *args);
-  place_workspace(&L.ws, (uint8_t*)workspace, *kv, *seqs, *args, L.n);
   L.sc.capped = args->softcap > 0.0f;
   L.sc.mul = score_factor(*args);
   L.sc.cap2 = fminf(args->softcap, kMostCap) * kLog2e;

@@ -530,7 +530,8 @@ def paged_append(kv, seqs, args, status=None, stream=None):
 
 
 def paged_attn_workspace(kv, seqs, args):
-    """Workspace bytes of paged_attn for these arguments (0: none, or refused)."""
+    """Workspace bytes of paged_attn for these arguments and every smaller batch
+    (0: none, or refused)."""
     return load().rlh_paged_attn_workspace(kv, seqs, args)
 
 

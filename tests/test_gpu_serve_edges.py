@@ -243,3 +243,28 @@ def test_attention_flat_rows_in_f16(n_seq, rows, kv, top):
     want = (seen - 1) * w / L
     bound = want * (2.0 ** -11 + 2 * (40 + n) * U) + seen * 2.0 ** -32 / L + 2.0 ** -25
     assert torch.all((out - want).abs() <= bound), (float(out.min()), float(out.max()), float(want.min()))
+
+
+def test_attention_one_workspace_for_limits():
+    """Prompts, single tokens, drafts and a shared prefix in the workspace of a
+    host's limits, one after the other."""
+    heads, kv, dim, page, ty = 8, 2, 128, 16, rlh.BF16
+    batches = [dict(seqs=[(700, 700)]), dict(seqs=[(1, 3000)]), dict(seqs=[(130, 2500), (1, 9)]), dict(seqs=[(4, 2000)] * 3),
+               dict(seqs=[(1, 40)] * 30), dict(seqs=[(1, 1100 + i) for i in range(9)], shared=1024),
+               dict(seqs=[(3, 1100), (40, 1500)], shared=1024), dict(seqs=[(200, 2999)])]
+    first = attn_case(seed=1, heads=heads, kv=kv, dim=dim, page=page, ty=ty, **batches[5])[0]
+    p = first.q_start.data_ptr()
+    limits = rlh.Seqs(30, 700, 700, 3000, -(-3000 // page), p, p, p)
+    args = rlh.AttnArgs(heads, 0, first.k.data_ptr(), first.v.data_ptr() + (1 << 40), heads * dim, heads * dim, 0.1, 0.0,
+                        None, None, p, 1024)
+    need = rlh.paged_attn_workspace(first.kv(), limits, args)
+    assert 0 < need < 64 << 20
+    guard = torch.full((need + 4096,), 0xa5, dtype=torch.uint8, device="cuda")
+    ws = guard[:need]
+    for i, batch in enumerate(batches):
+        ws.fill_(0xff)
+        b, q, out, opts = attn_case(seed=30 + i, heads=heads, kv=kv, dim=dim, page=page, ty=ty, **batch)
+        run_attn(b, q, out, heads, ws=ws, **opts)
+        torch.cuda.synchronize()
+        check_attn(b, q, out, heads, opts)
+    assert torch.all(guard[need:] == 0xa5)

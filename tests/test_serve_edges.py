@@ -6,6 +6,8 @@ import subprocess
 import numpy as np
 import pytest
 
+import rlh
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
@@ -43,3 +45,55 @@ def test_items_fit_their_list(plan_shim, goal):
     for steps, times in cases:
         n, per = items(plan_shim, steps, times, goal)
         assert 1 <= per <= 1 << 24 and int(np.sum(times)) <= n <= int(np.sum(times)) + goal, (steps, times, n, per)
+
+
+# ---- one workspace for all batches within limits ------------------------------------
+
+A = 1 << 40  # spacing of addresses that are never read
+
+
+def attention_args(heads, kv, dim, n_seq, n_rows, max_q, max_kv, shared, page=64):
+    pool = rlh.KvPages(rlh.F16, kv, dim, page, 16, A, 2 * A)
+    seqs = rlh.Seqs(n_seq, n_rows, max_q, max_kv, -(-max_kv // page), 3 * A, 4 * A, 5 * A)
+    att = rlh.AttnArgs(heads, 0, 6 * A, 8 * A, heads * dim, heads * dim, 0.1, 0.0, None, None, 10 * A if shared else None,
+                       shared)
+    return pool, seqs, att
+
+
+def log_int(rng, lo, hi):
+    return int(np.exp(rng.uniform(np.log(lo), np.log(hi + 1))))
+
+
+@pytest.mark.parametrize("heads,kv", [(64, 8), (16, 8), (8, 8), (12, 1), (40, 2), (28, 4), (128, 128), (512, 512)])
+def test_a_workspace_serves_every_smaller_batch(heads, kv):
+    """The size for some limits is accepted (as the checks before the device
+    go) by every batch within them, and does not fall as limits rise."""
+    rng = np.random.default_rng(heads)
+    lib = rlh.load()
+    for _ in range(60):
+        most_q = log_int(rng, 1, 4096)
+        n_seq = log_int(rng, 1, 600)
+        n_rows = most_q + log_int(rng, 1, 6000) - 1
+        max_kv = max(most_q, log_int(rng, 1, 60000))
+        shared = 64 * log_int(rng, 1, 400) if rng.random() < 0.4 else 0
+        limits = attention_args(heads, kv, 128, n_seq, n_rows, most_q, max_kv, shared)
+        size = lib.rlh_paged_attn_workspace(*limits)
+        for _ in range(40):
+            rows = log_int(rng, 1, n_rows)
+            q = min(rows, log_int(rng, 1, most_q))
+            less = attention_args(heads, kv, 128, log_int(rng, 1, n_seq), rows, q, max(q, log_int(rng, 1, max_kv)),
+                                  64 * int(rng.integers(0, shared // 64 + 1)))
+            rc = lib.rlh_paged_attn(*less, 16 * A, size, None, None)
+            assert rc in (rlh.RLH_EDEVICE, rlh.RLH_EINVAL), rc
+            assert not lib.rlh_last_error().startswith(b"workspace"), (lib.rlh_last_error(), size)
+            assert lib.rlh_paged_attn_workspace(*less) <= size
+
+
+def test_workspace_of_a_server():
+    """A prompt chunk's limits hold a token's and a short chunk's calls, and stay small."""
+    lib = rlh.load()
+    size = lib.rlh_paged_attn_workspace(*attention_args(64, 8, 128, 64, 4096, 4096, 40000, 0))
+    assert 0 < size < 64 << 20
+    for rows in (1, 100, 256, 300, 512, 2048, 4096):
+        assert lib.rlh_paged_attn(*attention_args(64, 8, 128, 1, rows, rows, 40000, 0), 16 * A, size, None, None) != rlh.RLH_OK
+        assert not lib.rlh_last_error().startswith(b"workspace")
