@@ -276,6 +276,14 @@ int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_app
       overlaps_pool(*kv, args->k, row_bytes_span(n, args->k_stride, kw, is)) ||
       overlaps_pool(*kv, args->v, row_bytes_span(n, args->v_stride, kw, is)))
     return serve_error(RLH_EINVAL, "the pool overlaps q, k, v or q_out");
+  const Area q_start = area_q_start(*seqs), kv_len = area_kv_len(*seqs), table = area_table(*seqs, kv->page_size),
+             q_norm = area("q_norm", args->q_norm, D * 4), k_norm = area("k_norm", args->k_norm, D * 4),
+             freqs = area("freqs", args->rot_dim ? args->freqs : nullptr, args->rot_dim / 2 * 8),
+             st = area("status", status, 4), q_out{"q_out", args->q_out, n, args->q_out_stride * 2, qw * 2};
+  for (const Area& written : {q_out, area("the pool", kv->k, pool_bytes(*kv)), area("the pool", kv->v, pool_bytes(*kv))})
+    RLH_TRY(check_apart(written, {q_start, kv_len, table, q_norm, k_norm, freqs, st}));
+  RLH_TRY(check_apart(st, {q_start, kv_len, table, q_norm, k_norm, freqs, Area{"q", args->q, n, args->q_stride * is, qw * is},
+                           Area{"k", args->k, n, args->k_stride * is, kw * is}, Area{"v", args->v, n, args->v_stride * is, kw * is}}));
   DeviceCheck dev;
   RLH_TRY(dev.begin());
   RLH_TRY(dev("k pages", kv->k));

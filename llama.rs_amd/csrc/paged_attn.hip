@@ -1437,6 +1437,16 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
       overlap(workspace, need, args->out, row_bytes_span(seqs->n_rows, args->out_stride, w, 2)) ||
       overlaps_pool(*kv, workspace, need))
     return serve_error(RLH_EINVAL, "workspace overlaps q, out or the pool");
+  const uint64_t rows = seqs->n_rows;
+  const Area q_start = area_q_start(*seqs), kv_len = area_kv_len(*seqs), table = area_table(*seqs, kv->page_size),
+             slopes = area("slopes", args->slopes, args->n_head * 4ull),
+             prefix_len = area("prefix_len", args->prefix_len, seqs->n_seq * 4ull),
+             shared = area("shared_table", args->shared_len ? args->shared_table : nullptr, args->shared_len / kv->page_size * 4ull),
+             st = area("status", status, 4);
+  for (const Area& written : {Area{"out", args->out, rows, args->out_stride * 2, w * 2}, area("workspace", need ? workspace : nullptr, need)})
+    RLH_TRY(check_apart(written, {q_start, kv_len, table, slopes, prefix_len, shared, st}));
+  RLH_TRY(check_apart(st, {q_start, kv_len, table, slopes, prefix_len, shared, Area{"q", args->q, rows, args->q_stride * 2, w * 2},
+                           area("the pool", kv->k, pool_bytes(*kv)), area("the pool", kv->v, pool_bytes(*kv))}));
   DeviceCheck dev;
   RLH_TRY(dev.begin());
   RLH_TRY(dev("k pages", kv->k));

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <string>
 
 #include "../../include/rlh_serve.h"
@@ -46,6 +47,37 @@ inline uint64_t pool_bytes(const rlh_kv_pages& kv) {
 }
 inline bool overlaps_pool(const rlh_kv_pages& kv, const void* p, uint64_t n) {
   return overlap(p, n, kv.k, pool_bytes(kv)) || overlap(p, n, kv.v, pool_bytes(kv));
+}
+
+// An argument's memory: `rows` of `width` bytes, `stride` bytes apart.
+struct Area {
+  const char* name;
+  const void* p;
+  uint64_t rows, stride, width;
+  uint64_t span() const { return rows ? (rows - 1) * stride + width : 0; }
+};
+inline Area area(const char* name, const void* p, uint64_t bytes) { return Area{name, p, 1, bytes, bytes}; }
+
+// Whether they share a byte; what lies between one's rows is not its own (of
+// two with gaps, the second counts as a whole).
+inline bool meet(const Area& a, const Area& b) {
+  if (!a.p || !b.p || !overlap(a.p, a.span(), b.p, b.span())) return false;
+  if (a.rows == 1 && b.rows > 1) return meet(b, a);
+  if ((uintptr_t)b.p < (uintptr_t)a.p) return true;
+  const uint64_t off = (uintptr_t)b.p - (uintptr_t)a.p, row = off / a.stride;
+  return off % a.stride < a.width || (row + 1 < a.rows && (row + 1) * a.stride < off + b.span());
+}
+inline int check_apart(const Area& written, std::initializer_list<Area> others) {
+  for (const Area& o : others)
+    if (meet(written, o)) return serve_error(RLH_EINVAL, std::string(written.name) + " overlaps " + o.name);
+  return RLH_OK;
+}
+
+// The batch's arrays.
+inline Area area_q_start(const rlh_seqs& s) { return area("q_start", s.q_start, ((uint64_t)s.n_seq + 1) * 4); }
+inline Area area_kv_len(const rlh_seqs& s) { return area("kv_len", s.kv_len, (uint64_t)s.n_seq * 4); }
+inline Area area_table(const rlh_seqs& s, uint32_t page_size) {
+  return Area{"table", s.table, s.n_seq, (uint64_t)s.table_stride * 4, ((uint64_t)s.max_kv + page_size - 1) / page_size * 4};
 }
 
 // The pool and the batch (no device needed).

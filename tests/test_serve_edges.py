@@ -97,3 +97,76 @@ def test_workspace_of_a_server():
     for rows in (1, 100, 256, 300, 512, 2048, 4096):
         assert lib.rlh_paged_attn(*attention_args(64, 8, 128, 1, rows, rows, 40000, 0), 16 * A, size, None, None) != rlh.RLH_OK
         assert not lib.rlh_last_error().startswith(b"workspace")
+
+
+# ---- what a call writes overlaps nothing else of it ----------------------------------
+
+B = 1 << 20
+D, HEADS, KV, ROWS, SEQS = 128, 4, 2, 6, 3
+PLACES = dict(k_pages=1 * B, v_pages=2 * B, q_start=3 * B, kv_len=4 * B, table=5 * B, q=6 * B, k=7 * B, v=8 * B, q_norm=9 * B,
+              k_norm=10 * B, freqs=11 * B, out=12 * B, slopes=13 * B, prefix_len=14 * B, shared_table=15 * B, status=16 * B,
+              workspace=17 * B)
+# bytes of each: 8 pages of 16 positions, rows of 640 values in all of which q takes 512
+SIZE = dict(k_pages=8 * KV * 16 * D * 2, v_pages=8 * KV * 16 * D * 2, q_start=4 * (SEQS + 1), kv_len=4 * SEQS,
+            table=4 * (2 * 6 + 4), q_norm=4 * D, k_norm=4 * D, freqs=8 * 64, slopes=4 * HEADS, prefix_len=4 * SEQS,
+            shared_table=4, status=4)
+STRIDE = 640
+
+
+def call(op, **moved):
+    at = {**PLACES, **moved}
+    kv = rlh.KvPages(rlh.F16, KV, D, 16, 8, at["k_pages"], at["v_pages"])
+    # rows of 6 page ids, of which 4 are used
+    seqs = rlh.Seqs(SEQS, ROWS, 2, 60, 6, at["q_start"], at["kv_len"], at["table"])
+    lib = rlh.load()
+    if op == "append":
+        args = rlh.AppendArgs(rlh.F16, HEADS, at["q"], at["k"], at["v"], STRIDE, STRIDE, STRIDE, at["q_norm"], at["k_norm"],
+                              1e-6, 1.0, at["freqs"], 128, 0, at["out"], STRIDE)
+        rc = lib.rlh_paged_append(kv, seqs, args, at["status"], None)
+    else:
+        args = rlh.AttnArgs(HEADS, 0, at["q"], at["out"], STRIDE, STRIDE, 0.1, 0.0, at["slopes"], at["prefix_len"],
+                            at["shared_table"], 16)
+        rc = lib.rlh_paged_attn(kv, seqs, args, at["workspace"], 1 << 40, at["status"], None)
+    return rc, lib.rlh_last_error().decode()
+
+
+READ = {"append": ["q_start", "kv_len", "table", "q_norm", "k_norm", "freqs"],
+        "attn": ["q_start", "kv_len", "table", "slopes", "prefix_len", "shared_table"]}
+WRITTEN = {"append": ["out", "k_pages", "v_pages"], "attn": ["out", "workspace"]}
+
+
+@pytest.mark.parametrize("op", ["append", "attn"])
+def test_written_memory_is_apart_from_the_arrays(op):
+    name = {"out": "q_out" if op == "append" else "out", "k_pages": "the pool", "v_pages": "the pool", "workspace": "workspace"}
+    assert "overlap" not in call(op)[1]
+    for w in WRITTEN[op]:
+        start = PLACES[w]
+        for r in READ[op] + ["status"]:
+            # its last bytes are the area's first, its first ones lie in a row
+            unit = 16 if r.endswith("norm") else 8 if r == "freqs" else 4  # (as it has to be aligned)
+            for place in (start - SIZE[r] + unit, start + 2 * STRIDE * 2 + 1008):
+                rc, said = call(op, **{r: place})
+                assert rc == rlh.RLH_EINVAL and said == "%s overlaps %s" % (name[w], r), (w, r, said)
+    for r in READ[op] + ["q"]:
+        rc, said = call(op, status=PLACES[r] + (0 if r == "q" else SIZE[r] - 4))
+        assert rc == rlh.RLH_EINVAL and said == "status overlaps " + r, (r, said)
+    for r in ("k_pages", "v_pages"):
+        rc, said = call(op, status=PLACES[r] + SIZE[r] - 4)
+        assert rc == rlh.RLH_EINVAL and "overlap" in said and "status" in said, (r, said)
+
+
+@pytest.mark.parametrize("op", ["append", "attn"])
+def test_memory_between_rows_is_free(op):
+    """Arrays in the gap behind each output row, a status word behind a row of
+    q or of the table: nothing overlaps."""
+    gap = PLACES["out"] + 512 * 2
+    for r in READ[op] + ["status"]:
+        if SIZE[r] > 256:
+            continue
+        rc, said = call(op, **{r: gap + STRIDE * 2})
+        assert "overlap" not in said, (r, said)
+    assert "overlap" not in call(op, status=PLACES["q"] + 512 * 2)[1]
+    assert "overlap" not in call(op, status=PLACES["table"] + 4 * 4)[1]
+    assert "overlaps" in call(op, status=PLACES["table"] + 6 * 4)[1]
+    assert "overlaps" in call(op, status=PLACES["table"] + (2 * 6 + 3) * 4)[1]
+    assert "overlap" not in call(op, status=PLACES["table"] + (2 * 6 + 4) * 4)[1]
