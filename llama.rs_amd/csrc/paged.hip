@@ -190,29 +190,20 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(AppendParams a) {
 }
 
 template <typename TI, typename TO, int D>
-void launch_append(const AppendParams& p, bool inter, hipStream_t s) {
+int launch_append(const AppendParams& p, bool inter, hipStream_t s) {
   const uint32_t per = kThreads / (D / 8);
   const dim3 grid(p.b.n_rows, (p.n_head + 2 * p.n_kv + per - 1) / per);
-  if (inter)
-    hipLaunchKernelGGL((k_paged_append<TI, TO, D, true>), grid, dim3(kThreads), 0, s, p);
-  else
-    hipLaunchKernelGGL((k_paged_append<TI, TO, D, false>), grid, dim3(kThreads), 0, s, p);
+  return enqueue("rlh_paged_append", inter ? k_paged_append<TI, TO, D, true> : k_paged_append<TI, TO, D, false>, grid, kThreads, 0, s, p);
 }
 
 template <typename TI, typename TO>
-void launch_append(const AppendParams& p, uint32_t dim, bool inter, hipStream_t s) {
-  if (dim == 64)
-    launch_append<TI, TO, 64>(p, inter, s);
-  else
-    launch_append<TI, TO, 128>(p, inter, s);
+int launch_append(const AppendParams& p, uint32_t dim, bool inter, hipStream_t s) {
+  return dim == 64 ? launch_append<TI, TO, 64>(p, inter, s) : launch_append<TI, TO, 128>(p, inter, s);
 }
 
 template <typename TI>
-void launch_append(const AppendParams& p, uint32_t type, uint32_t dim, bool inter, hipStream_t s) {
-  if (type == RLH_TYPE_F16)
-    launch_append<TI, _Float16>(p, dim, inter, s);
-  else
-    launch_append<TI, __bf16>(p, dim, inter, s);
+int launch_append(const AppendParams& p, uint32_t type, uint32_t dim, bool inter, hipStream_t s) {
+  return type == RLH_TYPE_F16 ? launch_append<TI, _Float16>(p, dim, inter, s) : launch_append<TI, __bf16>(p, dim, inter, s);
 }
 
 }  // namespace
@@ -324,13 +315,9 @@ int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_app
   p.pool_v = kv->v;
   p.status = status;
   const bool inter = args->interleaved != 0;
-  if (args->in_type == RLH_TYPE_F32)
-    launch_append<float>(p, kv->type, D, inter, (hipStream_t)stream);
-  else if (args->in_type == RLH_TYPE_F16)
-    launch_append<_Float16>(p, kv->type, D, inter, (hipStream_t)stream);
-  else
-    launch_append<__bf16>(p, kv->type, D, inter, (hipStream_t)stream);
-  return launched("rlh_paged_append");
+  if (args->in_type == RLH_TYPE_F32) return launch_append<float>(p, kv->type, D, inter, (hipStream_t)stream);
+  if (args->in_type == RLH_TYPE_F16) return launch_append<_Float16>(p, kv->type, D, inter, (hipStream_t)stream);
+  return launch_append<__bf16>(p, kv->type, D, inter, (hipStream_t)stream);
 }
 
 }  // extern "C"

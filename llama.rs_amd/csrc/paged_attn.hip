@@ -1375,24 +1375,22 @@ int allow_lds(int device) {
 template <typename T, int D, int MOD>
 int launch_attn(const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
-  if (L.n.planned) hipLaunchKernelGGL(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, L);
+  const char* what = "rlh_paged_attn";
+  if (L.n.planned) RLH_TRY(enqueue(what, k_attn_plan, dim3(1), kPlanThreads, 0, s, L));
   if (L.a.shared_len || L.n.tiled) {
     RLH_TRY((allow_lds<T, D, MOD>(device)));
     const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts) * G + (L.n.items * G + 1) / 2;
-    hipLaunchKernelGGL((k_attn_mixed<T, D, MOD>), dim3(blocks), dim3(64 * kTileWaves), kMixedLds<D>, s, L);
+    RLH_TRY(enqueue(what, k_attn_mixed<T, D, MOD>, dim3(blocks), 64 * kTileWaves, kMixedLds<D>, s, L));
   } else if (L.n.whole) {
     RLH_TRY((allow_lds<T, D, MOD>(device)));
-    hipLaunchKernelGGL((k_attn_small<T, D, MOD, kTileWaves>), dim3(L.n.items * G), dim3(64 * kTileWaves),
-                       (kSmallLds<D, kTileWaves>), s, L);
+    RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kTileWaves>, dim3(L.n.items * G), 64 * kTileWaves, kSmallLds<D, kTileWaves>, s, L));
   } else {
-    hipLaunchKernelGGL((k_attn_small<T, D, MOD, kWaves>), dim3(L.n.items * G), dim3(kThreads), (kSmallLds<D, kWaves>), s, L);
+    RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kWaves>, dim3(L.n.items * G), kThreads, kSmallLds<D, kWaves>, s, L));
   }
-  if (L.n.merge) {
-    const uint64_t blocks = L.n.merge_small ? (uint64_t)L.a.b.n_seq * L.n.merge_rows * G
-                                            : ((uint64_t)L.a.b.n_rows * L.a.n_head + kWaves - 1) / kWaves;
-    hipLaunchKernelGGL((k_attn_merge<T, D>), dim3((uint32_t)blocks), dim3(kThreads), 0, s, L);
-  }
-  return launched("rlh_paged_attn");
+  if (!L.n.merge) return RLH_OK;
+  const uint64_t blocks = L.n.merge_small ? (uint64_t)L.a.b.n_seq * L.n.merge_rows * G
+                                          : ((uint64_t)L.a.b.n_rows * L.a.n_head + kWaves - 1) / kWaves;
+  return enqueue(what, k_attn_merge<T, D>, dim3((uint32_t)blocks), kThreads, 0, s, L);
 }
 
 template <typename T, int D>

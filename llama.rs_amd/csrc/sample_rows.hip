@@ -1133,12 +1133,12 @@ Space sample_space(void* base, uint64_t n) {
 }
 
 template <typename T>
-void launch_sample(const void* logits, uint64_t n_rows, uint64_t n, uint64_t stride, const rlh_row_sampling* options,
-                   const float* u, uint32_t* tokens, const Space& space, hipStream_t s) {
-  hipLaunchKernelGGL(k_sample_scan<T>, dim3(space.chunks * (uint32_t)n_rows), dim3(kScanThreads), 0, s, (const T*)logits,
-                     (uint32_t)n, stride, options, space);
-  hipLaunchKernelGGL(k_sample_pick<T>, dim3((uint32_t)n_rows), dim3(kThreads), 0, s, (const T*)logits, (uint32_t)n,
-                     stride, options, u, tokens, space);
+int launch_sample(const void* logits, uint64_t n_rows, uint64_t n, uint64_t stride, const rlh_row_sampling* options,
+                  const float* u, uint32_t* tokens, const Space& space, hipStream_t s) {
+  RLH_TRY(enqueue("rlh_sample_rows", k_sample_scan<T>, dim3(space.chunks * (uint32_t)n_rows), kScanThreads, 0, s, (const T*)logits,
+                  (uint32_t)n, stride, options, space));
+  return enqueue("rlh_sample_rows", k_sample_pick<T>, dim3((uint32_t)n_rows), kThreads, 0, s, (const T*)logits, (uint32_t)n, stride,
+                 options, u, tokens, space);
 }
 
 }  // namespace
@@ -1188,13 +1188,9 @@ int rlh_sample_rows(uint32_t type, const void* logits, uint64_t n_rows, uint64_t
   if (need) RLH_TRY(dev("workspace", workspace));
   hipStream_t s = (hipStream_t)stream;
   const Space space = sample_space(workspace, n);
-  if (type == RLH_TYPE_F32)
-    launch_sample<float>(logits, n_rows, n, stride, options, u, tokens, space, s);
-  else if (type == RLH_TYPE_F16)
-    launch_sample<_Float16>(logits, n_rows, n, stride, options, u, tokens, space, s);
-  else
-    launch_sample<__bf16>(logits, n_rows, n, stride, options, u, tokens, space, s);
-  return launched("rlh_sample_rows");
+  if (type == RLH_TYPE_F32) return launch_sample<float>(logits, n_rows, n, stride, options, u, tokens, space, s);
+  if (type == RLH_TYPE_F16) return launch_sample<_Float16>(logits, n_rows, n, stride, options, u, tokens, space, s);
+  return launch_sample<__bf16>(logits, n_rows, n, stride, options, u, tokens, space, s);
 }
 
 }  // extern "C"

@@ -116,9 +116,19 @@ class DeviceCheck {
     if (rc_ != RLH_OK) return rc_; \
   } while (0)
 
-inline int launched(const char* what) {
-  const hipError_t e = hipGetLastError();
+// Enqueues a kernel; `what` is the entry that does. The launch's own status
+// counts: the thread's last error may be one that the caller left.
+template <typename T>
+struct as_is {
+  typedef T type;
+};
+template <typename... P>
+int enqueue(const char* what, void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t lds, hipStream_t stream,
+            typename as_is<P>::type... args) {
+  void* p[] = {(void*)&args...};
+  const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3(threads), p, lds, stream);
   if (e == hipSuccess) return RLH_OK;
+  (void)hipGetLastError();
   return serve_error(RLH_EDEVICE, std::string(what) + ": " + hipGetErrorString(e));
 }
 

@@ -1,12 +1,15 @@
 """Ends of the ranges that the batched serving operators accept, on the GPU
 against 64-bit forms."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import rlh
 import serve_ref as ref
-from test_gpu_serve import ATTN, attn_case, check_attn, run_attn, run_sample
+from test_gpu_serve import (ATTN, append_inputs, attn_case, check_attn, options_tensor, run_append, run_attn,
+                            run_sample)
 
 pytestmark = pytest.mark.gpu
 
@@ -268,3 +271,36 @@ def test_attention_one_workspace_for_limits():
         torch.cuda.synchronize()
         check_attn(b, q, out, heads, opts)
     assert torch.all(guard[need:] == 0xa5)
+
+
+# ---- errors of the caller's own ------------------------------------------------------
+
+def test_errors_that_a_caller_left_are_not_a_calls_own():
+    """A HIP error that the host caused before and has not asked for: the calls
+    are enqueued and say so."""
+    hip = ctypes.CDLL(rlh.LIB_PATH)  # (its symbols include those of the runtime that it is linked to)
+    n = 5000
+    x = torch.randn((2, n), generator=torch.Generator().manual_seed(1)).cuda()
+    opt = options_tensor([(0.0, 0, 1.0, 0.0)] * 2)
+    u = torch.zeros(2, device="cuda")
+    tok = torch.full((2,), -1, dtype=torch.int32, device="cuda")
+    ws = torch.empty(rlh.sample_rows_workspace(2, n), dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    b = ref.Batch([(3, 20), (1, 700), (40, 40)], 2, 128, 16, rlh.BF16, seed=1)
+    rows = append_inputs(b, 4, rlh.F32, 2)
+    q = torch.randn((b.n_rows, 512), generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    out, q_out = torch.zeros_like(q), torch.zeros_like(q)
+    try:
+        for call in (lambda: rlh.sample_rows(rlh.F32, x.data_ptr(), 2, n, n, opt.data_ptr(), u.data_ptr(), tok.data_ptr(),
+                                             ws.data_ptr(), ws.numel(), st),
+                     lambda: run_append(b, rows, rlh.F32, 4, q_out, None, None, None, 1.0, 0, False)):
+            assert hip.hipSetDevice(-7) != 0
+            call()
+        args = rlh.AttnArgs(4, 0, q.data_ptr(), out.data_ptr(), 512, 512, 0.1, 0.0, None, None, None, 0)
+        space = torch.empty(rlh.paged_attn_workspace(b.kv(), b.desc(), args) + 16, dtype=torch.uint8, device="cuda")
+        assert hip.hipSetDevice(-7) != 0
+        rlh.paged_attn(b.kv(), b.desc(), args, space.data_ptr(), space.numel() // 16 * 16, None, st)
+    finally:
+        hip.hipGetLastError()
+    torch.cuda.synchronize()
+    assert tok.cpu().tolist() == x.argmax(1).cpu().tolist()
