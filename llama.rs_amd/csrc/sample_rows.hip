@@ -127,7 +127,10 @@ __device__ __noinline__ double weight_called(uint32_t key, uint32_t top_key, dou
 }
 // Bins of a histogram: the value's logarithm of its weight, rounded to
 // sixteenths of a power of two and counted from the largest's (`base`) down.
-__device__ __forceinline__ double edge_of(double x16) { return (x16 + kRound) - kRound; }
+// From 2^51 on, where adding kRound rounds to more than whole numbers, they are
+// taken as they are: two f32 values are equal there or 2^27 apart.
+constexpr double kLastRounded = 0x1p51;
+__device__ __forceinline__ double edge_of(double x16) { return fabs(x16) < kLastRounded ? (x16 + kRound) - kRound : x16; }
 __device__ __forceinline__ double edge_of(uint32_t key, double c) { return edge_of((double)value_of(key) * (c * 16.0)); }
 __device__ __forceinline__ uint32_t bin_of(uint32_t key, uint32_t top_key, double base, double c) {
   if (key == top_key) return 0u;
@@ -136,8 +139,7 @@ __device__ __forceinline__ uint32_t bin_of(uint32_t key, uint32_t top_key, doubl
 }
 // Their words: a bin's count from bit 51 on, below it its mass as multiples of
 // 2^-38 of the weight at the bin's middle. A value's weight is 2^(-1/32) to
-// 2^(1/32) of that (at most 2^(1/16) where numbers above 2^51 are rounded), so
-// 4096 of them fit 51 bits, and each is rounded by 2^-39 of itself, however
+// 2^(1/32) of that, so 4096 of them fit 51 bits, and each is rounded by 2^-39 of itself, however
 // small the bin's weights are.
 constexpr int kBinShift = 51;
 constexpr uint64_t kBinMask = (1ull << kBinShift) - 1;
@@ -309,12 +311,13 @@ __global__ void __launch_bounds__(kScanThreads) k_sample_scan(const T* logits, u
   double sum = 0.0;
   if (top != 0u && plan.bins) {
     const double c16 = plan.c * 16.0, round = exp2.round;
+    const double edge_round = fabs(tv * c16) < kLastRounded ? round : 0.0;  // (what is near the largest goes by it)
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
         const float x = (float)line[i][e];
-        const double x16 = (double)x * c16, edge = (x16 + round) - round, d = base - edge;
+        const double x16 = (double)x * c16, edge = (x16 + edge_round) - edge_round, d = base - edge;
         if (d < (double)(kBins - 1))  // (not for NaN, and not for an infinite top)
           atomicAdd((unsigned long long*)&bin[(uint32_t)__builtin_bit_cast(uint64_t, d + round)],
                     (unsigned long long)bin_word(x16 - edge, bin_exp2));

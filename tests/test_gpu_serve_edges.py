@@ -304,3 +304,29 @@ def test_errors_that_a_caller_left_are_not_a_calls_own():
         hip.hipGetLastError()
     torch.cuda.synchronize()
     assert tok.cpu().tolist() == x.argmax(1).cpu().tolist()
+
+
+# ---- tiny temperatures ---------------------------------------------------------------
+
+# A logit over such a temperature is near a power of two from 2^54 to 2^62,
+# where doubles are whole numbers apart and rounding by addition is coarser still.
+TINY = [(5.933965826196662e-18, 18.966964721679688), (6.960958119566468e-18, 5.561732769012451),
+        (1.6533624045163976e-18, 21.140241622924805), (2.3351737171929274e-17, 18.65730857849121),
+        (2.107113983893586e-18, 13.470561027526855), (1.1937834601465037e-15, 14.591938972473145), (1e-12, 20.0), (1e-25, 3.0)]
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("n", [500, 9000])
+def test_sample_ties_at_tiny_temperatures(n, sign):
+    """Only equal largest logits have weight: top-p, top-k and min-p count them."""
+    rng = np.random.default_rng(n)
+    xs, rows, us = [], [], []
+    for temperature, top in TINY:
+        for opt in [(0, 0.5, 0.0), (0, 0.97, 0.0), (n // 2, 1.0, 0.0), (n - 1, 0.3, 0.5), (0, 1.0, 0.9)]:
+            for u in (0.0, 0.4, 0.9, 1.0):
+                v = (sign * top - 5.0 - 5.0 * rng.random(n)).astype(np.float32)
+                v[rng.choice(n, 100, replace=False)] = np.float32(sign * top)
+                xs.append(v)
+                rows.append((temperature,) + opt)
+                us.append(u)
+    compare_samples(xs, rows, us)
