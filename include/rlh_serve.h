@@ -57,9 +57,10 @@ typedef struct rlh_kv_pages {
  * new = q_start[s+1] - q_start[s] and kv_len[s] counts these rows. Position p
  * lies in page table[s * table_stride + p / page_size], slot p % page_size.
  * q_start (n_seq + 1 values) does not fall; a sequence may bring no rows,
- * and rows behind the last sequence are left as they were. max_q and max_kv
- * bound the new rows and kv_len of every sequence (max_kv <= table_stride *
- * page_size < 2^30): work is divided by them, so near bounds are faster.
+ * and rows before the first or behind the last one are left as they were.
+ * max_q and max_kv bound the new rows and kv_len of every sequence (max_kv <=
+ * table_stride * page_size < 2^30): work is divided by them, so near bounds are
+ * faster.
  * n_seq < 2^16, n_rows <= 2^23, n_rows * n_head <= 2^25 and n_seq * n_head_kv
  * <= 2^21 (RLH_EUNSUP beyond). */
 typedef struct rlh_seqs {

@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(AppendParams a) {
   if (s >= a.b.n_seq) return;  // behind the last sequence
   bool bad;
   const SeqView sv = load_seq(a.b, s, &bad);
+  if (s == 0 && !bad && row < sv.q0) return;  // before the first sequence
   if (!sv.ok || row < sv.q0 || row - sv.q0 >= sv.q_len) {  // (starts that fall may name a sequence that ends before it)
     if (threadIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
     return;

@@ -330,3 +330,41 @@ def test_sample_ties_at_tiny_temperatures(n, sign):
                 rows.append((temperature,) + opt)
                 us.append(u)
     compare_samples(xs, rows, us)
+
+
+# ---- batches that begin behind the first row -------------------------------------------
+
+@pytest.mark.parametrize("many", [0, 300])
+@pytest.mark.parametrize("first", [[], [(0, 30)]])
+def test_rows_before_the_first_sequence(first, many):
+    """A part of a larger batch: the first start is not 0. The rows before it
+    are left as they were, and nothing is wrong with the batch."""
+    heads, kv, dim, skip = 4, 2, 64, 5
+    seqs = first + [(3, 40), (0, 9), (1, 700), (70, 90)] + [(1, 1 + i % 50) for i in range(many)]
+    for shared in (0, 32):
+        b, q, out, opts = attn_case([(skip, skip)] + seqs, heads, kv, dim, 16, rlh.F16, seed=many + shared, shared=shared)
+        desc = b.desc()
+        part = rlh.Seqs(desc.n_seq - 1, desc.n_rows, desc.max_q, desc.max_kv, desc.table_stride, b.q_start[1:].data_ptr(),
+                        b.kv_len[1:].data_ptr(), b.table[1:].data_ptr())
+        keep = out[:skip].clone()
+        b.desc = lambda: part
+        st = torch.zeros(1, dtype=torch.int32, device="cuda")
+        run_attn(b, q, out, heads, status=st, **opts)
+        torch.cuda.synchronize()
+        assert int(st) == 0 and torch.equal(out[:skip], keep)
+        whole = out.clone()
+        b.desc = lambda: desc
+        run_attn(b, q, whole, heads, **opts)
+        torch.cuda.synchronize()
+        check_attn(b, q, whole, heads, opts)
+        out[:skip] = whole[:skip]
+        check_attn(b, q, out, heads, opts)
+        if shared:
+            continue  # (some of the new rows are in the shared pages, which no sequence owns)
+        b.desc = lambda: part
+        x = append_inputs(b, heads, rlh.F32, 3)
+        q_out = torch.full((b.n_rows, heads * dim), 7.0, dtype=torch.float16, device="cuda")
+        run_append(b, x, rlh.F32, heads, q_out, None, None, None, 1.0, 0, False, st)
+        torch.cuda.synchronize()
+        assert int(st) == 0
+        assert torch.all(q_out[:skip] == 7.0) and torch.equal(q_out[skip:], x[skip:, :heads * dim].half())
