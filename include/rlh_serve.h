@@ -17,8 +17,8 @@
  *    Data and workspaces are aligned to 16 bytes, strides count elements and
  *    span a multiple of 16 bytes, index arrays are aligned to 4 bytes, rotary
  *    frequencies to 8. What a call writes overlaps nothing else of it.
- *  - The calls enqueue kernels on `stream` (a hipStream_t, NULL for the null
- *    stream), allocate nothing and do not synchronize, so they may be captured
+ *  - The calls enqueue kernels on `stream` (a hipStream_t of the current device,
+ *    NULL for the null stream), allocate nothing and do not synchronize, so they may be captured
  *    into a graph; lengths, positions, page ids and sampling options are read
  *    when the kernels run. Calls that may overlap (two streams, or two
  *    graphs replayed at once) need workspaces of their own; between calls a
@@ -94,7 +94,7 @@ int rlh_rope_freqs(const rlh_rope* rope, double* freqs, float* magnitude);
  * src/ops.rs:336-446, for many sequences). q, k and v are rows of in_type
  * (RLH_TYPE_F32, F16 or BF16) with strides of their own, e.g. the slices of
  * one product. q_norm / k_norm (f32[head_dim], each may be NULL):
- * x * w / sqrt(mean(x^2) + eps). The first rot_dim values of a head (a
+ * x * w / sqrt(mean(x^2) + eps), the squares summed in f32. The first rot_dim values of a head (a
  * multiple of 16, 0: none) are rotated by position * freqs[i], computed in
  * 64 bits, and multiplied by `magnitude`: pairs (i, i + rot_dim / 2), or
  * (2i, 2i + 1) when `interleaved`. q_out receives the rows of q, k and v
@@ -125,6 +125,8 @@ int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_app
  *   seen: j <= i, and j > i - window when window > 0; and every
  *   j < prefix_len[s] (u32[n_seq], may be NULL), also ahead of i; always
  *   j < kv_len[s]. What is not seen contributes nothing, whatever it holds.
+ * The bias is signed as written: a prefix position ahead of a row (j > i) gets
+ * slopes[h] times how far ahead it is, not minus that.
  * A row that sees nothing, or only scores of minus infinity, is zero. q and
  * out are [n_rows][n_head][head_dim] of the pool's type with row strides, and
  * must not overlap. Scores, maxima and sums are f32; the probabilities are
@@ -165,7 +167,7 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
  * options per row. The filters are rlh_sample's (top-k, then top-p over the
  * softmax of the whole row) and min-p; the draw runs over the kept tokens in
  * index order, so it needs no sorted list:
- *   w_i = exp((l_i - max l) / temperature), in 64 bits
+ *   w_i = exp((l_i - max l) / temperature), in 64 bits, to 2^-37 of itself
  *   order: l descending, equal ones by index
  *   kept: the first top_k (0: all), the shortest head of the order whose
  *   mass reaches top_p * sum(w) (for 0 < top_p < 1), w_i >= min_p (for
@@ -173,11 +175,12 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
  *   token: the lowest index whose running kept mass exceeds u * kept mass
  * temperature <= 0 (or NaN): the first of the order. NaN logits have no mass;
  * at +infinity only those logits have; a row without a value above -infinity
- * gives 0. Masses below 2^-43 of the largest may count as none. u outside
- * [0, 1) (or NaN) is taken as the nearer end (0); at 1 and above the token is
- * the last kept one of at least 2^-43 of the largest weight. n <= 2^21, n_rows <= 2^21
- * and n_rows * n <= 2^35. The token does not depend on the run: masses are
- * summed in a fixed order, or as whole numbers. */
+ * gives 0. Borders of mass and the draw are met to 2^-36 of sum(w); masses
+ * below 2^-43 of the largest may count as none. u outside [0, 1) (or NaN) is
+ * taken as the nearer end (0); at 1 and above the token is the last kept one of
+ * at least 2^-43 of the largest weight. n <= 2^21, n_rows <= 2^21 and
+ * n_rows * n <= 2^35. The token does not depend on the run: masses are summed in
+ * a fixed order, or as whole numbers. */
 typedef struct rlh_row_sampling {
   float temperature;
   uint32_t top_k;

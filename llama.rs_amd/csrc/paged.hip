@@ -194,7 +194,8 @@ template <typename TI, typename TO, int D>
 int launch_append(const AppendParams& p, bool inter, hipStream_t s) {
   const uint32_t per = kThreads / (D / 8);
   const dim3 grid(p.b.n_rows, (p.n_head + 2 * p.n_kv + per - 1) / per);
-  return enqueue("rlh_paged_append", inter ? k_paged_append<TI, TO, D, true> : k_paged_append<TI, TO, D, false>, grid, kThreads, 0, s, p);
+  const auto kernel = inter ? k_paged_append<TI, TO, D, true> : k_paged_append<TI, TO, D, false>;
+  return enqueue("rlh_paged_append", kernel, grid, kThreads, 0, s, p);
 }
 
 template <typename TI, typename TO>
@@ -275,7 +276,8 @@ int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_app
   for (const Area& written : {q_out, area("the pool", kv->k, pool_bytes(*kv)), area("the pool", kv->v, pool_bytes(*kv))})
     RLH_TRY(check_apart(written, {q_start, kv_len, table, q_norm, k_norm, freqs, st}));
   RLH_TRY(check_apart(st, {q_start, kv_len, table, q_norm, k_norm, freqs, Area{"q", args->q, n, args->q_stride * is, qw * is},
-                           Area{"k", args->k, n, args->k_stride * is, kw * is}, Area{"v", args->v, n, args->v_stride * is, kw * is}}));
+                           Area{"k", args->k, n, args->k_stride * is, kw * is},
+                           Area{"v", args->v, n, args->v_stride * is, kw * is}}));
   DeviceCheck dev;
   RLH_TRY(dev.begin());
   RLH_TRY(dev("k pages", kv->k));

@@ -313,8 +313,8 @@ __device__ __forceinline__ uint32_t small_steps(const AttnParams& a, uint32_t s,
 // by half a step of each; the sum takes them unrounded), all else is f32.
 // Bound by HBM: 61 tokens of 32 heads on 940 MB of pages take 166 us (5.7
 // TB/s; a copy of 2 GiB moves 5.1), 3 of 64 heads on 459 MB 90 us. The
-// positions are divided so that the parts are of one length and fill the card
-// once; a single short sequence costs the chain of loads from its start to its
+// positions are divided so that the parts are of one length, 768 blocks of them
+// (of the two or three that a CU runs at once); a single short sequence costs the chain of loads from its start to its
 // pages (6 us) and the second launch that joins the parts (4 us).
 template <int D, int W>
 constexpr uint32_t kSmallLds = (W * 32 * (D * 2 + 32) > W * 16 * (D + 4) * 4 ? W * 32 * (D * 2 + 32) : W * 16 * (D + 4) * 4) + W * 128;
@@ -528,7 +528,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
     }
   }
   l = sum_across_16(sum_across_32(l));
-  // the four waves' results
+  // the waves' results
   __syncthreads();
   float* ol = (float*)lds;
 #pragma unroll
@@ -585,16 +585,17 @@ __global__ void __launch_bounds__(64 * W, 2) k_attn_small(Launch L) {
 // pieces that are exchanged within a row so that the products' reads meet no
 // bank twice. Each of eight waves has 32 rows: scores are K times Q^T
 // (32x32x16: positions down, rows across), so that a row is a lane column as
-// above. What bounds it: a step's 32 MFMAs take 1024 cycles of a SIMD and its
-// exponentials, maxima and sums as many, and the two overlap only between
-// two waves that are at different places; copies are issued at 48 cycles a
+// above. What bounds it: a step's 32 MFMAs take a wave 1024 cycles of its SIMD
+// and its exponentials, maxima and sums as many; within a wave they are one
+// chain, and the two waves of a SIMD overlap little of it (a step takes 2.3 us,
+// the sum of both waves' 4096 cycles 1.7). Copies are issued at 48 cycles a
 // KB, so four waves per tile would spend 1550 cycles a step on them. 4096
-// tokens of 64 heads: 275 GFLOP in 303 us, 907 TFLOP/s (340 us in a row of
-// passes; a product of 16384^3 reaches 1357 TFLOP/s; there, tiles of 128 rows took 382 us, operand reads that do not run
-// ahead of the products 349). A cap adds an exponential and a reciprocal per
+// tokens of 64 heads: 275 GFLOP in 300 us, 916 TFLOP/s (a product of 16384^3
+// reaches 1357). In a row of passes it is 340 us; there, tiles of 128 rows took
+// 382, operand reads that do not run ahead of the products 349. A cap adds an exponential and a reciprocal per
 // score; a bias is linear in the position, so that a row's share at the step's
 // first position is kept out of the scores and joins the running maximum only
-// (5 prompts of 6895 tokens with a bias: 147 us with it in each score, 107).
+// (5 prompts of 6895 tokens with a bias: 147 us with it in each score, 104).
 template <int D>
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
   return D == 128 ? ((r & 3) << 2 | (r >> 2 & 3)) : ((r >> 1 & 1) << 2 | (r >> 2 & 3));
@@ -1145,7 +1146,8 @@ constexpr uint32_t kWhole = 512;
 // Where each sequence's items and tiles begin, by one block. Up to kPlanned
 // sequences every wave of the other kernels finds that out by itself, which
 // costs less than a launch; beyond, their loops over all sequences would take
-// longer than the attention (2048 of 300 positions: 5 + 448 us instead of 1024).
+// longer than the attention (2048 tokens of 32 heads over 8 of 128, 300
+// positions each: 5 + 448 us instead of 1024).
 constexpr uint32_t kPlanned = 256;
 constexpr int kPlanThreads = 1024;
 
@@ -1211,7 +1213,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
   }
 }
 
-constexpr uint32_t kSmallBlocks = 768;  // blocks that the small kernel's work is divided into (three to a CU)
+// Blocks that the small kernel's work is divided into: three to a CU. So many
+// run at once with cap or bias (162 registers) and for head_dim 64, two
+// without at 128 (173).
+constexpr uint32_t kSmallBlocks = 768;
 
 uint32_t item_goal(uint32_t n_head_kv) { return std::max(1u, kSmallBlocks / n_head_kv); }
 
@@ -1276,8 +1281,8 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
     n.prefix_parts = n.last_parts = tile_parts((uint64_t)n.prefix_tiles * kv.n_head_kv, args.shared_len);
     // A last tile of up to 128 rows has one wave per SIMD, whose steps take
     // about 0.55 of the time, and is divided into fewer parts (576 rows of a
-    // KV head against 16384 positions: 12, 12 and 8 parts instead of 10 each,
-    // 70 us instead of 75).
+    // KV head against 16384 positions, the only size it was measured at: 12, 12
+    // and 8 parts instead of 10 each, 70 us instead of 75).
     const uint64_t most = 256 / kv.n_head_kv, last = rows - (uint64_t)(n.prefix_tiles - 1) * kTileRows;
     const uint64_t p = std::min<uint64_t>(most * 20 / (20 * n.prefix_tiles - 9), args.shared_len / 256);
     if (n.prefix_tiles > 1 && last <= kTileRows / 2 && p > n.prefix_parts) {
@@ -1383,7 +1388,8 @@ int launch_attn(const Launch& L, int device, hipStream_t s) {
     RLH_TRY(enqueue(what, k_attn_mixed<T, D, MOD>, dim3(blocks), 64 * kTileWaves, kMixedLds<D>, s, L));
   } else if (L.n.whole) {
     RLH_TRY((allow_lds<T, D, MOD>(device)));
-    RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kTileWaves>, dim3(L.n.items * G), 64 * kTileWaves, kSmallLds<D, kTileWaves>, s, L));
+    RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kTileWaves>, dim3(L.n.items * G), 64 * kTileWaves,
+                    kSmallLds<D, kTileWaves>, s, L));
   } else {
     RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kWaves>, dim3(L.n.items * G), kThreads, kSmallLds<D, kWaves>, s, L));
   }
@@ -1439,11 +1445,14 @@ int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   const Area q_start = area_q_start(*seqs), kv_len = area_kv_len(*seqs), table = area_table(*seqs, kv->page_size),
              slopes = area("slopes", args->slopes, args->n_head * 4ull),
              prefix_len = area("prefix_len", args->prefix_len, seqs->n_seq * 4ull),
-             shared = area("shared_table", args->shared_len ? args->shared_table : nullptr, args->shared_len / kv->page_size * 4ull),
+             shared = area("shared_table", args->shared_len ? args->shared_table : nullptr,
+                           args->shared_len / kv->page_size * 4ull),
              st = area("status", status, 4);
-  for (const Area& written : {Area{"out", args->out, rows, args->out_stride * 2, w * 2}, area("workspace", need ? workspace : nullptr, need)})
+  for (const Area& written :
+       {Area{"out", args->out, rows, args->out_stride * 2, w * 2}, area("workspace", need ? workspace : nullptr, need)})
     RLH_TRY(check_apart(written, {q_start, kv_len, table, slopes, prefix_len, shared, st}));
-  RLH_TRY(check_apart(st, {q_start, kv_len, table, slopes, prefix_len, shared, Area{"q", args->q, rows, args->q_stride * 2, w * 2},
+  RLH_TRY(check_apart(st, {q_start, kv_len, table, slopes, prefix_len, shared,
+                           Area{"q", args->q, rows, args->q_stride * 2, w * 2},
                            area("the pool", kv->k, pool_bytes(*kv)), area("the pool", kv->v, pool_bytes(*kv))}));
   DeviceCheck dev;
   RLH_TRY(dev.begin());

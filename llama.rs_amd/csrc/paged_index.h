@@ -49,7 +49,8 @@ RLH_HD RowSpan row_span(int32_t pos, uint32_t kv_len, uint32_t window, uint32_t 
 // (no short-circuits: the kernels ask for every score of a border tile)
 RLH_HD bool row_sees(const RowSpan& r, int32_t j) { return ((j >= r.lo) & (j < r.hi)) | (j < r.prefix); }
 
-// First and end position that any row of positions [first, last] sees.
+// First and end position that any row of positions [first, last] sees (with
+// both a prefix and a window, what lies between them is stepped through).
 RLH_HD int32_t span_begin(const RowSpan& first) { return first.prefix > 0 ? 0 : first.lo; }
 RLH_HD int32_t span_end(const RowSpan& last) { return last.hi > last.prefix ? last.hi : last.prefix; }
 

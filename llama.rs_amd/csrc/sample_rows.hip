@@ -537,7 +537,8 @@ __device__ __forceinline__ bool narrow(PickShared& sh, Range& r, const Goal& goa
   // (2^21 values of at most 2^42 units: below 2^64)
   double unit = 0.0, units = 0.0;  // of a mass; in a weight of one
   if (goal.p < INFINITY) {
-    unit = fmax(weight_called(min(r.hi, goal.top_key), goal.top_key, goal.top, goal.c), kLeastWeight) * (1.0 / (double)(1ull << kMassBits));
+    const double most = weight_called(min(r.hi, goal.top_key), goal.top_key, goal.top, goal.c);
+    unit = fmax(most, kLeastWeight) * (1.0 / (double)(1ull << kMassBits));
     units = 1.0 / unit;
   }
   __syncthreads();
@@ -1138,10 +1139,10 @@ Space sample_space(void* base, uint64_t n) {
 template <typename T>
 int launch_sample(const void* logits, uint64_t n_rows, uint64_t n, uint64_t stride, const rlh_row_sampling* options,
                   const float* u, uint32_t* tokens, const Space& space, hipStream_t s) {
-  RLH_TRY(enqueue("rlh_sample_rows", k_sample_scan<T>, dim3(space.chunks * (uint32_t)n_rows), kScanThreads, 0, s, (const T*)logits,
-                  (uint32_t)n, stride, options, space));
-  return enqueue("rlh_sample_rows", k_sample_pick<T>, dim3((uint32_t)n_rows), kThreads, 0, s, (const T*)logits, (uint32_t)n, stride,
-                 options, u, tokens, space);
+  const dim3 chunks(space.chunks * (uint32_t)n_rows), rows((uint32_t)n_rows);
+  const T* x = (const T*)logits;
+  RLH_TRY(enqueue("rlh_sample_rows", k_sample_scan<T>, chunks, kScanThreads, 0, s, x, (uint32_t)n, stride, options, space));
+  return enqueue("rlh_sample_rows", k_sample_pick<T>, rows, kThreads, 0, s, x, (uint32_t)n, stride, options, u, tokens, space);
 }
 
 }  // namespace
@@ -1163,7 +1164,7 @@ int rlh_sample_rows(uint32_t type, const void* logits, uint64_t n_rows, uint64_t
   if (!size) return serve_error(RLH_EUNSUP, "logits are not F32, F16 or BF16");
   if (n == 0 || n > kMaxRow) return serve_error(RLH_EINVAL, "n outside [1, 2^21]");
   if (n_rows > kMaxRows || n_rows * sample_space(nullptr, n).chunks >= (1ull << 24))
-    return serve_error(RLH_EUNSUP, "more than 2^21 rows, or 2^36 logits");
+    return serve_error(RLH_EUNSUP, "more than 2^21 rows, or 2^35 logits");
   if (n_rows == 0) return RLH_OK;
   if (!logits) return serve_error(RLH_EINVAL, "logits is null");
   if (!aligned(logits, size)) return serve_error(RLH_EINVAL, "logits is not aligned to its type");
