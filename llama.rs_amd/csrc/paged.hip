@@ -3,6 +3,7 @@
 // head, position rotation, write to the pages) in one pass.
 #include <math.h>
 
+#include "../../include/rlh_cache.h"
 #include "paged_device.h"
 #include "serve_check.h"
 
@@ -86,6 +87,7 @@ struct AppendParams {
   uint64_t q_stride, k_stride, v_stride, q_out_stride;
   const float *q_norm, *k_norm;
   const double* freqs;
+  const uint32_t* positions;  // rotary, per row; null: the rows' places
   float eps, magnitude;
   uint32_t n_head, n_kv, page_shift, n_pages, rot_dim;
   void *q_out, *pool_k, *pool_v;
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(AppendParams a) {
   const uint32_t half = a.rot_dim / 2;
   if (threadIdx.x < half) {
     // turns in 64 bits: at a position of 10^6 an f32 angle is off by 0.03
-    const double turns = (double)pos * a.freqs[threadIdx.x] * 0.15915494309189535;
+    const double turns = (double)(a.positions ? a.positions[row] : pos) * a.freqs[threadIdx.x] * 0.15915494309189535;
     const float f = (float)(turns - rint(turns));
     float sv_, cv_;
     sincospif(2.0f * f, &sv_, &cv_);
@@ -208,6 +210,91 @@ int launch_append(const AppendParams& p, uint32_t type, uint32_t dim, bool inter
   return type == RLH_TYPE_F16 ? launch_append<TI, _Float16>(p, dim, inter, s) : launch_append<TI, __bf16>(p, dim, inter, s);
 }
 
+// Checks and enqueues an append; `positions` may be null.
+int run_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_append_args* args, const uint32_t* positions,
+               uint32_t* status, void* stream) {
+  if (!args) return serve_error(RLH_EINVAL, "null argument");
+  RLH_TRY(check_batch(kv, seqs, args->n_head));
+  const uint32_t is = float_type_size(args->in_type);
+  if (!is) return serve_error(RLH_EUNSUP, "in_type is not F32, F16 or BF16");
+  if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;
+  const uint32_t D = kv->head_dim;
+  const uint64_t qw = (uint64_t)args->n_head * D, kw = (uint64_t)kv->n_head_kv * D;
+  RLH_TRY(check_rows("q", args->q, args->q_stride, qw, is));
+  RLH_TRY(check_rows("k", args->k, args->k_stride, kw, is));
+  RLH_TRY(check_rows("v", args->v, args->v_stride, kw, is));
+  RLH_TRY(check_rows("q_out", args->q_out, args->q_out_stride, qw, 2));
+  if (args->rot_dim % 16 || args->rot_dim > D)
+    return serve_error(RLH_EINVAL, "rot_dim is not a multiple of 16 up to head_dim");
+  if (args->rot_dim && !args->freqs) return serve_error(RLH_EINVAL, "freqs is null");
+  if (!aligned(args->freqs, 8) || !aligned(args->q_norm, 16) || !aligned(args->k_norm, 16) || !aligned(status, 4))
+    return serve_error(RLH_EINVAL, "freqs, q_norm, k_norm or status is misaligned");
+  const uint64_t n = seqs->n_rows;
+  const uint64_t ow = row_bytes_span(n, args->q_out_stride, qw, 2);
+  if (overlap(args->q_out, ow, args->q, row_bytes_span(n, args->q_stride, qw, is)) ||
+      overlap(args->q_out, ow, args->k, row_bytes_span(n, args->k_stride, kw, is)) ||
+      overlap(args->q_out, ow, args->v, row_bytes_span(n, args->v_stride, kw, is)))
+    return serve_error(RLH_EINVAL, "q_out overlaps q, k or v");
+  if (overlaps_pool(*kv, args->q_out, ow) || overlaps_pool(*kv, args->q, row_bytes_span(n, args->q_stride, qw, is)) ||
+      overlaps_pool(*kv, args->k, row_bytes_span(n, args->k_stride, kw, is)) ||
+      overlaps_pool(*kv, args->v, row_bytes_span(n, args->v_stride, kw, is)))
+    return serve_error(RLH_EINVAL, "the pool overlaps q, k, v or q_out");
+  const Area q_start = area_q_start(*seqs), kv_len = area_kv_len(*seqs), table = area_table(*seqs, kv->page_size),
+             q_norm = area("q_norm", args->q_norm, D * 4), k_norm = area("k_norm", args->k_norm, D * 4),
+             freqs = area("freqs", args->rot_dim ? args->freqs : nullptr, args->rot_dim / 2 * 8),
+             at = area("positions", positions, n * 4), st = area("status", status, 4), q_out{"q_out", args->q_out, n, args->q_out_stride * 2, qw * 2};
+  for (const Area& written : {q_out, area("the pool", kv->k, pool_bytes(*kv)), area("the pool", kv->v, pool_bytes(*kv))})
+    RLH_TRY(check_apart(written, {q_start, kv_len, table, q_norm, k_norm, freqs, at, st}));
+  RLH_TRY(check_apart(st, {q_start, kv_len, table, q_norm, k_norm, freqs, at, Area{"q", args->q, n, args->q_stride * is, qw * is},
+                           Area{"k", args->k, n, args->k_stride * is, kw * is},
+                           Area{"v", args->v, n, args->v_stride * is, kw * is}}));
+  DeviceCheck dev;
+  RLH_TRY(dev.begin());
+  RLH_TRY(dev("k pages", kv->k));
+  RLH_TRY(dev("v pages", kv->v));
+  RLH_TRY(dev("q_start", seqs->q_start));
+  RLH_TRY(dev("kv_len", seqs->kv_len));
+  RLH_TRY(dev("table", seqs->table));
+  RLH_TRY(dev("q", args->q));
+  RLH_TRY(dev("k", args->k));
+  RLH_TRY(dev("v", args->v));
+  RLH_TRY(dev("q_norm", args->q_norm));
+  RLH_TRY(dev("k_norm", args->k_norm));
+  if (args->rot_dim) RLH_TRY(dev("freqs", args->freqs));
+  RLH_TRY(dev("positions", positions));
+  RLH_TRY(dev("q_out", args->q_out));
+  RLH_TRY(dev("status", status));
+  AppendParams p{};
+  p.b = Batch{seqs->n_seq, seqs->n_rows, seqs->max_q, seqs->max_kv, seqs->table_stride,
+              seqs->q_start, seqs->kv_len, seqs->table};
+  p.q = args->q;
+  p.k = args->k;
+  p.v = args->v;
+  p.q_stride = args->q_stride;
+  p.k_stride = args->k_stride;
+  p.v_stride = args->v_stride;
+  p.q_out_stride = args->q_out_stride;
+  p.q_norm = args->q_norm;
+  p.k_norm = args->k_norm;
+  p.freqs = args->freqs;
+  p.positions = positions;
+  p.eps = args->eps;
+  p.magnitude = args->magnitude;
+  p.n_head = args->n_head;
+  p.n_kv = kv->n_head_kv;
+  p.page_shift = (uint32_t)__builtin_ctz(kv->page_size);
+  p.n_pages = (uint32_t)kv->n_pages;
+  p.rot_dim = args->rot_dim;
+  p.q_out = args->q_out;
+  p.pool_k = kv->k;
+  p.pool_v = kv->v;
+  p.status = status;
+  const bool inter = args->interleaved != 0;
+  if (args->in_type == RLH_TYPE_F32) return launch_append<float>(p, kv->type, D, inter, (hipStream_t)stream);
+  if (args->in_type == RLH_TYPE_F16) return launch_append<_Float16>(p, kv->type, D, inter, (hipStream_t)stream);
+  return launch_append<__bf16>(p, kv->type, D, inter, (hipStream_t)stream);
+}
+
 }  // namespace
 }  // namespace rlh
 
@@ -243,84 +330,14 @@ int rlh_rope_freqs(const rlh_rope* r, double* freqs, float* magnitude) {
 
 int rlh_paged_append(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_append_args* args, uint32_t* status,
                      void* stream) {
-  if (!args) return serve_error(RLH_EINVAL, "null argument");
-  RLH_TRY(check_batch(kv, seqs, args->n_head));
-  const uint32_t is = float_type_size(args->in_type);
-  if (!is) return serve_error(RLH_EUNSUP, "in_type is not F32, F16 or BF16");
-  if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;
-  const uint32_t D = kv->head_dim;
-  const uint64_t qw = (uint64_t)args->n_head * D, kw = (uint64_t)kv->n_head_kv * D;
-  RLH_TRY(check_rows("q", args->q, args->q_stride, qw, is));
-  RLH_TRY(check_rows("k", args->k, args->k_stride, kw, is));
-  RLH_TRY(check_rows("v", args->v, args->v_stride, kw, is));
-  RLH_TRY(check_rows("q_out", args->q_out, args->q_out_stride, qw, 2));
-  if (args->rot_dim % 16 || args->rot_dim > D)
-    return serve_error(RLH_EINVAL, "rot_dim is not a multiple of 16 up to head_dim");
-  if (args->rot_dim && !args->freqs) return serve_error(RLH_EINVAL, "freqs is null");
-  if (!aligned(args->freqs, 8) || !aligned(args->q_norm, 16) || !aligned(args->k_norm, 16) || !aligned(status, 4))
-    return serve_error(RLH_EINVAL, "freqs, q_norm, k_norm or status is misaligned");
-  const uint64_t n = seqs->n_rows;
-  const uint64_t ow = row_bytes_span(n, args->q_out_stride, qw, 2);
-  if (overlap(args->q_out, ow, args->q, row_bytes_span(n, args->q_stride, qw, is)) ||
-      overlap(args->q_out, ow, args->k, row_bytes_span(n, args->k_stride, kw, is)) ||
-      overlap(args->q_out, ow, args->v, row_bytes_span(n, args->v_stride, kw, is)))
-    return serve_error(RLH_EINVAL, "q_out overlaps q, k or v");
-  if (overlaps_pool(*kv, args->q_out, ow) || overlaps_pool(*kv, args->q, row_bytes_span(n, args->q_stride, qw, is)) ||
-      overlaps_pool(*kv, args->k, row_bytes_span(n, args->k_stride, kw, is)) ||
-      overlaps_pool(*kv, args->v, row_bytes_span(n, args->v_stride, kw, is)))
-    return serve_error(RLH_EINVAL, "the pool overlaps q, k, v or q_out");
-  const Area q_start = area_q_start(*seqs), kv_len = area_kv_len(*seqs), table = area_table(*seqs, kv->page_size),
-             q_norm = area("q_norm", args->q_norm, D * 4), k_norm = area("k_norm", args->k_norm, D * 4),
-             freqs = area("freqs", args->rot_dim ? args->freqs : nullptr, args->rot_dim / 2 * 8),
-             st = area("status", status, 4), q_out{"q_out", args->q_out, n, args->q_out_stride * 2, qw * 2};
-  for (const Area& written : {q_out, area("the pool", kv->k, pool_bytes(*kv)), area("the pool", kv->v, pool_bytes(*kv))})
-    RLH_TRY(check_apart(written, {q_start, kv_len, table, q_norm, k_norm, freqs, st}));
-  RLH_TRY(check_apart(st, {q_start, kv_len, table, q_norm, k_norm, freqs, Area{"q", args->q, n, args->q_stride * is, qw * is},
-                           Area{"k", args->k, n, args->k_stride * is, kw * is},
-                           Area{"v", args->v, n, args->v_stride * is, kw * is}}));
-  DeviceCheck dev;
-  RLH_TRY(dev.begin());
-  RLH_TRY(dev("k pages", kv->k));
-  RLH_TRY(dev("v pages", kv->v));
-  RLH_TRY(dev("q_start", seqs->q_start));
-  RLH_TRY(dev("kv_len", seqs->kv_len));
-  RLH_TRY(dev("table", seqs->table));
-  RLH_TRY(dev("q", args->q));
-  RLH_TRY(dev("k", args->k));
-  RLH_TRY(dev("v", args->v));
-  RLH_TRY(dev("q_norm", args->q_norm));
-  RLH_TRY(dev("k_norm", args->k_norm));
-  if (args->rot_dim) RLH_TRY(dev("freqs", args->freqs));
-  RLH_TRY(dev("q_out", args->q_out));
-  RLH_TRY(dev("status", status));
-  AppendParams p{};
-  p.b = Batch{seqs->n_seq, seqs->n_rows, seqs->max_q, seqs->max_kv, seqs->table_stride,
-              seqs->q_start, seqs->kv_len, seqs->table};
-  p.q = args->q;
-  p.k = args->k;
-  p.v = args->v;
-  p.q_stride = args->q_stride;
-  p.k_stride = args->k_stride;
-  p.v_stride = args->v_stride;
-  p.q_out_stride = args->q_out_stride;
-  p.q_norm = args->q_norm;
-  p.k_norm = args->k_norm;
-  p.freqs = args->freqs;
-  p.eps = args->eps;
-  p.magnitude = args->magnitude;
-  p.n_head = args->n_head;
-  p.n_kv = kv->n_head_kv;
-  p.page_shift = (uint32_t)__builtin_ctz(kv->page_size);
-  p.n_pages = (uint32_t)kv->n_pages;
-  p.rot_dim = args->rot_dim;
-  p.q_out = args->q_out;
-  p.pool_k = kv->k;
-  p.pool_v = kv->v;
-  p.status = status;
-  const bool inter = args->interleaved != 0;
-  if (args->in_type == RLH_TYPE_F32) return launch_append<float>(p, kv->type, D, inter, (hipStream_t)stream);
-  if (args->in_type == RLH_TYPE_F16) return launch_append<_Float16>(p, kv->type, D, inter, (hipStream_t)stream);
-  return launch_append<__bf16>(p, kv->type, D, inter, (hipStream_t)stream);
+  return run_append(kv, seqs, args, nullptr, status, stream);
+}
+
+int rlh_paged_append_at(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_append_args* args,
+                        const uint32_t* positions, uint32_t* status, void* stream) {
+  if (!positions && seqs && seqs->n_seq != 0 && seqs->n_rows != 0) return serve_error(RLH_EINVAL, "positions is null");
+  if (!aligned(positions, 4)) return serve_error(RLH_EINVAL, "positions is not aligned to 4 bytes");
+  return run_append(kv, seqs, args, positions, status, stream);
 }
 
 }  // extern "C"

@@ -54,6 +54,41 @@ RLH_HD bool row_sees(const RowSpan& r, int32_t j) { return ((j >= r.lo) & (j < r
 RLH_HD int32_t span_begin(const RowSpan& first) { return first.prefix > 0 ? 0 : first.lo; }
 RLH_HD int32_t span_end(const RowSpan& last) { return last.hi > last.prefix ? last.hi : last.prefix; }
 
+// ---- drafted rows -----------------------------------------------------------------
+// What a drafted row sees before its batch, whose first position is `first`: with
+// a window, `seen` (the new rows that it sees) take their part of it. lo may be
+// past hi: then nothing.
+RLH_HD RowSpan tree_span(int32_t first, uint32_t seen, uint32_t window) {
+  RowSpan r;
+  const uint64_t end = (uint64_t)(uint32_t)first + seen;
+  r.hi = first;
+  r.lo = window != 0 && end > window ? (int32_t)(end - window) : 0;
+  r.prefix = 0;
+  return r;
+}
+
+// The low `rows` bits of x.
+RLH_HD uint64_t only_rows(uint64_t x, int64_t rows) { return rows <= 0 ? 0 : rows >= 64 ? x : x & ((1ull << rows) - 1); }
+
+// New rows that a mask of `words` words names.
+RLH_HD uint32_t tree_seen(const uint64_t* mask, uint32_t words, uint32_t q_len) {
+  uint32_t n = 0;
+  for (uint32_t w = 0; w < words && w * 64 < q_len; w++)
+    n += (uint32_t)__builtin_popcountll(only_rows(mask[w], (int64_t)q_len - w * 64));
+  return n;
+}
+
+// Bits off .. off + 63 of the mask (off may lie before or behind it).
+RLH_HD uint64_t tree_bits(const uint64_t* mask, uint32_t words, uint32_t q_len, int32_t off) {
+  if (off <= -64 || off >= (int32_t)q_len) return 0;
+  const int32_t w = off >> 6;  // floor
+  const uint32_t sh = (uint32_t)off & 63;
+  const uint64_t a = w >= 0 && (uint32_t)w < words ? mask[w] : 0;
+  const uint64_t b = w + 1 >= 0 && (uint32_t)(w + 1) < words && sh ? mask[w + 1] : 0;
+  const uint64_t x = sh ? a >> sh | b << (64 - sh) : a;
+  return only_rows(x, (int64_t)q_len - off);
+}
+
 // Steps of an item when the `steps` of all sequences (fewer than 2^24 each, so
 // that 32 bits hold the sum of 256 of them, not of 65535) are divided into
 // `goal` items: the sequences' own, rounded up, are at most `goal` and one each.

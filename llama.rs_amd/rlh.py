@@ -309,7 +309,29 @@ class RowSampling(ctypes.Structure):
                 ("min_p", ctypes.c_float)]
 
 
+class AcceptArgs(ctypes.Structure):
+    """rlh_accept_args (include/rlh_cache.h): drafted trees in, the kept branches out."""
+    _fields_ = [("parents", ctypes.c_void_p), ("tokens", ctypes.c_void_p), ("sampled", ctypes.c_void_p),
+                ("path", ctypes.c_void_p), ("path_stride", ctypes.c_uint32), ("count", ctypes.c_void_p),
+                ("next", ctypes.c_void_p), ("new_len", ctypes.c_void_p)]
+
+
+class MoveArgs(ctypes.Structure):
+    """rlh_move_args."""
+    _fields_ = [("index", ctypes.c_void_p), ("index_stride", ctypes.c_uint32), ("per_head", ctypes.c_uint32),
+                ("count", ctypes.c_void_p), ("max_count", ctypes.c_uint32), ("base", ctypes.c_void_p),
+                ("mass", ctypes.c_void_p), ("mass_out", ctypes.c_void_p)]
+
+
+class EvictArgs(ctypes.Structure):
+    """rlh_evict_args."""
+    _fields_ = [("mass", ctypes.c_void_p), ("budget", ctypes.c_uint32), ("first_kept", ctypes.c_uint32),
+                ("last_kept", ctypes.c_uint32), ("keep_stride", ctypes.c_uint32), ("keep", ctypes.c_void_p),
+                ("count", ctypes.c_void_p)]
+
+
 SERVE_BAD_PAGE, SERVE_BAD_SEQ = 1, 2
+NO_PARENT = 0xffffffff
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS = 0, 1, 2
 
 _lib = None
@@ -422,6 +444,18 @@ def load():
         "rlh_paged_attn_workspace": (U64, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs)]),
         "rlh_paged_attn": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs), P, U64, P,
                                  P]),
+        "rlh_paged_append_at": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AppendArgs), P, P,
+                                      P]),
+        "rlh_paged_attn_lse": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs), P, P, U64,
+                                     P, P]),
+        "rlh_tree_masks": (I32, [ctypes.POINTER(Seqs), P, P, P, U32, P, P, P]),
+        "rlh_tree_attn_workspace": (U64, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs)]),
+        "rlh_tree_attn": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs), P, U32, P, P,
+                                U64, P, P]),
+        "rlh_tree_accept": (I32, [ctypes.POINTER(Seqs), ctypes.POINTER(AcceptArgs), P, P]),
+        "rlh_paged_move": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(MoveArgs), P, P]),
+        "rlh_paged_mass": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(AttnArgs), P, F, P, P, P]),
+        "rlh_evict_select": (I32, [ctypes.POINTER(KvPages), ctypes.POINTER(Seqs), ctypes.POINTER(EvictArgs), P, P]),
         "rlh_sample_rows_workspace": (U64, [U64, U64]),
         "rlh_sample_rows": (I32, [U32, P, U64, U64, U64, P, P, P, P, U64, P]),
     }
@@ -541,6 +575,72 @@ def paged_attn(kv, seqs, args, workspace=None, workspace_bytes=0, status=None, s
     if rc:
         check(rc)
 
+
+# ---- operators that edit the paged cache (include/rlh_cache.h) ------------------------
+
+def paged_append_at(kv, seqs, args, positions, status=None, stream=None):
+    """paged_append with row r rotated by positions[r]."""
+    rc = load().rlh_paged_append_at(kv, seqs, args, positions, status, stream)
+    if rc:
+        check(rc)
+
+
+def paged_attn_lse(kv, seqs, args, lse, workspace=None, workspace_bytes=0, status=None, stream=None):
+    """paged_attn, and the log of each row's sum of exponentials."""
+    rc = load().rlh_paged_attn_lse(kv, seqs, args, lse, workspace, workspace_bytes, status, stream)
+    if rc:
+        check(rc)
+
+
+def tree_masks(seqs, parents, base, masks, mask_words, positions=None, status=None, stream=None):
+    """Who sees whom in trees of drafted rows, and the rows' rotary positions."""
+    rc = load().rlh_tree_masks(seqs, parents, base, masks, mask_words, positions, status, stream)
+    if rc:
+        check(rc)
+
+
+def tree_attn_workspace(kv, seqs, args):
+    """Workspace bytes of tree_attn for these arguments and every smaller batch
+    (0: none, or refused)."""
+    return load().rlh_tree_attn_workspace(kv, seqs, args)
+
+
+def tree_attn(kv, seqs, args, masks, mask_words, lse=None, workspace=None, workspace_bytes=0, status=None, stream=None):
+    """Attention of drafted rows over the pages, their own by bitmask."""
+    rc = load().rlh_tree_attn(kv, seqs, args, masks, mask_words, lse, workspace, workspace_bytes, status, stream)
+    if rc:
+        check(rc)
+
+
+def tree_accept(seqs, args, status=None, stream=None):
+    """The branch of each tree that the model's own tokens follow."""
+    rc = load().rlh_tree_accept(seqs, args, status, stream)
+    if rc:
+        check(rc)
+
+
+def paged_move(kv, seqs, args, status=None, stream=None):
+    """The rows that stay, moved together in place."""
+    rc = load().rlh_paged_move(kv, seqs, args, status, stream)
+    if rc:
+        check(rc)
+
+
+def paged_mass(kv, seqs, args, lse, decay, mass, status=None, stream=None):
+    """Adds each position's attention weights to its mass."""
+    rc = load().rlh_paged_mass(kv, seqs, args, lse, decay, mass, status, stream)
+    if rc:
+        check(rc)
+
+
+def evict_select(kv, seqs, args, status=None, stream=None):
+    """The positions of largest mass that stay, per sequence and KV head."""
+    rc = load().rlh_evict_select(kv, seqs, args, status, stream)
+    if rc:
+        check(rc)
+
+
+# ---- sampling of rows (include/rlh_serve.h) ---------------------------------------------
 
 def sample_rows_workspace(n_rows, n):
     """Workspace bytes of sample_rows."""
