@@ -271,21 +271,6 @@ __device__ __forceinline__ SeqSpan seq_span(const AttnParams& a, uint32_t s, boo
   return r;
 }
 
-// x moved between lanes by a DPP control; 0 where none comes.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp0(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-}
-// Inclusive sum over the wave in lane order.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x += dpp0<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
-  x += dpp0<0x112, 0xf>(x);
-  x += dpp0<0x114, 0xf>(x);
-  x += dpp0<0x118, 0xf>(x);
-  x += dpp0<0x142, 0xa>(x);  // row_bcast 15, 31
-  x += dpp0<0x143, 0xc>(x);
-  return x;
-}
 __device__ __forceinline__ uint32_t lane_value(uint32_t x, int lane) {
   return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
 }

@@ -25,6 +25,22 @@ __device__ __forceinline__ void raise(uint32_t* status, uint32_t bit) {
   if (status) atomicOr(status, bit);
 }
 
+// x moved between lanes by a DPP control; 0 where none comes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+// Inclusive sum over the wave in lane order.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += dpp0<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += dpp0<0x112, 0xf>(x);
+  x += dpp0<0x114, 0xf>(x);
+  x += dpp0<0x118, 0xf>(x);
+  x += dpp0<0x142, 0xa>(x);  // row_bcast 15, 31
+  x += dpp0<0x143, 0xc>(x);
+  return x;
+}
+
 // How many of the n values a[0], a[stride], ... that do not fall are at most x:
 // a wave's 64 lanes try places of the range that is left. (Ends within [0, n]
 // also where they fall.)

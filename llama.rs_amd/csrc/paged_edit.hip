@@ -16,6 +16,9 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__shfl((int)(uint32_t)x, lane) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(x >> 32), lane) << 32;
 }
 
+// A value every lane of the wave has.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // ---- trees --------------------------------------------------------------------------
 
 struct TreeParams {
@@ -136,18 +139,20 @@ struct MoveParams {
   uint32_t n_seq, n_kv, max_kv, table_stride, index_stride, per_head, max_count, page_shift, n_pages;
 };
 
-// A block takes K or V of one KV head of one sequence and goes through the list
-// in order, kAhead rows per thread at a time: all of a round's rows are read
-// before one of them is written. A row comes from its place or from behind it,
-// so what a round writes no later round reads.
-constexpr int kMoveThreads = 256;
-constexpr int kMoveAhead = 4;
-
-template <int D>
-__global__ void __launch_bounds__(kMoveThreads) k_paged_move(MoveParams a) {
-  constexpr uint32_t L = D / 8, R = kMoveThreads / L;  // lanes of a row, rows of a pass
-  const bool is_v = blockIdx.x & 1;
-  const uint32_t h = (blockIdx.x >> 1) % a.n_kv, s = (blockIdx.x >> 1) / a.n_kv;
+// A block takes a slice of 16 L bytes of the rows of K or V of one KV head of one
+// sequence and goes through the list in order, AHEAD rows per thread at a
+// time: all of a round's values are read before one of them is written. A row
+// comes from its place or from behind it, so what a round writes no later round
+// reads; slices have nothing to do with each other. While a round's values are
+// on their way the next one's places are looked up.
+template <int D, int L, int THREADS, int AHEAD>
+__global__ void __launch_bounds__(THREADS) k_paged_move(MoveParams a) {
+  constexpr uint32_t kSlices = D / 8 / L, R = THREADS / L;  // rows of a pass
+  // the slices of a row go to one XCD (blocks are dealt to the eight in turn), whose L2 holds its lines
+  const uint32_t slice = blockIdx.x / 8 % kSlices, of = blockIdx.x / (8 * kSlices) * 8 + blockIdx.x % 8;
+  const bool is_v = of & 1;
+  const uint32_t h = (of >> 1) % a.n_kv, s = (of >> 1) / a.n_kv;
+  if (s >= a.n_seq) return;
   const uint32_t n = a.kv_len[s], count = a.count[s], base = a.base ? a.base[s] : 0;
   if (count == 0) return;
   if (n > a.max_kv || count > a.max_count || base > n || count > n - base) {
@@ -157,48 +162,71 @@ __global__ void __launch_bounds__(kMoveThreads) k_paged_move(MoveParams a) {
   const uint32_t* index = a.index + ((size_t)s * (a.per_head ? a.n_kv : 1) + (a.per_head ? h : 0)) * a.index_stride;
   const uint32_t* table = a.table + (size_t)s * a.table_stride;
   const uint32_t c = threadIdx.x % L, r0 = threadIdx.x / L, page_mask = (1u << a.page_shift) - 1;
-  u32x4_t* pool = (u32x4_t*)(is_v ? a.pool_v : a.pool_k);
-  const bool masses = !is_v && a.mass && c == 0, apart = a.mass != a.mass_out;
-  for (uint32_t j0 = 0; j0 < count; j0 += R * kMoveAhead) {
-    u32x4_t row[kMoveAhead];
-    float mass[kMoveAhead];
-    size_t to[kMoveAhead];
-    uint32_t what[kMoveAhead];  // bits: a row, a mass
+  u32x4_t* pool = (u32x4_t*)(is_v ? a.pool_v : a.pool_k) + slice * L + c;
+  const bool masses = !is_v && slice == 0 && a.mass && c == 0, apart = a.mass != a.mass_out;
+  uint32_t at[AHEAD], to[AHEAD];  // rows of the pool (which no memory holds 2^32 of)
+  uint32_t what[AHEAD];                // bits: a row, a mass
+  // (loads of places that exist, checked afterwards: branches would put them one behind the other)
+  auto look_up = [&](uint32_t j0) {
+    uint32_t from[AHEAD], ps[AHEAD], pd[AHEAD], bad = 0;
 #pragma unroll
-    for (int u = 0; u < kMoveAhead; u++) {
-      const uint32_t j = j0 + u * R + r0;
-      what[u] = 0;
-      if (j >= count) continue;
-      const uint32_t from = index[j];
-      if (from < j || from >= n - base) {
-        raise(c == 0 ? a.status : nullptr, RLH_SERVE_BAD_SEQ);
-        continue;
-      }
-      if (from == j && !(masses && apart)) continue;
-      const uint32_t ps = table[(base + from) >> a.page_shift], pd = table[(base + j) >> a.page_shift];
-      if (ps >= a.n_pages || pd >= a.n_pages) {
-        raise(c == 0 ? a.status : nullptr, RLH_SERVE_BAD_PAGE);
-        continue;
-      }
-      const size_t at = ((((size_t)ps * a.n_kv + h) << a.page_shift) + ((base + from) & page_mask));
-      to[u] = ((((size_t)pd * a.n_kv + h) << a.page_shift) + ((base + j) & page_mask));
-      if (from != j) {
-        row[u] = pool[at * L + c];
-        what[u] = 1;
-      }
-      if (masses) {
-        mass[u] = a.mass[at];
-        what[u] |= 2;
-      }
+    for (int u = 0; u < AHEAD; u++) from[u] = index[min(j0 + u * R + r0, count - 1)];
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) {
+      ps[u] = table[(base + min(from[u], n - base - 1)) >> a.page_shift];
+      pd[u] = table[(base + min(j0 + u * R + r0, count - 1)) >> a.page_shift];
     }
-    wait_vmcnt<0>();  // the loads have arrived: another wave may write there
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) {
+      const uint32_t j = j0 + u * R + r0;
+      const bool any = j < count && (from[u] != j || (masses && apart)), fits = from[u] >= j && from[u] < n - base;
+      const bool exist = ps[u] < a.n_pages && pd[u] < a.n_pages, ok = any && fits && exist;
+      bad |= (any && !fits ? RLH_SERVE_BAD_SEQ : 0u) | (any && fits && !exist ? RLH_SERVE_BAD_PAGE : 0u);
+      at[u] = ok ? ((ps[u] * a.n_kv + h) << a.page_shift) + ((base + from[u]) & page_mask) : 0;
+      to[u] = ok ? ((pd[u] * a.n_kv + h) << a.page_shift) + ((base + j) & page_mask) : 0;
+      what[u] = ok ? (from[u] != j ? 1u : 0u) | (masses ? 2u : 0u) : 0u;
+    }
+    if (bad && c == 0) raise(a.status, bad);
+  };
+  look_up(0);
+  for (uint32_t j0 = 0; j0 < count; j0 += R * AHEAD) {
+    u32x4_t row[AHEAD];
+    float mass[AHEAD];
+    uint32_t dst[AHEAD], moves[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) {
+      if (__ballot(what[u] & 1)) row[u] = pool[(size_t)at[u] * (D / 8)];
+      dst[u] = to[u];
+      moves[u] = what[u];
+    }
+    if (masses) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; u++) mass[u] = a.mass[at[u]];
+    }
+    if (j0 + R * AHEAD < count) look_up(j0 + R * AHEAD);
+    wait_vmcnt<0>();  // the values have arrived: another wave may write where they were
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kMoveAhead; u++) {
-      if (what[u] & 1) pool[to[u] * L + c] = row[u];
-      if (what[u] & 2) a.mass_out[to[u]] = mass[u];
+    for (int u = 0; u < AHEAD; u++)
+      if (moves[u] & 1) pool[(size_t)dst[u] * (D / 8)] = row[u];
+    if (masses) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; u++)
+        if (moves[u] & 2) a.mass_out[dst[u]] = mass[u];
     }
   }
+}
+
+template <int D, int L, int THREADS, int AHEAD>
+int launch_move(const MoveParams& p, hipStream_t stream) {
+  const uint32_t of = (p.n_seq * p.n_kv * 2 + 7) / 8 * 8;
+  return enqueue("rlh_paged_move", k_paged_move<D, L, THREADS, AHEAD>, dim3(of * (D / 8 / L)), THREADS, 0, stream, p);
+}
+template <int D>
+int launch_move(const MoveParams& p, hipStream_t stream) {
+  // short lists: whole rows by small blocks; long ones: slices of 64 bytes
+  if (p.max_count <= 256) return launch_move<D, D / 8, 256, 1>(p, stream);
+  return launch_move<D, 4, 1024, 8>(p, stream);
 }
 
 // ---- what stays -------------------------------------------------------------------------
@@ -218,13 +246,21 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
 }
 constexpr uint32_t kKeptKey = 0xffffffffu;  // above every mass
 
+// How many lanes below this one are in the mask.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
-constexpr int kEvictBins = 2048;
+constexpr int kEvictBits[3] = {13, 10, 9};  // of a key, from the top
+constexpr int kEvictBins = 1 << 13;
 
 // A block takes one KV head of one sequence. The smallest kept key is found
-// from three histograms of 11, 11 and 10 of its bits; then each wave counts the
-// larger and the equal ones of its stretch and lists those that stay.
+// from three histograms of 13, 10 and 9 of its bits; then each wave counts the
+// larger and the equal ones of its stretch and lists those that stay. With up
+// to 1024 R positions the keys stay in registers (R = 0: read anew each time).
+template <int R>
 __global__ void __launch_bounds__(kEvictThreads) k_evict_select(EvictParams a) {
   __shared__ uint32_t bins[kEvictBins];
   __shared__ uint32_t sums[2][kEvictWaves];
@@ -259,34 +295,91 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(EvictParams a) {
   // each wave's stretch, 64 positions at a time
   const uint32_t rounds = (n + kEvictThreads - 1) / kEvictThreads;
   const uint32_t j0 = wave * rounds * 64 + lane;
+  uint32_t keys[R ? R : 1];
+  // f(position, key) for the wave's positions in order
+  auto each = [&](auto f) {
+    if constexpr (R != 0) {
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        if ((uint32_t)r >= rounds) continue;
+        asm volatile("" : "+v"(keys[r]));  // (no comparison is kept from one sweep for the next)
+        f(j0 + r * 64, keys[r]);
+      }
+    } else {
+      for (uint32_t r = 0; r < rounds; r++) f(j0 + r * 64, key_of(j0 + r * 64));
+    }
+  };
+  if constexpr (R != 0) {
+    // pages, then masses, kAtOnce at a time: what is not a mass is read from the sequence's first place
+    // (a branch among them would put one load behind the other)
+    bool missing = false;
+    constexpr int kAtOnce = R < 20 ? R : 20;
+#pragma unroll
+    for (int r0 = 0; r0 < R; r0 += kAtOnce) {
+      uint32_t page[kAtOnce];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; r++) {
+        const uint32_t j = j0 + (r0 + r) * 64;
+        page[r] = table[(j < n ? j : 0u) >> a.page_shift];
+      }
+      float x[kAtOnce];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; r++) {
+        const uint32_t slot = (j0 + (r0 + r) * 64) & ((1u << a.page_shift) - 1);
+        x[r] = a.mass[(((size_t)(page[r] < a.n_pages ? page[r] : 0u) * a.n_kv + h) << a.page_shift) + slot];
+      }
+#pragma unroll
+      for (int r = 0; r < kAtOnce; r++) {
+        asm volatile("" : "+v"(x[r]));  // (or the load would move behind the conditions below)
+        const uint32_t j = j0 + (r0 + r) * 64;
+        const bool middle = j >= a.first && j < n - a.last, exists = page[r] < a.n_pages;
+        missing |= middle && !exists;
+        keys[r0 + r] = j >= n ? 0u : !middle ? kKeptKey : !exists ? 1u : mass_key(x[r]);
+      }
+    }
+    if (missing) raise(a.status, RLH_SERVE_BAD_PAGE);
+  }
   uint32_t prefix = 0, left = a.budget;  // keys that begin with `prefix`: so many of them stay
 #pragma unroll
   for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
-    for (uint32_t b = t; b < kEvictBins; b += kEvictThreads) bins[b] = 0;
+    const int width = kEvictBits[pass], shift = pass == 0 ? 32 - width : pass == 1 ? kEvictBits[2] : 0;
+    const int kMine = pass == 0 ? kEvictBins / kEvictThreads : 1;  // bins of a thread
+    for (uint32_t b = t; b < 1u << width; b += kEvictThreads) bins[b] = 0;
     __syncthreads();
-    for (uint32_t r = 0; r < rounds; r++) {
-      const uint32_t k = key_of(j0 + r * 64);
-      if (pass == 0 || k >> (shift + width) == prefix) atomicAdd(&bins[k >> shift & ((1u << width) - 1)], 1u);
-    }
+    each([&](uint32_t, uint32_t k) {
+      if (pass != 0 && k >> (shift + width) != prefix) return;
+      const uint32_t bin = k >> shift & ((1u << width) - 1);
+      // (lanes of one bin would take turns at it: where all are, one counts for them)
+      const uint32_t bin0 = uniform(bin);
+      const uint64_t here = __ballot(true);
+      if (__ballot(bin == bin0) != here)
+        atomicAdd(&bins[bin], 1u);
+      else if (lane == (uint32_t)__builtin_ctzll(here))
+        atomicAdd(&bins[bin], (uint32_t)__popcll(here));
+    });
     __syncthreads();
     // from the top: the bin in which the count passes what is left
-    const uint32_t b0 = kEvictBins - 2 - 2 * t;  // thread t: bins b0 + 1 and b0
-    const uint32_t hi = bins[b0 + 1], lo = bins[b0];
-    uint32_t upto = hi + lo;
+    uint32_t mine[kEvictBins / kEvictThreads], sum = 0;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t x = __shfl_up(upto, d);
-      if (lane >= (uint32_t)d) upto += x;
+    for (int i = 0; i < kMine; i++) {
+      const uint32_t b = t * kMine + i;
+      mine[i] = b < 1u << width ? bins[(1u << width) - 1 - b] : 0;
+      sum += mine[i];
     }
+    uint32_t upto = wave_scan(sum);
     if (lane == 63) sums[0][wave] = upto;
     __syncthreads();
     for (uint32_t w = 0; w < wave; w++) upto += sums[0][w];
-    const uint32_t before = upto - hi - lo;
+    uint32_t before = upto - sum;
     if (before < left && upto >= left) {
-      const bool high = before + hi >= left;
-      found[0] = high ? b0 + 1 : b0;
-      found[1] = left - before - (high ? 0 : hi);
+#pragma unroll
+      for (int i = 0; i < kMine; i++) {
+        if (before < left && before + mine[i] >= left) {
+          found[0] = (1u << width) - 1 - (t * kMine + i);
+          found[1] = left - before;
+        }
+        before += mine[i];
+      }
     }
     __syncthreads();
     prefix = prefix << width | found[0];
@@ -295,31 +388,37 @@ __global__ void __launch_bounds__(kEvictThreads) k_evict_select(EvictParams a) {
   }
   // `prefix` is the smallest key that stays, of `left` positions
   uint32_t above = 0, equal = 0;
-  for (uint32_t r = 0; r < rounds; r++) {
-    const uint32_t k = key_of(j0 + r * 64);
+  each([&](uint32_t, uint32_t k) {
     above += (uint32_t)__popcll(__ballot(k > prefix));
     equal += (uint32_t)__popcll(__ballot(k == prefix));
-  }
+  });
   if (lane == 0) {
     sums[0][wave] = above;
     sums[1][wave] = equal;
   }
   __syncthreads();
-  uint32_t at = 0, ties = 0;
-  for (uint32_t w = 0; w < wave; w++) {
-    at += sums[0][w];
-    ties += sums[1][w];
+  uint32_t at = 0, ties = 0, all_ties = 0;
+  for (uint32_t w = 0; w < kEvictWaves; w++) {
+    at += w < wave ? sums[0][w] : 0u;
+    ties += w < wave ? sums[1][w] : 0u;
+    all_ties += sums[1][w];
   }
   at += min(ties, left);
-  const uint64_t below = (1ull << lane) - 1;
-  for (uint32_t r = 0; r < rounds; r++) {
-    const uint32_t j = j0 + r * 64, k = key_of(j);
-    const uint64_t same = __ballot(k == prefix);
-    const bool stays = k > prefix || (k == prefix && ties + (uint32_t)__popcll(same & below) < left);
-    const uint64_t all = __ballot(stays);
-    if (stays) keep[at + (uint32_t)__popcll(all & below)] = j;
-    at += (uint32_t)__popcll(all);
-    ties += (uint32_t)__popcll(same);
+  if (all_ties == left) {
+    each([&](uint32_t j, uint32_t k) {
+      const uint64_t all = __ballot(k >= prefix);
+      if (k >= prefix) keep[at + lanes_below(all)] = j;
+      at += (uint32_t)__popcll(all);
+    });
+  } else {
+    each([&](uint32_t j, uint32_t k) {
+      const uint64_t same = __ballot(k == prefix);
+      const bool stays = k > prefix || (k == prefix && ties + lanes_below(same) < left);
+      const uint64_t all = __ballot(stays);
+      if (stays) keep[at + lanes_below(all)] = j;
+      at += (uint32_t)__popcll(all);
+      ties += (uint32_t)__popcll(same);
+    });
   }
 }
 
@@ -507,9 +606,7 @@ int rlh_paged_move(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_move_
   p.max_count = args->max_count;
   p.page_shift = (uint32_t)__builtin_ctz(kv->page_size);
   p.n_pages = (uint32_t)kv->n_pages;
-  const dim3 grid(seqs->n_seq * kv->n_head_kv * 2);
-  return enqueue("rlh_paged_move", kv->head_dim == 64 ? k_paged_move<64> : k_paged_move<128>, grid, kMoveThreads, 0,
-                 (hipStream_t)stream, p);
+  return kv->head_dim == 64 ? launch_move<64>(p, (hipStream_t)stream) : launch_move<128>(p, (hipStream_t)stream);
 }
 
 int rlh_evict_select(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_evict_args* args, uint32_t* status,
@@ -557,8 +654,10 @@ int rlh_evict_select(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_evi
   p.first = args->first_kept;
   p.last = args->last_kept;
   p.keep_stride = args->keep_stride;
-  return enqueue("rlh_evict_select", k_evict_select, dim3(seqs->n_seq * kv->n_head_kv), kEvictThreads, 0,
-                 (hipStream_t)stream, p);
+  const uint32_t rounds = (seqs->max_kv + kEvictThreads - 1) / kEvictThreads;
+  const auto kernel = rounds <= 8 ? k_evict_select<8> : rounds <= 16 ? k_evict_select<16>
+                      : rounds <= 40 ? k_evict_select<40> : k_evict_select<0>;
+  return enqueue("rlh_evict_select", kernel, dim3(seqs->n_seq * kv->n_head_kv), kEvictThreads, 0, (hipStream_t)stream, p);
 }
 
 }  // extern "C"
