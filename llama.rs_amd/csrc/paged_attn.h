@@ -191,6 +191,7 @@ struct Workspace {
   float* item_ml;    // [items * n_kv][16][2]
   uint32_t* plan;    // [n_seq][2]: first item, items
   uint32_t* tiles;   // [n_seq][2]: first tile, tiles (where `planned`)
+  uint64_t* line;    // of drafted rows: a block's units, then each sequence's first one
 };
 
 struct Sizes {
@@ -207,6 +208,8 @@ struct Sizes {
   bool planned;           // a launch before found where each sequence's items and tiles begin
   bool merge_small;       // only its sequences have parts to join
   uint32_t merge_rows;    // then: blocks per sequence and KV head
+  uint32_t line_blocks;   // not 0: drafted rows as a line of tiles that so many blocks per KV head share
+  uint32_t slot_rows;     // rows of a part of theirs
 };
 
 // Blocks of a KV head for the shared prefix.
@@ -629,10 +632,9 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t r) {
 }
 
 // Tiles of sequence s.
-template <bool TREE>
 __device__ __forceinline__ uint32_t tiles_of_seq(const Launch& L, uint32_t s) {
   bool bad;
-  const SeqView v = load_attn_seq<TREE>(L.a, s, &bad);
+  const SeqView v = load_seq(L.a.b, s, &bad);
   const uint32_t r = v.ok ? v.q_len * L.a.group : 0;
   return r > L.n.small_rows ? (r + kTileRows - 1) / kTileRows : 0u;
 }
@@ -641,11 +643,26 @@ struct TileShared {
   uint64_t special[2];  // positions of a step whose V row holds infinities or NaN
   int32_t ranges[kTileWaves][8];
 };
-template <int D>
-constexpr uint32_t kTileLds = 4 * kTileKv * D * 2 + sizeof(TileShared);
+// Steps that LDS holds: one in use, the others on their way. Prompts find
+// theirs one step ahead; drafted rows, whose steps are often shorter than what
+// HBM takes under load (of up to 128 rows 1.3 us, 2.2 us), three.
+template <bool TREE>
+constexpr int kTileBufs = TREE ? 4 : 2;
+template <int D, bool TREE>
+constexpr uint32_t kTileLds = 2 * kTileBufs<TREE> * kTileKv * D * 2 + sizeof(TileShared);
+
+// What a block does at a time: steps of 64 positions of a tile.
+struct TileJob {
+  uint32_t h, s, row0, rows;  // KV head, sequence (own positions), the tile's first row and all rows
+  bool prefix;                // the shared positions, of the rows of all sequences
+  uint32_t part, parts;       // TREE false: the part of the tile's positions
+  int32_t begin, end;         // TREE: the positions that steps count from, and their end
+  uint32_t st0, st1;          // TREE: its steps
+  float *o, *ml;              // TREE: where a part of the tile goes (null: the tile is whole)
+};
 
 template <typename T, int D, int MOD, bool TREE>
-__device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool prefix, uint8_t* lds) {
+__device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, uint8_t* lds) {
   constexpr int kRowB = D * 2;
   constexpr int kBuf = kTileKv * kRowB;   // bytes of a K or V step
   constexpr int kSteps = D / 16;
@@ -654,41 +671,17 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   constexpr int kThreads = 64 * kTileWaves;
   constexpr int kMine = kTileKv / kTileWaves;           // positions of a step that a wave copies
   constexpr int kCopies = kMine / (64 / kLanes);        // in 1 KB pieces
-  // K, V of two steps first
-  TileShared& sh = *(TileShared*)(lds + 4 * kBuf);
+  constexpr int kBufs = kTileBufs<TREE>;
+  // K, V of the steps first
+  TileShared& sh = *(TileShared*)(lds + 2 * kBufs * kBuf);
   uint64_t* special = sh.special;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(RLH_LDS uint8_t*)lds;
   const AttnParams& a = L.a;
   const uint32_t t = threadIdx.x;
   const uint32_t wave = uniform(t >> 6), lane = t & 63;
-  const uint32_t h = block % a.n_kv, of_head = block / a.n_kv;
-  uint32_t parts = prefix ? L.n.prefix_parts : L.n.tile_parts, tile = of_head / parts, part = of_head % parts;
-  if (prefix && tile >= L.n.prefix_tiles - 1) {
-    tile = L.n.prefix_tiles - 1;
-    part = of_head - tile * parts;
-    parts = L.n.last_parts;
-  }
-  // the tile's sequence (own positions), or all rows (the prefix)
-  uint32_t s = 0, row0 = 0, rows = 0;
-  if (prefix) {
-    row0 = tile * kTileRows;
-    rows = a.b.n_rows * a.group;
-  } else {
-    if (block == 0 && !L.n.planned)
-      for (uint32_t i = t; i < a.b.n_seq; i += kThreads) {
-        bool bad;
-        load_attn_seq<TREE>(a, i, &bad);
-        if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
-      }
-    Found f;
-    if (L.n.planned ? !find_planned(L.ws.tiles, a.b.n_seq, tile, &f)
-                    : !find_item(a.b.n_seq, tile, [&](uint32_t i) { return tiles_of_seq<TREE>(L, i); }, &f))
-      return;
-    s = f.s;
-    row0 = (f.n - 1 - (tile - f.first)) * kTileRows;  // the last rows, with the most positions, first
-    bool bad;
-    rows = load_seq(a.b, s, &bad).q_len * a.group;
-  }
+  const bool prefix = job.prefix;
+  if (TREE) __syncthreads();  // every wave is done with the job before
+  const uint32_t h = job.h, part = job.part, parts = job.parts, s = job.s, row0 = job.row0, rows = job.rows;
   // the lane's row
   const uint32_t col = lane & 31, half = lane >> 5;
   const uint32_t rr = row0 + wave * 32 + col;
@@ -777,8 +770,13 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   t_hi = (int32_t)uniform(t_hi);
   t_prefix = (int32_t)uniform(t_prefix);
   t_min_lo = (int32_t)uniform(t_min_lo);
+  if (TREE) {
+    t_lo = job.begin;
+    t_hi = min(t_hi, job.end);
+  }
   const uint32_t n_steps = t_hi > t_lo ? (uint32_t)(t_hi - t_lo + kTileKv - 1) / kTileKv : 0;
-  const uint32_t st0 = (uint32_t)((uint64_t)n_steps * part / parts), st1 = (uint32_t)((uint64_t)n_steps * (part + 1) / parts);
+  const uint32_t st0 = TREE ? job.st0 : (uint32_t)((uint64_t)n_steps * part / parts);
+  const uint32_t st1 = TREE ? min(job.st1, n_steps) : (uint32_t)((uint64_t)n_steps * (part + 1) / parts);
 
   const float slope2 = MOD && a.slopes && active ? a.slopes[head] * kLog2e : 0.0f;
   vec8<T> q[kSteps];
@@ -865,22 +863,35 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   if (st0 < st1) {
     pages = look_up(st0);
     exist = __ballot(pages != kNone);
-    copy(t_lo + (int32_t)st0 * kTileKv, pages, 0, 0);
+    for (uint32_t i = 0; i < kBufs - 1 && st0 + i < st1; i++) copy(t_lo + (int32_t)(st0 + i) * kTileKv, pages, i, i);
   }
+  uint64_t next_exist = 0;
   for (uint32_t st = st0; st < st1; st++) {
-    const uint32_t buf = (st - st0) & 1;
+    const uint32_t buf = (st - st0) & (kBufs - 1);
     const int32_t p = t_lo + (int32_t)st * kTileKv;
     const uint32_t k = (st - st0) & 15;
+    if (k == 0 && st != st0) exist = next_exist;
     const uint32_t ok = (uint32_t)(exist >> (4 * k)) & 15;
-    if (t == 0) special[buf] = 0;  // last read two barriers ago
-    wait_vmcnt<0>();               // this wave's copies of the step have landed
-    lds_barrier();                 // ... everyone's; every wave is done with the other buffer
-    if (k == 8) next_pages = look_up(st + 8);
-    if (k == 15) {
-      pages = next_pages;
-      exist = __ballot(pages != kNone);
+    if (t == 0) special[buf & 1] = 0;  // last read two barriers ago
+    // this wave's copies of the step have landed (those of the steps behind it may be on their way)
+    if constexpr (kBufs == 4) {
+      if (st + 2 < st1)
+        wait_vmcnt<4 * kCopies>();
+      else if (st + 1 < st1)
+        wait_vmcnt<2 * kCopies>();
+      else
+        wait_vmcnt<0>();
+    } else {
+      wait_vmcnt<0>();
     }
-    if (st + 1 < st1) copy(p + kTileKv, pages, (k + 1) & 15, buf ^ 1);
+    lds_barrier();  // ... everyone's; every wave is done with the buffer before this one
+    if (k == 8) next_pages = look_up(st + 8);
+    if (k == 17 - kBufs) {
+      pages = next_pages;
+      next_exist = __ballot(pages != kNone);
+    }
+    if (st + kBufs - 1 < st1)
+      copy(p + (kBufs - 1) * kTileKv, pages, (k + kBufs - 1) & 15, (buf + kBufs - 1) & (kBufs - 1));
     const uint8_t RLH_LDS* kb = (const uint8_t RLH_LDS*)lds + buf * 2 * kBuf;
     uint8_t RLH_LDS* vb = (uint8_t RLH_LDS*)lds + buf * 2 * kBuf + kBuf;
     const bool full = ok == 15 && ((p >= w_lo && p + kTileKv <= w_hi) || p + kTileKv <= w_prefix);
@@ -893,10 +904,10 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
       for (int i = 0; i < kBuf / (kThreads * 16); i++) {
         const uint32_t at = (i * kThreads + t) * 16;
         if (any_special<T>(*(const RLH_LDS_PTR(u32x4_t)*)(vb + at)))
-          atomicOr((unsigned long long*)&special[buf], 1ull << (at / kRowB));
+          atomicOr((unsigned long long*)&special[buf & 1], 1ull << (at / kRowB));
       }
       lds_barrier();
-      odd = special[buf];
+      odd = special[buf & 1];
     }
     f32x16_t sc[2];
     vec8<T> pr[4];
@@ -1015,7 +1026,7 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   }
   l = sum_across_32(l);
   if (!active) return;
-  if (!prefix && parts == 1 && a.shared_len == 0) {
+  if (!prefix && (TREE ? job.o == nullptr : parts == 1) && a.shared_len == 0) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* dst = (T*)a.out + (size_t)row * a.out_stride + (size_t)head * D;
 #pragma unroll
@@ -1029,9 +1040,10 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
       }
     if (a.lse && half == 0) a.lse[(size_t)row * a.n_head + head] = log_sum<T>(m, l);
   } else {
-    const size_t at = ((size_t)part * a.b.n_rows + row) * a.n_head + head;
-    float* dst = (prefix ? L.ws.prefix_o : L.ws.tile_o) + at * D;
-    float* mlp = (prefix ? L.ws.prefix_ml : L.ws.tile_ml) + at * 2;
+    const bool slot = TREE && job.o;
+    const size_t at = slot ? rr - row0 : ((size_t)(TREE ? 0 : part) * a.b.n_rows + row) * a.n_head + head;
+    float* dst = (slot ? job.o : prefix ? L.ws.prefix_o : L.ws.tile_o) + at * D;
+    float* mlp = (slot ? job.ml : prefix ? L.ws.prefix_ml : L.ws.tile_ml) + at * 2;
 #pragma unroll
     for (int i = 0; i < kOut; i++)
 #pragma unroll
@@ -1044,22 +1056,215 @@ __device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool
   }
 }
 
+template <typename T, int D, int MOD>
+__device__ __forceinline__ void tile_block(const Launch& L, uint32_t block, bool prefix, uint8_t* lds) {
+  const AttnParams& a = L.a;
+  const uint32_t h = block % a.n_kv, of_head = block / a.n_kv;
+  uint32_t parts = prefix ? L.n.prefix_parts : L.n.tile_parts, tile = of_head / parts, part = of_head % parts;
+  if (prefix && tile >= L.n.prefix_tiles - 1) {
+    tile = L.n.prefix_tiles - 1;
+    part = of_head - tile * parts;
+    parts = L.n.last_parts;
+  }
+  // the tile's sequence (own positions), or all rows (the prefix)
+  uint32_t s = 0, row0 = 0, rows = 0;
+  if (prefix) {
+    row0 = tile * kTileRows;
+    rows = a.b.n_rows * a.group;
+  } else {
+    if (block == 0 && !L.n.planned)
+      for (uint32_t i = threadIdx.x; i < a.b.n_seq; i += 64 * kTileWaves) {
+        bool bad;
+        load_seq(a.b, i, &bad);
+        if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
+      }
+    Found f;
+    if (L.n.planned ? !find_planned(L.ws.tiles, a.b.n_seq, tile, &f)
+                    : !find_item(a.b.n_seq, tile, [&](uint32_t i) { return tiles_of_seq(L, i); }, &f))
+      return;
+    s = f.s;
+    row0 = (f.n - 1 - (tile - f.first)) * kTileRows;  // the last rows, with the most positions, first
+    bool bad;
+    rows = load_seq(a.b, s, &bad).q_len * a.group;
+  }
+  TileJob job{};
+  job.h = h;
+  job.s = s;
+  job.row0 = row0;
+  job.rows = rows;
+  job.prefix = prefix;
+  job.part = part;
+  job.parts = parts;
+  tile_run<T, D, MOD, false>(L, job, lds);
+}
+
 // Prefix tiles, tiles and items of few rows in one launch, long blocks first:
 // each kind leaves parts of the card idle that the others fill (64 tokens of
 // 32 heads behind 4096 shared positions: 28 us, in launches of their own
 // 20 + 17; 72 of 64 heads behind 16384: 70 us, apart 65 + 14 + 5; a prompt
 // alone loses 1 % by it).
-template <typename T, int D, int MOD, bool TREE>
+template <typename T, int D, int MOD>
 __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
   const uint32_t n_prefix = prefix_blocks(L.n) * L.a.n_kv;
   const uint32_t n_tiles = n_prefix + L.n.tiles * L.n.tile_parts * L.a.n_kv;
   const uint32_t b = blockIdx.x;
   if (b < n_tiles) {
-    tile_block<T, D, MOD, TREE>(L, b < n_prefix ? b : b - n_prefix, b < n_prefix, lds);
+    tile_block<T, D, MOD>(L, b < n_prefix ? b : b - n_prefix, b < n_prefix, lds);
   } else {  // two items, of four waves each
     const uint32_t half = uniform(threadIdx.x / kThreads);
-    small_block<T, D, MOD, kWaves, TREE>(L, 2 * (b - n_tiles) + half, lds + half * kSmallLds<D, kWaves>);
+    small_block<T, D, MOD, kWaves, false>(L, 2 * (b - n_tiles) + half, lds + half * kSmallLds<D, kWaves>);
+  }
+}
+
+// ---- drafted rows as a line of tiles -------------------------------------------------
+// Every drafted row sees nearly all of its sequence, so that a tile's time is
+// its sequence's length, and batches have few and unequal tiles. The tiles of a KV
+// head (of the shared positions first, then the sequences' own) are therefore
+// laid out as one line and divided equally among as many blocks as run at once.
+struct LineSeq {
+  SeqSpan q;
+  uint32_t steps;
+  uint64_t units;
+};
+__device__ __forceinline__ LineSeq line_seq(const AttnParams& a, uint32_t s, bool* bad) {
+  LineSeq r;
+  r.q = seq_span<true>(a, s, bad);
+  r.steps = r.q.rows ? (uint32_t)(r.q.end - r.q.begin + kTileKv - 1) / kTileKv : 0;
+  r.units = line_units(r.q.rows, r.steps);
+  return r;
+}
+// Inclusive sum over the wave in lane order, of 64 bits.
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
+  const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t y = (uint64_t)__shfl_up((unsigned long long)x, d);
+    x += lane >= (uint32_t)d ? y : 0;
+  }
+  return x;
+}
+__device__ __forceinline__ uint64_t lane_value64(uint64_t x, int lane) {
+  return (uint64_t)lane_value((uint32_t)(x >> 32), lane) << 32 | lane_value((uint32_t)x, lane);
+}
+__device__ __forceinline__ uint32_t prefix_steps(const AttnParams& a) { return (a.shared_len + kTileKv - 1) / kTileKv; }
+__device__ __forceinline__ uint64_t prefix_units(const AttnParams& a) {
+  return a.shared_len ? line_units(a.b.n_rows * a.group, prefix_steps(a)) : 0;
+}
+
+// Up to so many sequences every block lays the line out by itself.
+constexpr uint32_t kPlanned = 256;
+
+template <typename T, int D, int MOD>
+__global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  __shared__ uint64_t line[2 + kPlanned];  // a block's share and all units, then each sequence's first one
+  const AttnParams& a = L.a;
+  const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const uint32_t h = blockIdx.x % a.n_kv, block = blockIdx.x / a.n_kv;
+  if (!L.n.planned) {
+    if (wave == 0) {
+      uint64_t before = prefix_units(a);
+      for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64) {
+        const uint32_t s = s0 + lane;
+        uint64_t u = 0;
+        if (s < a.b.n_seq) {
+          bool bad;
+          u = line_seq(a, s, &bad).units;
+          if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
+        }
+        const uint64_t upto = before + wave_scan64(u);
+        if (s < a.b.n_seq) {
+          line[2 + s] = upto - u;
+          if (blockIdx.x == 0) L.ws.line[2 + s] = upto - u;  // for the launch that joins parts
+        }
+        before = lane_value64(upto, 63);
+      }
+      if (lane == 0) {
+        line[0] = line_share(before, L.n.line_blocks);
+        line[1] = before;
+        if (blockIdx.x == 0) L.ws.line[0] = line[0];
+      }
+    }
+    __syncthreads();
+  }
+  const uint64_t share = lane_value64(L.n.planned ? L.ws.line[0] : line[0], 0);
+  const uint64_t total = lane_value64(L.n.planned ? L.ws.line[1] : line[1], 0);
+  const uint64_t x1 = min((block + 1) * share, total);
+  for (uint64_t x = block * share; x < x1;) {
+    TileJob job{};
+    job.h = h;
+    job.prefix = x < prefix_units(a);
+    uint64_t first = 0;  // unit of the sequence's first tile
+    uint32_t steps;
+    if (job.prefix) {
+      job.rows = a.b.n_rows * a.group;
+      job.end = (int32_t)a.shared_len;
+      steps = prefix_steps(a);
+    } else {
+      // the last sequence that begins at x or before (those without units share their first one with the next)
+      uint32_t n = 0;
+      if (L.n.planned) {
+        n = count_upto<uint64_t>(L.ws.line + 2, 1, a.b.n_seq, x);
+      } else {
+        for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64)
+          n += (uint32_t)__popcll(__ballot(s0 + lane < a.b.n_seq && line[2 + s0 + lane] <= x));
+      }
+      job.s = uniform(n - 1);
+      first = lane_value64(L.n.planned ? L.ws.line[2 + job.s] : line[2 + job.s], 0);
+      bool bad;
+      const LineSeq q = line_seq(a, job.s, &bad);
+      job.rows = uniform(q.q.rows);
+      job.begin = (int32_t)uniform((uint32_t)q.q.begin);
+      job.end = (int32_t)uniform((uint32_t)q.q.end);
+      steps = uniform(q.steps);
+    }
+    const uint32_t k = line_at(first, job.rows, steps, x);
+    const LineTile tile = line_tile(first, job.rows, steps, k);
+    const uint64_t end = line_end(tile);
+    job.row0 = k * kTileRows;
+    job.st0 = uniform(line_step(tile, x));
+    job.st1 = end <= x1 ? steps : uniform(line_step(tile, x1));
+    if (job.st0 != 0 || job.st1 != steps) {
+      const size_t slot = ((size_t)line_slot(tile, block, share) * a.n_kv + h) * L.n.slot_rows;
+      job.o = L.ws.item_o + slot * D;
+      job.ml = L.ws.item_ml + slot * 2;
+    }
+    if (job.st0 < job.st1) tile_run<T, D, MOD, true>(L, job, lds);
+    x = end;
+  }
+}
+
+// The line of more than kPlanned sequences, by one block: its share, its
+// length and each sequence's first unit.
+constexpr int kPlanThreads = 1024;
+__global__ void __launch_bounds__(kPlanThreads) k_line_plan(Launch L) {
+  __shared__ uint64_t sums[kPlanThreads / 64];
+  const AttnParams& a = L.a;
+  const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  uint64_t before = prefix_units(a);
+  for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += kPlanThreads) {
+    uint64_t u = 0;
+    if (s0 + t < a.b.n_seq) {
+      bool bad;
+      u = line_seq(a, s0 + t, &bad).units;
+      if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
+    }
+    uint64_t upto = wave_scan64(u);
+    __syncthreads();
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    uint64_t all = 0;
+    for (uint32_t w = 0; w < kPlanThreads / 64; w++) {
+      upto += w < wave ? sums[w] : 0;
+      all += sums[w];
+    }
+    if (s0 + t < a.b.n_seq) L.ws.line[2 + s0 + t] = before + upto - u;
+    before += all;
+  }
+  if (t == 0) {
+    L.ws.line[0] = line_share(before, L.n.line_blocks);
+    L.ws.line[1] = before;
   }
 }
 
@@ -1174,6 +1379,83 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
   if (a.lse && c0 == 0) a.lse[rh] = log_sum<T>(m, l);
 }
 
+// The same for a line of tiles: a wave takes four heads of a row, 16 lanes each,
+// and goes through their parts with a running maximum, eight parts' loads at a time.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) k_line_merge(Launch L) {
+  constexpr int N = D / 16;   // values per lane
+  constexpr uint32_t kAhead = 8;
+  const AttnParams& a = L.a;
+  const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const uint32_t per_row = (a.n_head + 3) / 4, w = blockIdx.x * kWaves + wave;
+  const uint32_t row = w / per_row, head = w % per_row * 4 + lane / 16;
+  if (row >= a.b.n_rows) return;
+  const uint64_t share = L.ws.line[0];
+  const uint32_t s = count_upto<uint32_t>(a.b.q_start + 1, 1, a.b.n_seq, row);
+  if (s >= a.b.n_seq) return;
+  bool bad;
+  const LineSeq q = line_seq(a, s, &bad);
+  if (row < q.q.v.q0 || !q.q.v.ok || head >= a.n_head) return;
+  const uint32_t h = head / a.group, r = (row - q.q.v.q0) * a.group + head % a.group;
+  const uint32_t in_head = row * a.group + head % a.group;  // among all rows of its KV head
+  const LineTile own = line_tile(L.ws.line[2 + s], q.q.rows, q.steps, r / kLineRows);
+  const uint32_t own0 = line_first_block(own, share), n_own = line_last_block(own, share) - own0 + 1;
+  LineTile shared{};  // the tile of the shared positions
+  uint32_t shared0 = 0, n_shared = 0;
+  if (a.shared_len) {
+    shared = line_tile(0, a.b.n_rows * a.group, prefix_steps(a), in_head / kLineRows);
+    shared0 = line_first_block(shared, share);
+    n_shared = line_last_block(shared, share) - shared0 + 1;
+  }
+  if (n_shared == 0 && n_own == 1) return;  // written already
+  const size_t rh = (size_t)row * a.n_head + head;
+  const uint32_t n = n_shared + n_own, c0 = lane % 16 * N;
+  float m = -INFINITY, l = 0.0f, acc[N] = {};
+  for (uint32_t i0 = 0; i0 < n; i0 += kAhead) {
+    f32x4_t v[kAhead][N / 4];
+    float mi[kAhead], li[kAhead], top = m;
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      const uint32_t i = min(i0 + k, n - 1);
+      const bool mine = i >= n_shared;
+      const float *o = mine ? L.ws.tile_o : L.ws.prefix_o, *ml = mine ? L.ws.tile_ml : L.ws.prefix_ml;
+      size_t at = rh;  // a whole tile's
+      if ((mine ? n_own : n_shared) > 1) {
+        const uint32_t slot = mine ? line_slot(own, own0 + i - n_shared, share) : line_slot(shared, shared0 + i, share);
+        at = ((size_t)slot * a.n_kv + h) * L.n.slot_rows + (mine ? r : in_head) % kLineRows;
+        o = L.ws.item_o;
+        ml = L.ws.item_ml;
+      }
+      mi[k] = i0 + k < n ? ml[at * 2] : -INFINITY;
+      li[k] = ml[at * 2 + 1];
+#pragma unroll
+      for (int e = 0; e < N / 4; e++) v[k][e] = *(const f32x4_t*)(o + at * D + c0 + 4 * e);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) top = fmaxf(top, mi[k]);
+    const float tb = top == -INFINITY ? 0.0f : top, f0 = __builtin_amdgcn_exp2f(m - tb);
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < N; e++) acc[e] *= f0;
+    m = top;
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; k++) {
+      if (i0 + k >= n) continue;
+      const float f = __builtin_amdgcn_exp2f(mi[k] - tb);
+      l = fmaf(li[k], f, l);
+#pragma unroll
+      for (int e = 0; e < N; e++) acc[e] = fmaf(v[k][e / 4][e % 4], f, acc[e]);
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  typedef T VO __attribute__((ext_vector_type(N)));
+  VO v;
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = (T)(acc[i] * inv);
+  *(VO*)((T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + c0) = v;
+  if (a.lse && c0 == 0) a.lse[rh] = log_sum<T>(m, l);
+}
+
 // Up to so many positions, and while all blocks run at once, a sequence of few
 // rows is not divided: its block then has eight waves (a step of 256 positions
 // takes 2 us) and there is no second launch (8 sequences of 250: 8.6 us
@@ -1187,9 +1469,6 @@ constexpr uint32_t kWhole = 512;
 // costs less than a launch; beyond, their loops over all sequences would take
 // longer than the attention (2048 tokens of 32 heads over 8 of 128, 300
 // positions each: 5 + 448 us instead of 1024).
-constexpr uint32_t kPlanned = 256;
-constexpr int kPlanThreads = 1024;
-
 template <bool TREE>
 __global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
   __shared__ uint32_t sums[2][kPlanThreads / 64];
@@ -1235,7 +1514,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_attn_plan(Launch L) {
       const uint32_t steps = small_steps<kWaves, TREE>(a, s, &bad, &mine);
       if (bad) raise(a.status, RLH_SERVE_BAD_SEQ);
       if (L.n.small) n[0] = steps ? items_of(steps, per_item) : mine ? 1u : 0u;
-      if (L.n.tiled) n[1] = tiles_of_seq<TREE>(L, s);
+      if (L.n.tiled) n[1] = tiles_of_seq(L, s);
     }
     uint32_t upto[2] = {n[0], n[1]};
     scan(upto, all);
@@ -1318,12 +1597,27 @@ Scoring scoring_of(const rlh_attn_args& args, int* mod) {
   return c;
 }
 
+// Blocks per KV head of a line of tiles: one to a CU.
+uint32_t line_blocks(uint32_t n_head_kv) { return std::max(1u, 256 / n_head_kv); }
+// Rows of a part of its tiles.
+uint32_t line_slot_rows(const rlh_seqs& q, uint64_t group, bool shared) {
+  return (uint32_t)std::min<uint64_t>(kLineRows, shared ? q.n_rows * group : q.max_q * group);
+}
+
 // How the work of a call is divided, from sizes that the host knows.
+template <bool TREE>
 Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
   Sizes n{};
   const uint64_t group = args.n_head / kv.n_head_kv, rows = (uint64_t)q.n_rows * group;
   const uint64_t own = q.max_kv > args.shared_len ? q.max_kv - args.shared_len : 0;
   n.tiled = q.max_q * group > kSmallRows;
+  if (TREE && (n.tiled || args.shared_len)) {
+    n.line_blocks = line_blocks(kv.n_head_kv);
+    n.slot_rows = line_slot_rows(q, group, args.shared_len != 0);
+    n.planned = q.n_seq > kPlanned;
+    n.merge = true;
+    return n;
+  }
   // a single sequence goes to one of the two kernels as a whole
   n.small = group <= kSmallRows && !(n.tiled && q.n_seq == 1);
   n.small_rows = n.small ? kSmallRows : 0;
@@ -1361,10 +1655,22 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
 struct Room {
   uint64_t prefix, tile, item;  // partial results of a row and head (or of an item's row)
   uint64_t plan, tiles;         // sequences
+  uint64_t line;                // units
 };
+
+// What the line of tiles takes. (Monotone in all sizes.)
+Room line_room(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
+  const uint64_t group = args.n_head / kv.n_head_kv, rows = (uint64_t)q.n_rows * args.n_head;
+  Room r{};
+  r.prefix = r.tile = args.shared_len ? rows : 0;
+  r.item = 2ull * line_blocks(kv.n_head_kv) * kv.n_head_kv * line_slot_rows(q, group, args.shared_len != 0);
+  r.line = q.n_seq + 2;
+  return r;
+}
 
 // What a call takes.
 Room attn_room(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args, const Sizes& n) {
+  if (n.line_blocks) return line_room(kv, q, args);
   const uint64_t rows = (uint64_t)q.n_rows * args.n_head;
   Room r{};
   r.prefix = args.shared_len ? n.prefix_parts * rows : 0;
@@ -1398,6 +1704,20 @@ Room attn_room_within(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_
   return r;
 }
 
+// The same of drafted rows: of a line of tiles if there may be one, and of the
+// small kernel, which smaller batches may go to.
+Room tree_room_within(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
+  const uint64_t group = args.n_head / kv.n_head_kv;
+  const bool small = group <= kSmallRows, line = q.max_q * group > kSmallRows || args.shared_len;
+  Room r{};
+  if (line) r = line_room(kv, q, args);
+  const bool whole = !line && q.max_kv <= kWhole && q.n_seq * kv.n_head_kv <= 256;
+  if (small && !whole && q.max_kv > 32 * kWaves)
+    r.item = std::max(r.item, ((uint64_t)q.n_seq + item_goal(kv.n_head_kv)) * kv.n_head_kv * kSmallRows);
+  r.plan = small ? q.n_seq : 0;
+  return r;
+}
+
 // Places the workspace's parts from `base` on (null: counts only); bytes.
 uint64_t place_workspace(Workspace* w, uint8_t* base, uint64_t dim, const Room& r) {
   uint64_t at = 0;
@@ -1414,20 +1734,28 @@ uint64_t place_workspace(Workspace* w, uint8_t* base, uint64_t dim, const Room& 
   w->item_ml = (float*)take(r.item * 8);
   w->plan = (uint32_t*)take(r.plan * 8);
   w->tiles = (uint32_t*)take(r.tiles * 8);
+  w->line = (uint64_t*)take(r.line * 8);
   return at;
 }
 
 // The mixed kernels take more LDS than a launch may by default; said once per
 // device (idempotent, so two threads may).
 template <int D>
-constexpr uint32_t kMixedLds = kTileLds<D> > 2 * kSmallLds<D, kWaves> ? kTileLds<D> : 2 * kSmallLds<D, kWaves>;
+constexpr uint32_t kMixedLds = kTileLds<D, false> > 2 * kSmallLds<D, kWaves> ? kTileLds<D, false> : 2 * kSmallLds<D, kWaves>;
+template <typename T, int D, int MOD, bool TREE>
+const void* tile_kernel() {
+  if constexpr (TREE)
+    return (const void*)k_attn_line<T, D, MOD>;
+  else
+    return (const void*)k_attn_mixed<T, D, MOD>;
+}
 template <typename T, int D, int MOD, bool TREE>
 int allow_lds(int device) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_acquire) & bit) return RLH_OK;
-  if (hipFuncSetAttribute((const void*)k_attn_mixed<T, D, MOD, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (int)kMixedLds<D>) != hipSuccess ||
+  if (hipFuncSetAttribute(tile_kernel<T, D, MOD, TREE>(), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)(TREE ? kTileLds<D, true> : kMixedLds<D>)) != hipSuccess ||
       hipFuncSetAttribute((const void*)k_attn_small<T, D, MOD, kTileWaves, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize,
                           (int)kSmallLds<D, kTileWaves>) != hipSuccess) {
     (void)hipGetLastError();
@@ -1440,11 +1768,15 @@ int allow_lds(int device) {
 template <typename T, int D, int MOD, bool TREE>
 int launch_attn(const char* what, const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
-  if (L.n.planned) RLH_TRY(enqueue(what, k_attn_plan<TREE>, dim3(1), kPlanThreads, 0, s, L));
+  if (L.n.planned) RLH_TRY(enqueue(what, TREE && L.n.line_blocks ? k_line_plan : k_attn_plan<TREE>, dim3(1), kPlanThreads, 0, s, L));
   if (L.a.shared_len || L.n.tiled) {
     RLH_TRY((allow_lds<T, D, MOD, TREE>(device)));
-    const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts) * G + (L.n.items * G + 1) / 2;
-    RLH_TRY(enqueue(what, k_attn_mixed<T, D, MOD, TREE>, dim3(blocks), 64 * kTileWaves, kMixedLds<D>, s, L));
+    if constexpr (TREE) {
+      RLH_TRY(enqueue(what, k_attn_line<T, D, MOD>, dim3(L.n.line_blocks * G), 64 * kTileWaves, kTileLds<D, true>, s, L));
+    } else {
+      const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts) * G + (L.n.items * G + 1) / 2;
+      RLH_TRY(enqueue(what, k_attn_mixed<T, D, MOD>, dim3(blocks), 64 * kTileWaves, kMixedLds<D>, s, L));
+    }
   } else if (L.n.whole) {
     RLH_TRY((allow_lds<T, D, MOD, TREE>(device)));
     RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kTileWaves, TREE>, dim3(L.n.items * G), 64 * kTileWaves,
@@ -1453,6 +1785,11 @@ int launch_attn(const char* what, const Launch& L, int device, hipStream_t s) {
     RLH_TRY(enqueue(what, k_attn_small<T, D, MOD, kWaves, TREE>, dim3(L.n.items * G), kThreads, kSmallLds<D, kWaves>, s, L));
   }
   if (!L.n.merge) return RLH_OK;
+  if constexpr (TREE)
+    if (L.n.line_blocks) {
+      const uint64_t waves = (uint64_t)L.a.b.n_rows * ((L.a.n_head + 3) / 4);
+      return enqueue(what, k_line_merge<T, D>, dim3((uint32_t)((waves + kWaves - 1) / kWaves)), kThreads, 0, s, L);
+    }
   const uint64_t blocks = L.n.merge_small ? (uint64_t)L.a.b.n_seq * L.n.merge_rows * G
                                           : ((uint64_t)L.a.b.n_rows * L.a.n_head + kWaves - 1) / kWaves;
   return enqueue(what, k_attn_merge<T, D, TREE>, dim3((uint32_t)blocks), kThreads, 0, s, L);
@@ -1480,7 +1817,7 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
     return serve_error(RLH_EINVAL, "status or lse is not aligned to 4 bytes");
   if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;
   Launch L{};
-  L.n = attn_sizes(*kv, *seqs, *args);
+  L.n = attn_sizes<TREE>(*kv, *seqs, *args);
   const uint64_t need = place_workspace(&L.ws, (uint8_t*)workspace, kv->head_dim, attn_room(*kv, *seqs, *args, L.n));
   if (need && !workspace) return serve_error(RLH_EINVAL, "workspace is null");
   if (need > workspace_bytes)
@@ -1553,9 +1890,10 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
   return launch_attn<__bf16, TREE>(what, L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
 }
 
+template <bool TREE>
 uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& seqs, const rlh_attn_args& args) {
   Workspace w;
-  return place_workspace(&w, nullptr, kv.head_dim, attn_room_within(kv, seqs, args));
+  return place_workspace(&w, nullptr, kv.head_dim, TREE ? tree_room_within(kv, seqs, args) : attn_room_within(kv, seqs, args));
 }
 
 }  // namespace

@@ -9,7 +9,7 @@ extern "C" {
 
 uint64_t rlh_paged_attn_workspace(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
   if (check_attn(kv, seqs, args) != RLH_OK || seqs->n_seq == 0 || seqs->n_rows == 0) return 0;
-  return attn_workspace(*kv, *seqs, *args);
+  return attn_workspace<false>(*kv, *seqs, *args);
 }
 
 int rlh_paged_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args, void* workspace,

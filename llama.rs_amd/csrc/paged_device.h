@@ -44,7 +44,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 // How many of the n values a[0], a[stride], ... that do not fall are at most x:
 // a wave's 64 lanes try places of the range that is left. (Ends within [0, n]
 // also where they fall.)
-__device__ __forceinline__ uint32_t count_upto(const uint32_t* a, uint32_t stride, uint32_t n, uint32_t x) {
+template <typename V>
+__device__ __forceinline__ uint32_t count_upto(const V* a, uint32_t stride, uint32_t n, V x) {
   uint32_t lo = 0, hi = n;
   while (lo < hi) {
     const uint32_t step = (hi - lo + 63) / 64, i = lo + (threadIdx.x & 63) * step;

@@ -89,6 +89,65 @@ RLH_HD uint64_t tree_bits(const uint64_t* mask, uint32_t words, uint32_t q_len, 
   return only_rows(x, (int64_t)q_len - off);
 }
 
+// ---- a line of tiles ------------------------------------------------------------------
+// The work of drafted rows: tiles of up to kLineRows rows of a KV head, each of
+// which takes the same `steps`; all tiles, one behind the other, make a line that
+// blocks share equally, so that a block may end inside a tile and go on
+// with the next. Lengths are in units: a step of a tile of more than half the
+// rows takes three, of another two (there one of a SIMD's two waves idles and
+// memory sets the pace: 2.3 and 1.6 us), a tile's start two steps more.
+constexpr uint32_t kLineRows = 256;
+constexpr uint32_t kLineStart = 2;
+// Units of a block at least: parts are joined by another launch, and a block
+// starts with a chain of loads that takes as long as three steps.
+constexpr uint32_t kLineLeast = 12;
+
+RLH_HD uint32_t line_weight(uint32_t rows) { return rows > kLineRows / 2 ? 3 : 2; }
+RLH_HD uint32_t line_tiles(uint32_t rows) { return (rows + kLineRows - 1) / kLineRows; }
+// Units of all tiles of `rows` rows.
+RLH_HD uint64_t line_units(uint32_t rows, uint32_t steps) {
+  if (rows == 0) return 0;
+  const uint32_t full = line_tiles(rows) - 1;
+  return ((uint64_t)full * 3 + line_weight(rows - full * kLineRows)) * (steps + kLineStart);
+}
+RLH_HD uint64_t line_share(uint64_t units, uint32_t blocks) {
+  const uint64_t n = (units + blocks - 1) / blocks;
+  return n > kLineLeast ? n : kLineLeast;
+}
+
+// Tile k of `rows` rows whose first tile begins at unit `first`.
+struct LineTile {
+  uint64_t begin;  // unit
+  uint32_t weight, steps;
+};
+RLH_HD LineTile line_tile(uint64_t first, uint32_t rows, uint32_t steps, uint32_t k) {
+  return LineTile{first + (uint64_t)k * 3 * (steps + kLineStart), line_weight(rows - k * kLineRows), steps};
+}
+RLH_HD uint64_t line_end(const LineTile& t) { return t.begin + (uint64_t)t.weight * (t.steps + kLineStart); }
+// The tile that unit x, at or behind `first`, lies in.
+RLH_HD uint32_t line_at(uint64_t first, uint32_t rows, uint32_t steps, uint64_t x) {
+  const uint64_t k = (x - first) / (3 * (uint64_t)(steps + kLineStart));
+  return k < line_tiles(rows) ? (uint32_t)k : line_tiles(rows) - 1;
+}
+// A step belongs to the block in whose units it begins: the first step that
+// begins at unit x or behind, and the blocks (of `share` units, more than a
+// step's) of the first and the last one.
+RLH_HD uint32_t line_step(const LineTile& t, uint64_t x) {
+  const uint64_t n = x > t.begin ? (x - t.begin + t.weight - 1) / t.weight : 0;
+  return n <= kLineStart ? 0 : n - kLineStart < t.steps ? (uint32_t)(n - kLineStart) : t.steps;
+}
+RLH_HD uint32_t line_first_block(const LineTile& t, uint64_t share) {
+  return (uint32_t)((t.begin + t.weight * kLineStart) / share);
+}
+RLH_HD uint32_t line_last_block(const LineTile& t, uint64_t share) {
+  return (uint32_t)((t.begin + (uint64_t)t.weight * (kLineStart + t.steps - 1)) / share);
+}
+// A block has two places for parts of tiles: the first for the tile that it
+// begins in or at, the second for one that it begins and does not end.
+RLH_HD uint32_t line_slot(const LineTile& t, uint32_t block, uint64_t share) {
+  return 2 * block + (block * share < t.begin ? 1 : 0);
+}
+
 // Steps of an item when the `steps` of all sequences (fewer than 2^24 each, so
 // that 32 bits hold the sum of 256 of them, not of 65535) are divided into
 // `goal` items: the sequences' own, rounded up, are at most `goal` and one each.

@@ -22,7 +22,7 @@ extern "C" {
 
 uint64_t rlh_tree_attn_workspace(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args) {
   if (check_tree(kv, seqs, args) != RLH_OK || seqs->n_seq == 0 || seqs->n_rows == 0) return 0;
-  return attn_workspace(*kv, *seqs, *args);
+  return attn_workspace<true>(*kv, *seqs, *args);
 }
 
 int rlh_tree_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args, const uint64_t* masks,
