@@ -11,8 +11,12 @@ struct MassLaunch {
   const float* lse;
   float* mass;
   float decay;
-  uint32_t stripes;  // blocks that share a KV head of a sequence
+  uint32_t stripes;     // blocks that share a KV head of a sequence
+  uint64_t per_group;   // 2^36 / group, rounded up
 };
+
+// r / group: exact while r * group < 2^36 (a batch has up to 2^25 rows of all heads, a group up to 2^10).
+__device__ __forceinline__ uint32_t of_group(const MassLaunch& L, uint32_t r) { return (uint32_t)(r * L.per_group >> 36); }
 
 constexpr int kMassThreads = 256;
 
@@ -35,14 +39,16 @@ struct MassRow {
 // The lse of row r of a KV head (minus infinity where there is none), and what follows from it.
 __device__ __forceinline__ float mass_lse(const MassLaunch& L, const SeqView& v, uint32_t rows, uint32_t r, uint32_t h) {
   const AttnParams& a = L.a;
-  return r < rows ? L.lse[(size_t)(v.q0 + r / a.group) * a.n_head + h * a.group + r % a.group] : -INFINITY;
+  const uint32_t i = of_group(L, r);
+  return r < rows ? L.lse[(size_t)(v.q0 + i) * a.n_head + h * a.group + r - i * a.group] : -INFINITY;
 }
 __device__ __forceinline__ MassRow mass_row(const MassLaunch& L, const SeqView& v, uint32_t r, uint32_t h, bool biased, float lse) {
   const AttnParams& a = L.a;
   MassRow m{0.0f, 0.0f, 0.0f, -1};
   if (lse == -INFINITY) return m;
-  if (biased && a.slopes) m.slope2 = a.slopes[h * a.group + r % a.group] * kLog2e;
-  m.pos = (int32_t)(v.kv_len - v.q_len + r / a.group);
+  const uint32_t i = of_group(L, r);
+  if (biased && a.slopes) m.slope2 = a.slopes[h * a.group + r - i * a.group] * kLog2e;
+  m.pos = (int32_t)(v.kv_len - v.q_len + i);
   m.lse2 = lse * kLog2e;
   const float rest = fmaf(lse, kLog2e, -m.lse2) + lse * kLog2eRest;
   m.rest = fabsf(m.lse2) < INFINITY ? __builtin_amdgcn_exp2f(-rest) : 1.0f;
@@ -173,16 +179,16 @@ __global__ void __launch_bounds__(kMassThreads) k_mass_few(MassLaunch L) {
 }
 
 // ---- many rows ------------------------------------------------------------------------
-// A wave keeps K of 64 positions of one KV head in registers; the block's rows
-// pass by in LDS, 128 at a time and the next ones on their way, as the other
+// A wave keeps K of 32 positions of one KV head in registers; the block's rows
+// pass by in LDS, 64 at a time and the next ones on their way, as the other
 // operand of 32x32x16 MFMAs (positions down, rows across). Each score becomes its
 // weight and joins one register per lane and position; the lanes of a position
 // meet once at the end.
-constexpr int kMassRows = 128;
-constexpr int kMassTile = 256;  // positions of a block
+constexpr int kMassRows = 64;
+constexpr int kMassTile = 128;  // positions of a block
 
 template <typename T, int D, int MOD>
-__global__ void __launch_bounds__(kMassThreads, 2) k_mass_many(MassLaunch L) {
+__global__ void __launch_bounds__(kMassThreads, 4) k_mass_many(MassLaunch L) {
   constexpr int kSteps = D / 16;
   constexpr int kLanes = D / 8;           // lanes of a row in a copy
   constexpr int kBuf = kMassRows * D * 2;
@@ -210,19 +216,20 @@ __global__ void __launch_bounds__(kMassThreads, 2) k_mass_many(MassLaunch L) {
 #pragma unroll
     for (int i = 0; i < kCopies; i++) {
       const uint32_t piece = wave * kCopies + i, r = piece * (64 / kLanes) + lane / kLanes, rr = min(c0 + r, rows - 1);
-      const T* row = (const T*)a.q + (size_t)(v.q0 + rr / a.group) * a.q_stride + (size_t)(h * a.group + rr % a.group) * D;
+      const uint32_t at = of_group(L, rr);
+      const T* row = (const T*)a.q + (size_t)(v.q0 + at) * a.q_stride + (size_t)(h * a.group + rr - at * a.group) * D;
       copy_to_lds(row + ((lane % kLanes) ^ swizzle<D>(r)) * 8, uniform(lds0 + buf * kBuf + piece * 1024));
     }
   };
   // what rows r .. end - 1 see of positions q .. q_end - 1: 0 nothing, 2 each row all, else 1
   auto sees = [&](uint32_t r, uint32_t end, int32_t q, int32_t q_end) -> int {
-    const RowSpan low = row_span(p0 + (int32_t)(r / a.group), v.kv_len, a.window, prefix);
-    const RowSpan high = row_span(p0 + (int32_t)((end - 1) / a.group), v.kv_len, a.window, prefix);
+    const RowSpan low = row_span(p0 + (int32_t)of_group(L, r), v.kv_len, a.window, prefix);
+    const RowSpan high = row_span(p0 + (int32_t)of_group(L, end - 1), v.kv_len, a.window, prefix);
     if (!((q < high.hi && q_end > low.lo) || q < low.prefix)) return 0;
     return (q >= high.lo && q_end <= low.hi) || q_end <= low.prefix ? 2 : 1;
   };
   for (int32_t b0 = (int32_t)(a.shared_len + stripe * kMassTile); b0 < n; b0 += (int32_t)(L.stripes * kMassTile)) {
-    const int32_t p = b0 + (int32_t)wave * 64, b1 = min(b0 + kMassTile, n);
+    const int32_t p = b0 + (int32_t)wave * 32, b1 = min(b0 + kMassTile, n);
     // the rows from c on that see any of the block's positions
     auto next_rows = [&](uint32_t c) {
       while (c < rows && sees(c, min(c + kMassRows, rows), b0, b1) == 0) c += kMassRows;
@@ -235,27 +242,26 @@ __global__ void __launch_bounds__(kMassThreads, 2) k_mass_many(MassLaunch L) {
       stage(c0, 0);
       if (t < kMassRows) lse = mass_lse(L, v, rows, c0 + t, h);
     }
-    // pages of the wave's four groups of 16 positions
-    uint32_t page[4], ok = 0;
-    size_t at[4];
+    // pages of the wave's two groups of 16 positions
+    uint32_t page[2], ok = 0;
+    size_t at[2];
 #pragma unroll
-    for (int u = 0; u < 4; u++) page[u] = p + 16 * u < n ? load_uniform(table, (uint32_t)(p + 16 * u) >> a.page_shift) : 0u;
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const bool live = p + 16 * u < n, exists = live && page[u] < a.n_pages;
-      ok |= (exists ? 1u << u : 0u) | (live && !exists ? 16u : 0u);
-      at[u] = exists ? (((size_t)page[u] * a.n_kv + h) << a.page_shift) + ((uint32_t)(p + 16 * u) & page_mask) : 0;
-    }
-    if (ok & 16) raise(lane == 0 ? a.status : nullptr, RLH_SERVE_BAD_PAGE);
-    vec8<T> k[2][kSteps];  // (negated where the scale is: the rows come unchanged)
+    for (int u = 0; u < 2; u++) page[u] = p + 16 * u < n ? load_uniform(table, (uint32_t)(p + 16 * u) >> a.page_shift) : 0u;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      const T* kp = (const T*)a.pool_k + ((col & 16 ? at[2 * u + 1] : at[2 * u]) + (col & 15)) * D + half * 8;
+      const bool live = p + 16 * u < n, exists = live && page[u] < a.n_pages;
+      ok |= (exists ? 1u << u : 0u) | (live && !exists ? 4u : 0u);
+      at[u] = exists ? (((size_t)page[u] * a.n_kv + h) << a.page_shift) + ((uint32_t)(p + 16 * u) & page_mask) : 0;
+    }
+    if (ok & 4) raise(lane == 0 ? a.status : nullptr, RLH_SERVE_BAD_PAGE);
+    vec8<T> k[kSteps];  // (negated where the scale is: the rows come unchanged)
+    {
+      const T* kp = (const T*)a.pool_k + ((col & 16 ? at[1] : at[0]) + (col & 15)) * D + half * 8;
 #pragma unroll
-      for (int i = 0; i < kSteps; i++) k[u][i] = __builtin_bit_cast(vec8<T>, *(const u32x4_t*)(kp + i * 16) ^ L.sc.flip);
+      for (int i = 0; i < kSteps; i++) k[i] = __builtin_bit_cast(vec8<T>, *(const u32x4_t*)(kp + i * 16) ^ L.sc.flip);
     }
     if (t < kMassRows) infos[0][t] = mass_row(L, v, c0 + t, h, MOD, lse);
-    float sum[2][16] = {};
+    float sum[16] = {};
     while (c0 < rows) {
       const uint32_t c1 = min(c0 + kMassRows, rows), c2 = next_rows(c0 + kMassRows);
       wait_vmcnt<0>();  // this wave's rows have landed
@@ -265,62 +271,56 @@ __global__ void __launch_bounds__(kMassThreads, 2) k_mass_many(MassLaunch L) {
         stage(c2, buf ^ 1);
       }
       const uint8_t* q0 = qs + buf * kBuf;
-      const int whole = sees(c0, c1, p, p + 64);
+      const int whole = sees(c0, c1, p, p + 32);
       for (uint32_t r0 = c0; r0 < c1; r0 += 32) {
-        const int see = whole == 1 ? sees(r0, min(r0 + 32, rows), p, p + 64) : whole;
+        const int see = whole == 1 ? sees(r0, min(r0 + 32, rows), p, p + 32) : whole;
         if (see == 0) continue;
         const uint32_t r = r0 - c0 + col;
         vec8<T> q[kSteps];
 #pragma unroll
         for (int i = 0; i < kSteps; i++) q[i] = *(const vec8<T>*)(q0 + r * D * 2 + ((2 * i + half) ^ swizzle<D>(r)) * 16);
         const MassRow m = infos[buf][r];
-        f32x16_t sc[2];
+        f32x16_t sc;
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) sc[u][e] = 0.0f;
+        for (int e = 0; e < 16; e++) sc[e] = 0.0f;
         __builtin_amdgcn_sched_barrier(0);  // (all reads before the first product: one takes some 250 cycles)
 #pragma unroll
-        for (int i = 0; i < kSteps; i++)
-#pragma unroll
-          for (int u = 0; u < 2; u++) sc[u] = mfma32(k[u][i], q[i], sc[u]);
-        // the lane's first position (opaque, so that 32 of them are not kept in registers)
+        for (int i = 0; i < kSteps; i++) sc = mfma32(k[i], q[i], sc);
+        // the lane's first position (opaque, so that 16 of them are not kept in registers)
         int32_t j0 = p + (int32_t)half * 4;
         asm volatile("" : "+v"(j0));
 #pragma unroll
-        for (int i = 0; i < 32; i++)
-          sc[i / 16][i % 16] = mass_weight<MOD>(L.sc, m, sc[i / 16][i % 16], j0 + i / 4 * 8 + i % 4);
+        for (int i = 0; i < 16; i++)
+          sc[i] = mass_weight<MOD>(L.sc, m, sc[i], j0 + i / 4 * 8 + i % 4);
         if (see != 2 || __ballot(m.pos < 0)) {
           const RowSpan span = row_span(max(m.pos, 0), v.kv_len, a.window, prefix);
           const bool counts = m.pos >= 0;
           const int32_t lo = counts ? span.lo - j0 : 0x7fffffff, hi = span.hi - j0, pre = counts ? span.prefix - j0 : -0x7fffffff;
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
+          for (int i = 0; i < 16; i++) {
             const int32_t d = i / 4 * 8 + i % 4;
-            sc[i / 16][i % 16] = (((d >= lo) & (d < hi)) | (d < pre)) ? sc[i / 16][i % 16] : 0.0f;
+            sc[i] = (((d >= lo) & (d < hi)) | (d < pre)) ? sc[i] : 0.0f;
           }
         }
 #pragma unroll
-        for (int i = 0; i < 32; i++) sum[i / 16][i % 16] = fmaf(sc[i / 16][i % 16], m.rest, sum[i / 16][i % 16]);
+        for (int i = 0; i < 16; i++) sum[i] = fmaf(sc[i], m.rest, sum[i]);
       }
       if (t < kMassRows && c2 < rows) infos[buf ^ 1][t] = mass_row(L, v, c2 + t, h, MOD, lse);
       c0 = c2;
       buf ^= 1;
     }
-    // Lane (col, half) has positions 8 g + 4 half + 0..3 of 32 u; lane col = 4 u + g writes its four.
+    // Lane (col, half) has positions 8 g + 4 half + 0..3; lane col = g writes its four.
     f32x4_t mine = {0, 0, 0, 0};
 #pragma unroll
-    for (int g = 0; g < 8; g++) {
+    for (int g = 0; g < 4; g++) {
       f32x4_t x;
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = sum_across_16(row_sum(sum[g / 4][g % 4 * 4 + i]));
+      for (int i = 0; i < 4; i++) x[i] = sum_across_16(row_sum(sum[g * 4 + i]));
       if (col == (uint32_t)g) mine = x;
     }
-    const uint32_t u = col >> 1;  // of the groups of 16 positions
-    if (col < 8 && (ok >> u & 1)) {
+    if (col < 4 && (ok >> (col >> 1) & 1)) {
       const int32_t j0 = p + (int32_t)(col * 8 + half * 4);
-      const size_t place = (u == 0 ? at[0] : u == 1 ? at[1] : u == 2 ? at[2] : at[3]) + (col & 1) * 8 + half * 4;
-      float* dst = L.mass + place;
+      float* dst = L.mass + (col >> 1 ? at[1] : at[0]) + (col & 1) * 8 + half * 4;
       const f32x4_t old = L.decay != 0.0f && j0 < p0 ? *(const f32x4_t*)dst : f32x4_t{0, 0, 0, 0};
       add_mass(dst, old, mine, L.decay, j0, p0, n);
     }
@@ -396,6 +396,7 @@ int rlh_paged_mass(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   L.a.n_pages = (uint32_t)kv->n_pages;
   L.a.window = args->window;
   L.a.shared_len = args->shared_len;
+  L.per_group = ((1ull << 36) + L.a.group - 1) / L.a.group;
   L.lse = lse;
   L.mass = mass;
   L.decay = decay;
