@@ -170,3 +170,219 @@ def test_a_line_past_32_bits(shim):
     for b in (0, 31):
         got = shim.shim_line_block(U64(0), U32(rows), U32(steps), U64(share), U32(b), out)
         assert out[0][0] == b * 4096 and got == 4096 and [out[got - 1][i] for i in range(3)] == [b * 4096 + 4095, 0, steps]
+
+
+# ---- refusals ------------------------------------------------------------------------
+# Addresses that are never read: every check below comes before the device.
+
+OPS = ["append_at", "attn_lse", "tree_masks", "tree_attn", "tree_accept", "paged_move", "paged_mass", "evict_select"]
+NODES = [f for f in BATCH if f[0] == "seqs" and f[1] in ("n_seq", "n_rows", "max_q", "q_start", "kv_len")]
+CACHED = [f for f in BATCH if (f[0] == "kv" and f[2] != 3) or f[1] in ("n_seq", "kv_len", "table", "table_stride") or f[1:3] == ("max_kv", 65)]  # (no query heads: any n_head_kv)
+SCORES = [("att", "n_head", 3, rlh.RLH_EINVAL), ("att", "q", 0, rlh.RLH_EINVAL), ("att", "q_stride", 513, rlh.RLH_EINVAL),
+          ("att", "scale", float("inf"), rlh.RLH_EINVAL), ("att", "scale", 3e38, rlh.RLH_EINVAL),
+          ("att", "softcap", -1.0, rlh.RLH_EINVAL), ("att", "slopes", A + 2, rlh.RLH_EINVAL),
+          ("att", "prefix_len", A + 1, rlh.RLH_EINVAL), ("att", "shared_len", 8, rlh.RLH_EINVAL),
+          ("att", "shared_len", 1 << 30, rlh.RLH_EUNSUP)]
+OUT = [("att", "out", 0, rlh.RLH_EINVAL), ("att", "out", 6 * A + 512, rlh.RLH_EINVAL), ("att", "out_stride", 500, rlh.RLH_EINVAL),
+       ("att", "shared_len", 16, rlh.RLH_EINVAL)]
+REFUSED = {
+    "append_at": test_serve.APPEND + [("", "positions", 0, rlh.RLH_EINVAL), ("", "positions", 13 * A + 2, rlh.RLH_EINVAL)],
+    "attn_lse": test_serve.ATTN + [("", "lse", 0, rlh.RLH_EINVAL), ("", "lse", 14 * A + 2, rlh.RLH_EINVAL),
+                                   ("", "workspace", 16 * A + 8, rlh.RLH_EINVAL)],
+    "tree_masks": NODES + [("", "parents", 0, rlh.RLH_EINVAL), ("", "parents", A + 2, rlh.RLH_EINVAL),
+                           ("", "masks", 0, rlh.RLH_EINVAL), ("", "masks", 15 * A + 4, rlh.RLH_EINVAL),
+                           ("", "words", 0, rlh.RLH_EINVAL), ("", "words", 1 << 31, rlh.RLH_EUNSUP),
+                           ("", "base", A + 1, rlh.RLH_EINVAL), ("", "positions", A + 2, rlh.RLH_EINVAL),
+                           ("", "status", A + 2, rlh.RLH_EINVAL)],
+    "tree_attn": BATCH + SCORES + OUT + [("att", "slopes", A, rlh.RLH_EUNSUP), ("att", "prefix_len", A, rlh.RLH_EUNSUP),
+                                         ("", "masks", 0, rlh.RLH_EINVAL), ("", "masks", 15 * A + 4, rlh.RLH_EINVAL),
+                                         ("", "words", 0, rlh.RLH_EINVAL), ("", "words", 1 << 31, rlh.RLH_EUNSUP),
+                                         ("", "lse", 14 * A + 2, rlh.RLH_EINVAL), ("", "status", A + 2, rlh.RLH_EINVAL)],
+    "tree_accept": NODES + [("acc", f, 0, rlh.RLH_EINVAL) for f in ("parents", "tokens", "sampled", "path", "count", "next",
+                                                                    "new_len")] +
+                   [("acc", "path", 20 * A + 1, rlh.RLH_EINVAL), ("acc", "path_stride", 4, rlh.RLH_EINVAL),
+                    ("", "status", A + 2, rlh.RLH_EINVAL)],
+    "paged_move": CACHED + [("mov", "index", 0, rlh.RLH_EINVAL), ("mov", "index", A + 2, rlh.RLH_EINVAL),
+                            ("mov", "count", 0, rlh.RLH_EINVAL), ("mov", "max_count", 21, rlh.RLH_EINVAL),
+                            ("mov", "mass", 0, rlh.RLH_EINVAL), ("mov", "mass_out", 0, rlh.RLH_EINVAL),
+                            ("mov", "base", A + 2, rlh.RLH_EINVAL), ("mov", "mass_out", 25 * A + 64, rlh.RLH_EINVAL),
+                            ("", "status", A + 2, rlh.RLH_EINVAL)],
+    "paged_mass": BATCH + SCORES + [("", "lse", 0, rlh.RLH_EINVAL), ("", "lse", A + 2, rlh.RLH_EINVAL), ("", "mass", 0, rlh.RLH_EINVAL),
+                                    ("", "mass", 25 * A + 8, rlh.RLH_EINVAL), ("", "decay", -0.5, rlh.RLH_EINVAL),
+                                    ("", "decay", float("inf"), rlh.RLH_EINVAL), ("", "decay", float("nan"), rlh.RLH_EINVAL),
+                                    ("", "status", A + 2, rlh.RLH_EINVAL)],
+    "evict_select": CACHED + [("evi", "mass", 0, rlh.RLH_EINVAL), ("evi", "mass", A + 2, rlh.RLH_EINVAL), ("evi", "keep", 0, rlh.RLH_EINVAL),
+                              ("evi", "count", 0, rlh.RLH_EINVAL), ("evi", "budget", 0, rlh.RLH_EINVAL),
+                              ("evi", "first_kept", 15, rlh.RLH_EINVAL), ("evi", "last_kept", 0xffffffff, rlh.RLH_EINVAL),
+                              ("evi", "keep_stride", 19, rlh.RLH_EINVAL), ("", "status", A + 2, rlh.RLH_EINVAL)],
+}
+
+
+def good():
+    args = test_serve.good()
+    args["acc"] = dict(parents=17 * A, tokens=18 * A, sampled=19 * A, path=20 * A, path_stride=5, count=21 * A, next=22 * A,
+                       new_len=23 * A)
+    args["mov"] = dict(index=24 * A, index_stride=20, per_head=1, count=21 * A, max_count=20, base=0, mass=25 * A, mass_out=26 * A)
+    args["evi"] = dict(mass=25 * A, budget=20, first_kept=4, last_kept=6, keep_stride=20, keep=27 * A, count=21 * A)
+    args[""] = dict(positions=13 * A, lse=14 * A, masks=15 * A, words=1, parents=17 * A, base=28 * A, workspace=16 * A, status=0,
+                    mass=25 * A, decay=0.5)
+    return args
+
+
+def call(op, args):
+    lib = rlh.load()
+    kv, seqs, app, att = test_serve.structs(args)
+    x = args[""]
+    st = x["status"] or None
+    if op == "append_at":
+        rc = lib.rlh_paged_append_at(kv, seqs, app, x["positions"], st, None)
+    elif op == "attn_lse":
+        rc = lib.rlh_paged_attn_lse(kv, seqs, att, x["lse"], x["workspace"], 1 << 40, st, None)
+    elif op == "tree_masks":
+        rc = lib.rlh_tree_masks(seqs, x["parents"], x["base"], x["masks"], x["words"], x["positions"], st, None)
+    elif op == "tree_attn":
+        rc = lib.rlh_tree_attn(kv, seqs, att, x["masks"], x["words"], x["lse"], x["workspace"], 1 << 40, st, None)
+    elif op == "tree_accept":
+        rc = lib.rlh_tree_accept(seqs, rlh.AcceptArgs(**args["acc"]), st, None)
+    elif op == "paged_move":
+        rc = lib.rlh_paged_move(kv, seqs, rlh.MoveArgs(**args["mov"]), st, None)
+    elif op == "paged_mass":
+        rc = lib.rlh_paged_mass(kv, seqs, att, x["lse"], x["decay"], x["mass"], st, None)
+    else:
+        rc = lib.rlh_evict_select(kv, seqs, rlh.EvictArgs(**args["evi"]), st, None)
+    return rc, lib.rlh_last_error().decode()
+
+
+def _has_gpu():
+    import torch
+
+    return torch.cuda.device_count() > 0
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_refusals(op):
+    for part, field, value, code in REFUSED[op]:
+        args = good()
+        args[part][field] = value
+        rc, said = call(op, args)
+        assert rc == code and said, (part, field, value, rc, said)
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_missing_structs(op):
+    lib, f = rlh.load(), {"append_at": "rlh_paged_append_at", "attn_lse": "rlh_paged_attn_lse"}.get(op, "rlh_" + op)
+    f = getattr(lib, f)
+    args = good()
+    kv, seqs, app, att = test_serve.structs(args)
+    own = {"append_at": app, "attn_lse": att, "tree_attn": att, "paged_mass": att, "tree_accept": rlh.AcceptArgs(**args["acc"]),
+           "paged_move": rlh.MoveArgs(**args["mov"]), "evict_select": rlh.EvictArgs(**args["evi"])}
+    lead = [seqs] if op in ("tree_masks", "tree_accept") else [kv, seqs]
+    lead += [own[op]] if op in own else []
+    rest = [0.5 if t is ctypes.c_float else 1 if t in (U32, U64) else 16 * A for t in f.argtypes[len(lead):]]
+    rest[-2:] = [None, None]
+    for i in range(len(lead)):
+        assert f(*(lead[:i] + [None] + lead[i + 1:]), *rest) == rlh.RLH_EINVAL
+
+
+@pytest.mark.skipif(_has_gpu(), reason="checks the no-GPU error path")
+@pytest.mark.parametrize("op", OPS)
+def test_what_is_accepted_needs_a_device(op):
+    rc, said = call(op, good())
+    assert rc == rlh.RLH_EDEVICE and "no HIP device" in said, said
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_empty_batches_do_nothing(op):
+    args = good()
+    args["seqs"]["n_seq"] = 0
+    assert call(op, args)[0] == rlh.RLH_OK
+    args = good()
+    args["seqs"]["n_rows"] = 0
+    if op in ("tree_accept", "paged_move", "evict_select"):  # these have work without rows
+        args["seqs"].update(max_q=0, q_start=3 * A if op == "tree_accept" else 0)
+        if op == "tree_accept":
+            args["acc"].update(parents=0, tokens=0, sampled=0, path=0)
+        assert call(op, args)[0] in (rlh.RLH_EDEVICE, rlh.RLH_EINVAL) and "null" not in call(op, args)[1]
+    else:
+        args[""].update(lse=0 if op == "attn_lse" else 14 * A, masks=0 if op == "tree_attn" else 15 * A)
+        assert call(op, args)[0] == rlh.RLH_OK
+    args = good()
+    args["mov"]["max_count"] = 0
+    if op == "paged_move":
+        assert call(op, args)[0] == rlh.RLH_OK
+
+
+# what a call writes and reads: (part, field) and bytes
+POOL = 8 * 2 * 16 * 128 * 2
+READS = {"q_start": ("seqs", "q_start", 12), "kv_len": ("seqs", "kv_len", 8), "table": ("seqs", "table", 32),
+         "positions": ("", "positions", 24), "masks": ("", "masks", 48), "parents": ("", "parents", 24), "base": ("", "base", 8),
+         "lse": ("", "lse", 96), "a.parents": ("acc", "parents", 24), "tokens": ("acc", "tokens", 24),
+         "sampled": ("acc", "sampled", 24), "index": ("mov", "index", 320), "m.count": ("mov", "count", 8),
+         "m.base": ("mov", "base", 8), "mass": ("", "mass", 1024), "e.mass": ("evi", "mass", 1024), "q": ("att", "q", 6144),
+         "k": ("kv", "k", POOL), "v": ("kv", "v", POOL)}
+APART = {
+    "append_at": [(("app", "q_out", 6144), ["positions"]), (("kv", "k", POOL), ["positions"])],
+    "attn_lse": [(("", "lse", 96), ["q_start", "kv_len", "table", "q", "k", "v"])],
+    "tree_masks": [(("", "masks", 48), ["q_start", "kv_len", "parents", "base", "positions"]),
+                   (("", "positions", 24), ["q_start", "kv_len", "parents", "base"])],
+    "tree_attn": [(("att", "out", 6144), ["masks"]), (("", "lse", 96), ["q_start", "kv_len", "table", "masks", "q", "k", "v"])],
+    "tree_accept": [(("acc", f, n), ["q_start", "kv_len", "a.parents", "tokens", "sampled"])
+                    for f, n in (("path", 40), ("count", 8), ("next", 8), ("new_len", 8))],
+    "paged_move": [(("kv", f, POOL), ["kv_len", "table", "index", "m.count", "m.base"]) for f in ("k", "v")] +
+                  [(("mov", "mass_out", 1024), ["kv_len", "table", "index", "m.count", "m.base", "k", "v"])],
+    "paged_mass": [(("", "mass", 1024), ["q_start", "kv_len", "table", "q", "lse", "k", "v"])],
+    "evict_select": [(("evi", "keep", 320), ["kv_len", "table", "e.mass"]), (("evi", "count", 8), ["kv_len", "table", "e.mass"])],
+}
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_written_memory_is_apart(op):
+    for (part, field, size), names in APART[op]:
+        for name in names + ["status"]:
+            for at in (0, 1):  # its first bytes are the area's last ones, its last ones the area's first
+                args = good()
+                start = args[part][field]
+                p2, f2, n2 = READS[name] if name != "status" else ("", "status", 4)
+                unit = 16 if name in ("q", "k", "v", "mass") else 8 if name == "masks" else 4
+                place = start + size - unit if at == 0 else start - n2 + unit
+                if place % unit or (field in ("masks", "mass", "k", "v", "q_out", "out") and n2 % unit):
+                    continue
+                args[p2][f2] = place
+                rc, said = call(op, args)
+                assert rc == rlh.RLH_EINVAL and "overlap" in said, (field, name, at, said)
+
+
+@pytest.mark.parametrize("heads,kv", [(64, 8), (16, 8), (12, 1), (40, 2), (28, 4), (128, 128), (512, 512), (24, 1)])
+def test_a_tree_workspace_serves_every_smaller_batch(heads, kv):
+    """As of rlh_paged_attn: the size for some limits is enough for every batch within them."""
+    from test_serve_edges import A as far
+    from test_serve_edges import attention_args, log_int
+
+    rng = np.random.default_rng(heads)
+    lib = rlh.load()
+    for _ in range(60):
+        most_q, n_seq, shared = log_int(rng, 1, 700), log_int(rng, 1, 600), 64 * log_int(rng, 1, 100) if rng.random() < 0.4 else 0
+        n_rows, max_kv = most_q + log_int(rng, 1, 6000) - 1, max(most_q, log_int(rng, 1, 60000))
+        size = lib.rlh_tree_attn_workspace(*attention_args(heads, kv, 128, n_seq, n_rows, most_q, max_kv, shared))
+        for _ in range(40):
+            rows = log_int(rng, 1, n_rows)
+            q = min(rows, log_int(rng, 1, most_q))
+            less = attention_args(heads, kv, 128, log_int(rng, 1, n_seq), rows, q, max(q, log_int(rng, 1, max_kv)),
+                                  64 * int(rng.integers(0, shared // 64 + 1)))
+            rc = lib.rlh_tree_attn(*less, 12 * far, 16, None, 16 * far, size, None, None)
+            assert rc in (rlh.RLH_EDEVICE, rlh.RLH_EINVAL), rc
+            assert not lib.rlh_last_error().startswith(b"workspace"), (lib.rlh_last_error(), size)
+            assert lib.rlh_tree_attn_workspace(*less) <= size
+
+
+def test_tree_workspace_of_a_server():
+    """64 sequences of up to 63 nodes at 40000 positions: parts of 256 blocks, two each."""
+    from test_serve_edges import A as far
+    from test_serve_edges import attention_args
+
+    lib = rlh.load()
+    args = attention_args(64, 8, 128, 64, 4032, 63, 40000, 0)
+    size = lib.rlh_tree_attn_workspace(*args)
+    assert 0 < size < 72 << 20
+    lib.rlh_tree_attn(*args, 12 * far, 1, None, 16 * far, size // 2, None, None)
+    assert lib.rlh_last_error().startswith(b"workspace")

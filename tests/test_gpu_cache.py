@@ -709,3 +709,328 @@ def test_evict_skips_contradictions_and_missing_pages():
             if s == 2:
                 row[16:32] = np.nan
             assert np.array_equal(keep[s, g, :30], cref.evict(row, 30, 2, 2))
+
+
+# ---- the operators together ---------------------------------------------------------------------------
+
+def test_a_step_with_drafts_captured_and_replayed():
+    """Masks, append at the nodes' positions, tree attention, a token per node,
+    the accepted branch and its move, as one captured step, for batches whose
+    lengths, trees and inputs change from replay to replay; eager calls of the
+    program's own lie between. The step is followed on the host: the pages hold
+    the kept rows, and the next step's attention sees them."""
+    heads, kv, dim, page, vocab, sizes = 8, 2, 64, 16, 200, [26, 7, 1, 70]
+    r = cref.rng(3)
+    lens = [150, 31, 77, 300]  # positions before the drafts
+    room = [(0, n + 6 * 80) for n in lens]
+    b = ref.Batch(room, kv, dim, page, rlh.F16, seed=5)
+    b.starts = np.cumsum([0] + sizes)
+    b.n_rows = b.n_live = int(b.starts[-1])
+    b.max_q = max(sizes)
+    b.q_start = ints(b.starts)
+    n, rows, most, words = len(sizes), b.n_rows, max(sizes), 2
+    freqs = torch.tensor(rlh.rope_freqs(dim, 1e4)[0]).cuda()
+    x = torch.zeros((rows, (heads + 2 * kv) * dim), device="cuda")
+    q_rows = torch.zeros((rows, heads * dim), dtype=torch.float16, device="cuda")
+    out = torch.zeros_like(q_rows)
+    g = torch.Generator().manual_seed(1)
+    w_logits = (0.3 * torch.randn((heads * dim, vocab), generator=g)).cuda()
+    parents, tokens, sampled, positions = (torch.zeros(rows, dtype=torch.int32, device="cuda") for _ in range(4))
+    base = ints(lens)
+    masks = torch.zeros((rows, words), dtype=torch.int64, device="cuda")
+    path = torch.zeros((n, most), dtype=torch.int32, device="cuda")
+    count, nxt, new_len = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(3))
+    options = torch.tensor(np.frombuffer(b"".join(bytes(rlh.RowSampling(0.0, 0, 1.0, 0.0)) for _ in range(rows)), np.uint8).copy()).cuda()
+    u, st = torch.zeros(rows, device="cuda"), word()
+    attn = rlh.AttnArgs(heads, 0, at(q_rows), at(out), q_rows.stride(0), out.stride(0), dim ** -0.5, 0.0, None, None, None, 0)
+    append = rlh.AppendArgs(rlh.F32, heads, at(x), at(x) + heads * dim * 4, at(x) + (heads + kv) * dim * 4, x.stride(0), x.stride(0),
+                            x.stride(0), None, None, 1e-6, 1.0, at(freqs), dim, 0, at(q_rows), q_rows.stride(0))
+    accept = rlh.AcceptArgs(at(parents), at(tokens), at(sampled), at(path), most, at(count), at(nxt), at(new_len))
+    move = rlh.MoveArgs(at(path), most, 0, at(count), most, at(base), None, None)
+    ws = torch.empty(rlh.tree_attn_workspace(b.kv(), b.desc(), attn), dtype=torch.uint8, device="cuda")
+    ws2 = torch.empty(rlh.sample_rows_workspace(rows, vocab), dtype=torch.uint8, device="cuda")
+
+    def step(s):
+        rlh.tree_masks(b.desc(), at(parents), at(base), at(masks), words, at(positions), at(st), s)
+        rlh.paged_append_at(b.kv(), b.desc(), append, at(positions), at(st), s)
+        rlh.tree_attn(b.kv(), b.desc(), attn, at(masks), words, None, at(ws), ws.numel(), at(st), s)
+        logits = out.float() @ w_logits
+        rlh.sample_rows(rlh.F32, at(logits), rows, vocab, vocab, at(options), at(u), at(sampled), at(ws2), ws2.numel(), s)
+        rlh.tree_accept(b.desc(), accept, at(st), s)
+        rlh.paged_move(b.kv(), b.desc(), move, at(st), s)
+        return logits
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    now, kept_all = list(lens), 0
+
+    def set_inputs(i):
+        trees = [cref.random_tree(r, m, 4) for m in sizes]
+        x.copy_(1.2 * torch.randn(x.shape, generator=g))
+        parents.copy_(ints(sum(trees, [])))
+        b.kv_len.copy_(ints([a + m for a, m in zip(now, sizes)]))
+        base.copy_(ints(now))
+        # half of the steps draft what the model would draw, found by an eager pass over copies
+        drafts = [r.randrange(vocab) for _ in range(rows)]
+        return trees, drafts
+
+    with torch.cuda.stream(side):
+        out.float() @ w_logits  # the product's library is loaded before the capture
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            logits = step(side.cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(5):
+        trees, drafts = set_inputs(i)
+        k0, v0 = b.k.clone(), b.v.clone()
+        # an eager pass: what each node draws does not depend on the drafted numbers
+        tokens.copy_(ints(drafts))
+        torch.cuda.synchronize()
+        step(stream())
+        drawn = sampled.cpu().numpy().copy()
+        for s, tree in enumerate(trees):
+            for c in range(1, len(tree)):
+                if r.random() < 0.7:
+                    drafts[int(b.starts[s]) + c] = int(drawn[int(b.starts[s]) + tree[c]])
+        b.k.copy_(k0)
+        b.v.copy_(v0)
+        tokens.copy_(ints(drafts))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(st) == 0
+        assert np.array_equal(sampled.cpu().numpy(), drawn)
+        assert torch.equal(logits.argmax(1).to(torch.int32), sampled)
+        # attention over what the pages held and the rows just appended
+        b.seqs = [(m, a + m) for m, a in zip(sizes, now)]
+        sees = [cref.tree_sees(cref.mask_matrix(t), a, 0) for t, a in zip(trees, now)]
+        full = b.k.clone(), b.v.clone()
+        k1, v1 = k0.clone(), v0.clone()  # the pages before the move
+        rowsx = x.double().view(rows, heads + 2 * kv, dim)
+        place = torch.tensor([now[s] + len(cref.lineage(t, c)) - 1 for s, t in enumerate(trees) for c in range(len(t))])
+        turned = ref.rotate(rowsx[:, :heads + kv], place.cuda(), freqs, 1.0, dim, False)
+        for s, m in enumerate(sizes):
+            kept = cref.accept(trees[s], drafts[int(b.starts[s]):int(b.starts[s + 1])], drawn[int(b.starts[s]):int(b.starts[s + 1])])
+            assert int(count[s]) == len(kept) and path[s, :len(kept)].tolist() == kept
+            assert int(nxt[s]) == drawn[int(b.starts[s]) + kept[-1]] and int(new_len[s]) == now[s] + len(kept)
+            for c in range(m):
+                p, row = now[s] + c, int(b.starts[s]) + c
+                v1[b.page_of(s, p), :, p % page] = rowsx[row, heads + kv:].half()
+                k1[b.page_of(s, p), :, p % page] = turned[row, heads:].half()
+            for j, c in enumerate(kept):  # (keys of a rotation: within the append's bound; values: the same bits)
+                p, row = now[s] + j, int(b.starts[s]) + c
+                want = turned[row, heads:]
+                big = rowsx[row, heads:heads + kv].abs().amax() * 2
+                assert torch.all((b.k[b.page_of(s, p), :, p % page].double() - want).abs() <= want.abs() * 2.0 ** -11 + big * 2.0 ** -20)
+                assert torch.equal(b.v[b.page_of(s, p), :, p % page], rowsx[row, heads + kv:].half())
+            kept_all += len(kept) - 1
+        # K as the kernel wrote it: the move changed only kept places, so the attention is checked against the rounded own form
+        b.k.copy_(k1)
+        b.v.copy_(v1)
+        eager = torch.full_like(out, 7.0)
+        args = rlh.AttnArgs(heads, 0, at(q_rows), at(eager), q_rows.stride(0), out.stride(0), dim ** -0.5, 0.0, None, None, None, 0)
+        rlh.tree_attn(b.kv(), b.desc(), args, at(masks), words, None, at(ws), ws.numel(), None, stream())
+        want, bound, _, _ = cref.attention(b, q_rows.view(-1, heads, dim), heads, sees, dim ** -0.5)
+        assert torch.all((eager.double().view(-1, heads, dim) - want).abs() <= bound + 1e-30)
+        b.k.copy_(full[0])
+        b.v.copy_(full[1])
+        now = [a + int(c) for a, c in zip(now, count.tolist())]
+        b.seqs = [(0, a) for a in now]
+    assert kept_all > 10
+
+
+def test_a_bounded_cache_captured_and_replayed():
+    """Attention with its sums, the weights that positions gather, and, when
+    the cache is full, the choice and the move: step by step as on the host."""
+    heads, kv, dim, page, budget = 8, 2, 128, 16, 96
+    lens = [60, 95, 80]
+    b = ref.Batch([(1, n + 60) for n in lens], kv, dim, page, rlh.BF16, seed=8)
+    q = torch.zeros((3, heads * dim), dtype=torch.bfloat16, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros((3, heads), device="cuda")
+    mass = torch.full(b.k.shape[:3], 0.25, device="cuda")
+    keep = torch.zeros((3, kv, budget), dtype=torch.int32, device="cuda")
+    count, st = torch.zeros(3, dtype=torch.int32, device="cuda"), word()
+    args = rlh.AttnArgs(heads, 0, at(q), at(out), q.stride(0), out.stride(0), dim ** -0.5, 0.0, None, None, None, 0)
+    ws = torch.empty(max(16, rlh.paged_attn_workspace(b.kv(), b.desc(), args)), dtype=torch.uint8, device="cuda")
+    choice = rlh.EvictArgs(at(mass), budget, 4, 16, budget, at(keep), at(count))
+    move = rlh.MoveArgs(at(keep), budget, 1, at(count), budget, None, at(mass), at(mass))
+
+    def step(s):
+        rlh.paged_attn_lse(b.kv(), b.desc(), args, at(lse), at(ws), ws.numel(), at(st), s)
+        rlh.paged_mass(b.kv(), b.desc(), args, at(lse), 0.9, at(mass), at(st), s)
+        rlh.evict_select(b.kv(), b.desc(), choice, at(st), s)
+        rlh.paged_move(b.kv(), b.desc(), move, at(st), s)
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        step(side.cuda_stream)
+    g = torch.Generator().manual_seed(2)
+    now = list(lens)
+    cut = 0
+    for i in range(12):
+        now = [n + 1 for n in now]
+        b.seqs = [(1, n) for n in now]
+        b.kv_len.copy_(ints(now))
+        q.copy_(torch.randn(q.shape, generator=g))
+        for s, n in enumerate(now):  # the new position's row
+            b.k[b.page_of(s, n - 1), :, (n - 1) % page] = torch.randn((kv, dim), generator=g).bfloat16().cuda()
+            b.v[b.page_of(s, n - 1), :, (n - 1) % page] = torch.randn((kv, dim), generator=g).bfloat16().cuda()
+        k0, v0, m0 = b.k.clone(), b.v.clone(), mass.clone()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(st) == 0
+        got = b.k.clone(), b.v.clone(), mass.clone()
+        b.k.copy_(k0)
+        b.v.copy_(v0)
+        sees = [cref.causal_sees(1, n) for n in now]
+        want, bound, want_lse, far = cref.attention(b, q.view(3, heads, dim), heads, sees, dim ** -0.5)
+        assert torch.all((out.double().view(3, heads, dim) - want).abs() <= bound + 1e-30)
+        assert torch.all((lse.double() - want_lse).abs() <= far)
+        expect, off = cref.mass(b, q.view(3, heads, dim), heads, sees, lse, dim ** -0.5, 0.9, m0)
+        # the masses that the choice saw are those of an eager call
+        eager = m0.clone()
+        rlh.paged_mass(b.kv(), b.desc(), args, at(lse), 0.9, at(eager), None, stream())
+        assert torch.all((eager.double() - expect).abs() <= off)
+        host = eager.cpu().numpy()
+        k, v, m = k0.clone(), v0.clone(), eager.clone()
+        for s, n in enumerate(now):
+            pages, slots = np.array([b.page_of(s, j) for j in range(n)]), np.arange(n) % page
+            for h in range(kv):
+                kept = cref.evict(host[pages, h, slots], budget, 4, 16)
+                assert int(count[s]) == len(kept) and keep[s, h, :len(kept)].tolist() == list(kept)
+                to, src = (pages[:len(kept)], h, slots[:len(kept)]), (pages[kept], h, slots[kept])
+                k[to], v[to], m[to] = k0[src], v0[src], eager[src]
+        assert torch.equal(got[0], k) and torch.equal(got[1], v) and torch.equal(got[2], m)
+        b.k.copy_(k)
+        b.v.copy_(v)
+        cut += sum(n > budget for n in now)
+        now = [min(n, budget) for n in now]
+    assert cut > 5
+
+
+def test_cache_two_streams_at_once():
+    """Tree attention, masses and the choice on two streams, workspaces of their own: the bits of calls alone."""
+    jobs = []
+    for i, name in enumerate(("ragged", "28 over 4")):
+        case = dict(TREE[name])
+        b, q, out, lse, masks, _ = tree_case(seed=30 + i, **case)
+        ws = run_tree(b, q, out, case["heads"], masks, lse)
+        m = masses(b.k.shape[:3], "spread", i)
+        args = rlh.AttnArgs(case["heads"], 0, at(q), None, q.stride(0), 0, b.dim ** -0.5, 0.0, None, None, None, 0)
+        rlh.paged_mass(b.kv(), b.desc(), args, at(lse), 0.5, at(m), None, stream())
+        keep = torch.zeros((b.desc().n_seq, b.kv_heads, 64), dtype=torch.int32, device="cuda")
+        count = torch.zeros(b.desc().n_seq, dtype=torch.int32, device="cuda")
+        b.kv_len[len(b.seqs):] = 0
+        rlh.evict_select(b.kv(), b.desc(), rlh.EvictArgs(at(m), 64, 4, 8, 64, at(keep), at(count)), None, stream())
+        jobs.append((b, q, lse, masks, args, case["heads"], ws, out, masses(b.k.shape[:3], "spread", i), m, keep, count,
+                     torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    hold = []
+    for _ in range(6):
+        for b, q, lse, masks, args, heads, ws, out, m0, m, keep, count, s in jobs:
+            o2, l2, m2 = torch.full_like(out, 7.0), torch.full_like(lse, 7.0), m0.clone()
+            k2, c2 = torch.zeros_like(keep), torch.zeros_like(count)
+            torch.cuda.synchronize()
+            hold.append((o2, l2, m2, k2, c2, out, lse, m, keep, count))
+        for j, (b, q, lse, masks, args, heads, ws, out, m0, m, keep, count, s) in enumerate(jobs):
+            o2, l2, m2, k2, c2 = hold[j - 2][:5]
+            run_tree(b, q, o2, heads, masks, l2, ws=ws, st=s.cuda_stream)
+            rlh.paged_mass(b.kv(), b.desc(), args, at(l2), 0.5, at(m2), None, s.cuda_stream)
+            rlh.evict_select(b.kv(), b.desc(), rlh.EvictArgs(at(m2), 64, 4, 8, 64, at(k2), at(c2)), None, s.cuda_stream)
+    torch.cuda.synchronize()
+    for o2, l2, m2, k2, c2, out, lse, m, keep, count in hold:
+        assert torch.equal(o2, out) and torch.equal(l2, lse) and torch.equal(m2, m)
+        assert torch.equal(k2, keep) and torch.equal(c2, count)
+
+
+def test_tree_one_workspace_for_limits():
+    """A workspace of a host's limits holds every smaller call, and nothing behind it is written."""
+    heads, kv, dim = 16, 2, 64
+    limits = rlh.Seqs(300, 4000, 300, 2000, 125, 1 << 40, 1 << 41, 1 << 42)
+    pool = rlh.KvPages(rlh.BF16, kv, dim, 16, 1 << 20, 1 << 43, 1 << 44)
+    most = rlh.AttnArgs(heads, 0, 1 << 45, 1 << 46, heads * dim, heads * dim, 0.1, 0.0, None, None, 1 << 47, 256)
+    size = rlh.tree_attn_workspace(pool, limits, most)
+    ws = torch.full((size + 256,), 0xff, dtype=torch.uint8, device="cuda")
+    for seqs, shared in (([(300, 2000)], 0), ([(1, 2000)], 0), ([(3, 300 + i) for i in range(280)], 256), ([(1, 9)] * 300, 0),
+                         ([(13, 13 + i) for i in range(290)], 0), ([(130, 700)] * 7, 256)):
+        b, q, out, lse, masks, sees = tree_case(seqs, heads, kv, dim, 16, rlh.BF16, seed=2, shared=shared)
+        args = rlh.AttnArgs(heads, 0, at(q), at(out), q.stride(0), out.stride(0), dim ** -0.5, 0.0, None, None,
+                            at(b.shared_table) if shared else None, shared)
+        rlh.tree_attn(b.kv(), b.desc(), args, at(masks), masks.shape[1], at(lse), at(ws), size, None, stream())
+        torch.cuda.synchronize()
+        assert torch.all(ws[size:] == 0xff)
+        check_tree(b, q, out, lse, heads, sees)
+
+
+@pytest.mark.parametrize("ty", [rlh.BF16])
+def test_cache_offsets_past_32_bits(ty):
+    """Pages whose values lie past 2^32 elements (9 GB of K and of V)."""
+    kv, dim, page = 8, 128, 256
+    n_pages = (1 << 32) // (kv * dim * page) + 40
+    k, v = (torch.zeros((n_pages, kv, page, dim), dtype=TORCH[ty], device="cuda") for _ in range(2))
+    pool = rlh.KvPages(ty, kv, dim, page, n_pages, at(k), at(v))
+    g = torch.Generator().manual_seed(4)
+    ids = [n_pages - 1, n_pages - 3, 2, n_pages - 2]
+    b = ref.Batch([(20, 1000)], kv, dim, page, ty, seed=3)
+    for i, p in enumerate(ids):
+        k[p], v[p] = b.k[b.page_of(0, i * page)], b.v[b.page_of(0, i * page)]
+    table, q_start, kv_len = ints([ids]), ints([0, 20]), ints([1000])
+    seqs = rlh.Seqs(1, 20, 20, 1000, 4, at(q_start), at(kv_len), at(table))
+    heads = 16
+    q = torch.randn((20, heads * dim), generator=g).to(TORCH[ty]).cuda()
+    see = cref.mask_matrix(cref.random_tree(cref.rng(1), 20))
+    masks = torch.tensor(cref.pack(see, 1), device="cuda")
+    out, lse, mass = torch.zeros_like(q), torch.zeros((20, heads), device="cuda"), torch.rand((n_pages, kv, page), device="cuda")
+    args = rlh.AttnArgs(heads, 0, at(q), at(out), q.stride(0), out.stride(0), dim ** -0.5, 0.0, None, None, None, 0)
+    ws = torch.empty(rlh.tree_attn_workspace(pool, seqs, args), dtype=torch.uint8, device="cuda")
+    rlh.tree_attn(pool, seqs, args, at(masks), 1, at(lse), at(ws), ws.numel(), None, stream())
+    want, bound, want_lse, far = cref.attention(b, q.view(20, heads, dim), heads, [cref.tree_sees(see, 980, 0)], dim ** -0.5)
+    assert torch.all((out.double().view(20, heads, dim) - want).abs() <= bound) and torch.all((lse.double() - want_lse).abs() <= far)
+    small = torch.zeros(b.k.shape[:3], device="cuda")
+    for i, p in enumerate(ids):
+        small[b.page_of(0, i * page)] = mass[p]
+    for rows in (20, 1):
+        qr, ls = q[20 - rows:], lse[20 - rows:].contiguous()
+        b.seqs, b.starts = [(rows, 1000)], np.array([0, rows])
+        starts = ints([0, rows])
+        one = rlh.Seqs(1, rows, rows, 1000, 4, at(starts), at(kv_len), at(table))
+        a2 = rlh.AttnArgs(heads, 0, at(qr), None, q.stride(0), 0, dim ** -0.5, 0.0, None, None, None, 0)
+        expect, off = cref.mass(b, qr.view(rows, heads, dim), heads, [cref.causal_sees(rows, 1000)], ls, dim ** -0.5, 1.0, small)
+        got = mass.clone()
+        rlh.paged_mass(pool, one, a2, at(ls), 1.0, at(got), None, stream())
+        for i, p in enumerate(ids):
+            e = (got[p].double() - expect[b.page_of(0, i * page)]).abs() - off[b.page_of(0, i * page)]
+            live = min(page, 1000 - i * page)
+            assert torch.all(e[:, :live] <= 0)
+    index = ints(np.sort(np.random.default_rng(1).choice(1000, 600, replace=False)))
+    c = ints([600])
+    rows_k = torch.cat([k[p] for p in ids], 1)[:, :1000][:, index.long()].clone()
+    rlh.paged_move(pool, seqs, rlh.MoveArgs(at(index), 600, 0, at(c), 600, None, None, None), None, stream())
+    assert torch.equal(torch.cat([k[p] for p in ids], 1)[:, :600], rows_k)
+
+
+def test_cache_refused_on_the_device():
+    """Host memory, and nothing written by a refused call."""
+    b, q, out, lse, masks, _ = tree_case([(5, 300)], 4, 2, 64, 16, rlh.F16, seed=1)
+    host = torch.zeros(4096, dtype=torch.int64)
+    args = rlh.AttnArgs(4, 0, at(q), at(out), q.stride(0), out.stride(0), 0.125, 0.0, None, None, None, 0)
+    ws = torch.empty(rlh.tree_attn_workspace(b.kv(), b.desc(), args), dtype=torch.uint8, device="cuda")
+    c = word()
+    calls = [
+        lambda: rlh.tree_attn(b.kv(), b.desc(), args, host.data_ptr(), 1, None, at(ws), ws.numel(), None, stream()),
+        lambda: rlh.tree_attn(b.kv(), b.desc(), args, at(masks), 1, host.data_ptr(), at(ws), ws.numel(), None, stream()),
+        lambda: rlh.tree_attn(b.kv(), b.desc(), args, at(masks), 1, None, at(ws), 16, None, stream()),
+        lambda: rlh.tree_masks(b.desc(), host.data_ptr(), None, at(masks), 1, None, None, stream()),
+        lambda: rlh.paged_mass(b.kv(), b.desc(), args, host.data_ptr(), 0.5, at(ws), None, stream()),
+        lambda: rlh.paged_move(b.kv(), b.desc(), rlh.MoveArgs(host.data_ptr(), 8, 0, at(c), 8, None, None, None), None, stream()),
+        lambda: rlh.evict_select(b.kv(), b.desc(), rlh.EvictArgs(at(ws), 8, 0, 0, 8, host.data_ptr(), at(c)), None, stream()),
+    ]
+    keep = masks.clone()
+    for f in calls:
+        with pytest.raises(rlh.RlhError) as e:
+            f()
+        assert e.value.code == rlh.RLH_EINVAL
+    torch.cuda.synchronize()
+    assert torch.all(out == 7.0) and torch.all(lse == 7.0) and torch.equal(masks, keep)
