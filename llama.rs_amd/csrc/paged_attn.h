@@ -700,7 +700,11 @@ __device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, ui
     active = active && sq < a.b.n_seq;
   }
   SeqView sv{};
-  if (active) {
+  if (TREE && !prefix) {  // (a tile's sequence is one that counts)
+    bool bad;
+    sv = load_attn_seq<TREE>(a, s, &bad);
+    row += sv.q0;
+  } else if (active) {
     bool bad;
     sv = load_attn_seq<TREE>(a, sq, &bad);
     if (!prefix) row += sv.q0;
@@ -719,60 +723,77 @@ __device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, ui
     span.prefix = min(span.prefix, limit);
   }
   // positions that the wave's rows all see lie in [w_lo, w_hi) or below
-  // w_prefix; those that any sees in [b_lo, b_hi)
-  int32_t w_lo = active ? span.lo : 0, w_hi = active ? span.hi : 0x7fffffff, w_prefix = active ? span.prefix : 0x7fffffff;
-  const int32_t lo1 = drafts ? min(span.lo, first) : span.lo;  // (a window may end among the new rows)
-  int32_t b_lo = active ? max(TREE ? lo1 : span_begin(span), prefix ? 0 : (int32_t)a.shared_len) : 0x7fffffff;
-  int32_t b_hi = active ? (drafts ? (int32_t)sv.kv_len : span_end(span)) : 0;
-  int32_t any_prefix = active ? span.prefix : 0, min_lo = active ? lo1 : 0x7fffffff;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    w_lo = max(w_lo, __shfl_xor(w_lo, d));
-    w_hi = min(w_hi, __shfl_xor(w_hi, d));
-    w_prefix = min(w_prefix, __shfl_xor(w_prefix, d));
-    b_lo = min(b_lo, __shfl_xor(b_lo, d));
-    b_hi = max(b_hi, __shfl_xor(b_hi, d));
-    any_prefix = max(any_prefix, __shfl_xor(any_prefix, d));
-    min_lo = min(min_lo, __shfl_xor(min_lo, d));
-  }
-  w_lo = (int32_t)uniform(w_lo);
-  w_hi = (int32_t)uniform(w_hi);
-  w_prefix = (int32_t)uniform(w_prefix);
-  const int32_t v_lo = (int32_t)uniform(b_lo), v_hi = (int32_t)uniform(b_hi);  // the wave's
-  if (lane == 0) {
-    int32_t* r = sh.ranges[wave];
-    r[0] = v_lo;
-    r[1] = v_hi;
-    r[2] = any_prefix;
-    r[3] = min_lo;
-    r[4] = w_lo;
-    r[5] = w_hi;
-    r[6] = w_prefix;
-  }
-  __syncthreads();
-  int32_t t_lo = 0x7fffffff, t_hi = 0, t_prefix = 0, t_min_lo = 0x7fffffff;  // the block's
-  int32_t c_lo = 0, c_hi = 0x7fffffff, c_prefix = 0x7fffffff;
-#pragma unroll
-  for (int w = 0; w < kTileWaves; w++) {
-    const int32_t* r = sh.ranges[w];
-    t_lo = min(t_lo, r[0]);
-    t_hi = max(t_hi, r[1]);
-    t_prefix = max(t_prefix, r[2]);
-    t_min_lo = min(t_min_lo, r[3]);
-    c_lo = max(c_lo, r[4]);
-    c_hi = min(c_hi, r[5]);
-    c_prefix = min(c_prefix, r[6]);
-  }
-  c_lo = (int32_t)uniform(c_lo);
-  c_hi = (int32_t)uniform(c_hi);
-  c_prefix = (int32_t)uniform(c_prefix);
-  t_lo = (int32_t)uniform(t_lo & ~15);
-  t_hi = (int32_t)uniform(t_hi);
-  t_prefix = (int32_t)uniform(t_prefix);
-  t_min_lo = (int32_t)uniform(t_min_lo);
-  if (TREE) {
+  // w_prefix; those that any sees in [v_lo, v_hi); t_ and c_: the block's
+  int32_t w_lo, w_hi, w_prefix, v_lo, v_hi, t_lo, t_hi, t_prefix, t_min_lo, c_lo, c_hi, c_prefix;
+  if (drafts) {
+    // bounds of what any row may see: a window's start moves with the new rows seen, none to all
+    const int32_t from = (int32_t)uniform((uint32_t)first), n = (int32_t)uniform(sv.kv_len);
+    const bool any = row0 + wave * 32 < rows;
+    c_lo = w_lo = tree_span(from, uniform(sv.q_len), a.window).lo;
+    c_hi = w_hi = from;
+    t_prefix = c_prefix = w_prefix = 0;
+    t_min_lo = min(tree_span(from, 0, a.window).lo, from);
     t_lo = job.begin;
-    t_hi = min(t_hi, job.end);
+    t_hi = n;
+    v_lo = any ? max(t_min_lo, (int32_t)a.shared_len) : 0x7fffffff;
+    v_hi = any ? n : 0;
+  } else {
+    w_lo = active ? span.lo : 0;
+    w_hi = active ? span.hi : 0x7fffffff;
+    w_prefix = active ? span.prefix : 0x7fffffff;
+    int32_t b_lo = active ? max(span_begin(span), prefix ? 0 : (int32_t)a.shared_len) : 0x7fffffff;
+    int32_t b_hi = active ? span_end(span) : 0;
+    int32_t any_prefix = active ? span.prefix : 0, min_lo = active ? span.lo : 0x7fffffff;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      w_lo = max(w_lo, __shfl_xor(w_lo, d));
+      w_hi = min(w_hi, __shfl_xor(w_hi, d));
+      w_prefix = min(w_prefix, __shfl_xor(w_prefix, d));
+      b_lo = min(b_lo, __shfl_xor(b_lo, d));
+      b_hi = max(b_hi, __shfl_xor(b_hi, d));
+      any_prefix = max(any_prefix, __shfl_xor(any_prefix, d));
+      min_lo = min(min_lo, __shfl_xor(min_lo, d));
+    }
+    w_lo = (int32_t)uniform(w_lo);
+    w_hi = (int32_t)uniform(w_hi);
+    w_prefix = (int32_t)uniform(w_prefix);
+    v_lo = (int32_t)uniform(b_lo);
+    v_hi = (int32_t)uniform(b_hi);
+    if (lane == 0) {
+      int32_t* r = sh.ranges[wave];
+      r[0] = v_lo;
+      r[1] = v_hi;
+      r[2] = any_prefix;
+      r[3] = min_lo;
+      r[4] = w_lo;
+      r[5] = w_hi;
+      r[6] = w_prefix;
+    }
+    __syncthreads();
+    t_lo = t_min_lo = c_hi = c_prefix = 0x7fffffff;
+    t_hi = t_prefix = c_lo = 0;
+#pragma unroll
+    for (int w = 0; w < kTileWaves; w++) {
+      const int32_t* r = sh.ranges[w];
+      t_lo = min(t_lo, r[0]);
+      t_hi = max(t_hi, r[1]);
+      t_prefix = max(t_prefix, r[2]);
+      t_min_lo = min(t_min_lo, r[3]);
+      c_lo = max(c_lo, r[4]);
+      c_hi = min(c_hi, r[5]);
+      c_prefix = min(c_prefix, r[6]);
+    }
+    c_lo = (int32_t)uniform(c_lo);
+    c_hi = (int32_t)uniform(c_hi);
+    c_prefix = (int32_t)uniform(c_prefix);
+    t_lo = (int32_t)uniform(t_lo & ~15);
+    t_hi = (int32_t)uniform(t_hi);
+    t_prefix = (int32_t)uniform(t_prefix);
+    t_min_lo = (int32_t)uniform(t_min_lo);
+    if (TREE) {
+      t_lo = job.begin;
+      t_hi = min(t_hi, job.end);
+    }
   }
   const uint32_t n_steps = t_hi > t_lo ? (uint32_t)(t_hi - t_lo + kTileKv - 1) / kTileKv : 0;
   const uint32_t st0 = TREE ? job.st0 : (uint32_t)((uint64_t)n_steps * part / parts);
