@@ -1034,3 +1034,32 @@ def test_cache_refused_on_the_device():
         assert e.value.code == rlh.RLH_EINVAL
     torch.cuda.synchronize()
     assert torch.all(out == 7.0) and torch.all(lse == 7.0) and torch.equal(masks, keep)
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_tree_attention_with_starts_that_fall(many):
+    """A sequence whose start falls is skipped; rows between that two others
+    name are written by one of them, and nothing else changes."""
+    n = 270 if many else 3
+    seqs = [(20, 200), (30, 100), (25, 130)] + [(0, 5)] * (n - 3)
+    b, q, out, lse, masks, sees = tree_case(seqs, 8, 2, 64, 16, rlh.F16, seed=13)
+    # rows 0 .. 19, then a fall from 50 to 40, then rows 40 .. 74
+    starts = b.q_start.clone()
+    starts[1], starts[2] = 50, 40
+    keep = b.q_start.clone()
+    b.q_start.copy_(starts)
+    b.max_q = 60
+    st = word()
+    masks = torch.zeros((b.n_rows, 1), dtype=torch.int64, device="cuda")
+    run_tree(b, q, out, 8, masks, lse, status=st)
+    torch.cuda.synchronize()
+    assert int(st) == rlh.SERVE_BAD_SEQ
+    assert torch.all(out[:, 8 * 64:] == 7.0)
+    b.q_start.copy_(keep)
+
+
+def test_tree_attention_of_many_heads():
+    """More KV heads than the card has CUs: a block to a head."""
+    b, q, out, lse, masks, sees = tree_case([(20, 70), (1, 33)], 300, 300, 64, 16, rlh.BF16, seed=14)
+    run_tree(b, q, out, 300, masks, lse)
+    check_tree(b, q, out, lse, 300, sees)
