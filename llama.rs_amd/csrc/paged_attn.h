@@ -22,10 +22,8 @@ struct AttnParams {
   uint64_t q_stride, out_stride;
   const float* slopes;
   const uint32_t *prefix_len, *shared_table;
-  const uint64_t* masks;  // TREE: [n_rows][mask_words]
-  float* lse;             // may be null
   uint32_t* status;
-  uint32_t n_head, n_kv, group, page_shift, n_pages, window, shared_len, mask_words;
+  uint32_t n_head, n_kv, group, page_shift, n_pages, window, shared_len;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -191,7 +189,6 @@ struct Workspace {
   float* item_ml;    // [items * n_kv][16][2]
   uint32_t* plan;    // [n_seq][2]: first item, items
   uint32_t* tiles;   // [n_seq][2]: first tile, tiles (where `planned`)
-  uint64_t* line;    // of drafted rows: a block's units, then each sequence's first one
 };
 
 struct Sizes {
@@ -208,8 +205,6 @@ struct Sizes {
   bool planned;           // a launch before found where each sequence's items and tiles begin
   bool merge_small;       // only its sequences have parts to join
   uint32_t merge_rows;    // then: blocks per sequence and KV head
-  uint32_t line_blocks;   // not 0: drafted rows as a line of tiles that so many blocks per KV head share
-  uint32_t slot_rows;     // rows of a part of theirs
 };
 
 // Blocks of a KV head for the shared prefix.
@@ -217,11 +212,22 @@ __host__ __device__ inline uint32_t prefix_blocks(const Sizes& n) {
   return n.prefix_tiles ? (n.prefix_tiles - 1) * n.prefix_parts + n.last_parts : 0;
 }
 
+// What a call may do beside: the log of its sums, drafted rows.
+struct Beside {
+  float* lse;             // may be null
+  const uint64_t* masks;  // TREE: [n_rows][mask_words]
+  uint64_t* line;         // of a line of tiles (workspace): a block's units, the line's, then each sequence's first one
+  uint32_t mask_words;
+  uint32_t line_blocks;   // not 0: drafted rows as a line of tiles that so many blocks per KV head share
+  uint32_t slot_rows;     // rows of a part of theirs
+};
+
 struct Launch {
   AttnParams a;
   Scoring sc;
   Workspace ws;
   Sizes n;
+  Beside b;
 };
 
 // The sequence s; drafted rows lie behind the shared positions.
@@ -237,11 +243,11 @@ __device__ __forceinline__ SeqView load_attn_seq(const AttnParams& a, uint32_t s
 
 // TREE: what row `row` (of q_len, the sequence's first at `first`) sees of the
 // positions before its batch; the new rows among the 64 positions from p on.
-__device__ __forceinline__ RowSpan tree_row(const AttnParams& a, uint32_t row, int32_t first, uint32_t q_len) {
-  return tree_span(first, a.window ? tree_seen(a.masks + (size_t)row * a.mask_words, a.mask_words, q_len) : 0, a.window);
+__device__ __forceinline__ RowSpan tree_row(const Launch& L, uint32_t row, int32_t first, uint32_t q_len) {
+  return tree_span(first, L.a.window ? tree_seen(L.b.masks + (size_t)row * L.b.mask_words, L.b.mask_words, q_len) : 0, L.a.window);
 }
-__device__ __forceinline__ uint64_t tree_row_bits(const AttnParams& a, uint32_t row, int32_t first, uint32_t q_len, int32_t p) {
-  return tree_bits(a.masks + (size_t)row * a.mask_words, a.mask_words, q_len, p - first);
+__device__ __forceinline__ uint64_t tree_row_bits(const Launch& L, uint32_t row, int32_t first, uint32_t q_len, int32_t p) {
+  return tree_bits(L.b.masks + (size_t)row * L.b.mask_words, L.b.mask_words, q_len, p - first);
 }
 
 // log of the sum of exp(score) from a maximum in units of log 2 and the sum relative to it
@@ -410,7 +416,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
   const uint32_t qi = active ? col / a.group : 0, g = active ? col % a.group : 0;
   const uint32_t row = sq.v.q0 + qi, head = h * a.group + g;
   const int32_t pos = sq.p0 + (int32_t)qi;
-  const RowSpan span = TREE ? tree_row(a, row, sq.p0, sq.v.q_len) : row_span(pos, sq.v.kv_len, a.window, sq.prefix);
+  const RowSpan span = TREE ? tree_row(L, row, sq.p0, sq.v.q_len) : row_span(pos, sq.v.kv_len, a.window, sq.prefix);
   // bounds of all rows' (TREE: from none to all of the new rows seen)
   const RowSpan span0 = TREE ? tree_span(sq.p0, 0, a.window) : row_span(sq.p0, sq.v.kv_len, a.window, sq.prefix);
   const RowSpan span1 = TREE ? tree_span(sq.p0, sq.v.q_len, a.window)
@@ -503,7 +509,7 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
       }
       uint64_t bits = 0;  // TREE: the new rows among the step's positions that the row sees
       if (!full) {
-        if (TREE && p + 32 > sq.p0) bits = tree_row_bits(a, row, sq.p0, sq.v.q_len, p);
+        if (TREE && p + 32 > sq.p0) bits = tree_row_bits(L, row, sq.p0, sq.v.q_len, p);
         const uint32_t b = (uint32_t)bits >> (quad * 4);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -588,8 +594,8 @@ __device__ __forceinline__ void small_block(const Launch& L, uint32_t block, uin
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = (T)(acc[i] * inv);
     *(VO*)dst = v;
-    if (a.lse && c0 == 0)
-      a.lse[(size_t)(sq.v.q0 + r / a.group) * a.n_head + h * a.group + r % a.group] = log_sum<T>(mm, ls);
+    if (L.b.lse && c0 == 0)
+      L.b.lse[(size_t)(sq.v.q0 + r / a.group) * a.n_head + h * a.group + r % a.group] = log_sum<T>(mm, ls);
   } else {
     const size_t at = ((size_t)item * a.n_kv + h) * kSmallRows + r;
     float* dst = L.ws.item_o + at * D + c0;
@@ -717,7 +723,7 @@ __device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, ui
   const int32_t first = (int32_t)(sv.kv_len - sv.q_len);
   const bool drafts = TREE && !prefix;  // the new rows are among the positions
   if (active) {
-    span = TREE ? tree_row(a, row, first, sv.q_len)
+    span = TREE ? tree_row(L, row, first, sv.q_len)
                 : row_span(pos, sv.kv_len, a.window, a.prefix_len ? a.prefix_len[sq] : 0);
     span.hi = min(span.hi, limit);
     span.prefix = min(span.prefix, limit);
@@ -877,39 +883,39 @@ __device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, ui
   };
   // TREE: the new rows among the step's positions that the row sees
   auto step_bits = [&](int32_t p) -> uint64_t {
-    return drafts && active && p + kTileKv > first ? tree_row_bits(a, row, first, sv.q_len, p) : 0;
+    return drafts && active && p + kTileKv > first ? tree_row_bits(L, row, first, sv.q_len, p) : 0;
   };
   uint32_t pages = kNone, next_pages = kNone;
   uint64_t exist = 0;  // the groups of `pages` whose page exists
   if (st0 < st1) {
     pages = look_up(st0);
     exist = __ballot(pages != kNone);
-    for (uint32_t i = 0; i < kBufs - 1 && st0 + i < st1; i++) copy(t_lo + (int32_t)(st0 + i) * kTileKv, pages, i, i);
+    copy(t_lo + (int32_t)st0 * kTileKv, pages, 0, 0);
+    if constexpr (kBufs == 4) {
+      if (st0 + 1 < st1) copy(t_lo + (int32_t)(st0 + 1) * kTileKv, pages, 1, 1);
+      if (st0 + 2 < st1) copy(t_lo + (int32_t)(st0 + 2) * kTileKv, pages, 2, 2);
+    }
   }
   uint64_t next_exist = 0;
   for (uint32_t st = st0; st < st1; st++) {
     const uint32_t buf = (st - st0) & (kBufs - 1);
     const int32_t p = t_lo + (int32_t)st * kTileKv;
     const uint32_t k = (st - st0) & 15;
-    if (k == 0 && st != st0) exist = next_exist;
+    if (kBufs == 4 && k == 0 && st != st0) exist = next_exist;
     const uint32_t ok = (uint32_t)(exist >> (4 * k)) & 15;
     if (t == 0) special[buf & 1] = 0;  // last read two barriers ago
     // this wave's copies of the step have landed (those of the steps behind it may be on their way)
-    if constexpr (kBufs == 4) {
-      if (st + 2 < st1)
-        wait_vmcnt<4 * kCopies>();
-      else if (st + 1 < st1)
-        wait_vmcnt<2 * kCopies>();
-      else
-        wait_vmcnt<0>();
-    } else {
+    if (kBufs == 4 && st + 2 < st1)
+      wait_vmcnt<4 * kCopies>();
+    else if (kBufs == 4 && st + 1 < st1)
+      wait_vmcnt<2 * kCopies>();
+    else
       wait_vmcnt<0>();
-    }
     lds_barrier();  // ... everyone's; every wave is done with the buffer before this one
     if (k == 8) next_pages = look_up(st + 8);
     if (k == 17 - kBufs) {
       pages = next_pages;
-      next_exist = __ballot(pages != kNone);
+      (kBufs == 4 ? next_exist : exist) = __ballot(pages != kNone);
     }
     if (st + kBufs - 1 < st1)
       copy(p + (kBufs - 1) * kTileKv, pages, (k + kBufs - 1) & 15, (buf + kBufs - 1) & (kBufs - 1));
@@ -1059,7 +1065,7 @@ __device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, ui
         for (int k = 0; k < 4; k++) v[k] = (T)(o[i][e + k] * inv);
         *(vec4<T>*)(dst + i * 32 + (e / 4) * 8 + half * 4) = v;
       }
-    if (a.lse && half == 0) a.lse[(size_t)row * a.n_head + head] = log_sum<T>(m, l);
+    if (L.b.lse && half == 0) L.b.lse[(size_t)row * a.n_head + head] = log_sum<T>(m, l);
   } else {
     const bool slot = TREE && job.o;
     const size_t at = slot ? rr - row0 : ((size_t)(TREE ? 0 : part) * a.b.n_rows + row) * a.n_head + head;
@@ -1203,20 +1209,20 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
         const uint64_t upto = before + wave_scan64(u);
         if (s < a.b.n_seq) {
           line[2 + s] = upto - u;
-          if (blockIdx.x == 0) L.ws.line[2 + s] = upto - u;  // for the launch that joins parts
+          if (blockIdx.x == 0) L.b.line[2 + s] = upto - u;  // for the launch that joins parts
         }
         before = lane_value64(upto, 63);
       }
       if (lane == 0) {
-        line[0] = line_share(before, L.n.line_blocks);
+        line[0] = line_share(before, L.b.line_blocks);
         line[1] = before;
-        if (blockIdx.x == 0) L.ws.line[0] = line[0];
+        if (blockIdx.x == 0) L.b.line[0] = line[0];
       }
     }
     __syncthreads();
   }
-  const uint64_t share = lane_value64(L.n.planned ? L.ws.line[0] : line[0], 0);
-  const uint64_t total = lane_value64(L.n.planned ? L.ws.line[1] : line[1], 0);
+  const uint64_t share = lane_value64(L.n.planned ? L.b.line[0] : line[0], 0);
+  const uint64_t total = lane_value64(L.n.planned ? L.b.line[1] : line[1], 0);
   const uint64_t x1 = min((block + 1) * share, total);
   for (uint64_t x = block * share; x < x1;) {
     TileJob job{};
@@ -1232,13 +1238,13 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
       // the last sequence that begins at x or before (those without units share their first one with the next)
       uint32_t n = 0;
       if (L.n.planned) {
-        n = count_upto<uint64_t>(L.ws.line + 2, 1, a.b.n_seq, x);
+        n = count_upto<uint64_t>(L.b.line + 2, 1, a.b.n_seq, x);
       } else {
         for (uint32_t s0 = 0; s0 < a.b.n_seq; s0 += 64)
           n += (uint32_t)__popcll(__ballot(s0 + lane < a.b.n_seq && line[2 + s0 + lane] <= x));
       }
       job.s = uniform(n - 1);
-      first = lane_value64(L.n.planned ? L.ws.line[2 + job.s] : line[2 + job.s], 0);
+      first = lane_value64(L.n.planned ? L.b.line[2 + job.s] : line[2 + job.s], 0);
       bool bad;
       const LineSeq q = line_seq(a, job.s, &bad);
       job.rows = uniform(q.q.rows);
@@ -1253,7 +1259,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
     job.st0 = uniform(line_step(tile, x));
     job.st1 = end <= x1 ? steps : uniform(line_step(tile, x1));
     if (job.st0 != 0 || job.st1 != steps) {
-      const size_t slot = ((size_t)line_slot(tile, block, share) * a.n_kv + h) * L.n.slot_rows;
+      const size_t slot = ((size_t)line_slot(tile, block, share) * a.n_kv + h) * L.b.slot_rows;
       job.o = L.ws.item_o + slot * D;
       job.ml = L.ws.item_ml + slot * 2;
     }
@@ -1286,12 +1292,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_line_plan(Launch L) {
       upto += w < wave ? sums[w] : 0;
       all += sums[w];
     }
-    if (s0 + t < a.b.n_seq) L.ws.line[2 + s0 + t] = before + upto - u;
+    if (s0 + t < a.b.n_seq) L.b.line[2 + s0 + t] = before + upto - u;
     before += all;
   }
   if (t == 0) {
-    L.ws.line[0] = line_share(before, L.n.line_blocks);
-    L.ws.line[1] = before;
+    L.b.line[0] = line_share(before, L.b.line_blocks);
+    L.b.line[1] = before;
   }
 }
 
@@ -1403,7 +1409,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_merge(Launch L) {
 #pragma unroll
   for (int i = 0; i < N; i++) v[i] = (T)(acc[i] * inv);
   *(VO*)((T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + c0) = v;
-  if (a.lse && c0 == 0) a.lse[rh] = log_sum<T>(m, l);
+  if (L.b.lse && c0 == 0) L.b.lse[rh] = log_sum<T>(m, l);
 }
 
 // The same for a line of tiles: a wave takes four heads of a row, 16 lanes each,
@@ -1418,7 +1424,7 @@ __global__ void __launch_bounds__(kThreads) k_line_merge(Launch L) {
   const uint32_t per_row = (a.n_head + 3) / 4, w = blockIdx.x * kWaves + wave;
   const uint32_t row = w / per_row, head = w % per_row * 4 + lane / 16;
   if (row >= a.b.n_rows) return;
-  const uint64_t share = L.ws.line[0];
+  const uint64_t share = L.b.line[0];
   const uint32_t s = count_upto<uint32_t>(a.b.q_start + 1, 1, a.b.n_seq, row);
   if (s >= a.b.n_seq) return;
   bool bad;
@@ -1427,7 +1433,7 @@ __global__ void __launch_bounds__(kThreads) k_line_merge(Launch L) {
   if (!q.q.v.ok || row < q.q.v.q0 || row >= q.q.v.q0 + q.q.v.q_len || head >= a.n_head) return;
   const uint32_t h = head / a.group, r = (row - q.q.v.q0) * a.group + head % a.group;
   const uint32_t in_head = row * a.group + head % a.group;  // among all rows of its KV head
-  const LineTile own = line_tile(L.ws.line[2 + s], q.q.rows, q.steps, r / kLineRows);
+  const LineTile own = line_tile(L.b.line[2 + s], q.q.rows, q.steps, r / kLineRows);
   const uint32_t own0 = line_first_block(own, share), n_own = line_last_block(own, share) - own0 + 1;
   LineTile shared{};  // the tile of the shared positions
   uint32_t shared0 = 0, n_shared = 0;
@@ -1451,7 +1457,7 @@ __global__ void __launch_bounds__(kThreads) k_line_merge(Launch L) {
       size_t at = rh;  // a whole tile's
       if ((mine ? n_own : n_shared) > 1) {
         const uint32_t slot = mine ? line_slot(own, own0 + i - n_shared, share) : line_slot(shared, shared0 + i, share);
-        at = ((size_t)slot * a.n_kv + h) * L.n.slot_rows + (mine ? r : in_head) % kLineRows;
+        at = ((size_t)slot * a.n_kv + h) * L.b.slot_rows + (mine ? r : in_head) % kLineRows;
         o = L.ws.item_o;
         ml = L.ws.item_ml;
       }
@@ -1482,7 +1488,7 @@ __global__ void __launch_bounds__(kThreads) k_line_merge(Launch L) {
 #pragma unroll
   for (int i = 0; i < N; i++) v[i] = (T)(acc[i] * inv);
   *(VO*)((T*)a.out + (size_t)row * a.out_stride + (size_t)head * D + c0) = v;
-  if (a.lse && c0 == 0) a.lse[rh] = log_sum<T>(m, l);
+  if (L.b.lse && c0 == 0) L.b.lse[rh] = log_sum<T>(m, l);
 }
 
 // Up to so many positions, and while all blocks run at once, a sequence of few
@@ -1641,8 +1647,6 @@ Sizes attn_sizes(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args&
   const uint64_t own = q.max_kv > args.shared_len ? q.max_kv - args.shared_len : 0;
   n.tiled = q.max_q * group > kSmallRows;
   if (TREE && (n.tiled || args.shared_len)) {
-    n.line_blocks = line_blocks(kv.n_head_kv);
-    n.slot_rows = line_slot_rows(q, group, args.shared_len != 0);
     n.planned = q.n_seq > kPlanned;
     n.merge = true;
     return n;
@@ -1699,7 +1703,6 @@ Room line_room(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& a
 
 // What a call takes.
 Room attn_room(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args, const Sizes& n) {
-  if (n.line_blocks) return line_room(kv, q, args);
   const uint64_t rows = (uint64_t)q.n_rows * args.n_head;
   Room r{};
   r.prefix = args.shared_len ? n.prefix_parts * rows : 0;
@@ -1748,7 +1751,7 @@ Room tree_room_within(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_
 }
 
 // Places the workspace's parts from `base` on (null: counts only); bytes.
-uint64_t place_workspace(Workspace* w, uint8_t* base, uint64_t dim, const Room& r) {
+uint64_t place_workspace(Workspace* w, uint64_t** line, uint8_t* base, uint64_t dim, const Room& r) {
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     uint8_t* p = base ? base + at : nullptr;
@@ -1763,7 +1766,7 @@ uint64_t place_workspace(Workspace* w, uint8_t* base, uint64_t dim, const Room& 
   w->item_ml = (float*)take(r.item * 8);
   w->plan = (uint32_t*)take(r.plan * 8);
   w->tiles = (uint32_t*)take(r.tiles * 8);
-  w->line = (uint64_t*)take(r.line * 8);
+  *line = (uint64_t*)take(r.line * 8);
   return at;
 }
 
@@ -1797,11 +1800,11 @@ int allow_lds(int device) {
 template <typename T, int D, int MOD, bool TREE>
 int launch_attn(const char* what, const Launch& L, int device, hipStream_t s) {
   const uint32_t G = L.a.n_kv;
-  if (L.n.planned) RLH_TRY(enqueue(what, TREE && L.n.line_blocks ? k_line_plan : k_attn_plan<TREE>, dim3(1), kPlanThreads, 0, s, L));
+  if (L.n.planned) RLH_TRY(enqueue(what, TREE && L.b.line_blocks ? k_line_plan : k_attn_plan<TREE>, dim3(1), kPlanThreads, 0, s, L));
   if (L.a.shared_len || L.n.tiled) {
     RLH_TRY((allow_lds<T, D, MOD, TREE>(device)));
     if constexpr (TREE) {
-      RLH_TRY(enqueue(what, k_attn_line<T, D, MOD>, dim3(L.n.line_blocks * G), 64 * kTileWaves, kTileLds<D, true>, s, L));
+      RLH_TRY(enqueue(what, k_attn_line<T, D, MOD>, dim3(L.b.line_blocks * G), 64 * kTileWaves, kTileLds<D, true>, s, L));
     } else {
       const uint32_t blocks = (prefix_blocks(L.n) + L.n.tiles * L.n.tile_parts) * G + (L.n.items * G + 1) / 2;
       RLH_TRY(enqueue(what, k_attn_mixed<T, D, MOD>, dim3(blocks), 64 * kTileWaves, kMixedLds<D>, s, L));
@@ -1815,7 +1818,7 @@ int launch_attn(const char* what, const Launch& L, int device, hipStream_t s) {
   }
   if (!L.n.merge) return RLH_OK;
   if constexpr (TREE)
-    if (L.n.line_blocks) {
+    if (L.b.line_blocks) {
       const uint64_t waves = (uint64_t)L.a.b.n_rows * ((L.a.n_head + 3) / 4);
       return enqueue(what, k_line_merge<T, D>, dim3((uint32_t)((waves + kWaves - 1) / kWaves)), kThreads, 0, s, L);
     }
@@ -1847,7 +1850,13 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
   if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;
   Launch L{};
   L.n = attn_sizes<TREE>(*kv, *seqs, *args);
-  const uint64_t need = place_workspace(&L.ws, (uint8_t*)workspace, kv->head_dim, attn_room(*kv, *seqs, *args, L.n));
+  const bool line = TREE && (L.n.tiled || args->shared_len);
+  if (line) {
+    L.b.line_blocks = line_blocks(kv->n_head_kv);
+    L.b.slot_rows = line_slot_rows(*seqs, args->n_head / kv->n_head_kv, args->shared_len != 0);
+  }
+  const uint64_t need = place_workspace(&L.ws, &L.b.line, (uint8_t*)workspace, kv->head_dim,
+                                        line ? line_room(*kv, *seqs, *args) : attn_room(*kv, *seqs, *args, L.n));
   if (need && !workspace) return serve_error(RLH_EINVAL, "workspace is null");
   if (need > workspace_bytes)
     return serve_error(RLH_EINVAL, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
@@ -1900,9 +1909,6 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
   p.slopes = args->slopes;
   p.prefix_len = args->prefix_len;
   p.shared_table = args->shared_table;
-  p.masks = masks;
-  p.mask_words = mask_words;
-  p.lse = lse;
   p.status = status;
   p.n_head = args->n_head;
   p.n_kv = kv->n_head_kv;
@@ -1912,6 +1918,9 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
   p.window = args->window;
   p.shared_len = args->shared_len;
   L.a = p;
+  L.b.lse = lse;
+  L.b.masks = masks;
+  L.b.mask_words = mask_words;
   int mod;
   L.sc = scoring_of(*args, &mod);
   if (kv->type == RLH_TYPE_F16)
@@ -1922,7 +1931,8 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
 template <bool TREE>
 uint64_t attn_workspace(const rlh_kv_pages& kv, const rlh_seqs& seqs, const rlh_attn_args& args) {
   Workspace w;
-  return place_workspace(&w, nullptr, kv.head_dim, TREE ? tree_room_within(kv, seqs, args) : attn_room_within(kv, seqs, args));
+  uint64_t* line;
+  return place_workspace(&w, &line, nullptr, kv.head_dim, TREE ? tree_room_within(kv, seqs, args) : attn_room_within(kv, seqs, args));
 }
 
 }  // namespace
