@@ -265,9 +265,9 @@ struct SeqSpan {
 };
 
 template <bool TREE>
-__device__ __forceinline__ SeqSpan seq_span(const AttnParams& a, uint32_t s, bool* bad) {
+__device__ __forceinline__ SeqSpan span_of_seq(const AttnParams& a, uint32_t s, const SeqView& v) {
   SeqSpan r;
-  r.v = load_attn_seq<TREE>(a, s, bad);
+  r.v = v;
   r.rows = r.v.ok ? r.v.q_len * a.group : 0;
   r.p0 = (int32_t)(r.v.kv_len - r.v.q_len);
   r.prefix = a.prefix_len ? a.prefix_len[s] : 0;
@@ -278,6 +278,10 @@ __device__ __forceinline__ SeqSpan seq_span(const AttnParams& a, uint32_t s, boo
     r.end = TREE ? (int32_t)r.v.kv_len : span_end(row_span((int32_t)r.v.kv_len - 1, r.v.kv_len, a.window, r.prefix));
   }
   return r;
+}
+template <bool TREE>
+__device__ __forceinline__ SeqSpan seq_span(const AttnParams& a, uint32_t s, bool* bad) {
+  return span_of_seq<TREE>(a, s, load_attn_seq<TREE>(a, s, bad));
 }
 
 __device__ __forceinline__ uint32_t lane_value(uint32_t x, int lane) {
@@ -662,6 +666,7 @@ struct TileJob {
   uint32_t h, s, row0, rows;  // KV head, sequence (own positions), the tile's first row and all rows
   bool prefix;                // the shared positions, of the rows of all sequences
   uint32_t part, parts;       // TREE false: the part of the tile's positions
+  SeqView v;                  // TREE: the sequence, as it counts
   int32_t begin, end;         // TREE: the positions that steps count from, and their end
   uint32_t st0, st1;          // TREE: its steps
   float *o, *ml;              // TREE: where a part of the tile goes (null: the tile is whole)
@@ -706,9 +711,8 @@ __device__ __forceinline__ void tile_run(const Launch& L, const TileJob& job, ui
     active = active && sq < a.b.n_seq;
   }
   SeqView sv{};
-  if (TREE && !prefix) {  // (a tile's sequence is one that counts)
-    bool bad;
-    sv = load_attn_seq<TREE>(a, s, &bad);
+  if (TREE && !prefix) {
+    sv = job.v;
     row += sv.q0;
   } else if (active) {
     bool bad;
@@ -1160,12 +1164,15 @@ struct LineSeq {
   uint32_t steps;
   uint64_t units;
 };
-__device__ __forceinline__ LineSeq line_seq(const AttnParams& a, uint32_t s, bool* bad) {
+__device__ __forceinline__ LineSeq line_seq(const AttnParams& a, uint32_t s, const SeqView& v) {
   LineSeq r;
-  r.q = seq_span<true>(a, s, bad);
+  r.q = span_of_seq<true>(a, s, v);
   r.steps = r.q.rows ? (uint32_t)(r.q.end - r.q.begin + kTileKv - 1) / kTileKv : 0;
   r.units = line_units(r.q.rows, r.steps);
   return r;
+}
+__device__ __forceinline__ LineSeq line_seq(const AttnParams& a, uint32_t s, bool* bad) {
+  return line_seq(a, s, load_attn_seq<true>(a, s, bad));
 }
 // Inclusive sum over the wave in lane order, of 64 bits.
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t x) {
@@ -1192,6 +1199,7 @@ template <typename T, int D, int MOD>
 __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
   extern __shared__ __align__(1024) uint8_t lds[];
   __shared__ uint64_t line[2 + kPlanned];  // a block's share and all units, then each sequence's first one
+  __shared__ uint32_t views[kPlanned][3];  // each sequence's first row, rows and positions
   const AttnParams& a = L.a;
   const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const uint32_t h = blockIdx.x % a.n_kv, block = blockIdx.x / a.n_kv;
@@ -1203,7 +1211,11 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
         uint64_t u = 0;
         if (s < a.b.n_seq) {
           bool bad;
-          u = line_seq(a, s, &bad).units;
+          const LineSeq q = line_seq(a, s, &bad);
+          u = q.units;
+          views[s][0] = q.q.v.q0;
+          views[s][1] = q.q.v.q_len;
+          views[s][2] = q.q.v.kv_len;
           if (bad && blockIdx.x == 0) raise(a.status, RLH_SERVE_BAD_SEQ);
         }
         const uint64_t upto = before + wave_scan64(u);
@@ -1246,11 +1258,23 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_line(Launch L) {
       job.s = uniform(n - 1);
       first = lane_value64(L.n.planned ? L.b.line[2 + job.s] : line[2 + job.s], 0);
       bool bad;
-      const LineSeq q = line_seq(a, job.s, &bad);
-      job.rows = uniform(q.q.rows);
-      job.begin = (int32_t)uniform((uint32_t)q.q.begin);
-      job.end = (int32_t)uniform((uint32_t)q.q.end);
-      steps = uniform(q.steps);
+      SeqView v{0, 0, 0, true};  // (one with units counts)
+      if (L.n.planned) {
+        v = load_attn_seq<true>(a, job.s, &bad);
+      } else {
+        v.q0 = views[job.s][0];
+        v.q_len = views[job.s][1];
+        v.kv_len = views[job.s][2];
+      }
+      v.q0 = uniform(v.q0);
+      v.q_len = uniform(v.q_len);
+      v.kv_len = uniform(v.kv_len);
+      const LineSeq q = line_seq(a, job.s, v);
+      job.v = v;
+      job.rows = q.q.rows;
+      job.begin = q.q.begin;
+      job.end = q.q.end;
+      steps = q.steps;
     }
     const uint32_t k = line_at(first, job.rows, steps, x);
     const LineTile tile = line_tile(first, job.rows, steps, k);

@@ -98,10 +98,16 @@ RLH_HD uint64_t tree_bits(const uint64_t* mask, uint32_t words, uint32_t q_len, 
 // memory sets the pace: 2.3 and 1.6 us), a tile's start two steps more.
 constexpr uint32_t kLineRows = 256;
 constexpr uint32_t kLineStart = 2;
-// Units of a block at least: parts are joined by another launch, and a block
-// starts with a chain of loads that takes as long as three steps.
-constexpr uint32_t kLineLeast = 12;
+// Units of a block at least: a step, so that the blocks of a tile follow one on
+// another. (A block starts with a chain of loads that takes as long as five
+// steps, but the starts of blocks that would otherwise not be there cost nothing:
+// a tree of 26 nodes at 640 positions takes 19 us by blocks of 12 units.)
+constexpr uint32_t kLineLeast = 4;
 
+// a / b, by 32 bits where they do (64 take some 200 instructions more).
+RLH_HD uint64_t line_div(uint64_t a, uint64_t b) {
+  return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 RLH_HD uint32_t line_weight(uint32_t rows) { return rows > kLineRows / 2 ? 3 : 2; }
 RLH_HD uint32_t line_tiles(uint32_t rows) { return (rows + kLineRows - 1) / kLineRows; }
 // Units of all tiles of `rows` rows.
@@ -111,7 +117,7 @@ RLH_HD uint64_t line_units(uint32_t rows, uint32_t steps) {
   return ((uint64_t)full * 3 + line_weight(rows - full * kLineRows)) * (steps + kLineStart);
 }
 RLH_HD uint64_t line_share(uint64_t units, uint32_t blocks) {
-  const uint64_t n = (units + blocks - 1) / blocks;
+  const uint64_t n = line_div(units + blocks - 1, blocks);
   return n > kLineLeast ? n : kLineLeast;
 }
 
@@ -126,21 +132,25 @@ RLH_HD LineTile line_tile(uint64_t first, uint32_t rows, uint32_t steps, uint32_
 RLH_HD uint64_t line_end(const LineTile& t) { return t.begin + (uint64_t)t.weight * (t.steps + kLineStart); }
 // The tile that unit x, at or behind `first`, lies in.
 RLH_HD uint32_t line_at(uint64_t first, uint32_t rows, uint32_t steps, uint64_t x) {
-  const uint64_t k = (x - first) / (3 * (uint64_t)(steps + kLineStart));
+  if (rows <= kLineRows) return 0;
+  const uint64_t k = line_div(x - first, 3 * (uint64_t)(steps + kLineStart));
   return k < line_tiles(rows) ? (uint32_t)k : line_tiles(rows) - 1;
 }
 // A step belongs to the block in whose units it begins: the first step that
 // begins at unit x or behind, and the blocks (of `share` units, more than a
 // step's) of the first and the last one.
 RLH_HD uint32_t line_step(const LineTile& t, uint64_t x) {
-  const uint64_t n = x > t.begin ? (x - t.begin + t.weight - 1) / t.weight : 0;
-  return n <= kLineStart ? 0 : n - kLineStart < t.steps ? (uint32_t)(n - kLineStart) : t.steps;
+  // (fewer than 2^26 units, or the tile is over)
+  const uint64_t u = x > t.begin ? x - t.begin : 0;
+  if (u >= (uint64_t)t.weight * (t.steps + kLineStart)) return t.steps;
+  const uint32_t n = t.weight == 2 ? ((uint32_t)u + 1) / 2 : ((uint32_t)u + 2) / 3;
+  return n <= kLineStart ? 0 : n - kLineStart < t.steps ? n - kLineStart : t.steps;
 }
 RLH_HD uint32_t line_first_block(const LineTile& t, uint64_t share) {
-  return (uint32_t)((t.begin + t.weight * kLineStart) / share);
+  return (uint32_t)line_div(t.begin + t.weight * kLineStart, share);
 }
 RLH_HD uint32_t line_last_block(const LineTile& t, uint64_t share) {
-  return (uint32_t)((t.begin + (uint64_t)t.weight * (kLineStart + t.steps - 1)) / share);
+  return (uint32_t)line_div(t.begin + (uint64_t)t.weight * (kLineStart + t.steps - 1), share);
 }
 // A block has two places for parts of tiles: the first for the tile that it
 // begins in or at, the second for one that it begins and does not end.

@@ -131,7 +131,7 @@ def test_a_line_of_tiles_is_divided_once(shim):
         if at == 0:
             continue
         share = shim.shim_line_share(U64(at), U32(n_blocks))
-        assert share >= 12 and share * n_blocks >= at
+        assert share >= 3 and share * n_blocks >= at
         used = {}
         done = [np.zeros(((r + 255) // 256, st), int) for r, st in zip(rows, steps)]
         whole = set()
