@@ -1153,12 +1153,13 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
 // its sequence's length, and batches have few and unequal tiles. The tiles of a KV
 // head (of the shared positions first, then the sequences' own) are therefore
 // laid out as one line and divided equally among as many blocks as run at once
-// (16 trees of 26 nodes, 32 heads, behind 1100 to 8200 positions: 63 + 6 us; with
+// (16 trees of 26 nodes, 32 heads, behind 1100 to 8200 positions: 62 + 6 us; with
 // a block to a tile 192 + 5). A step of up to 64 rows takes 1.63 us (32 KB on each
 // CU: 5.05 TB/s, HBM), of 128 rows 1.9, of 256 2.6 (766 TFLOP/s: reads of LDS,
 // products and exponentials of all eight waves one behind the other; halves of the
-// block taking turns at them were measured at 2.9). A launch starts and ends with 13
-// us beside its steps: sequences, pages and first copies are a chain of loads.
+// block taking turns at them were measured at 2.9). A launch starts and ends with 9
+// to 11 us beside its steps: sequences, pages and first copies are a chain of loads,
+// and parts are written (133 KB of 256 rows).
 struct LineSeq {
   SeqSpan q;
   uint32_t steps;
