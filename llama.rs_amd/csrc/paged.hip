@@ -27,7 +27,7 @@ int check_batch(const rlh_kv_pages* kv, const rlh_seqs* seqs, uint32_t n_head) {
   if (overlap(kv->k, pool, kv->v, pool)) return serve_error(RLH_EINVAL, "the pool's k and v overlap");
   if (seqs->n_seq > 65535) return serve_error(RLH_EUNSUP, "more than 65535 sequences");
   if (seqs->n_rows > 0x800000u) return serve_error(RLH_EUNSUP, "more than 2^23 rows");
-  // launches hold fewer than 2^24 blocks
+  // launches hold fewer than 2^24 blocks of 256 threads
   if ((uint64_t)seqs->n_rows * n_head > (1ull << 25)) return serve_error(RLH_EUNSUP, "n_rows * n_head above 2^25");
   if ((uint64_t)seqs->n_seq * kv->n_head_kv > (1ull << 21)) return serve_error(RLH_EUNSUP, "n_seq * n_head_kv above 2^21");
   if (seqs->n_seq == 0 || seqs->n_rows == 0) return RLH_OK;  // nothing to do

@@ -230,8 +230,9 @@ int launch_move(const MoveParams& p, hipStream_t stream) {
 template <int D>
 int launch_move(const MoveParams& p, hipStream_t stream) {
   // Short lists (accepted branches): whole rows by small blocks, one row ahead (three
-  // rows of 96 sequences: 3.7 us, by the other form 7.7). Long ones: slices of 64 bytes.
-  if (p.max_count <= 256) return launch_move<D, D / 8, 256, 1>(p, stream);
+  // rows of 96 sequences: 3.7 us, by the other form 7.7). Long ones: slices of 64 bytes,
+  // while a launch holds them (fewer than 2^32 threads): 2^18 lists fill the card without.
+  if (p.max_count <= 256 || (uint64_t)p.n_seq * p.n_kv > (1u << 18)) return launch_move<D, D / 8, 256, 1>(p, stream);
   return launch_move<D, 4, 1024, 8>(p, stream);
 }
 

@@ -141,6 +141,8 @@ struct as_is {
 template <typename... P>
 int enqueue(const char* what, void (*kernel)(P...), dim3 grid, uint32_t threads, uint32_t lds, hipStream_t stream,
             typename as_is<P>::type... args) {
+  // (a launch of 2^32 threads or more is not refused: it leaves blocks out)
+  if ((uint64_t)grid.x * threads >> 32) return serve_error(RLH_EUNSUP, std::string(what) + ": a launch of 2^32 threads");
   void* p[] = {(void*)&args...};
   const hipError_t e = hipLaunchKernel((const void*)kernel, grid, dim3(threads), p, lds, stream);
   if (e == hipSuccess) return RLH_OK;
