@@ -65,10 +65,14 @@ int rlh_tree_masks(const rlh_seqs* seqs, const uint32_t* parents, const uint32_t
  * position before its sequence's new rows (of which the window, if any, leaves
  * the last window - c, c being the new rows that it sees), and the new rows
  * whose bit its mask has, also behind it; bits of no new row are ignored. Any
- * masks will do, those of rlh_tree_masks among them. slopes and prefix_len are
- * RLH_EUNSUP; shared_len must not reach into the new rows (RLH_SERVE_BAD_SEQ).
- * lse may be NULL. The workspace is as rlh_paged_attn_workspace says of its
- * own. n_rows * mask_words <= 2^32. */
+ * masks will do, those of rlh_tree_masks among them. The window alone does not
+ * bound c: with RLH_WINDOW_DRAFTS | window a row that sees more than `window` new
+ * rows sees the last `window` of them (and nothing before), as rlh_paged_attn's
+ * row of the same line of tokens does. A model with a window needs it wherever a
+ * branch may be longer than the window. slopes and prefix_len are RLH_EUNSUP; shared_len must not reach into the new rows (RLH_SERVE_BAD_SEQ).
+ * lse may be NULL. The workspace is as rlh_paged_attn_workspace says of its own; for
+ * calls with RLH_WINDOW_DRAFTS it is asked for with it. n_rows * mask_words <= 2^32. */
+#define RLH_WINDOW_DRAFTS 0x80000000u
 uint64_t rlh_tree_attn_workspace(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args);
 int rlh_tree_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args, const uint64_t* masks,
                   uint32_t mask_words, float* lse, void* workspace, uint64_t workspace_bytes, uint32_t* status,

@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "../../include/rlh_cache.h"
 #include "paged_device.h"
 #include "rlh_device.h"
 #include "serve_check.h"
@@ -189,6 +190,7 @@ struct Workspace {
   float* item_ml;    // [items * n_kv][16][2]
   uint32_t* plan;    // [n_seq][2]: first item, items
   uint32_t* tiles;   // [n_seq][2]: first tile, tiles (where `planned`)
+  uint64_t* masks;   // [n_rows][words of max_q]: what a window leaves of the drafted rows' masks
 };
 
 struct Sizes {
@@ -1326,6 +1328,18 @@ __global__ void __launch_bounds__(kPlanThreads) k_line_plan(Launch L) {
   }
 }
 
+// What the window leaves of the masks, where it bounds the drafts too: a block to
+// a sequence, a thread to a row. (A launch of its own, of calls whose drafts may
+// pass the window: with the bound in the attention's own look at the masks every
+// call took 0.6 to 1.6 % longer.)
+__global__ void __launch_bounds__(kThreads) k_window_masks(Launch L, uint32_t words) {
+  bool bad;
+  const SeqView v = load_seq(L.a.b, blockIdx.x, &bad);
+  if (!v.ok) return;
+  for (uint32_t i = threadIdx.x; i < v.q_len; i += kThreads)
+    tree_window(L.b.masks + (size_t)(v.q0 + i) * L.b.mask_words, words, v.q_len, L.a.window, L.ws.masks + (size_t)(v.q0 + i) * words);
+}
+
 // ---- joining the parts of a row ------------------------------------------------------
 // A wave takes a row of a query head, its four groups of 16 lanes every
 // fourth part: all maxima at once, then the parts' values, four parts' loads
@@ -1714,7 +1728,11 @@ struct Room {
   uint64_t prefix, tile, item;  // partial results of a row and head (or of an item's row)
   uint64_t plan, tiles;         // sequences
   uint64_t line;                // units
+  uint64_t masks;               // words
 };
+
+// Words of the masks that a window leaves, of all rows.
+uint64_t window_words(const rlh_seqs& q) { return (uint64_t)q.n_rows * ((q.max_q + 63) / 64); }
 
 // What the line of tiles takes. (Monotone in all sizes.)
 Room line_room(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_args& args) {
@@ -1772,6 +1790,7 @@ Room tree_room_within(const rlh_kv_pages& kv, const rlh_seqs& q, const rlh_attn_
   if (small && !whole && q.max_kv > 32 * kWaves)
     r.item = std::max(r.item, ((uint64_t)q.n_seq + item_goal(kv.n_head_kv)) * kv.n_head_kv * kSmallRows);
   r.plan = small ? q.n_seq : 0;
+  r.masks = args.window & RLH_WINDOW_DRAFTS ? window_words(q) : 0;
   return r;
 }
 
@@ -1792,6 +1811,7 @@ uint64_t place_workspace(Workspace* w, uint64_t** line, uint8_t* base, uint64_t 
   w->plan = (uint32_t*)take(r.plan * 8);
   w->tiles = (uint32_t*)take(r.tiles * 8);
   *line = (uint64_t*)take(r.line * 8);
+  w->masks = (uint64_t*)take(r.masks * 8);
   return at;
 }
 
@@ -1880,8 +1900,12 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
     L.b.line_blocks = line_blocks(kv->n_head_kv);
     L.b.slot_rows = line_slot_rows(*seqs, args->n_head / kv->n_head_kv, args->shared_len != 0);
   }
-  const uint64_t need = place_workspace(&L.ws, &L.b.line, (uint8_t*)workspace, kv->head_dim,
-                                        line ? line_room(*kv, *seqs, *args) : attn_room(*kv, *seqs, *args, L.n));
+  const uint32_t window = TREE ? args->window & ~RLH_WINDOW_DRAFTS : args->window;
+  // whether a row may see more drafts than the window, which bounds them
+  const bool bounded = TREE && window != args->window && window != 0 && seqs->max_q > window;
+  Room room = line ? line_room(*kv, *seqs, *args) : attn_room(*kv, *seqs, *args, L.n);
+  if (bounded) room.masks = window_words(*seqs);
+  const uint64_t need = place_workspace(&L.ws, &L.b.line, (uint8_t*)workspace, kv->head_dim, room);
   if (need && !workspace) return serve_error(RLH_EINVAL, "workspace is null");
   if (need > workspace_bytes)
     return serve_error(RLH_EINVAL, "workspace of " + std::to_string(workspace_bytes) + " bytes, " + std::to_string(need) + " needed");
@@ -1940,7 +1964,7 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
   p.group = args->n_head / kv->n_head_kv;
   p.page_shift = (uint32_t)__builtin_ctz(kv->page_size);
   p.n_pages = (uint32_t)kv->n_pages;
-  p.window = args->window;
+  p.window = window;
   p.shared_len = args->shared_len;
   L.a = p;
   L.b.lse = lse;
@@ -1948,6 +1972,13 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
   L.b.mask_words = mask_words;
   int mod;
   L.sc = scoring_of(*args, &mod);
+  if constexpr (TREE)
+    if (bounded) {
+      const uint32_t words = (seqs->max_q + 63) / 64;
+      RLH_TRY(enqueue(what, k_window_masks, dim3(seqs->n_seq), kThreads, 0, (hipStream_t)stream, L, words));
+      L.b.masks = L.ws.masks;
+      L.b.mask_words = words;
+    }
   if (kv->type == RLH_TYPE_F16)
     return launch_attn<_Float16, TREE>(what, L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);
   return launch_attn<__bf16, TREE>(what, L, kv->head_dim, mod, dev.device(), (hipStream_t)stream);

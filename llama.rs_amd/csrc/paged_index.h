@@ -89,6 +89,18 @@ RLH_HD uint64_t tree_bits(const uint64_t* mask, uint32_t words, uint32_t q_len, 
   return only_rows(x, (int64_t)q_len - off);
 }
 
+// The last `window` of the new rows that a mask names, as a mask of as many words.
+RLH_HD void tree_window(const uint64_t* mask, uint32_t words, uint32_t q_len, uint32_t window, uint64_t* out) {
+  uint32_t left = window;
+  for (uint32_t w = words; w-- > 0;) {
+    uint64_t x = only_rows(mask[w], (int64_t)q_len - (int64_t)w * 64);
+    uint32_t n = (uint32_t)__builtin_popcountll(x);
+    for (; n > left; n--) x &= x - 1;
+    left -= n;
+    out[w] = x;
+  }
+}
+
 // ---- a line of tiles ------------------------------------------------------------------
 // The work of drafted rows: tiles of up to kLineRows rows of a KV head, each of
 // which takes the same `steps`; all tiles, one behind the other, make a line that

@@ -332,6 +332,7 @@ class EvictArgs(ctypes.Structure):
 
 SERVE_BAD_PAGE, SERVE_BAD_SEQ = 1, 2
 NO_PARENT = 0xffffffff
+WINDOW_DRAFTS = 0x80000000
 ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS = 0, 1, 2
 
 _lib = None
