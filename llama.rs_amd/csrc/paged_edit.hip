@@ -457,6 +457,10 @@ int check_cached(const rlh_kv_pages* kv, const rlh_seqs* seqs) {
   rlh_seqs s = *seqs;
   s.n_rows = s.max_q = 1;
   s.q_start = s.kv_len;
+  if (s.max_kv == 0) {  // all sequences are empty
+    s.max_kv = 1;
+    s.table_stride = std::max(s.table_stride, 1u);
+  }
   return check_batch(kv, &s, kv->n_head_kv);
 }
 

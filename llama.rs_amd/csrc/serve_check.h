@@ -54,6 +54,7 @@ struct Area {
   const char* name;
   const void* p;
   uint64_t rows, stride, width;
+  bool empty() const { return !p || rows == 0 || width == 0; }
   uint64_t span() const { return rows ? (rows - 1) * stride + width : 0; }
 };
 inline Area area(const char* name, const void* p, uint64_t bytes) { return Area{name, p, 1, bytes, bytes}; }
@@ -61,7 +62,7 @@ inline Area area(const char* name, const void* p, uint64_t bytes) { return Area{
 // Whether they share a byte; what lies between one's rows is not its own (of
 // two with gaps, the second counts as a whole).
 inline bool meet(const Area& a, const Area& b) {
-  if (!a.p || !b.p || !overlap(a.p, a.span(), b.p, b.span())) return false;
+  if (a.empty() || b.empty() || !overlap(a.p, a.span(), b.p, b.span())) return false;
   if (a.rows == 1 && b.rows > 1) return meet(b, a);
   if ((uintptr_t)b.p < (uintptr_t)a.p) return true;
   const uint64_t off = (uintptr_t)b.p - (uintptr_t)a.p, row = off / a.stride;

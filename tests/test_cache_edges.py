@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import rlh
-from test_cache import ROOT, I32, U32, ptr
+from test_cache import ROOT, I32, U32, _has_gpu, call, good, ptr
 from test_serve_edges import A as far
 from test_serve_edges import attention_args, log_int
 
@@ -97,3 +97,18 @@ def test_a_tree_workspace_for_windows_serves_every_smaller_batch(heads, kv):
 
     assert needed(rlh.WINDOW_DRAFTS | 4) == needed(4) + 256
     assert needed(rlh.WINDOW_DRAFTS | 8) == needed(rlh.WINDOW_DRAFTS) == needed(4)
+
+
+@pytest.mark.skipif(_has_gpu(), reason="checks the no-GPU error path")
+@pytest.mark.parametrize("stride", [0, 4])
+@pytest.mark.parametrize("op", ["paged_move", "evict_select"])
+def test_batches_of_empty_sequences_are_taken(op, stride):
+    """max_kv 0: every sequence is empty, its count is written all the same.
+    An array of no bytes overlaps nothing."""
+    args = good()
+    args["seqs"].update(max_kv=0, max_q=0, n_rows=0, q_start=0, table_stride=stride)
+    args["evi"]["keep_stride"] = 0
+    for table in (args["seqs"]["table"], args["evi"]["mass"] + 64, args["kv"]["k"] + 64):
+        args["seqs"]["table"] = table
+        rc, said = call(op, args)
+        assert rc == rlh.RLH_EDEVICE and "no HIP device" in said, (said, table)

@@ -133,3 +133,22 @@ def test_a_bounding_window_captured_and_replayed():
         tighter = [last_seen(see[:, n - rows:], n - rows, 2) for see, (rows, n) in zip(sees, case["seqs"])]
         run_tree(b, q, out, heads, masks, lse, window=rlh.WINDOW_DRAFTS | 2, ws=ws)
         check_tree(b, q, out, lse, heads, tighter)
+
+
+# ---- empty sequences ------------------------------------------------------------------
+
+def test_a_batch_of_empty_sequences():
+    """With max_kv 0 every count is 0 and nothing moves; a sequence that is not empty is skipped."""
+    b = ref.Batch([(0, 0), (0, 0), (0, 0)], 2, 64, 16, rlh.F16, seed=1, pad_rows=1)
+    b.kv_len[1] = 5
+    keep = torch.full((3, 2, 4), 99, dtype=torch.int32, device="cuda")
+    count, mass, st = torch.full((3,), 99, dtype=torch.int32, device="cuda"), torch.rand(b.k.shape[:3], device="cuda"), word()
+    for stride in (0, b.table.shape[1]):
+        seqs = rlh.Seqs(3, 0, 0, 0, stride, None, at(b.kv_len), at(b.table))
+        st.zero_()
+        rlh.evict_select(b.kv(), seqs, rlh.EvictArgs(at(mass), 4, 1, 1, 4, at(keep), at(count)), at(st), stream())
+        assert int(st) == rlh.SERVE_BAD_SEQ and count.tolist() == [0, 0, 0] and torch.all(keep == 99)
+        k, m = b.k.clone(), mass.clone()
+        st.zero_()
+        rlh.paged_move(b.kv(), seqs, rlh.MoveArgs(at(keep), 4, 1, at(count), 4, None, at(mass), at(mass)), at(st), stream())
+        assert int(st) == 0 and torch.equal(b.k, k) and torch.equal(mass, m)
