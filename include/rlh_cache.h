@@ -138,7 +138,7 @@ int rlh_paged_move(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_move_
  * Rows whose lse is minus infinity add nothing. decay is finite and not
  * negative. Scores, exponentials and sums are f32; a term is off by about 2^-21
  * of itself (a score of 16; more for larger ones) and as a cap is in
- * rlh_paged_attn. v of kv is not read. Sequences own the pages from shared_len on;
+ * rlh_paged_attn; terms below 2^-126 may count as none. v of kv is not read. Sequences own the pages from shared_len on;
  * a sequence without rows is left alone. */
 int rlh_paged_mass(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args, const float* lse,
                    float decay, float* mass, uint32_t* status, void* stream);

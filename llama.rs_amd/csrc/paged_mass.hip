@@ -31,7 +31,8 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // What a weight needs to know of its row: exp(s - lse) is formed as 2^(s2 - lse2)
 // * rest, where the log in units of log 2 is taken in two parts (one would put
-// 2^-21 into every weight).
+// 2^-21 into every weight). The hardware's exponential has no values below 2^-126:
+// such a weight is 0, which no sum with a larger one can tell.
 struct MassRow {
   float lse2, rest, slope2;
   int32_t pos;  // of the row; below zero: it adds nothing
