@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import rlh
-from test_cache import ROOT, I32, U32, _has_gpu, call, good, ptr
+from test_cache import ROOT, I32, U32, U64, _has_gpu, call, good, ptr
 from test_serve_edges import A as far
 from test_serve_edges import attention_args, log_int
 
@@ -112,3 +112,50 @@ def test_batches_of_empty_sequences_are_taken(op, stride):
         args["seqs"]["table"] = table
         rc, said = call(op, args)
         assert rc == rlh.RLH_EDEVICE and "no HIP device" in said, (said, table)
+
+
+# ---- that the GPU tests reach what they are for -----------------------------------------
+
+@pytest.fixture(scope="module")
+def line(tmp_path_factory):
+    out = tmp_path_factory.mktemp("line") / "libtree_index_shim.so"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(out), os.path.join(HERE, "tree_index_shim.cpp")], check=True)
+    lib = ctypes.CDLL(str(out))
+    lib.shim_line_units.restype = lib.shim_line_share.restype = U64
+    return lib
+
+
+def test_long_jobs_are_long(line):
+    """The steps that one block takes of one tile, in the batches of
+    test_gpu_cache_edges.py: more than 32, and the first job of the line too."""
+    from test_gpu_cache_edges import LONG_JOBS
+
+    out = (U32 * 4 * 4096)()
+    for name, case in LONG_JOBS.items():
+        group, shared, window = case["heads"] // case["kv"], case.get("shared", 0), case.get("window", 0)
+        tiles = [(sum(q for q, _ in case["seqs"]) * group, shared // 64)] if shared else []
+        for q, n in case["seqs"]:
+            begin = max(shared, n - q - window if window else 0) // 16 * 16
+            tiles.append((q * group, -(-(n - begin) // 64)))
+        at, firsts = 0, []
+        for rows, steps in tiles:
+            firsts.append(at)
+            at += line.shim_line_units(U32(rows), U32(steps))
+        blocks = max(1, 256 // case["kv"])
+        share = line.shim_line_share(U64(at), U32(blocks))
+        jobs = []
+        for first, (rows, steps) in zip(firsts, tiles):
+            for block in range(blocks):
+                for i in range(line.shim_line_block(U64(first), U32(rows), U32(steps), U64(share), U32(block), out)):
+                    jobs.append(out[i][2] - out[i][1])
+        assert jobs[0] > 36, (name, jobs)
+
+
+def test_weights_go_on_from_step_to_step():
+    from test_gpu_cache_edges import GOES_ON
+
+    for name, case in GOES_ON.items():
+        few = max(q for q, _ in case["seqs"]) * (case["heads"] // case["kv"]) <= 16
+        steps = -(-(max(n for _, n in case["seqs"]) - case.get("shared", 0)) // 128)
+        blocks = max(1, (4096 if few else 65536) // (len(case["seqs"]) * case["kv"]))
+        assert steps > 2 * blocks and few == ("rows" not in name), name
