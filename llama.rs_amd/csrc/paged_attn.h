@@ -656,8 +656,9 @@ struct TileShared {
   int32_t ranges[kTileWaves][8];
 };
 // Steps that LDS holds: one in use, the others on their way. Prompts find
-// theirs one step ahead; drafted rows, whose steps are often shorter than what
-// HBM takes under load (of up to 128 rows 1.3 us, 2.2 us), three.
+// theirs one step ahead; drafted rows, whose steps of few rows are over before HBM
+// under load answers, three (32 trees of 7 nodes at 5120 positions: 135 us, with
+// one ahead 146).
 template <bool TREE>
 constexpr int kTileBufs = TREE ? 4 : 2;
 template <int D, bool TREE>
@@ -1156,12 +1157,14 @@ __global__ void __launch_bounds__(64 * kTileWaves, 2) k_attn_mixed(Launch L) {
 // head (of the shared positions first, then the sequences' own) are therefore
 // laid out as one line and divided equally among as many blocks as run at once
 // (16 trees of 26 nodes, 32 heads, behind 1100 to 8200 positions: 62 + 6 us; with
-// a block to a tile 192 + 5). A step of up to 64 rows takes 1.63 us (32 KB on each
-// CU: 5.05 TB/s, HBM), of 128 rows 1.9, of 256 2.6 (766 TFLOP/s: reads of LDS,
-// products and exponentials of all eight waves one behind the other; halves of the
-// block taking turns at them were measured at 2.9). A launch starts and ends with 9
-// to 11 us beside its steps: sequences, pages and first copies are a chain of loads,
-// and parts are written (133 KB of 256 rows).
+// a block to a tile 192 + 5). A step of 64 rows takes 1.49 us (32 KB on each CU:
+// 5.6 TB/s, HBM), of 128 rows 1.55 in bf16 and 1.69 in f16, of 256 2.1 and 2.3 (1027
+// and 926 TFLOP/s: reads of LDS, products and exponentials of all eight waves one
+// behind the other; halves of the block taking turns at them took 14 % longer); with
+// a cap 1.9, 2.0 and 2.8. (32 sequences of 4096 and of 12288 positions, passes apart;
+// in a row of passes the clocks fall and a step of 256 rows takes 3.0.) A call has 12
+// to 24 us beside its steps: sequences, pages and first copies are a chain of loads,
+// parts are written (133 KB of 256 rows) and joined.
 struct LineSeq {
   SeqSpan q;
   uint32_t steps;

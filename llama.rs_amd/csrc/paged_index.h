@@ -107,7 +107,7 @@ RLH_HD void tree_window(const uint64_t* mask, uint32_t words, uint32_t q_len, ui
 // blocks share equally, so that a block may end inside a tile and go on
 // with the next. Lengths are in units: a step of a tile of more than half the
 // rows takes three, of another two (there one of a SIMD's two waves idles and
-// memory sets the pace: 2.3 and 1.6 us), a tile's start two steps more.
+// memory sets the pace: 2.1 to 2.3 us, and 1.5 to 1.7), a tile's start two steps more.
 constexpr uint32_t kLineRows = 256;
 constexpr uint32_t kLineStart = 2;
 // Units of a block at least: a step, so that the blocks of a tile follow one on
