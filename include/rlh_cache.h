@@ -69,9 +69,12 @@ int rlh_tree_masks(const rlh_seqs* seqs, const uint32_t* parents, const uint32_t
  * bound c: with RLH_WINDOW_DRAFTS | window a row that sees more than `window` new
  * rows sees the last `window` of them (and nothing before), as rlh_paged_attn's
  * row of the same line of tokens does. A model with a window needs it wherever a
- * branch may be longer than the window. slopes and prefix_len are RLH_EUNSUP; shared_len must not reach into the new rows (RLH_SERVE_BAD_SEQ).
- * lse may be NULL. The workspace is as rlh_paged_attn_workspace says of its own; for
- * calls with RLH_WINDOW_DRAFTS it is asked for with it. n_rows * mask_words <= 2^32. */
+ * branch may be longer than the window. (rlh_paged_attn and the entries that
+ * score as it does take the flag too: there a window bounds all rows as it is.)
+ * slopes and prefix_len are RLH_EUNSUP; shared_len must not reach into the new
+ * rows (RLH_SERVE_BAD_SEQ). lse may be NULL. The workspace is as
+ * rlh_paged_attn_workspace says of its own; for calls with RLH_WINDOW_DRAFTS it
+ * is asked for with it. n_rows * mask_words <= 2^32. */
 #define RLH_WINDOW_DRAFTS 0x80000000u
 uint64_t rlh_tree_attn_workspace(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args);
 int rlh_tree_attn(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_args* args, const uint64_t* masks,

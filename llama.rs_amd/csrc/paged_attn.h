@@ -1903,7 +1903,7 @@ int run_attn(const char* what, const rlh_kv_pages* kv, const rlh_seqs* seqs, con
     L.b.line_blocks = line_blocks(kv->n_head_kv);
     L.b.slot_rows = line_slot_rows(*seqs, args->n_head / kv->n_head_kv, args->shared_len != 0);
   }
-  const uint32_t window = TREE ? args->window & ~RLH_WINDOW_DRAFTS : args->window;
+  const uint32_t window = args->window & ~RLH_WINDOW_DRAFTS;
   // whether a row may see more drafts than the window, which bounds them
   const bool bounded = TREE && window != args->window && window != 0 && seqs->max_q > window;
   Room room = line ? line_room(*kv, *seqs, *args) : attn_room(*kv, *seqs, *args, L.n);

@@ -400,7 +400,7 @@ int rlh_paged_mass(const rlh_kv_pages* kv, const rlh_seqs* seqs, const rlh_attn_
   L.a.group = args->n_head / kv->n_head_kv;
   L.a.page_shift = (uint32_t)__builtin_ctz(kv->page_size);
   L.a.n_pages = (uint32_t)kv->n_pages;
-  L.a.window = args->window;
+  L.a.window = args->window & ~RLH_WINDOW_DRAFTS;
   L.a.shared_len = args->shared_len;
   L.per_group = ((1ull << 36) + L.a.group - 1) / L.a.group;
   L.lse = lse;

@@ -136,6 +136,25 @@ def test_a_bounding_window_captured_and_replayed():
         check_tree(b, q, out, lse, heads, tighter)
 
 
+def test_the_flag_changes_nothing_where_a_window_bounds_all_rows():
+    """One set of arguments serves a layer's entries: attention and weights with
+    the flag are those without it."""
+    seqs, heads = [(40, 300), (3, 64), (1, 700)], 8
+    for window in (0, 5, 100):
+        got = []
+        for flag in (0, rlh.WINDOW_DRAFTS):
+            b, q, out, args, _, sees = plain_case(seqs, heads, 2, 64, 16, rlh.F16, seed=2, window=window)
+            args.window |= flag
+            lse, mass = torch.full((b.n_rows, heads), 7.0, device="cuda"), torch.ones(b.k.shape[:3], device="cuda")
+            ws = torch.empty(max(16, rlh.paged_attn_workspace(b.kv(), b.desc(), args)), dtype=torch.uint8, device="cuda")
+            rlh.paged_attn_lse(b.kv(), b.desc(), args, at(lse), at(ws), ws.numel(), None, stream())
+            rlh.paged_mass(b.kv(), b.desc(), args, at(lse), 0.5, at(mass), None, stream())
+            want, bound, _, _ = cref.attention(b, q, heads, sees, 0.125)
+            assert torch.all((out.double() - want).abs() <= bound + 1e-30)
+            got.append((out, lse, mass))
+        assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
 # ---- empty sequences ------------------------------------------------------------------
 
 def test_a_batch_of_empty_sequences():
